@@ -294,6 +294,72 @@ int vitk_sdpa_row_bwd(const float *q, int64_t ld_q, const float *k, const float 
                       float scale, int32_t dk_mode, float *dq, int64_t ld_dq, float *dk, float *dv, int64_t ld_dkv,
                       vitk_stream_t stream);
 
+/* ---- cross attention: queries of one sequence read the keys / values of another ----------------
+ * (a decoder, a prompt or learned latents reading the encoder's states; no counterpart in the
+ * reference, whose attention is over one sequence: src/layers/MultiHeadAttention.cpp:96-156.)
+ * Element (b, n, h, d) of q / out / dout / dq is at ptr[(b*Nq + n)*ld + h*dh + d], h < H; of
+ * k / v / dk / dv at ptr[(b*Nk + n)*ld + h*dh + d], h < Hkv.  H is a multiple of Hkv: query head h
+ * reads key head h / (H/Hkv), and dk / dv sum over the query heads that share one.
+ *   s = scale * q k^T over the first key_len[b] keys, p = softmax(s), out = p v
+ *   ds = p * (dout v^T - dout . out), dq = scale * ds k, dk = scale * ds^T q, dv = p^T dout
+ * key_len: device array of B lengths, values outside [0, Nk] are clamped; NULL = all Nk.  Keys and
+ * values behind the length are never read (they may hold anything, NaN too) and their dk / dv are
+ * written as 0.  A row without a key gives out = 0, stats = {0, 0} and no gradient.
+ * stats (optional in the forward, required by the backward; [B*H][Nq][2]): {row maximum of the
+ * scaled scores times log2(e), row sum of exp(score - maximum)}.
+ * Any Nq, Nk >= 0, 1 <= dh <= 128, any alignment.  Operands are finite fp32 numbers below 3.38e38 (an infinity
+ * among them gives NaN).  Outputs must not overlap inputs.  The sum over a row's
+ * keys may be split over workgroups, a rule on the sizes; every result has a fixed order of sums.
+ * workspace: vitk_cross_sdpa_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments (0 =
+ * none needed); one call at a time may use it (two captured graphs replayed at once need two). */
+typedef struct vitk_cross_sdpa_args {
+  int32_t B, H, Hkv, Nq, Nk, dh;
+  float scale;
+  int32_t reserved; /* 0 */
+  const float *q;
+  int64_t ld_q;
+  const float *k;
+  int64_t ld_k;
+  const float *v;
+  int64_t ld_v;
+  const int32_t *key_len;
+  float *out;
+  int64_t ld_out;
+  float *stats;
+  /* backward only */
+  const float *dout;
+  int64_t ld_dout;
+  float *dq;
+  int64_t ld_dq;
+  float *dk;
+  int64_t ld_dk;
+  float *dv;
+  int64_t ld_dv;
+  float *workspace;
+  size_t workspace_bytes;
+} vitk_cross_sdpa_args;
+size_t vitk_cross_sdpa_fwd_workspace_bytes(const vitk_cross_sdpa_args *args);
+int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *args, vitk_stream_t stream);
+size_t vitk_cross_sdpa_bwd_workspace_bytes(const vitk_cross_sdpa_args *args);
+int vitk_cross_sdpa_bwd(const vitk_cross_sdpa_args *args, vitk_stream_t stream);
+
+/* ---- token embedding with scaling, and its gradient by sorted tokens ---------------------------
+ * (the input side of a decoder; no counterpart in the reference.)
+ * forward:  out[i][:] = scale * table[index[i]][:]
+ * backward: dtable[t][:] = scale * sum over i with index[i] == t of dout[i][:], or with accumulate != 0
+ *           dtable[t][:] += the same (a table whose gradient another product already wrote: tied
+ *           input and output weights).
+ * index: device array of `rows` int32 values; a value outside [0, V) (padding) gives a row of zeros
+ * and adds to no gradient.  table / dtable are [V][D], out / dout [rows][D].  The backward sorts
+ * the tokens (stable) and adds each token's rows in a fixed order: no floating-point atomics, the
+ * same bits on every call.  accumulate == 0 writes every row of dtable. */
+int vitk_embedding_fwd(const float *table, int64_t V, const int32_t *index, int64_t rows, int64_t D, float scale,
+                       float *out, vitk_stream_t stream);
+size_t vitk_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D);
+int vitk_embedding_bwd(const float *dout, const int32_t *index, int64_t rows, int64_t V, int64_t D, float scale,
+                       int32_t accumulate, float *dtable, float *workspace, size_t workspace_bytes,
+                       vitk_stream_t stream);
+
 /* ---- batch assembly: dst[r][:] = src[index[r]][:]  (the per-batch gather of shuffled samples,
  * src/model/Trainer.cpp:163-199, done on the device from a dataset that stays resident in HBM).
  * index is a device array of `rows` int32 values in [0, src_rows). */
@@ -373,6 +439,48 @@ int vitk_argmax_rows(const float *x, int32_t B, int32_t K, int32_t *out, vitk_st
  * (1 normally; 1/world when averaging all-reduced gradients). */
 int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float lr, float beta1, float beta2,
                  float beta1_t, float beta2_t, float eps, float wd, float grad_scale, vitk_stream_t stream);
+
+/* ---- orthogonalised update: Newton-Schulz products, and the Muon step on them ------------------
+ * (an optimiser for weight matrices beside Adam; no counterpart in the reference.)
+ * For each of `batch` matrices of rows x cols (element (i, j) of matrix k at
+ * ptr[k*stride + i*ld + j]):
+ *   y = x / (|x|_F + eps);  `steps` times: g = y y^T, y = a y + (b g + c g g) y;  out = y
+ * (y^T y on the other side where rows > cols: the same polynomial of the singular values.)  The
+ * Frobenius norm is summed in double precision; products take fp32 operands as two fp16 parts each
+ * (22 significant bits, three matrix products, fp32 sums), the iterate y itself stays in fp32.
+ * out may be x.  0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1]
+ * within [-4, 4], with |b t^2 + c t^4| below 31 (checked on 65 points), which every useful triple does.
+ * vitk_muon_f32 (p, g, m share ld and stride, as arenas of one layout do):
+ *   m = momentum*m + grad_scale*g;  u = nesterov ? grad_scale*g + momentum*m : m
+ *   p = p * (1 - lr*weight_decay) - lr*update_scale * NS(u)
+ * workspace: *_workspace_bytes of the same arguments, 16-byte aligned, one call at a time. */
+typedef struct vitk_newton_schulz_args {
+  int32_t rows, cols, batch, steps;
+  const float *x;
+  int64_t ld_x, stride_x;
+  float *out;
+  int64_t ld_out, stride_out;
+  float a, b, c, eps;
+  float *workspace;
+  size_t workspace_bytes;
+} vitk_newton_schulz_args;
+size_t vitk_newton_schulz_workspace_bytes(int32_t rows, int32_t cols, int32_t batch);
+int vitk_newton_schulz_f32(const vitk_newton_schulz_args *args, vitk_stream_t stream);
+
+typedef struct vitk_muon_args {
+  int32_t rows, cols, batch, steps;
+  float *p;
+  const float *g;
+  float *m;
+  int64_t ld, stride;
+  float lr, momentum, weight_decay, update_scale, grad_scale;
+  int32_t nesterov;
+  float a, b, c, eps;
+  float *workspace;
+  size_t workspace_bytes;
+} vitk_muon_args;
+size_t vitk_muon_workspace_bytes(int32_t rows, int32_t cols, int32_t batch);
+int vitk_muon_f32(const vitk_muon_args *args, vitk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,647 @@
+"""Cross attention, token embeddings and the orthogonalised optimiser step against float64.
+
+Tolerances come from the arithmetic, u = 2^-24 (half a step of fp32).  A sum of n rounded terms is off by
+at most LAM * sqrt(n) * u times the sum of their magnitudes, but for a chance of 2 exp(-LAM^2 / 2) (rounding
+errors as independent, mean-zero variables); LAM = 6 makes that 3e-8.  The helpers below carry that
+through softmax and its gradient element by element, so the bound of every element is its own.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+U = 2.0 ** -24
+LAM = 6.0
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K():
+    from visiontransformer_amd import vitk
+    vitk.init(0)
+    return vitk
+
+
+def rng(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+def within(got, want, tol, what=""):
+    got, want = got.double().cpu(), want.cpu()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = (got - want).abs() - tol.cpu()
+    worst = over.argmax()
+    assert (over <= 0).all(), (f"{what}: element {int(worst)} of {tuple(got.shape)} is {got.flatten()[worst].item()}, expected "
+                               f"{want.flatten()[worst].item()} +- {tol.cpu().expand_as(want).flatten()[worst].item()}")
+
+
+# ------------------------------------------------------------------------------- cross attention
+def attention64(q, k, v, lens, scale, dout=None):
+    """float64 out (dq, dk, dv) and the bound of each element of each, one (batch, head) at a time."""
+    B, Nq, H, dh = q.shape
+    Nk, Hkv = k.shape[1:3]
+    q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
+    res = {n: torch.zeros_like(x) for n, x in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    tol = {n: torch.zeros_like(x) for n, x in res.items()}
+    stats = torch.zeros(B, H, Nq, 2, dtype=torch.float64)
+    root = lambda n: LAM * np.sqrt(n) * U  # noqa: E731
+    for b in range(B):
+        n = Nk if lens is None else min(max(int(lens[b]), 0), Nk)
+        if n == 0:
+            continue
+        for h in range(H):
+            j = h // (H // Hkv)
+            Q, Kk, Vv = q[b, :, h], k[b, :n, j], v[b, :n, j]
+            s = scale * Q @ Kk.T
+            m = s.amax(1, keepdim=True)
+            e = torch.exp(s - m)
+            l = e.sum(1, keepdim=True)
+            p = e / l
+            out = p @ Vv
+            res["out"][b, :, h] = out
+            stats[b, h, :, 0], stats[b, h, :, 1] = m[:, 0], l[:, 0]
+            # score: a dot of dh terms, the product with scale log2 e (2 roundings, of s and of the maximum)
+            es = root(dh) * abs(scale) * (Q.abs() @ Kk.abs().T) + 4 * U * (s.abs() + m.abs())
+            # probability, relative: exponent errors of the key and of the maximum's stand-in, exp2 (2 u), sum, 1/l
+            rel = es + (p * es).sum(1, keepdim=True) + (root(n) + 8 * U)
+            ep = p * rel
+            eo = ep @ Vv.abs() + root(n) * (p @ Vv.abs()) + 2 * U * out.abs()
+            tol["out"][b, :, h] = eo
+            if dout is None:
+                continue
+            G = dout[b, :, h].double().cpu()
+            dp = G @ Vv.T
+            delta = (G * out).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            edp = root(dh) * (G.abs() @ Vv.abs().T)
+            edl = (G.abs() * eo).sum(1, keepdim=True) + root(dh) * (G.abs() * out.abs()).sum(1, keepdim=True)
+            eds = p * (edp + edl + 2 * U * (dp.abs() + delta.abs())) + ep * (dp - delta).abs()
+            res["dq"][b, :, h] = scale * ds @ Kk
+            tol["dq"][b, :, h] = abs(scale) * (eds @ Kk.abs() + (root(n) + 2 * U) * (ds.abs() @ Kk.abs()))
+            res["dk"][b, :n, j] += scale * ds.T @ Q
+            # rows of all heads of the group go into one sum
+            r = root(Nq * (H // Hkv)) + 2 * U
+            tol["dk"][b, :n, j] += abs(scale) * (eds.T @ Q.abs() + r * (ds.abs().T @ Q.abs()))
+            res["dv"][b, :n, j] += p.T @ G
+            tol["dv"][b, :n, j] += ep.T @ G.abs() + r * (p.T @ G.abs())
+    return res, tol, stats
+
+
+def pitched(g, B, N, heads, dh, pad, offset=0):
+    """[B, N, heads, dh] inside rows of heads*dh + pad floats, `offset` floats into the allocation."""
+    flat = randn(g, B * N * (heads * dh + pad) + offset)[offset:]
+    return flat.reshape(B, N, heads * dh + pad)[:, :, :heads * dh].unflatten(2, (heads, dh))
+
+
+ATTENTION = {
+    # B, H, Hkv, Nq, Nk, dh, lengths, row padding, offset
+    "one_by_one": (1, 1, 1, 1, 1, 1, None, 0, 0),
+    "token_over_197": (4, 12, 12, 1, 197, 64, None, 0, 0),
+    "token_shared_heads_long": (3, 8, 2, 1, 5001, 128, [5001, 0, 1234], 0, 0),
+    "token_all_heads_share_one": (2, 7, 1, 1, 333, 48, [1, 332], 4, 0),
+    "prompt": (2, 3, 3, 33, 197, 64, None, 0, 0),
+    "one_key": (3, 4, 4, 70, 1, 64, None, 0, 0),
+    "ragged": (5, 6, 6, 65, 130, 32, [130, 0, 1, 129, 64], 0, 0),
+    "lengths_outside": (3, 2, 2, 9, 40, 64, [-5, 41, 2 ** 31 - 1], 0, 0),
+    "odd_dh_unaligned": (2, 3, 1, 37, 75, 33, [75, 31], 1, 1),
+    "dh_96_shared": (2, 8, 2, 130, 261, 96, [200, 261], 0, 0),
+    "dh_128_masked": (1, 2, 2, 257, 129, 128, None, 4, 4),
+    "dh_7": (2, 5, 5, 17, 19, 7, None, 0, 0),
+    "few_keys_many_rows": (2, 6, 6, 147, 50, 64, None, 0, 0),
+    "long_keys_split": (1, 2, 1, 40, 3001, 64, [2999], 0, 0),
+    "long_rows": (1, 2, 1, 1500, 70, 80, None, 0, 0),
+}
+
+
+@gpu
+@pytest.mark.parametrize("name", list(ATTENTION))
+def test_cross_attention_forward_and_backward(K, name):
+    B, H, Hkv, Nq, Nk, dh, lens, pad, off = ATTENTION[name]
+    g = rng(100 + list(ATTENTION).index(name))
+    q, k, v = (pitched(g, B, n, h, dh, pad, off) for n, h in ((Nq, H), (Nk, Hkv), (Nk, Hkv)))
+    dout = pitched(g, B, Nq, H, dh, pad, off)
+    out, dq = torch.full_like(q, 7.0), pitched(g, B, Nq, H, dh, pad, off)
+    dk, dv = (pitched(g, B, Nk, Hkv, dh, pad, off) for _ in range(2))
+    klen = None
+    if lens is not None:
+        klen = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        for b, n in enumerate(lens):  # what lies behind a length is never read
+            k[b, max(n, 0):] = float("nan")
+            v[b, max(n, 0):] = float("nan")
+    stats = torch.full((B * H, Nq, 2), 7.0, device="cuda")
+    want, tol, wstats = attention64(q, k.nan_to_num(), v.nan_to_num(), lens, dh ** -0.5, dout)
+    args = K.cross_sdpa_args(q, k, v, out, key_len=klen, stats=stats, dout=dout, dq=dq, dk=dk, dv=dv)
+    K.cross_sdpa_fwd(args)
+    within(out, want["out"], tol["out"], "out")
+    got = stats.double().cpu().view(B, H, Nq, 2)
+    m = got[..., 0] / np.log2(np.e)
+    assert ((m - wstats[..., 0]).abs() <= 1e-5 * (1 + wstats[..., 0].abs())).all()
+    assert ((got[..., 1] - wstats[..., 1]).abs() <= 1e-4 * (1 + wstats[..., 1])).all()
+    K.cross_sdpa_bwd(args)
+    for n, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+        within(t, want[n], tol[n], n)
+    # same bits again, and without statistics
+    first = [t.clone() for t in (out, dq, dk, dv)]
+    K.cross_sdpa_fwd(args)
+    K.cross_sdpa_bwd(args)
+    for a, b in zip(first, (out, dq, dk, dv)):
+        assert torch.equal(a, b)
+    out2 = torch.full_like(q, 7.0)
+    K.cross_sdpa_fwd(K.cross_sdpa_args(q, k, v, out2, key_len=klen))
+    assert torch.equal(out2, out)
+
+
+@gpu
+def test_cross_attention_leaves_what_is_between_the_rows(K):
+    g = rng(5)
+    B, H, N, dh = 2, 3, 11, 20
+    bufs = {n: torch.full((B, N + (n[-1] in "kv") * 8, H * dh + 12), 3.0, device="cuda") for n in ("out", "dq", "dk", "dv")}
+    view = {n: t[:, :, :H * dh].unflatten(2, (H, dh)) for n, t in bufs.items()}
+    q, k, v, dout = randn(g, B, N, H, dh), randn(g, B, N + 8, H, dh), randn(g, B, N + 8, H, dh), randn(g, B, N, H, dh)
+    stats = torch.empty(B * H, N, 2, device="cuda")
+    args = K.cross_sdpa_args(q, k, v, view["out"], stats=stats, dout=dout, dq=view["dq"], dk=view["dk"], dv=view["dv"])
+    K.cross_sdpa_fwd(args)
+    K.cross_sdpa_bwd(args)
+    for n, t in bufs.items():
+        assert (t[:, :, H * dh:] == 3.0).all(), n
+        assert (t[:, :, :H * dh] != 3.0).all(), n
+
+
+@gpu
+def test_cross_attention_without_queries_or_keys(K):
+    B, H, dh = 2, 3, 16
+    g = rng(6)
+    e = lambda n: torch.full((B, n, H, dh), 7.0, device="cuda")  # noqa: E731
+    # no keys: zeros out, zero gradient
+    out, dq, st = e(5), e(5), torch.full((B * H, 5, 2), 7.0, device="cuda")
+    a = K.cross_sdpa_args(randn(g, B, 5, H, dh), e(0), e(0), out, stats=st, dout=e(5), dq=dq, dk=e(0), dv=e(0))
+    K.cross_sdpa_fwd(a)
+    K.cross_sdpa_bwd(a)
+    assert (out == 0).all() and (st == 0).all() and (dq == 0).all()
+    # no queries: the key gradients are zeros
+    dk, dv = e(6), e(6)
+    st = torch.empty(B * H, 0, 2, device="cuda")
+    a = K.cross_sdpa_args(e(0), e(6), e(6), e(0), stats=st, dout=e(0), dq=e(0), dk=dk, dv=dv)
+    K.cross_sdpa_fwd(a)
+    K.cross_sdpa_bwd(a)
+    assert (dk == 0).all() and (dv == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("amplitude", [1e-18, 30.0])
+def test_cross_attention_extreme_scores(K, amplitude):
+    """Scores that underflow to one uniform row, and scores in the thousands (one key takes all)."""
+    g = rng(7)
+    B, H, Nq, Nk, dh = 1, 2, 40, 300, 64
+    q, k = randn(g, B, Nq, H, dh) * amplitude, randn(g, B, Nk, H, dh) * amplitude
+    v, dout = randn(g, B, Nk, H, dh), randn(g, B, Nq, H, dh) * 1e-6
+    want, tol, _ = attention64(q, k, v, None, dh ** -0.5, dout)
+    out, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+    stats = torch.empty(B * H, Nq, 2, device="cuda")
+    a = K.cross_sdpa_args(q, k, v, out, stats=stats, dout=dout, dq=dq, dk=dk, dv=dv)
+    K.cross_sdpa_fwd(a)
+    K.cross_sdpa_bwd(a)
+    tiny = 2.0 ** -126  # subnormal results may be flushed
+    for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        within(t, want[n], tol[n] + tiny, n)
+
+
+@gpu
+def test_cross_attention_gradients_against_differences(K):
+    """Central differences of sum(out * dout) in float64 of the definition, at single entries."""
+    g = rng(8)
+    B, H, Hkv, Nq, Nk, dh = 2, 4, 2, 5, 9, 12
+    q, k, v, dout = randn(g, B, Nq, H, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nq, H, dh)
+    lens = [9, 4]
+    out, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+    stats = torch.empty(B * H, Nq, 2, device="cuda")
+    a = K.cross_sdpa_args(q, k, v, out, key_len=torch.tensor(lens, dtype=torch.int32, device="cuda"), stats=stats, dout=dout,
+                          dq=dq, dk=dk, dv=dv)
+    K.cross_sdpa_fwd(a)
+    K.cross_sdpa_bwd(a)
+    base = {"q": q.double().cpu(), "k": k.double().cpu(), "v": v.double().cpu()}
+    G = dout.double().cpu()
+
+    def f(**kw):
+        x = dict(base, **kw)
+        o = torch.zeros_like(x["q"])
+        for b in range(B):
+            for h in range(H):
+                n, j = lens[b], h // 2
+                p = torch.softmax(dh ** -0.5 * x["q"][b, :, h] @ x["k"][b, :n, j].T, 1)
+                o[b, :, h] = p @ x["v"][b, :n, j]
+        return (o * G).sum().item()
+
+    step = 1e-5
+    for n, t in (("q", dq), ("k", dk), ("v", dv)):
+        for at in ((0, 1, 1, 3), (1, 3, 0, 0), (1, 4, 1, 7)):
+            plus, minus = base[n].clone(), base[n].clone()
+            plus[at] += step
+            minus[at] -= step
+            d = (f(**{n: plus}) - f(**{n: minus})) / (2 * step)
+            # differences: 1e-10 of the third derivative, 1e-11 / step of rounding; the kernel: about 1e-6
+            assert abs(t[at].item() - d) <= 2e-5 * (1 + abs(d)), (n, at)
+
+
+@gpu
+def test_cross_attention_captured_and_replayed_on_another_stream(K):
+    """Forward and backward in one graph, replayed with other inputs and lengths, eager work between."""
+    g = rng(9)
+    B, H, Hkv, Nq, Nk, dh = 2, 4, 2, 1, 2000, 64
+    q, k, v, dout = randn(g, B, Nq, H, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nq, H, dh)
+    klen = torch.tensor([Nk, 7], dtype=torch.int32, device="cuda")
+    mk = lambda: [torch.full_like(x, 7.0) for x in (q, q, k, v)]  # noqa: E731
+    (out, dq, dk, dv), eager = mk(), mk()
+    stats = [torch.empty(B * H, Nq, 2, device="cuda") for _ in range(2)]
+    a = K.cross_sdpa_args(q, k, v, out, key_len=klen, stats=stats[0], dout=dout, dq=dq, dk=dk, dv=dv)
+    e = K.cross_sdpa_args(q, k, v, eager[0], key_len=klen, stats=stats[1], dout=dout, dq=eager[1], dk=eager[2], dv=eager[3])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        K.cross_sdpa_fwd(a)
+        K.cross_sdpa_bwd(a)
+    for i in range(4):
+        q.copy_(randn(g, *q.shape))
+        v.copy_(randn(g, *v.shape))
+        klen.copy_(torch.tensor([i * 600, Nk - i], dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        K.cross_sdpa_fwd(e)
+        K.cross_sdpa_bwd(e)
+        torch.cuda.synchronize()
+        for x, y in zip((out, dq, dk, dv), eager):
+            assert torch.equal(x, y), i
+
+
+# ---------------------------------------------------------------------------------- embeddings
+EMBED = {
+    # V, D, rows, how the tokens are drawn
+    "one": (1, 1, 1, "uniform"),
+    "odd_width": (37, 33, 100, "uniform"),
+    "wide": (1000, 768, 528, "rank"),
+    "one_token_takes_all": (500, 192, 5000, "same"),
+    "padded": (300, 500, 1111, "padded"),
+    "all_padding": (64, 64, 77, "all_padding"),
+    "outside": (100, 96, 400, "outside"),
+    "many_tokens": (5000, 96, 70001, "rank"),
+    "large_table_few_tokens": (100003, 32, 9, "uniform"),
+}
+
+
+def tokens(kind, V, rows, seed):
+    r = np.random.default_rng(seed)
+    t = r.integers(0, V, rows)
+    if kind == "rank":
+        t = np.clip((float(V) ** r.random(rows)).astype(np.int64) - 1, 0, V - 1)
+    if kind == "same":
+        t[:] = V // 3
+        t[::501] = V - 1
+    if kind == "padded":
+        t[r.random(rows) < 0.4] = -1
+    if kind == "all_padding":
+        t[:] = -1
+    if kind == "outside":
+        t[::3] = V
+        t[1::7] = -2 ** 31
+        t[2::11] = 2 ** 31 - 1
+    return torch.from_numpy(t.astype(np.int32)).cuda()
+
+
+@gpu
+@pytest.mark.parametrize("name", list(EMBED))
+def test_embedding_lookup_and_gradient(K, name):
+    V, D, rows, kind = EMBED[name]
+    g = rng(200)
+    index = tokens(kind, V, rows, 1)
+    there = (index >= 0) & (index < V)
+    safe = torch.where(there, index, 0).long()
+    scale = float(np.float32(D ** 0.5))
+    table, out = randn(g, V, D), torch.full((rows, D), 7.0, device="cuda")
+    K.embedding_fwd(table, index, out, scale=scale)
+    assert torch.equal(out, torch.where(there[:, None], table[safe] * scale, 0.0))  # one product, rounded once
+    dout = randn(g, rows, D)
+    dout[~there] = float("nan")  # rows without a token add nothing, whatever they hold
+    clean = torch.where(there[:, None], dout, 0.0).double()
+    want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, safe, clean) * scale
+    mag = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, safe, clean.abs()) * scale
+    count = torch.zeros(V, device="cuda", dtype=torch.float64).index_add_(0, safe, there.double())
+    tol = (LAM * count.sqrt()[:, None] + 2) * U * mag
+    dt = torch.full((V, D), float("nan"), device="cuda")
+    K.embedding_bwd(dout, index, dt, scale=scale)
+    within(dt, want, tol, "dtable")
+    again = torch.full((V, D), float("nan"), device="cuda")
+    K.embedding_bwd(dout, index, again, scale=scale)
+    assert torch.equal(dt, again)
+    base = randn(g, V, D)
+    acc = base.clone()
+    K.embedding_bwd(dout, index, acc, scale=scale, accumulate=True)
+    within(acc, base.double() + want, tol + 2 * U * (base.double() + want).abs(), "accumulated")
+    untouched = count == 0
+    assert torch.equal(acc[untouched], base[untouched])
+
+
+@gpu
+def test_embedding_unaligned_and_empty(K):
+    g = rng(201)
+    V, D, rows = 50, 64, 200
+    flat = randn(g, V * D + 1)[1:]
+    table, index = flat.view(V, D), tokens("uniform", V, rows, 2)
+    out = torch.empty(rows * D + 1, device="cuda")[1:].view(rows, D)
+    K.embedding_fwd(table, index, out, scale=0.5)
+    assert torch.equal(out, table[index.long()] * 0.5)
+    dt = torch.empty(V * D + 1, device="cuda")[1:].view(V, D)
+    K.embedding_bwd(out, index, dt, scale=1.0)
+    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, index.long(), out.double())
+    within(dt, want, 64 * U * (1 + want.abs()), "dtable")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    dt.fill_(7.0)
+    K.embedding_bwd(torch.empty(0, D, device="cuda"), none, dt)
+    assert (dt == 0).all()
+    K.embedding_fwd(table, none, torch.empty(0, D, device="cuda"))
+
+
+@gpu
+def test_embedding_gradient_captured_and_replayed(K):
+    g = rng(202)
+    V, D, rows = 3000, 96, 6000
+    index, dout = tokens("rank", V, rows, 3), randn(g, rows, D)
+    dt, eager = torch.empty(V, D, device="cuda"), torch.empty(V, D, device="cuda")
+    ws = K.embedding_bwd(dout, index, dt)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.embedding_bwd(dout, index, dt, workspace=ws)
+    for i in range(4):
+        index.copy_(tokens(["rank", "padded", "same", "uniform"][i], V, rows, 10 + i))
+        dout.copy_(randn(g, rows, D))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        K.embedding_bwd(dout, index, eager)
+        assert torch.equal(dt, eager), i
+
+
+# ------------------------------------------------------------------------- orthogonalised updates
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(x, steps, coef, eps, dtype):
+    a, b, c = (dtype(v) for v in coef)
+    x = x.astype(np.float64)
+    y = (x / (np.sqrt((x * x).sum()) + eps)).astype(dtype)
+    tall = y.shape[0] > y.shape[1]
+    y = y.T if tall else y
+    for _ in range(steps):
+        g = y @ y.T
+        y = a * y + (b * g + c * (g @ g)) @ y
+    return y.T if tall else y
+
+
+def ns_tolerance(x, want, steps, coef, eps):
+    """Frobenius bound.  The same steps in fp32 are off by some E.  Here the operands of the products carry
+    22 instead of 24 bits: 4 u each, independent, so a sum of n terms gains 4 u / sqrt(n) of its norm
+    product where the fp32 sum itself loses about u: the same order for n >= 16, and 4 E covers it.
+    Short sums (n < 16): five steps of at most 12 u each, passed on with a factor of at most 4 in all."""
+    plain = newton_schulz(x, steps, coef, eps, np.float32)
+    return 4 * np.linalg.norm(plain - want) + 256 * U * np.linalg.norm(want)
+
+
+ORTHO = {
+    # rows, cols, batch, steps, pitch padding
+    "one": (1, 1, 1, 5, 0),
+    "row": (1, 70, 2, 5, 0),
+    "column": (300, 1, 1, 5, 3),
+    "square_96": (96, 96, 1, 5, 0),
+    "square_64_batch": (64, 64, 5, 5, 0),
+    "wide": (65, 200, 2, 5, 0),
+    "tall": (257, 100, 2, 5, 1),
+    "odd": (131, 129, 1, 3, 7),
+    "no_steps": (40, 50, 2, 0, 2),
+    "one_step": (50, 40, 1, 1, 0),
+    "longer": (192, 576, 3, 5, 0),
+    "ten_steps": (128, 128, 1, 10, 0),
+}
+
+
+@gpu
+@pytest.mark.parametrize("name", list(ORTHO))
+def test_newton_schulz(K, name):
+    r, c, batch, steps, pad = ORTHO[name]
+    g = rng(300 + list(ORTHO).index(name))
+    full = randn(g, batch, r, c + pad) * 1e-3
+    x = full[:, :, :c]
+    out = torch.full((batch, r, c + pad), 7.0, device="cuda")
+    K.newton_schulz(K.newton_schulz_args(x, out[:, :, :c], steps=steps, coefficients=COEF, eps=1e-7))
+    assert (out[:, :, c:] == 7.0).all()
+    for i in range(batch):
+        h = x[i].cpu().numpy()
+        want = newton_schulz(h, steps, COEF, 1e-7, np.float64)
+        err = np.linalg.norm(out[i, :, :c].double().cpu().numpy() - want)
+        assert err <= ns_tolerance(h, want, steps, COEF, 1e-7), (i, err, np.linalg.norm(want))
+    # in place, the same bits
+    inplace = full.clone()
+    K.newton_schulz(K.newton_schulz_args(inplace[:, :, :c], inplace[:, :, :c], steps=steps, coefficients=COEF, eps=1e-7))
+    assert torch.equal(inplace[:, :, :c], out[:, :, :c])
+
+
+@gpu
+def test_newton_schulz_orthogonalises(K):
+    """With the convergent triple (15, -10, 3) / 8 the singular values go to 1."""
+    x = randn(rng(320), 80, 120)
+    out = torch.empty_like(x)
+    K.newton_schulz(K.newton_schulz_args(x, out, steps=20, coefficients=(15 / 8, -10 / 8, 3 / 8), eps=0.0))
+    s = torch.linalg.svdvals(out.double().cpu())
+    assert (s - 1).abs().max() < 1e-4, (s.min(), s.max())
+
+
+@gpu
+def test_newton_schulz_scales(K):
+    """Tiny, huge, zero and spiked matrices: the norm is formed in double precision."""
+    g = rng(321)
+    x = randn(g, 5, 70, 90)
+    x[1] *= 1e-30
+    x[2] *= 1e30
+    x[3] = 0
+    x[4] *= 1e-6
+    x[4, 3, 5] = 1.0
+    out = torch.empty_like(x)
+    K.newton_schulz(K.newton_schulz_args(x, out, eps=0.0 + 1e-38))
+    assert (out[3] == 0).all()
+    for i in (0, 1, 2, 4):
+        h = x[i].cpu().numpy()
+        want = newton_schulz(h, 5, COEF, 1e-38, np.float64)
+        # one strong direction beside a floor 1e-6 below: fp16 parts keep 2^-36 of the largest entry absolutely
+        floor = 2.0 ** -36 * 3.4445 ** 5 * np.sqrt(h.size) if i == 4 else 0.0
+        err = np.linalg.norm(out[i].double().cpu().numpy() - want)
+        assert err <= ns_tolerance(h, want, 5, COEF, 1e-38) + floor, (i, err)
+
+
+@gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("shape", [(96, 288, 3), (288, 96, 2), (10, 192, 1)])
+def test_muon_steps(K, nesterov, shape):
+    r, c, batch = shape
+    g = rng(330)
+    p, m = randn(g, batch, r, c) * 0.02, torch.zeros(batch, r, c, device="cuda")
+    p64, m64 = p.double().cpu().numpy(), m.double().cpu().numpy()
+    lr, mu, wd, us, gs = 0.02, 0.95, 0.1, 1.5, 0.25
+    for step in range(3):
+        grad = randn(g, batch, r, c) * 1e-2
+        K.muon(K.muon_args(p, grad, m, lr=lr, momentum=mu, weight_decay=wd, update_scale=us, grad_scale=gs,
+                           nesterov=nesterov))
+        gd = grad.double().cpu().numpy() * gs
+        m64 = mu * m64 + gd
+        tol_m = (step + 1) * 4 * U * (np.abs(m64) + np.abs(gd) + 1e-2)
+        assert (np.abs(m.double().cpu().numpy() - m64) <= tol_m).all()
+        u = gd + mu * m64 if nesterov else m64
+        for i in range(batch):
+            o = newton_schulz(u[i].astype(np.float32), 5, COEF, 1e-7, np.float64)
+            p64[i] = p64[i] * (1 - lr * wd) - lr * us * o
+            # the direction: bound of the products plus what 12 u in u becomes (a factor of at most 3.4445^5)
+            e = ns_tolerance(u[i].astype(np.float32), o, 5, COEF, 1e-7) + 12 * U * 485
+            err = np.linalg.norm(p[i].double().cpu().numpy() - p64[i])
+            assert err <= (step + 1) * (lr * us * e + 4 * U * np.linalg.norm(p64[i])), (step, i, err)
+
+
+@gpu
+def test_muon_captured_and_replayed(K):
+    g = rng(340)
+    shape = (2, 64, 160)
+    p, m = randn(g, *shape), torch.zeros(*shape, device="cuda")
+    grad = torch.empty(*shape, device="cuda")
+    pe, me = p.clone(), m.clone()
+    a, e = K.muon_args(p, grad, m, lr=0.1), K.muon_args(pe, grad, me, lr=0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.muon(a)
+    for i in range(4):
+        grad.copy_(randn(g, *shape))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        K.muon(e)
+        assert torch.equal(p, pe) and torch.equal(m, me), i
+
+
+# ------------------------------------------------------------------------------------- refusals
+def _xargs(vitk, **kw):
+    a = vitk.CrossSdpaArgs()
+    d = dict(B=2, H=4, Hkv=2, Nq=3, Nk=5, dh=8, scale=1.0, q=4096, ld_q=32, k=4096, ld_k=16, v=4096, ld_v=16, out=4096,
+             ld_out=32, stats=4096, dout=4096, ld_dout=32, dq=4096, ld_dq=32, dk=4096, ld_dk=16, dv=4096, ld_dv=16,
+             workspace=4096, workspace_bytes=1 << 20)
+    d.update(kw)
+    for n, x in d.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(B=-1), "negative size"), (dict(Hkv=3), "query heads over"), (dict(Hkv=0), "query heads over"),
+    (dict(H=0), "query heads over"), (dict(dh=0), "outside"), (dict(dh=129), "outside"),
+    (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(q=0), "null pointer"),
+    (dict(k=0), "null pointer"), (dict(out=0), "null pointer"), (dict(ld_q=31), "pitch"), (dict(ld_k=15), "pitch"),
+    (dict(ld_out=1), "pitch"), (dict(reserved=1), "reserved"), (dict(Nq=2 ** 30, H=8), "too many rows")])
+def test_cross_attention_refuses(change, message):
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    for fn in (d.vitk_cross_sdpa_fwd, d.vitk_cross_sdpa_bwd):
+        assert fn(C.byref(_xargs(vitk, **change)), None) != 0
+        assert message in d.vitk_last_error().decode()
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(dout=0), "null pointer"), (dict(dq=0), "null pointer"), (dict(dk=0), "null pointer"), (dict(dv=0), "null pointer"),
+    (dict(stats=0), "null pointer"), (dict(ld_dq=31), "pitch"), (dict(ld_dv=15), "pitch"),
+    (dict(workspace=0), "workspace"), (dict(workspace_bytes=4), "workspace"), (dict(workspace=4100), "aligned")])
+def test_cross_attention_backward_refuses(change, message):
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    assert d.vitk_cross_sdpa_bwd(C.byref(_xargs(vitk, **change)), None) != 0
+    assert message in d.vitk_last_error().decode()
+
+
+def test_cross_attention_refuses_null_arguments_and_a_missing_workspace():
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    assert d.vitk_cross_sdpa_fwd(None, None) != 0
+    assert d.vitk_cross_sdpa_bwd(None, None) != 0
+    a = _xargs(vitk, B=1, H=1, Hkv=1, Nq=1, Nk=100000, dh=64, ld_q=64, ld_k=64, ld_v=64, ld_out=64, workspace=0)
+    assert d.vitk_cross_sdpa_fwd_workspace_bytes(C.byref(a)) > 0  # split over keys
+    assert d.vitk_cross_sdpa_fwd(C.byref(a), None) != 0
+    assert "workspace" in d.vitk_last_error().decode()
+
+
+@pytest.mark.parametrize("name, args, message", [
+    ("vitk_embedding_fwd", (4096, 10, 4096, -1, 8, 1.0, 4096, None), "bad shape"),
+    ("vitk_embedding_fwd", (None, 10, 4096, 3, 8, 1.0, 4096, None), "null pointer"),
+    ("vitk_embedding_fwd", (4096, 10, None, 3, 8, 1.0, 4096, None), "null pointer"),
+    ("vitk_embedding_fwd", (4096, 2 ** 31, 4096, 3, 8, 1.0, 4096, None), "table of"),
+    ("vitk_embedding_bwd", (4096, 4096, 3, -10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "bad shape"),
+    ("vitk_embedding_bwd", (None, 4096, 3, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "null pointer"),
+    ("vitk_embedding_bwd", (4096, 4096, 3, 10, 8, 1.0, 0, None, 4096, 1 << 20, None), "null pointer"),
+    ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "tokens over"),
+])
+def test_embedding_refuses(name, args, message):
+    from visiontransformer_amd import vitk
+    with pytest.raises(vitk.VitkError, match=message):
+        vitk.call(name, *args)
+
+
+def _nargs(vitk, cls, **kw):
+    a = cls()
+    d = dict(rows=8, cols=8, batch=2, steps=5, a=COEF[0], b=COEF[1], c=COEF[2], eps=1e-7, workspace=4096, workspace_bytes=1 << 30)
+    if cls is vitk.MuonArgs:
+        d.update(p=4096, g=8192, m=16384, ld=8, stride=64)
+    else:
+        d.update(x=4096, out=4096, ld_x=8, ld_out=8, stride_x=64, stride_out=64)
+    d.update(kw)
+    for n, x in d.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(rows=-1), "bad shape"), (dict(cols=2 ** 21), "bad shape"), (dict(steps=-1), "steps"), (dict(steps=33), "steps"),
+    (dict(a=9.0), "bounded"), (dict(c=float("nan")), "bounded"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(workspace=0), "workspace"), (dict(workspace_bytes=64), "workspace"), (dict(workspace=4104), "aligned")])
+def test_newton_schulz_and_muon_refuse(change, message):
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    for fn, cls in ((d.vitk_newton_schulz_f32, vitk.NewtonSchulzArgs), (d.vitk_muon_f32, vitk.MuonArgs)):
+        assert fn(C.byref(_nargs(vitk, cls, **change)), None) != 0
+        assert message in d.vitk_last_error().decode()
+
+
+@pytest.mark.parametrize("cls, change, message", [
+    ("NewtonSchulzArgs", dict(x=0), "null pointer"), ("NewtonSchulzArgs", dict(out=0), "null pointer"),
+    ("NewtonSchulzArgs", dict(ld_x=7), "pitch"), ("NewtonSchulzArgs", dict(stride_out=63), "overlap"),
+    ("MuonArgs", dict(p=0), "null pointer"), ("MuonArgs", dict(m=8192), "different buffers"),
+    ("MuonArgs", dict(ld=7), "pitch"), ("MuonArgs", dict(stride=63), "overlap")])
+def test_newton_schulz_and_muon_refuse_their_own(cls, change, message):
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    fn = d.vitk_muon_f32 if cls == "MuonArgs" else d.vitk_newton_schulz_f32
+    assert fn(C.byref(_nargs(vitk, getattr(vitk, cls), **change)), None) != 0
+    assert message in d.vitk_last_error().decode()
+
+
+def test_bindings_refuse_wrong_tensors():
+    from visiontransformer_amd import vitk
+    cpu = torch.zeros(2, 3, 4, 8)
+    with pytest.raises(vitk.VitkError, match="CUDA"):
+        vitk.cross_sdpa_args(cpu, cpu, cpu, cpu)
+    with pytest.raises(vitk.VitkError, match="CUDA"):
+        vitk.embedding_fwd(torch.zeros(4, 4), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4))
+    with pytest.raises(vitk.VitkError, match="CUDA"):
+        vitk.newton_schulz_args(torch.zeros(4, 4), torch.zeros(4, 4))
+    with pytest.raises(vitk.VitkError, match="CUDA"):
+        vitk.muon_args(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), lr=0.1)

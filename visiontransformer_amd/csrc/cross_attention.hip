@@ -1,0 +1,277 @@
+// Cross attention forward: softmax(scale * q k^T) v with queries and keys of different sequences.
+//
+// One workgroup = 128 query rows of one (batch, key head); the query heads that share the key head are
+// rows of the same block, so shared keys are read once per block.  A wave holds 32 rows as the columns of
+// S^T[key][row] = K Q^T on v_mfma_f32_32x32x2_f32; register i of lane (c = lane & 31, g = lane >> 5) is key
+// 8 (i / 4) + 4 g + i % 4 of row c, which is the operand the second product O^T[d][row] += V^T P^T
+// wants for contraction index g, so probabilities never leave their registers.  One pass over the
+// keys with a running maximum and sum per row.
+#include "cross_attention.h"
+
+#include <cmath>
+
+namespace vitk {
+namespace cross {
+
+int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Params *p) {
+  VITK_REQUIRE(a != nullptr, "%s: null arguments", who);
+  VITK_REQUIRE(a->reserved == 0, "%s: reserved must be 0", who);
+  VITK_REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0, "%s: negative size", who);
+  VITK_REQUIRE(a->H > 0 && a->Hkv > 0 && a->H % a->Hkv == 0, "%s: %d query heads over %d key heads", who, a->H, a->Hkv);
+  VITK_REQUIRE(a->dh >= 1 && a->dh <= 128, "%s: head dimension %d outside [1, 128]", who, a->dh);
+  VITK_REQUIRE(std::isfinite(a->scale), "%s: scale is not a finite number", who);
+  const long long wq = (long long)a->H * a->dh, wk = (long long)a->Hkv * a->dh;
+  const bool any_q = a->B > 0 && a->Nq > 0, any_k = a->B > 0 && a->Nk > 0;
+  VITK_REQUIRE((long long)(a->H / a->Hkv) * a->Nq < 2147482624 && a->Nk < 2147482624,
+               "%s: too many rows", who);
+  if (any_q) {
+    VITK_REQUIRE(a->q && a->out, "%s: null pointer", who);
+    VITK_REQUIRE(a->ld_q >= wq && a->ld_out >= wq, "%s: row pitch below H*dh", who);
+  }
+  if (any_k) {
+    VITK_REQUIRE(a->k && a->v, "%s: null pointer", who);
+    VITK_REQUIRE(a->ld_k >= wk && a->ld_v >= wk, "%s: row pitch below Hkv*dh", who);
+  }
+  p->q = {a->q, a->ld_q};
+  p->k = {a->k, a->ld_k};
+  p->v = {a->v, a->ld_v};
+  p->out = {a->out, a->ld_out};
+  p->o = {a->out, a->ld_out};
+  p->len = a->key_len;
+  p->stats = a->stats;
+  p->B = a->B, p->H = a->H, p->Hkv = a->Hkv, p->G = a->H / a->Hkv, p->Nq = a->Nq, p->Nk = a->Nk, p->dh = a->dh;
+  p->rows = p->G * p->Nq;
+  p->scale = a->scale, p->c = a->scale * kLog2e;
+  bool vec = a->dh % 4 == 0;
+  auto quad = [&](const void *ptr, int64_t ld) { vec = vec && aligned16(ptr) && ld % 4 == 0; };
+  quad(a->q, a->ld_q), quad(a->k, a->ld_k), quad(a->v, a->ld_v), quad(a->out, a->ld_out);
+  if (backward) {
+    if (any_q) {
+      VITK_REQUIRE(a->dout && a->dq && a->stats, "%s: null pointer", who);
+      VITK_REQUIRE(a->ld_dout >= wq && a->ld_dq >= wq, "%s: row pitch below H*dh", who);
+    }
+    if (any_k) {
+      VITK_REQUIRE(a->dk && a->dv, "%s: null pointer", who);
+      VITK_REQUIRE(a->ld_dk >= wk && a->ld_dv >= wk, "%s: row pitch below Hkv*dh", who);
+    }
+    p->dout = {a->dout, a->ld_dout};
+    p->dq = {a->dq, a->ld_dq};
+    p->dk = {a->dk, a->ld_dk};
+    p->dv = {a->dv, a->ld_dv};
+    quad(a->dout, a->ld_dout), quad(a->dq, a->ld_dq), quad(a->dk, a->ld_dk), quad(a->dv, a->ld_dv);
+  }
+  p->vec = vec;
+  return 0;
+}
+
+}  // namespace cross
+}  // namespace vitk
+
+namespace {
+
+using namespace vitk::cross;
+
+constexpr int KT = 32;   // keys per tile
+constexpr int RB = 128;  // rows per workgroup
+
+template <int DH>
+__global__ __launch_bounds__(256) void cross_fwd_kernel(const Params p) {
+  constexpr int LP = DH + 4, NB = DH / 32;
+  __shared__ __attribute__((aligned(16))) float kt[KT * LP], vt[KT * LP];
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
+  long long wg = blockIdx.x;
+  const int rb = (int)(wg % p.blocks);
+  wg /= p.blocks;
+  const int hk = (int)(wg % p.Hkv);
+  wg /= p.Hkv;
+  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int len = valid_keys(p, b);
+  const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
+  const int row = rb * RB + wave * 32 + c;
+  const bool row_ok = row < p.rows;
+
+  float qf[DH / 2];  // columns g*DH/2 .. of this lane's row
+#pragma unroll
+  for (int i = 0; i < DH / 2; i += 4) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (row_ok) x = load_quad(p.q.ptr + row_offset(p, p.q.ld, b, hk, row), g * (DH / 2) + i, p.dh, p.vec);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qf[i + e] = x[e];
+  }
+  f32x16 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  for (int t = k0; t < k1; t += KT) {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < DH / 32; ++u) {
+      const int quad = threadIdx.x + 256 * u, key = quad / (DH / 4), d = 4 * (quad % (DH / 4));
+      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+      if (t + key < k1) {
+        x = load_quad(p.k.ptr + key_offset(p, p.k.ld, b, hk, t + key), d, p.dh, p.vec);
+        y = load_quad(p.v.ptr + key_offset(p, p.v.ld, b, hk, t + key), d, p.dh, p.vec);
+      }
+      *reinterpret_cast<f32x4 *>(kt + key * LP + d) = x;
+      *reinterpret_cast<f32x4 *>(vt + key * LP + d) = y;
+    }
+    __syncthreads();
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DH / 2; i += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(kt + c * LP + g * (DH / 2) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[i + e], s, 0, 0, 0);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = t + 8 * (i / 4) + 4 * g + i % 4;
+      s[i] = key < k1 ? s[i] * p.c : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m_new = fmaxf(m, top);
+    const float fall = __builtin_amdgcn_exp2f(m - m_new);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] - m_new);
+      sum += s[i];
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    l = l * fall + sum;
+    m = m_new;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][i] *= fall;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vt[(8 * (i / 4) + 4 * g + i % 4) * LP + 32 * n + c], s[i], o[n], 0, 0, 0);
+    }
+  }
+  if (!row_ok) return;
+  const long long stat = row_stat(p, b, hk, row);
+  float *dst, *st;
+  float f = 1.f;
+  if (p.splits > 1) {
+    const long long all = (long long)p.B * p.H * p.Nq;
+    dst = p.part + (split * all + stat) * p.dh;
+    st = p.part + p.splits * all * p.dh + (split * all + stat) * 2;
+  } else {
+    dst = p.out.ptr + row_offset(p, p.out.ld, b, hk, row);
+    st = p.stats ? p.stats + stat * 2 : nullptr;
+    f = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (l == 0.f) m = 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = o[n][4 * j + e] * f;
+      store_quad(dst, 32 * n + 8 * j + 4 * g, p.dh, p.vec, x);
+    }
+  if (st && g == 0) {
+    st[0] = m;
+    st[1] = l;
+  }
+}
+
+// Joins the parts of a split row: one wave per row, lanes over the columns.
+__global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
+  const long long all = (long long)p.B * p.H * p.Nq;
+  const int lane = threadIdx.x & 63;
+  const long long r = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (r >= all) return;
+  const float *st = p.part + p.splits * all * p.dh;
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, st[(s * all + r) * 2]);
+  if (m == -INFINITY) m = 0.f;  // no key at all
+  float l = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(st[(s * all + r) * 2] - m);
+    l += f * st[(s * all + r) * 2 + 1];
+    const float *src = p.part + (s * all + r) * p.dh;
+    if (lane < p.dh) x0 += f * src[lane];
+    if (lane + 64 < p.dh) x1 += f * src[lane + 64];
+  }
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  const long long bh = r / p.Nq, n = r % p.Nq, b = bh / p.H, h = bh % p.H;
+  float *dst = p.out.ptr + (b * p.Nq + n) * p.out.ld + h * p.dh;
+  if (lane < p.dh) dst[lane] = x0 * f;
+  if (lane + 64 < p.dh) dst[lane + 64] = x1 * f;
+  if (lane == 0 && p.stats) {
+    p.stats[2 * r] = m;
+    p.stats[2 * r + 1] = l;
+  }
+}
+
+// Row blocks, and over how many workgroups the keys of one block are split.
+void plan_fwd(Params *p) {
+  p->blocks = (p->rows + RB - 1) / RB;
+  const long long groups = (long long)p->B * p->Hkv * p->blocks;
+  long long splits = 1;
+  if (groups > 0) splits = 2ll * vitk::cu_count() / groups;
+  const long long tiles = (p->Nk + KT - 1) / KT;
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  p->chunk = (int)((tiles + splits - 1) / splits) * KT;
+  if (p->chunk == 0) p->chunk = KT;
+  p->splits = (p->Nk + p->chunk - 1) / p->chunk;
+  if (p->splits < 1) p->splits = 1;
+}
+
+size_t fwd_bytes(const Params &p) {
+  if (p.splits <= 1) return 0;
+  return (size_t)p.splits * p.B * p.H * p.Nq * (p.dh + 2) * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" size_t vitk_cross_sdpa_fwd_workspace_bytes(const vitk_cross_sdpa_args *a) {
+  if (!a || a->B <= 0 || a->Nq <= 0 || a->Nk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->dh < 1) return 0;
+  Params p = {};
+  p.B = a->B, p.H = a->H, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Nq = a->Nq, p.Nk = a->Nk, p.dh = a->dh;
+  p.rows = p.G * p.Nq;
+  plan_fwd(&p);
+  return fwd_bytes(p);
+}
+
+extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t stream) {
+  Params p = {};
+  if (check_args("vitk_cross_sdpa_fwd", a, false, &p)) return 1;
+  if (p.B == 0 || p.Nq == 0) return 0;
+  plan_fwd(&p);
+  const size_t need = fwd_bytes(p);
+  VITK_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
+               "vitk_cross_sdpa_fwd: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
+  VITK_REQUIRE(need == 0 || vitk::aligned16(a->workspace), "vitk_cross_sdpa_fwd: workspace is not 16-byte aligned");
+  p.part = a->workspace;
+  const long long wgs = (long long)p.B * p.Hkv * p.blocks * p.splits;
+  VITK_REQUIRE(wgs < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
+  hipStream_t st = vitk::as_stream(stream);
+  const dim3 grid((unsigned)wgs), block(256);
+  if (p.dh <= 32)
+    hipLaunchKernelGGL(cross_fwd_kernel<32>, grid, block, 0, st, p);
+  else if (p.dh <= 64)
+    hipLaunchKernelGGL(cross_fwd_kernel<64>, grid, block, 0, st, p);
+  else if (p.dh <= 96)
+    hipLaunchKernelGGL(cross_fwd_kernel<96>, grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL(cross_fwd_kernel<128>, grid, block, 0, st, p);
+  if (p.splits > 1) {
+    const long long all = (long long)p.B * p.H * p.Nq;
+    VITK_REQUIRE((all + 3) / 4 < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
+    hipLaunchKernelGGL(cross_join_kernel, dim3((unsigned)((all + 3) / 4)), block, 0, st, p);
+  }
+  return vitk::check_launch("vitk_cross_sdpa_fwd");
+}

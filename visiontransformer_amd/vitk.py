@@ -34,6 +34,40 @@ class GemmArgs(C.Structure):
     ]
 
 
+class CrossSdpaArgs(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("Nq", C.c_int32), ("Nk", C.c_int32), ("dh", C.c_int32),
+        ("scale", C.c_float), ("reserved", C.c_int32),
+        ("q", C.c_void_p), ("ld_q", C.c_int64), ("k", C.c_void_p), ("ld_k", C.c_int64),
+        ("v", C.c_void_p), ("ld_v", C.c_int64), ("key_len", C.c_void_p),
+        ("out", C.c_void_p), ("ld_out", C.c_int64), ("stats", C.c_void_p),
+        ("dout", C.c_void_p), ("ld_dout", C.c_int64), ("dq", C.c_void_p), ("ld_dq", C.c_int64),
+        ("dk", C.c_void_p), ("ld_dk", C.c_int64), ("dv", C.c_void_p), ("ld_dv", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class NewtonSchulzArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int32), ("cols", C.c_int32), ("batch", C.c_int32), ("steps", C.c_int32),
+        ("x", C.c_void_p), ("ld_x", C.c_int64), ("stride_x", C.c_int64),
+        ("out", C.c_void_p), ("ld_out", C.c_int64), ("stride_out", C.c_int64),
+        ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class MuonArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int32), ("cols", C.c_int32), ("batch", C.c_int32), ("steps", C.c_int32),
+        ("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("ld", C.c_int64), ("stride", C.c_int64),
+        ("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("update_scale", C.c_float),
+        ("grad_scale", C.c_float), ("nesterov", C.c_int32),
+        ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _p, _i32, _i64, _u64, _f, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); every function of include/vitk.h
@@ -89,6 +123,17 @@ SIGNATURES = {
     "vitk_sdpa_row_fwd": (C.c_int, [_p, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _f, _p, _i64, _p, _p]),
     "vitk_sdpa_row_bwd": (C.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _f, _i32, _p, _i64,
                                     _p, _p, _i64, _p]),
+    "vitk_cross_sdpa_fwd_workspace_bytes": (_sz, [C.POINTER(CrossSdpaArgs)]),
+    "vitk_cross_sdpa_fwd": (C.c_int, [C.POINTER(CrossSdpaArgs), _p]),
+    "vitk_cross_sdpa_bwd_workspace_bytes": (_sz, [C.POINTER(CrossSdpaArgs)]),
+    "vitk_cross_sdpa_bwd": (C.c_int, [C.POINTER(CrossSdpaArgs), _p]),
+    "vitk_embedding_fwd": (C.c_int, [_p, _i64, _p, _i64, _i64, _f, _p, _p]),
+    "vitk_embedding_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "vitk_embedding_bwd": (C.c_int, [_p, _p, _i64, _i64, _i64, _f, _i32, _p, _p, _sz, _p]),
+    "vitk_newton_schulz_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "vitk_newton_schulz_f32": (C.c_int, [C.POINTER(NewtonSchulzArgs), _p]),
+    "vitk_muon_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "vitk_muon_f32": (C.c_int, [C.POINTER(MuonArgs), _p]),
     "vitk_add2d_f32": (C.c_int, [_p, _i64, _p, _i64, _i64, _i64, _p]),
     "vitk_patch_gather": (C.c_int, [_p, _i32, _i32, _i32, _i32, _i32, _p, _p]),
     "vitk_patch_scatter_bwd": (C.c_int, [_p, _i32, _i32, _i32, _i32, _i32, _p, _p]),
@@ -201,6 +246,168 @@ def gemm_pair(dx, dw, st=None):
     keep = (_give_workspace(ax, None), _give_workspace(aw, None))
     check(dll().vitk_gemm_pair_f32(C.byref(ax), C.byref(aw), st if st is not None else stream()))
     return keep
+
+
+def _need(cond, message):
+    if not cond:
+        raise VitkError(message)
+
+
+def _f32(name, t, shape=None):
+    _need(str(t.dtype) == "torch.float32" and t.is_cuda, f"{name}: a float32 CUDA tensor is needed")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {shape}")
+
+
+def _head_rows(name, t, shape):
+    """Pitch of a [B, N, heads, dh] tensor whose rows (b, n) lie one after the other, heads packed."""
+    _f32(name, t, shape)
+    B, N, heads, dh = shape
+    if t.numel() == 0:
+        return heads * dh
+    _need((dh == 1 or t.stride(3) == 1) and (heads == 1 or t.stride(2) == dh),
+          f"{name}: the heads of a row have to be packed")
+    if N > 1:
+        ld = t.stride(1)
+        _need(B == 1 or t.stride(0) == N * ld, f"{name}: batch entries have to follow each other at the row pitch")
+    else:
+        ld = t.stride(0) if B > 1 else heads * dh
+    _need(ld >= heads * dh, f"{name}: rows overlap")
+    return ld
+
+
+def cross_sdpa_args(q, k, v, out, *, key_len=None, scale=None, stats=None, dout=None, dq=None, dk=None, dv=None,
+                    workspace=None):
+    """Arguments of cross_sdpa_fwd / cross_sdpa_bwd for q, out [B, Nq, H, dh] and k, v [B, Nk, Hkv, dh] (rows may be
+    pitched, e.g. slices of a packed projection); the object keeps its tensors and, unless one is passed, a
+    workspace.  Build it once and call as often as the same buffers are used."""
+    _need(q.dim() == 4 and k.dim() == 4, "cross_sdpa: q and k have four dimensions [B, N, heads, dh]")
+    B, Nq, H, dh = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    a = CrossSdpaArgs()
+    a.B, a.H, a.Hkv, a.Nq, a.Nk, a.dh = B, H, Hkv, Nq, Nk, dh
+    a.scale = dh ** -0.5 if scale is None else scale
+    rows, keys = (B, Nq, H, dh), (B, Nk, Hkv, dh)
+    for name, t, shape in (("q", q, rows), ("k", k, keys), ("v", v, keys), ("out", out, rows), ("dout", dout, rows),
+                           ("dq", dq, rows), ("dk", dk, keys), ("dv", dv, keys)):
+        if t is not None:
+            setattr(a, name, ptr(t))
+            setattr(a, "ld_" + name, _head_rows(name, t, shape))
+    if key_len is not None:
+        _need(str(key_len.dtype) == "torch.int32" and key_len.is_cuda and key_len.is_contiguous()
+              and tuple(key_len.shape) == (B,), "key_len: B contiguous int32 values on the GPU are needed")
+        a.key_len = ptr(key_len)
+    if stats is not None:
+        _f32("stats", stats)
+        _need(stats.is_contiguous() and stats.numel() == B * H * Nq * 2, "stats: [B*H, Nq, 2] contiguous is needed")
+        a.stats = ptr(stats)
+    need = dll().vitk_cross_sdpa_fwd_workspace_bytes(C.byref(a))
+    if dq is not None:
+        need = max(need, dll().vitk_cross_sdpa_bwd_workspace_bytes(C.byref(a)))
+    if need and workspace is None:
+        import torch
+        workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=q.device)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
+    a.keep = (q, k, v, out, key_len, stats, dout, dq, dk, dv, workspace)
+    return a
+
+
+def cross_sdpa_fwd(args, st=None):
+    """Softmax attention of args.q over args.k / args.v; see include/vitk.h."""
+    check(dll().vitk_cross_sdpa_fwd(C.byref(args), st if st is not None else stream()))
+
+
+def cross_sdpa_bwd(args, st=None):
+    check(dll().vitk_cross_sdpa_bwd(C.byref(args), st if st is not None else stream()))
+
+
+def _rows_2d(name, t, dtype="torch.float32"):
+    _need(str(t.dtype) == dtype and t.is_cuda and t.is_contiguous(), f"{name}: a contiguous {dtype} CUDA tensor is needed")
+
+
+def embedding_fwd(table, index, out, *, scale=1.0, st=None):
+    """out[i] = scale * table[index[i]]; an index outside the table gives zeros."""
+    _rows_2d("table", table), _rows_2d("out", out), _rows_2d("index", index, "torch.int32")
+    V, D = table.shape
+    rows = index.numel()
+    _need(out.numel() == rows * D, f"out: {rows} rows of {D} are needed")
+    check(dll().vitk_embedding_fwd(ptr(table), V, ptr(index), rows, D, scale, ptr(out),
+                                   st if st is not None else stream()))
+
+
+def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace=None, st=None):
+    """dtable[t] (+)= scale * sum of dout[i] over index[i] == t.  Without a workspace one is allocated."""
+    _rows_2d("dout", dout), _rows_2d("dtable", dtable), _rows_2d("index", index, "torch.int32")
+    V, D = dtable.shape
+    rows = index.numel()
+    _need(dout.numel() == rows * D, f"dout: {rows} rows of {D} are needed")
+    if workspace is None:
+        import torch
+        need = dll().vitk_embedding_bwd_workspace_bytes(rows, V, D)
+        workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=dout.device)
+    check(dll().vitk_embedding_bwd(ptr(dout), ptr(index), rows, V, D, scale, int(bool(accumulate)), ptr(dtable),
+                                   ptr(workspace), workspace.numel() * workspace.element_size(),
+                                   st if st is not None else stream()))
+    return workspace
+
+
+def _matrices(name, t, rows=None):
+    """(batch, rows, cols, ld, stride) of a [batch, rows, cols] or [rows, cols] tensor with unit column stride."""
+    _f32(name, t)
+    _need(t.dim() in (2, 3), f"{name}: [rows, cols] or [batch, rows, cols] is needed")
+    if t.dim() == 2:
+        t = t.unsqueeze(0)
+    batch, r, c = t.shape
+    _need(c <= 1 or t.stride(2) == 1, f"{name}: unit column stride is needed")
+    ld = t.stride(1) if r > 1 else max(c, 1)
+    return batch, r, c, ld, t.stride(0) if batch > 1 else r * ld
+
+
+def newton_schulz_args(x, out, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, workspace=None):
+    """Arguments of newton_schulz for [batch, rows, cols] (or one matrix); see include/vitk.h."""
+    a = NewtonSchulzArgs()
+    a.batch, a.rows, a.cols, a.ld_x, a.stride_x = _matrices("x", x)
+    shape = _matrices("out", out)
+    _need(shape[:3] == (a.batch, a.rows, a.cols), "out: the shape of x is needed")
+    a.ld_out, a.stride_out = shape[3:]
+    a.x, a.out = ptr(x), ptr(out)
+    a.steps, a.eps = steps, eps
+    a.a, a.b, a.c = coefficients
+    need = dll().vitk_newton_schulz_workspace_bytes(a.rows, a.cols, a.batch)
+    return _with_workspace(a, need, workspace, x, (x, out))
+
+
+def muon_args(p, g, m, *, lr, momentum=0.95, weight_decay=0.0, update_scale=1.0, grad_scale=1.0, nesterov=True, steps=5,
+              coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, workspace=None):
+    """Arguments of muon for parameters, gradients and momentum of one layout; see include/vitk.h."""
+    a = MuonArgs()
+    a.batch, a.rows, a.cols, a.ld, a.stride = _matrices("p", p)
+    for name, t in (("g", g), ("m", m)):
+        _need(_matrices(name, t) == (a.batch, a.rows, a.cols, a.ld, a.stride), f"{name}: the layout of p is needed")
+    a.p, a.g, a.m = ptr(p), ptr(g), ptr(m)
+    a.lr, a.momentum, a.weight_decay, a.update_scale, a.grad_scale = lr, momentum, weight_decay, update_scale, grad_scale
+    a.nesterov, a.steps, a.eps = int(bool(nesterov)), steps, eps
+    a.a, a.b, a.c = coefficients
+    need = dll().vitk_muon_workspace_bytes(a.rows, a.cols, a.batch)
+    return _with_workspace(a, need, workspace, p, (p, g, m))
+
+
+def _with_workspace(a, need, workspace, like, keep):
+    if need and workspace is None:
+        import torch
+        workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=like.device)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
+    a.keep = keep + (workspace,)
+    return a
+
+
+def newton_schulz(args, st=None):
+    check(dll().vitk_newton_schulz_f32(C.byref(args), st if st is not None else stream()))
+
+
+def muon(args, st=None):
+    check(dll().vitk_muon_f32(C.byref(args), st if st is not None else stream()))
 
 
 def planning_cu_count(cus):
