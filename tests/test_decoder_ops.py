@@ -292,6 +292,11 @@ EMBED = {
     "all_padding": (64, 64, 77, "all_padding"),
     "outside": (100, 96, 400, "outside"),
     "many_tokens": (5000, 96, 70001, "rank"),
+    "few_tokens_one_takes_most": (40, 300, 1023, "same"),
+    "sorted_small_table": (7, 64, 1025, "uniform"),
+    "sorted_few_tokens": (4097, 260, 65, "padded"),
+    "one_chunk": (5000, 48, 32, "rank"),
+    "three_passes": (70001, 36, 3000, "rank"),
     "large_table_few_tokens": (100003, 32, 9, "uniform"),
 }
 
@@ -588,6 +593,9 @@ def test_cross_attention_refuses_null_arguments_and_a_missing_workspace():
     ("vitk_embedding_bwd", (4096, 4096, 3, -10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "bad shape"),
     ("vitk_embedding_bwd", (None, 4096, 3, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "null pointer"),
     ("vitk_embedding_bwd", (4096, 4096, 3, 10, 8, 1.0, 0, None, 4096, 1 << 20, None), "null pointer"),
+    ("vitk_embedding_bwd", (4096, 4096, 3, 5000, 8, 1.0, 0, 4096, None, 1 << 20, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 4096, 4096, 16, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 4096, 4100, 1 << 20, None), "aligned"),
     ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "tokens over"),
 ])
 def test_embedding_refuses(name, args, message):
