@@ -253,8 +253,18 @@ def _need(cond, message):
         raise VitkError(message)
 
 
+_DTYPES = {}
+
+
+def _is(t, dtype):
+    if not _DTYPES:
+        import torch
+        _DTYPES.update(float32=torch.float32, int32=torch.int32)
+    return t.dtype is _DTYPES[dtype] and t.is_cuda
+
+
 def _f32(name, t, shape=None):
-    _need(str(t.dtype) == "torch.float32" and t.is_cuda, f"{name}: a float32 CUDA tensor is needed")
+    _need(_is(t, "float32"), f"{name}: a float32 CUDA tensor is needed")
     _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {shape}")
 
 
@@ -293,7 +303,7 @@ def cross_sdpa_args(q, k, v, out, *, key_len=None, scale=None, stats=None, dout=
             setattr(a, name, ptr(t))
             setattr(a, "ld_" + name, _head_rows(name, t, shape))
     if key_len is not None:
-        _need(str(key_len.dtype) == "torch.int32" and key_len.is_cuda and key_len.is_contiguous()
+        _need(_is(key_len, "int32") and key_len.is_contiguous()
               and tuple(key_len.shape) == (B,), "key_len: B contiguous int32 values on the GPU are needed")
         a.key_len = ptr(key_len)
     if stats is not None:
@@ -321,13 +331,14 @@ def cross_sdpa_bwd(args, st=None):
     check(dll().vitk_cross_sdpa_bwd(C.byref(args), st if st is not None else stream()))
 
 
-def _rows_2d(name, t, dtype="torch.float32"):
-    _need(str(t.dtype) == dtype and t.is_cuda and t.is_contiguous(), f"{name}: a contiguous {dtype} CUDA tensor is needed")
+def _rows_2d(name, t, dtype="float32"):
+    if not (_is(t, dtype) and t.is_contiguous()):
+        raise VitkError(f"{name}: a contiguous {dtype} CUDA tensor is needed")
 
 
 def embedding_fwd(table, index, out, *, scale=1.0, st=None):
     """out[i] = scale * table[index[i]]; an index outside the table gives zeros."""
-    _rows_2d("table", table), _rows_2d("out", out), _rows_2d("index", index, "torch.int32")
+    _rows_2d("table", table), _rows_2d("out", out), _rows_2d("index", index, "int32")
     V, D = table.shape
     rows = index.numel()
     _need(out.numel() == rows * D, f"out: {rows} rows of {D} are needed")
@@ -337,7 +348,7 @@ def embedding_fwd(table, index, out, *, scale=1.0, st=None):
 
 def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace=None, st=None):
     """dtable[t] (+)= scale * sum of dout[i] over index[i] == t.  Without a workspace one is allocated."""
-    _rows_2d("dout", dout), _rows_2d("dtable", dtable), _rows_2d("index", index, "torch.int32")
+    _rows_2d("dout", dout), _rows_2d("dtable", dtable), _rows_2d("index", index, "int32")
     V, D = dtable.shape
     rows = index.numel()
     _need(dout.numel() == rows * D, f"dout: {rows} rows of {D} are needed")
