@@ -436,6 +436,14 @@ ORTHO = {
     "one_step": (50, 40, 1, 1, 0),
     "longer": (192, 576, 3, 5, 0),
     "ten_steps": (128, 128, 1, 10, 0),
+    "one_launch_ragged": (33, 128, 3, 5, 0),
+    "one_launch_tall": (127, 97, 2, 5, 3),
+    "small_tiles": (257, 1000, 1, 5, 0),
+    "small_tiles_thin": (3, 2500, 1, 5, 0),
+    "tiles_64": (130, 520, 8, 5, 4),
+    "tiles_64_tall": (700, 190, 9, 3, 1),
+    "tiles_128": (300, 900, 9, 5, 0),
+    "tiles_128_tall": (1001, 385, 7, 2, 0),
 }
 
 
@@ -609,11 +617,11 @@ def test_embedding_refuses(name, args, message):
 
 def _nargs(vitk, cls, **kw):
     a = cls()
-    d = dict(rows=8, cols=8, batch=2, steps=5, a=COEF[0], b=COEF[1], c=COEF[2], eps=1e-7, workspace=4096, workspace_bytes=1 << 30)
+    d = dict(rows=200, cols=200, batch=2, steps=5, a=COEF[0], b=COEF[1], c=COEF[2], eps=1e-7, workspace=4096, workspace_bytes=1 << 30)
     if cls is vitk.MuonArgs:
-        d.update(p=4096, g=8192, m=16384, ld=8, stride=64)
+        d.update(p=4096, g=8192, m=16384, ld=200, stride=40000)
     else:
-        d.update(x=4096, out=4096, ld_x=8, ld_out=8, stride_x=64, stride_out=64)
+        d.update(x=4096, out=4096, ld_x=200, ld_out=200, stride_x=40000, stride_out=40000)
     d.update(kw)
     for n, x in d.items():
         setattr(a, n, x)

@@ -2,7 +2,7 @@
 // and the Muon step that applies the result to a parameter.
 //
 // The matrices are held with their shorter side (r) as rows (a taller matrix is transposed on the way in and
-// out: the polynomial acts on singular values only) and padded with zeros to multiples of 64.
+// out: the polynomial acts on singular values only), padded with zeros to whole tiles.
 // Products run on v_mfma_f32_32x32x16_f16 with every fp32 operand x split in two fp16 parts,
 //   2^S x = hi + lo,  hi = fp16(2^S x), lo = fp16(2^S x - hi),
 // and x y = hi hi' + hi lo' + lo hi' with fp32 sums: 22 significant bits (the dropped lo lo' is below
@@ -11,24 +11,31 @@
 // and |b g + c g g| < 31 with S = 10 (head room 64).  Against 64 bits the result is as close as the
 // same steps in fp32 throughout (the error is that of the long sums, not of the operands).
 // The iterate itself and the norms stay in fp32 / fp64.
+//
+// A split matrix ("planes") lies in memory as [row][column / 32][part][32]: the two parts of 32 columns are
+// one 128-byte line, 8 units of 16 bytes.
+//
+// Three ways to run the products, by size:
+//   both sides <= 128: the whole iteration in one launch, a workgroup per matrix, planes in LDS;
+//   few tiles: 32 x 32 tiles, the contraction split over the four waves of a workgroup, operands straight
+//     from memory (every load of a wave in flight: the time is a few round trips);
+//   otherwise: 64 x 64 or 128 x 128 tiles staged through LDS.
+// y y^T and g g are symmetric: only tiles on and below the diagonal are computed, and mirrored.
 #include "common.h"
 
 #include <cmath>
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int T = 64;         // output tile
-constexpr int KS = 32;        // contraction per slab
-constexpr int LP = KS + 8;    // LDS pitch in fp16
-constexpr int PARTS = 64;     // partial sums of a norm
+constexpr int PARTS = 64;                  // partial sums of a norm
 constexpr float kY = 4096.f, kG = 1024.f;  // 2^S of the planes of y and of g, b g + c g g
-
-struct Planes {  // hi and lo part of an fp32 matrix
-  _Float16 *hi, *lo;
-};
+constexpr int ONE = 128;                   // largest side of the one-launch form
 
 struct NsParams {
   // the user's matrices (row-major, as given)
@@ -38,19 +45,70 @@ struct NsParams {
   int rows, cols, batch, tall;  // tall: rows > cols
   float momentum, grad_scale, keep, step;
   int nesterov;
+  bool flat;  // x (and m) without gaps inside a matrix, 16-byte aligned
+  bool vec;   // out / p rows may be written 16 bytes at a time
   float a, b, c, eps;
+  int steps;
   // workspace
   int r, n, rp, np;
-  float *y, *g;                     // [batch][rp][np], [batch][rp][rp]
-  Planes yp, yt[2], gp, bp;         // y, y^T ([np][rp]; read and written by one product, so two), g, b g + c g g
-  double *sums;                     // [batch][PARTS]
+  float *y, *g;               // [batch][rp][np], [batch][rp][rp] (tiles on and below the diagonal)
+  _Float16 *yp[2], *gp, *bp;  // planes of y (read and written by one product, so two), g, b g + c g g
+  double *sums;               // [batch][PARTS]
 };
 
+// ------------------------------------------------------------------------------------- the planes
 __device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
+// fp16 offset of the hi part of element (row, col) of a matrix of `cols` columns; the lo part lies 32 behind
+__device__ __forceinline__ long long plane_at(long long row, int col, int cols) {
+  return row * (2ll * cols) + (col >> 5) * 64 + (col & 31);
+}
+__device__ __forceinline__ void store_split4(_Float16 *at, f32x4 v, float scale) {
+  f16x4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    _Float16 h, l;
+    split(v[e] * scale, h, l);
+    hi[e] = h, lo[e] = l;
+  }
+  *reinterpret_cast<f16x4 *>(at) = hi;
+  *reinterpret_cast<f16x4 *>(at + 32) = lo;
+}
+__device__ __forceinline__ void store_split(_Float16 *at, float v, float scale) {
+  _Float16 h, l;
+  split(v * scale, h, l);
+  at[0] = h;
+  at[32] = l;
+}
+// In LDS unit u of row `row` sits at u ^ swizzle(row): eight rows of one unit, and four rows of two
+// neighbouring units (a transposed read), then fall on different banks.
+__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
 
+// Transposed read: lane l of each 16 gets rows 0..3 of column l of the 4 x 16 block whose row l / 4,
+// columns 4 (l % 4) .. + 3, its address names.
+__device__ __forceinline__ f16x4 read_transposed(const _Float16 *at) {
+  const i16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) i16x4 *)(at));
+  return __builtin_bit_cast(f16x4, r);
+}
+__device__ __forceinline__ f16x8 join(f16x4 a, f16x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f32x16 product3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 acc) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// ----------------------------------------------------------------------------- norm and first y
 // The update before normalisation.  `first`: the momentum is still the old one and is written.
 __device__ __forceinline__ float update_value(const NsParams &p, long long at, bool first) {
   const float x = p.x[at];
@@ -63,21 +121,59 @@ __device__ __forceinline__ float update_value(const NsParams &p, long long at, b
   }
   return p.nesterov ? gs + p.momentum * m : m;
 }
+__device__ __forceinline__ f32x4 update_quad(const NsParams &p, long long at, bool first) {
+  const f32x4 x = *reinterpret_cast<const f32x4 *>(p.x + at);
+  if (!p.m) return x;
+  f32x4 m = *reinterpret_cast<const f32x4 *>(p.m + at), u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float gs = p.grad_scale * x[e];
+    if (first) m[e] = p.momentum * m[e] + gs;
+    u[e] = p.nesterov ? gs + p.momentum * m[e] : m[e];
+  }
+  if (first) *reinterpret_cast<f32x4 *>(p.m + at) = m;
+  return u;
+}
 
-// Sum of squares of one matrix in PARTS parts, each over whole rows in a fixed order; Muon: the new momentum.
+__device__ __forceinline__ double wave_sum(double s) {
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  return s;
+}
+
+// Sum of squares of one matrix in PARTS parts in a fixed order; Muon: the new momentum.
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsParams p) {
   __shared__ double red[4];
   const int part = blockIdx.x % PARTS;
   const long long k = blockIdx.x / PARTS;
-  const long long size = (long long)p.rows * p.cols, chunk = (size + PARTS - 1) / PARTS;
-  const long long end = (part + 1) * chunk < size ? (part + 1) * chunk : size;
+  const long long size = (long long)p.rows * p.cols, chunk = ((size + PARTS - 1) / PARTS + 3) / 4 * 4;
+  const long long begin = part * chunk < size ? part * chunk : size;
+  const long long end = begin + chunk < size ? begin + chunk : size;
   double s = 0.0;
-  for (long long i = part * chunk + threadIdx.x; i < end; i += 256) {
-    const long long row = i / p.cols;
-    const float u = update_value(p, k * p.stride_x + row * p.ld_x + (i - row * p.cols), true);
-    s += (double)u * (double)u;
+  if (p.flat) {
+    const long long quads = (end - begin) / 4;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < quads; i += 256) {
+      const f32x4 u = update_quad(p, k * p.stride_x + begin + 4 * i, true);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (double)u[e] * (double)u[e];
+    }
+    const long long i = begin + 4 * quads + threadIdx.x;
+    if (i < end) {
+      const float u = update_value(p, k * p.stride_x + i, true);
+      s += (double)u * (double)u;
+    }
+  } else {
+    long long i = begin + threadIdx.x, row = i / p.cols;
+    int col = (int)(i - row * p.cols);
+    const int step_rows = 256 / p.cols, step_cols = 256 % p.cols;
+    for (; i < end; i += 256) {
+      const float u = update_value(p, k * p.stride_x + row * p.ld_x + col, true);
+      s += (double)u * (double)u;
+      row += step_rows, col += step_cols;
+      if (col >= p.cols) col -= p.cols, ++row;
+    }
   }
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) p.sums[k * PARTS + part] = (red[0] + red[1]) + (red[2] + red[3]);
@@ -92,121 +188,461 @@ __device__ __forceinline__ void emit(const NsParams &p, long long k, int i, int 
   else
     p.out[at] = v;
 }
+__device__ __forceinline__ void emit4(const NsParams &p, long long k, int i, int j, f32x4 v) {
+  if (p.tall || !p.vec || j + 3 >= p.n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) emit(p, k, i, j + e, v[e]);
+    return;
+  }
+  if (i >= p.r) return;
+  const long long at = k * p.stride_out + i * p.ld_out + j;
+  if (p.p) {
+    f32x4 x = *reinterpret_cast<const f32x4 *>(p.p + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = x[e] * p.keep - p.step * v[e];
+    *reinterpret_cast<f32x4 *>(p.p + at) = x;
+  } else {
+    *reinterpret_cast<f32x4 *>(p.out + at) = v;
+  }
+}
 
-// y = u / (|u| + eps) with its planes and transposed planes, one 64 x 64 tile per workgroup; `last`: only the result.
+// y = u / (|u| + eps) with its planes, one 64 x 64 tile per workgroup; `last`: only the result.
 __global__ __launch_bounds__(256) void ns_start_kernel(const NsParams p, int last) {
+  constexpr int T = 64;
   __shared__ float tile[T][T + 1];
   const int tj = p.np / T, tiles = (p.rp / T) * tj;
   const long long k = blockIdx.x / tiles;
   const int t = blockIdx.x % tiles, i0 = t / tj * T, j0 = t % tj * T;
-  double s = 0.0;
-  for (int part = 0; part < PARTS; ++part) s += p.sums[k * PARTS + part];
-  const float norm = (float)sqrt(s) + p.eps;
-  for (int u = threadIdx.x; u < T * T; u += 256) {  // walk the user's matrix along its rows
-    const int a = u / T, b = u % T, i = p.tall ? b : a, j = p.tall ? a : b;
-    float v = 0.f;
-    if (i0 + i < p.r && j0 + j < p.n) {
-      const long long row = p.tall ? j0 + j : i0 + i, col = p.tall ? i0 + i : j0 + j;
-      v = update_value(p, k * p.stride_x + row * p.ld_x + col, false) / norm;
+  const float norm = (float)sqrt(wave_sum(p.sums[k * PARTS + (threadIdx.x & 63)])) + p.eps;
+  if (p.tall) {  // rows of the user's matrix are columns here
+    for (int u = threadIdx.x; u < T * T; u += 256) {
+      const int j = u / T, i = u % T;
+      float v = 0.f;
+      if (i0 + i < p.r && j0 + j < p.n) v = update_value(p, k * p.stride_x + (j0 + j) * p.ld_x + i0 + i, false) / norm;
+      tile[i][j] = v;
     }
-    tile[i][j] = v;
+    __syncthreads();
   }
-  __syncthreads();
-  for (int u = threadIdx.x; u < T * T; u += 256) {
-    const int i = u / T, j = u % T;
-    const float v = tile[i][j];
+  for (int u = threadIdx.x; u < T * T / 4; u += 256) {
+    const int i = u / (T / 4), j = u % (T / 4) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (p.tall) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = tile[i][j + e];
+    } else if (i0 + i < p.r) {
+      const long long at = k * p.stride_x + (i0 + i) * p.ld_x + j0 + j;
+      if (p.flat && p.cols % 4 == 0) {
+        if (j0 + j < p.n) v = update_quad(p, at, false);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j0 + j + e < p.n) v[e] = update_value(p, at + e, false);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j0 + j + e < p.n) v[e] /= norm;
+    }
     if (last) {
-      emit(p, k, i0 + i, j0 + j, v);
+      emit4(p, k, i0 + i, j0 + j, v);
       continue;
     }
-    const long long at = (k * p.rp + i0 + i) * p.np + j0 + j;
-    p.y[at] = v;
-    split(v * kY, p.yp.hi[at], p.yp.lo[at]);
-    const long long tt = (k * p.np + j0 + i) * p.rp + i0 + j;
-    split(tile[j][i] * kY, p.yt[0].hi[tt], p.yt[0].lo[tt]);
+    const long long row = k * p.rp + i0 + i;
+    *reinterpret_cast<f32x4 *>(p.y + row * p.np + j0 + j) = v;
+    store_split4(p.yp[0] + plane_at(row, j0 + j, p.np), v, kY);
   }
 }
 
+// --------------------------------------------------------------------------------------- products
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
-// C[i][j] = sum_k P[i][k] Q[j][k], one 64 x 64 tile per workgroup, a wave per 32 x 32 quarter.
+// C[i][j] = sum_k P[i][k] Q[j][k]:
 //   GRAM: P = Q = y      -> g and its planes
 //   POLY: P = Q = g      -> planes of b g + c g g
 //   APPLY: P = that, Q = y^T -> y = a y + C with its planes;  LAST: the same, result to the user's matrix
+// What becomes of four neighbouring elements (i, j..j+3) of the sum; returns the value (scale: of its planes).
 template <int MODE>
-__global__ __launch_bounds__(256) void ns_product_kernel(const NsParams p, int flip) {
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2][T * LP];  // operand, part
-  const int cols = MODE >= APPLY ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
-  const int tj = cols / T, tiles = (p.rp / T) * tj;
-  const long long k = blockIdx.x / tiles;
-  const int t = blockIdx.x % tiles, i0 = t / tj * T, j0 = t % tj * T;
-  const Planes P = MODE == GRAM ? p.yp : MODE == POLY ? p.gp : p.bp;
-  const Planes Q = MODE == GRAM ? p.yp : MODE == POLY ? p.gp : p.yt[flip];
-  const long long pb = (k * p.rp + i0) * depth, qb = (k * (long long)cols + j0) * depth;
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  const int lr = threadIdx.x >> 2, lc = (threadIdx.x & 3) * 8;  // this thread's 16 bytes of a slab
-  f32x16 acc;
+__device__ __forceinline__ f32x4 finish(const NsParams &p, int flip, long long k, int i, int j, f32x4 acc) {
+  const int cols = MODE >= APPLY ? p.np : p.rp;
+  const long long row = k * p.rp + i, at = row * cols + j;
+  f32x4 v;
+  if constexpr (MODE == GRAM) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int k0 = 0; k0 < depth; k0 += KS) {
-    const long long po = pb + (long long)lr * depth + k0 + lc, qo = qb + (long long)lr * depth + k0 + lc;
-    const f16x8 x0 = *reinterpret_cast<const f16x8 *>(P.hi + po), x1 = *reinterpret_cast<const f16x8 *>(P.lo + po);
-    const f16x8 y0 = *reinterpret_cast<const f16x8 *>(Q.hi + qo), y1 = *reinterpret_cast<const f16x8 *>(Q.lo + qo);
-    __syncthreads();
-    *reinterpret_cast<f16x8 *>(&lds[0][0][lr * LP + lc]) = x0;
-    *reinterpret_cast<f16x8 *>(&lds[0][1][lr * LP + lc]) = x1;
-    *reinterpret_cast<f16x8 *>(&lds[1][0][lr * LP + lc]) = y0;
-    *reinterpret_cast<f16x8 *>(&lds[1][1][lr * LP + lc]) = y1;
-    __syncthreads();
+    for (int e = 0; e < 4; ++e) v[e] = acc[e] * (1.f / (kY * kY));
+    *reinterpret_cast<f32x4 *>(p.g + at) = v;
+    store_split4(p.gp + plane_at(row, j, cols), v, kG);
+  } else if constexpr (MODE == POLY) {
+    const f32x4 g = *reinterpret_cast<const f32x4 *>(p.g + at);
 #pragma unroll
-    for (int h = 0; h < KS; h += 16) {
-      const f16x8 ph = *reinterpret_cast<const f16x8 *>(&lds[0][0][(wi + c) * LP + h + 8 * g]);
-      const f16x8 pl = *reinterpret_cast<const f16x8 *>(&lds[0][1][(wi + c) * LP + h + 8 * g]);
-      const f16x8 qh = *reinterpret_cast<const f16x8 *>(&lds[1][0][(wj + c) * LP + h + 8 * g]);
-      const f16x8 ql = *reinterpret_cast<const f16x8 *>(&lds[1][1][(wj + c) * LP + h + 8 * g]);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    for (int e = 0; e < 4; ++e) v[e] = p.b * g[e] + p.c * (acc[e] * (1.f / (kG * kG)));
+    store_split4(p.bp + plane_at(row, j, cols), v, kG);
+  } else {
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(p.y + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
+    if constexpr (MODE == LAST) {
+      emit4(p, k, i, j, v);
+    } else {
+      *reinterpret_cast<f32x4 *>(p.y + at) = v;
+      store_split4(p.yp[1 - flip] + plane_at(row, j, cols), v, kY);
     }
   }
-  const int j = j0 + wj + c;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int i = i0 + wi + 8 * (e / 4) + 4 * g + e % 4;
-    const long long at = (k * p.rp + i) * cols + j;
-    if (MODE == GRAM) {
-      const float v = acc[e] * (1.f / (kY * kY));
-      p.g[at] = v;
-      split(v * kG, p.gp.hi[at], p.gp.lo[at]);
-    } else if (MODE == POLY) {
-      const float v = p.b * p.g[at] + p.c * (acc[e] * (1.f / (kG * kG)));
-      split(v * kG, p.bp.hi[at], p.bp.lo[at]);
-    } else {
-      const float v = p.a * p.y[at] + acc[e] * (1.f / (kG * kY));
-      if (MODE == LAST) {
-        emit(p, k, i, j, v);
-      } else {
-        p.y[at] = v;
-        _Float16 hi, lo;
-        split(v * kY, hi, lo);
-        p.yp.hi[at] = hi, p.yp.lo[at] = lo;
-        const long long tt = (k * p.np + j) * p.rp + i;
-        p.yt[1 - flip].hi[tt] = hi, p.yt[1 - flip].lo[tt] = lo;
-      }
-    }
+  return v;
+}
+
+// Tile t of a list: all tiles row by row, or those on and below the diagonal.
+template <bool LOWER>
+__device__ __forceinline__ void tile_of(int t, int tj, int &i, int &j) {
+  if constexpr (LOWER) {
+    i = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) / 2 > t) --i;
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    j = t - i * (i + 1) / 2;
+  } else {
+    i = t / tj;
+    j = t - i * tj;
   }
 }
 
-long long padded(long long x) { return (x + T - 1) / T * T; }
+// T x T tiles, four waves of T/2 x T/2 each, slabs of 32 k double-buffered in LDS.
+// The workgroups of an XCD (every eighth) take neighbouring tiles, so that they share operands in its L2.
+template <int MODE, int T>
+__global__ __launch_bounds__(256, 2) void ns_tile_kernel(const NsParams p, int flip, int total) {
+  constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
+  constexpr int NB = T / 64;                 // 32-wide blocks of a wave in each direction
+  constexpr int UNITS = T * 8;               // 16-byte units of an operand's slab
+  constexpr int LOADS = UNITS / 256;
+  __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][UNITS];
+  const int per = (total + 7) / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (id >= total || (int)blockIdx.x / 8 >= per) return;
+  const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
+  const int ti = p.rp / T, tj = cols / T, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
+  const long long k = id / tiles;
+  int bi, bj;
+  tile_of<LOWER>(id % tiles, tj, bi, bj);
+  const int i0 = bi * T, j0 = bj * T;
+  const _Float16 *P = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.bp;
+  const _Float16 *Q = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.yp[flip];
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
+  const int wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2);
+
+  // this thread's units of a slab: source (advancing by `psteps` / `qsteps` units per slab) and place in LDS
+  const f16x8 *ps[LOADS], *qs[LOADS];
+  int pd[LOADS], qd[LOADS];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int id = threadIdx.x + 256 * u, row = id / 8, unit = id % 8;
+    ps[u] = reinterpret_cast<const f16x8 *>(P + (k * p.rp + i0 + row) * 2ll * depth) + unit;
+    pd[u] = row * 8 + (unit ^ swizzle(row));
+    if constexpr (TR) {  // 32 rows of T columns
+      const int qrow = id / (T / 4), qunit = id % (T / 4);
+      qs[u] = reinterpret_cast<const f16x8 *>(Q + (k * p.rp + qrow) * 2ll * cols + 2 * j0) + qunit;
+      qd[u] = qrow * (T / 4) + (qunit ^ swizzle(qrow));
+    } else {
+      qs[u] = reinterpret_cast<const f16x8 *>(Q + (k * p.rp + j0 + row) * 2ll * depth) + unit;
+      qd[u] = pd[u];
+    }
+  }
+  const long long qstep = TR ? 32ll * cols * 2 / 8 : 8;
+
+  f32x16 acc[NB][NB];
+#pragma unroll
+  for (int x = 0; x < NB; ++x)
+#pragma unroll
+    for (int y = 0; y < NB; ++y) acc[x][y] = zero16();
+  f16x8 pr[LOADS], qr[LOADS];
+  const int slabs = depth / 32;
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) pr[u] = *ps[u], qr[u] = *qs[u];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) lds[0][0][pd[u]] = pr[u], lds[0][1][qd[u]] = qr[u];
+  __syncthreads();
+  for (int s = 0; s < slabs; ++s) {
+    const bool more = s + 1 < slabs;
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) {
+        ps[u] += 8, qs[u] += qstep;
+        pr[u] = *ps[u], qr[u] = *qs[u];
+      }
+    }
+    const f16x8 *lp = lds[s & 1][0], *lq = lds[s & 1][1];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f16x8 a[NB][2], b[NB][2];  // [block][part] of P (columns of the result tile's MFMA form) and Q
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const int row = wi + 32 * x + c;
+          a[x][part] = lp[row * 8 + ((4 * part + 2 * h + g) ^ swizzle(row))];
+          if constexpr (TR) {
+            const int sub = (lane >> 4) & 1, k0 = 16 * h + 8 * g + ((lane & 15) >> 2);
+            const int unit = ((wj >> 5) + x) * 8 + 4 * part + 2 * sub + ((lane & 3) >> 1);
+            const _Float16 *base = reinterpret_cast<const _Float16 *>(lq) + 4 * (lane & 1);
+            b[x][part] = join(read_transposed(base + (k0 * (T / 4) + (unit ^ swizzle(k0))) * 8),
+                              read_transposed(base + ((k0 + 4) * (T / 4) + (unit ^ swizzle(k0 + 4))) * 8));
+          } else {
+            const int qrow = wj + 32 * x + c;
+            b[x][part] = lq[qrow * 8 + ((4 * part + 2 * h + g) ^ swizzle(qrow))];
+          }
+        }
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int y = 0; y < NB; ++y) acc[x][y] = product3(b[y][0], b[y][1], a[x][0], a[x][1], acc[x][y]);
+    }
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) lds[(s + 1) & 1][0][pd[u]] = pr[u], lds[(s + 1) & 1][1][qd[u]] = qr[u];
+    }
+    __syncthreads();
+  }
+  // register 4 q + e of lane (c, g) is element (i = c, j = 8 q + 4 g + e) of a block
+#pragma unroll
+  for (int x = 0; x < NB; ++x)
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + wi + 32 * x + c, j = j0 + wj + 32 * y + 8 * q + 4 * g;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * q + e];
+        v = finish<MODE>(p, flip, k, i, j, v);
+        if (LOWER && bi != bj) {
+          _Float16 *dst = MODE == GRAM ? p.gp : p.bp;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) store_split(dst + plane_at(k * p.rp + j + e, i, cols), v[e], kG);
+        }
+      }
+}
+
+// 32 x 32 tiles, a quarter of the contraction per wave, operands straight from memory.
+template <int MODE>
+__global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int flip) {
+  constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
+  constexpr int U = TR ? 4 : 8;       // steps of 16 k in flight
+  constexpr int PITCH = 80;           // fp16 pitch of a row of transposed operand (64 + a shift of 32 bytes)
+  constexpr int SUM_PITCH = 36, REGION = TR ? U * 16 * PITCH * 2 : 32 * SUM_PITCH * 4;  // bytes of a wave
+  static_assert(REGION >= 32 * SUM_PITCH * 4, "the wave's sums go where its operand was");
+  __shared__ __attribute__((aligned(16))) char lds[4][REGION];
+  const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
+  const int ti = (p.r + 31) / 32, tj = TR ? (p.n + 31) / 32 : ti, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
+  const long long k = blockIdx.x / tiles;
+  int bi, bj;
+  tile_of<LOWER>(blockIdx.x % tiles, tj, bi, bj);
+  const int i0 = bi * 32, j0 = bj * 32;
+  const _Float16 *P = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.bp;
+  const _Float16 *Q = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.yp[flip];
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int steps = ((MODE == GRAM ? p.n : p.r) + 15) / 16, quarter = (steps + 3) / 4;  // k behind n / r is padding
+  const int s0 = min(wave * quarter, steps), s1 = min(s0 + quarter, steps);
+  const _Float16 *prow = P + (k * p.rp + i0 + c) * 2ll * depth + 8 * g;
+  const _Float16 *qrow = TR ? Q + (k * p.rp + (lane >> 2)) * 2ll * cols + 2 * j0 + 8 * (lane & 3)
+                            : Q + (k * p.rp + j0 + c) * 2ll * depth + 8 * g;
+  f32x16 acc = zero16();
+  [[maybe_unused]] _Float16 *qt = reinterpret_cast<_Float16 *>(lds[wave]);
+  for (int s = s0; s < s1; s += U) {
+    f16x8 a[U][2], b[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = min(s + u, s1 - 1), off = (t >> 1) * 64 + (t & 1) * 16;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        a[u][part] = *reinterpret_cast<const f16x8 *>(prow + off + 32 * part);
+        if constexpr (TR)
+          b[u][part] = *reinterpret_cast<const f16x8 *>(qrow + t * 16ll * 2 * cols + 32 * part);
+        else
+          b[u][part] = *reinterpret_cast<const f16x8 *>(qrow + off + 32 * part);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // keep them all in flight
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s + u >= s1) a[u][0] = a[u][1] = f16x8{};  // (a step that was loaded twice adds nothing)
+    if constexpr (TR) {  // through the wave's own part of LDS
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          *reinterpret_cast<f16x8 *>(qt + (u * 16 + (lane >> 2)) * PITCH + 32 * part + 8 * (lane & 3)) = b[u][part];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const int row = u * 16 + 8 * g + ((lane & 15) >> 2), col = 32 * part + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          b[u][part] = join(read_transposed(qt + row * PITCH + col), read_transposed(qt + (row + 4) * PITCH + col));
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc = product3(b[u][0], b[u][1], a[u][0], a[u][1], acc);
+  }
+  float *mine = reinterpret_cast<float *>(lds[wave]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e];
+    *reinterpret_cast<f32x4 *>(mine + c * SUM_PITCH + 8 * q + 4 * g) = v;
+  }
+  __syncthreads();
+  const int i = threadIdx.x >> 3, j = (threadIdx.x & 7) * 4;
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float w[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) w[x] = reinterpret_cast<const float *>(lds[x])[i * SUM_PITCH + j + e];
+    v[e] = (w[0] + w[1]) + (w[2] + w[3]);
+  }
+  v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v);
+  if (LOWER && bi != bj) {
+    __syncthreads();
+    float *turn = reinterpret_cast<float *>(lds[0]);
+    *reinterpret_cast<f32x4 *>(turn + i * SUM_PITCH + j) = v;
+    __syncthreads();
+    f32x4 w;  // (j0 + i, i0 + j ..)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = turn[(j + e) * SUM_PITCH + i];
+    store_split4((MODE == GRAM ? p.gp : p.bp) + plane_at(k * p.rp + j0 + i, i0 + j, cols), w, kG);
+  }
+}
+
+// Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; y stays in
+// registers, its planes and those of g and b g + c g g in LDS (64 KiB each).
+__global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
+  extern __shared__ __attribute__((aligned(16))) f16x8 one_lds[];
+  __shared__ double red[16];
+  const int tr = (p.r + 31) / 32, tn = (p.n + 31) / 32;  // blocks of 32 in use
+  f16x8 *yl = one_lds, *gl = one_lds + tr * 32 * tn * 8;  // [row][column block][8 units]
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long k = blockIdx.x;
+  const int yi = wave / 4, yj = wave % 4;  // this wave's block of y and of g
+  const bool y_mine = yi < tr && yj < tn, g_mine = yi < tr && yj < tr;
+  float y[16];
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int i = 32 * yi + c, j = 32 * yj + 8 * (e / 4) + 4 * g + e % 4;
+    y[e] = 0.f;
+    if (i < p.r && j < p.n) y[e] = update_value(p, k * p.stride_x + (p.tall ? j * p.ld_x + i : i * p.ld_x + j), true);
+    s += (double)y[e] * (double)y[e];
+  }
+  s = wave_sum(s);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += red[w];
+  const float norm = (float)sqrt(s) + p.eps;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int i = 32 * yi + c, j = 32 * yj + 8 * (e / 4) + 4 * g + e % 4;
+    if (i < p.r && j < p.n) y[e] /= norm;
+  }
+  // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout
+  auto store = [&](f16x8 *m, int blocks, const float (&v)[16], float scale) {
+    const int row = 32 * yi + c;
+    _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + yj) * 8);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f16x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 h, l;
+        split(v[4 * q + e] * scale, h, l);
+        hi[e] = h, lo[e] = l;
+      }
+      *reinterpret_cast<f16x4 *>(line + 8 * (q ^ swizzle(row)) + 4 * g) = hi;
+      *reinterpret_cast<f16x4 *>(line + 8 * ((4 + q) ^ swizzle(row)) + 4 * g) = lo;
+    }
+  };
+  auto operand = [&](const f16x8 *m, int blocks, int block, int h, int part) {  // row `32 block + c`, k 16 h + 8 g ..
+    const int row = 32 * block + c;
+    return m[(row * blocks + (h >> 1)) * 8 + ((4 * part + 2 * (h & 1) + g) ^ swizzle(row))];
+  };
+  if (p.steps > 0 && y_mine) store(yl, tn, y, kY);
+  __syncthreads();
+  for (int step = 0; step < p.steps; ++step) {
+    float v[16], gv[16];
+    if (g_mine) {  // g = y y^T
+      f32x16 acc = zero16();
+#pragma unroll 1
+      for (int h = 0; h < 2 * tn; ++h)
+        acc = product3(operand(yl, tn, yj, h, 0), operand(yl, tn, yj, h, 1), operand(yl, tn, yi, h, 0),
+                       operand(yl, tn, yi, h, 1), acc);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) gv[e] = acc[e] * (1.f / (kY * kY));
+      store(gl, tr, gv, kG);
+    }
+    __syncthreads();
+    if (g_mine) {  // b g + c g g
+      f32x16 acc = zero16();
+#pragma unroll 1
+      for (int h = 0; h < 2 * tr; ++h)
+        acc = product3(operand(gl, tr, yj, h, 0), operand(gl, tr, yj, h, 1), operand(gl, tr, yi, h, 0),
+                       operand(gl, tr, yi, h, 1), acc);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = p.b * gv[e] + p.c * (acc[e] * (1.f / (kG * kG)));
+    }
+    __syncthreads();
+    if (g_mine) store(gl, tr, v, kG);
+    __syncthreads();
+    if (y_mine) {  // y = a y + that y
+      f32x16 acc = zero16();
+      const int sub = (lane >> 4) & 1, rr = (lane & 15) >> 2;
+#pragma unroll 1
+      for (int h = 0; h < 2 * tr; ++h) {
+        f16x8 b[2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const int row = 16 * h + 8 * g + rr, unit = 4 * part + 2 * sub + ((lane & 3) >> 1);
+          const _Float16 *base = reinterpret_cast<const _Float16 *>(yl + yj * 8) + 4 * (lane & 1);
+          b[part] = join(read_transposed(base + (row * tn * 8 + (unit ^ swizzle(row))) * 8),
+                         read_transposed(base + ((row + 4) * tn * 8 + (unit ^ swizzle(row + 4))) * 8));
+        }
+        acc = product3(b[0], b[1], operand(gl, tr, yi, h, 0), operand(gl, tr, yi, h, 1), acc);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
+    }
+    __syncthreads();
+    if (step + 1 < p.steps) {
+      if (y_mine) store(yl, tn, y, kY);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) emit(p, k, 32 * yi + c, 32 * yj + 8 * (e / 4) + 4 * g + e % 4, y[e]);
+}
+
+// ------------------------------------------------------------------------------------------- plan
+enum { FORM_ONE, FORM_SMALL, FORM_64, FORM_128 };
+
+long long padded(long long x, int t) { return (x + t - 1) / t * t; }
+
+int plan_form(int r, int n, int batch) {
+  if (n <= ONE) return FORM_ONE;
+  const long long enough = vitk::cu_count() * 3 / 4;
+  if (batch * (padded(r, 128) / 128) * (padded(n, 128) / 128) >= enough) return FORM_128;
+  if (batch * (padded(r, 64) / 64) * (padded(n, 64) / 64) >= enough) return FORM_64;
+  return FORM_SMALL;
+}
 
 // Workspace of one call: sums, then y, g (fp32), then the planes.
-size_t plan(NsParams *p, float *workspace) {
+size_t plan(NsParams *p, float *workspace, int *form) {
   p->tall = p->rows > p->cols;
   p->r = p->tall ? p->cols : p->rows;
   p->n = p->tall ? p->rows : p->cols;
-  p->rp = (int)padded(p->r);
-  p->np = (int)padded(p->n);
+  *form = plan_form(p->r, p->n, p->batch);
+  if (*form == FORM_ONE) return 0;
+  const int t = *form == FORM_128 ? 128 : 64;
+  p->rp = (int)padded(p->r, t);
+  p->np = (int)padded(p->n, t);
   const size_t b = p->batch, yy = b * p->rp * p->np, gg = b * p->rp * p->rp;
   char *at = reinterpret_cast<char *>(workspace);
   size_t used = 0;
@@ -218,13 +654,8 @@ size_t plan(NsParams *p, float *workspace) {
   p->sums = reinterpret_cast<double *>(take(b * PARTS * sizeof(double)));
   p->y = reinterpret_cast<float *>(take(yy * 4));
   p->g = reinterpret_cast<float *>(take(gg * 4));
-  auto planes = [&](size_t count) {
-    Planes r;
-    r.hi = reinterpret_cast<_Float16 *>(take(count * 2));
-    r.lo = reinterpret_cast<_Float16 *>(take(count * 2));
-    return r;
-  };
-  p->yp = planes(yy), p->yt[0] = planes(yy), p->yt[1] = planes(yy), p->gp = planes(gg), p->bp = planes(gg);
+  for (auto *planes : {&p->yp[0], &p->yp[1]}) *planes = reinterpret_cast<_Float16 *>(take(yy * 4));
+  for (auto *planes : {&p->gp, &p->bp}) *planes = reinterpret_cast<_Float16 *>(take(gg * 4));
   return used;
 }
 
@@ -246,24 +677,53 @@ bool bounded(float a, float b, float c, int steps) {
   return true;
 }
 
-int run(const char *who, NsParams *p, int steps, float *workspace, size_t bytes, hipStream_t st) {
-  const size_t need = plan(p, nullptr);
+template <int MODE>
+void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
+  const int t = form == FORM_128 ? 128 : form == FORM_64 ? 64 : 32;
+  const long long ti = (p.r + t - 1) / t, tj = (p.n + t - 1) / t;
+  const long long total = p.batch * (MODE <= POLY ? ti * (ti + 1) / 2 : ti * tj);
+  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(256);
+  if (form == FORM_128)
+    hipLaunchKernelGGL((ns_tile_kernel<MODE, 128>), grid, block, 0, st, p, flip, (int)total);
+  else if (form == FORM_64)
+    hipLaunchKernelGGL((ns_tile_kernel<MODE, 64>), grid, block, 0, st, p, flip, (int)total);
+  else
+    hipLaunchKernelGGL(ns_small_kernel<MODE>, dim3((unsigned)total), block, 0, st, p, flip);
+}
+
+std::atomic<unsigned long long> g_one_lds{0};
+
+int run(const char *who, NsParams *p, float *workspace, size_t bytes, hipStream_t st) {
+  int form;
+  const size_t need = plan(p, nullptr, &form);
+  const dim3 block(256);
+  if (form == FORM_ONE) {
+    const int tr = (p->r + 31) / 32, tn = (p->n + 31) / 32;
+    const size_t lds = (size_t)tr * 32 * (tn + tr) * 128;
+    if (vitk::first_use_on_device(&g_one_lds)) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(ns_one_kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 2 * ONE * ONE * 4);
+      VITK_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(ns_one_kernel, dim3(p->batch), dim3(1024), lds, st, *p);
+    return vitk::check_launch(who);
+  }
   VITK_REQUIRE(workspace && bytes >= need, "%s: workspace of %zu bytes needed, %zu given", who, need,
                workspace ? bytes : 0);
   VITK_REQUIRE(vitk::aligned16(workspace), "%s: workspace is not 16-byte aligned", who);
-  plan(p, workspace);
-  const long long ti = p->rp / T, tj = p->np / T, yb = p->batch * ti * tj, gb = p->batch * ti * ti;
-  VITK_REQUIRE(yb < (1ll << 31) && p->batch * (long long)PARTS < (1ll << 31), "%s: too many matrices for one launch", who);
-  const dim3 block(256);
+  plan(p, workspace, &form);
+  const long long yb = (long long)p->batch * (p->rp / 64) * (p->np / 64);
+  VITK_REQUIRE(4 * yb < (1ll << 31) - 8 && p->batch * (long long)PARTS < (1ll << 31),
+               "%s: too many matrices for one launch", who);
   hipLaunchKernelGGL(ns_norm_kernel, dim3(p->batch * PARTS), block, 0, st, *p);
-  hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)yb), block, 0, st, *p, steps == 0 ? 1 : 0);
-  for (int s = 0; s < steps; ++s) {
-    hipLaunchKernelGGL(ns_product_kernel<GRAM>, dim3((unsigned)gb), block, 0, st, *p, 0);
-    hipLaunchKernelGGL(ns_product_kernel<POLY>, dim3((unsigned)gb), block, 0, st, *p, 0);
-    if (s + 1 < steps)
-      hipLaunchKernelGGL(ns_product_kernel<APPLY>, dim3((unsigned)yb), block, 0, st, *p, s & 1);
+  hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)yb), block, 0, st, *p, p->steps == 0 ? 1 : 0);
+  for (int s = 0; s < p->steps; ++s) {
+    launch_product<GRAM>(*p, form, s & 1, st);
+    launch_product<POLY>(*p, form, s & 1, st);
+    if (s + 1 < p->steps)
+      launch_product<APPLY>(*p, form, s & 1, st);
     else
-      hipLaunchKernelGGL(ns_product_kernel<LAST>, dim3((unsigned)yb), block, 0, st, *p, s & 1);
+      launch_product<LAST>(*p, form, s & 1, st);
   }
   return vitk::check_launch(who);
 }
@@ -272,7 +732,8 @@ size_t bytes_of(int32_t rows, int32_t cols, int32_t batch) {
   if (!size_ok(rows, cols, batch) || rows == 0 || cols == 0 || batch == 0) return 0;
   NsParams p = {};
   p.rows = rows, p.cols = cols, p.batch = batch;
-  return plan(&p, nullptr);
+  int form;
+  return plan(&p, nullptr, &form);
 }
 
 int check(const char *who, int64_t rows, int64_t cols, int64_t batch, int steps, float a, float b, float c, float eps) {
@@ -304,9 +765,11 @@ extern "C" int vitk_newton_schulz_f32(const vitk_newton_schulz_args *a, vitk_str
   NsParams p = {};
   p.x = a->x, p.out = a->out;
   p.ld_x = a->ld_x, p.stride_x = a->stride_x, p.ld_out = a->ld_out, p.stride_out = a->stride_out;
-  p.rows = a->rows, p.cols = a->cols, p.batch = a->batch;
+  p.rows = a->rows, p.cols = a->cols, p.batch = a->batch, p.steps = a->steps;
+  p.flat = (a->ld_x == a->cols || a->rows == 1) && vitk::aligned16(a->x) && (a->batch == 1 || a->stride_x % 4 == 0);
+  p.vec = vitk::aligned16(a->out) && a->ld_out % 4 == 0 && (a->batch == 1 || a->stride_out % 4 == 0);
   p.a = a->a, p.b = a->b, p.c = a->c, p.eps = a->eps;
-  return run(who, &p, a->steps, a->workspace, a->workspace_bytes, vitk::as_stream(stream));
+  return run(who, &p, a->workspace, a->workspace_bytes, vitk::as_stream(stream));
 }
 
 extern "C" int vitk_muon_f32(const vitk_muon_args *a, vitk_stream_t stream) {
@@ -321,9 +784,12 @@ extern "C" int vitk_muon_f32(const vitk_muon_args *a, vitk_stream_t stream) {
   NsParams p = {};
   p.x = a->g, p.m = a->m, p.p = a->p;
   p.ld_x = p.ld_out = a->ld, p.stride_x = p.stride_out = a->stride;
-  p.rows = a->rows, p.cols = a->cols, p.batch = a->batch;
+  p.rows = a->rows, p.cols = a->cols, p.batch = a->batch, p.steps = a->steps;
+  p.flat = (a->ld == a->cols || a->rows == 1) && vitk::aligned16(a->g) && vitk::aligned16(a->m) &&
+           (a->batch == 1 || a->stride % 4 == 0);
+  p.vec = vitk::aligned16(a->p) && a->ld % 4 == 0 && (a->batch == 1 || a->stride % 4 == 0);
   p.momentum = a->momentum, p.grad_scale = a->grad_scale, p.nesterov = a->nesterov;
   p.keep = 1.f - a->lr * a->weight_decay, p.step = a->lr * a->update_scale;
   p.a = a->a, p.b = a->b, p.c = a->c, p.eps = a->eps;
-  return run(who, &p, a->steps, a->workspace, a->workspace_bytes, vitk::as_stream(stream));
+  return run(who, &p, a->workspace, a->workspace_bytes, vitk::as_stream(stream));
 }
