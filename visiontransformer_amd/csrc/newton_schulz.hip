@@ -5,12 +5,15 @@
 // out: the polynomial acts on singular values only), padded with zeros to whole tiles.
 // Products run on v_mfma_f32_32x32x16_f16 with every fp32 operand x split in two fp16 parts,
 //   2^S x = hi + lo,  hi = fp16(2^S x), lo = fp16(2^S x - hi),
-// and x y = hi hi' + hi lo' + lo hi' with fp32 sums: 22 significant bits (the dropped lo lo' is below
-// 2^-22), on matrix cores that do fp16 at 16 times the rate of fp32.  The steps are normalised, so
-// the range is known and the scales are constants: |y| <= 4 with S = 12 (a head room of 16), |y y^T| <= 16
-// and |b g + c g g| < 31 with S = 10 (head room 64).  Against 64 bits the result is as close as the
-// same steps in fp32 throughout (the error is that of the long sums, not of the operands).
-// The iterate itself and the norms stay in fp32 / fp64.
+// and x y = hi hi' + hi lo' + lo hi' with fp32 sums, on matrix cores that do fp16 at 16 times the rate of
+// fp32.  hi is off by at most half a step of 11 bits and lo, which has a sign, by half a step of 11
+// more: a pair is within 2^-23 of x, one bit short of fp32, in the same 32 bits; the dropped lo lo' is
+// below 2^-22.  The steps are normalised, so the range is known and the scales are constants: |y| <= 4
+// with S = 12 (a head room of 4), |y y^T| <= 16 and |b g + c g g| < 31 with S = 10 (head rooms 4 and 2).
+// Against 64 bits the result is as close as the same steps in fp32 throughout (the error is that of the
+// long sums, not of the operands).  Sums are fp32, the norm is fp64; the pairs are also where y and g
+// are kept between products: what the products move is what bounds them, and an fp32 copy beside the
+// pairs would double it.
 //
 // A split matrix ("planes") lies in memory as [row][column / 32][part][32]: the two parts of 32 columns are
 // one 128-byte line, 8 units of 16 bytes.
@@ -51,7 +54,6 @@ struct NsParams {
   int steps;
   // workspace
   int r, n, rp, np;
-  float *y, *g;               // [batch][rp][np], [batch][rp][rp] (tiles on and below the diagonal)
   _Float16 *yp[2], *gp, *bp;  // planes of y (read and written by one product, so two), g, b g + c g g
   double *sums;               // [batch][PARTS]
 };
@@ -188,22 +190,34 @@ __device__ __forceinline__ void emit(const NsParams &p, long long k, int i, int 
   else
     p.out[at] = v;
 }
-__device__ __forceinline__ void emit4(const NsParams &p, long long k, int i, int j, f32x4 v) {
-  if (p.tall || !p.vec || j + 3 >= p.n) {
+// Four neighbouring elements (row, col ..) of the user's matrix; `old`: the parameter, loaded before (p.vec).
+__device__ __forceinline__ f32x4 emit_old(const NsParams &p, long long k, int row, int col) {
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (p.p && p.vec && row < p.rows && col + 3 < p.cols)
+    x = *reinterpret_cast<const f32x4 *>(p.p + k * p.stride_out + row * p.ld_out + col);
+  return x;
+}
+__device__ __forceinline__ void emit4(const NsParams &p, long long k, int row, int col, f32x4 v, f32x4 old) {
+  if (row >= p.rows) return;
+  const long long at = k * p.stride_out + row * p.ld_out + col;
+  if (p.vec && col + 3 < p.cols) {
+    if (p.p) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) emit(p, k, i, j + e, v[e]);
+      for (int e = 0; e < 4; ++e) v[e] = old[e] * p.keep - p.step * v[e];
+      *reinterpret_cast<f32x4 *>(p.p + at) = v;
+    } else {
+      *reinterpret_cast<f32x4 *>(p.out + at) = v;
+    }
     return;
   }
-  if (i >= p.r) return;
-  const long long at = k * p.stride_out + i * p.ld_out + j;
-  if (p.p) {
-    f32x4 x = *reinterpret_cast<const f32x4 *>(p.p + at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = x[e] * p.keep - p.step * v[e];
-    *reinterpret_cast<f32x4 *>(p.p + at) = x;
-  } else {
-    *reinterpret_cast<f32x4 *>(p.out + at) = v;
-  }
+  for (int e = 0; e < 4; ++e)
+    if (col + e < p.cols) {
+      if (p.p)
+        p.p[at + e] = p.p[at + e] * p.keep - p.step * v[e];
+      else
+        p.out[at + e] = v[e];
+    }
 }
 
 // y = u / (|u| + eps) with its planes, one 64 x 64 tile per workgroup; `last`: only the result.
@@ -243,11 +257,15 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsParams p, int las
         if (j0 + j + e < p.n) v[e] /= norm;
     }
     if (last) {
-      emit4(p, k, i0 + i, j0 + j, v);
+      if (p.tall) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) emit(p, k, i0 + i, j0 + j + e, v[e]);
+      } else {
+        emit4(p, k, i0 + i, j0 + j, v, emit_old(p, k, i0 + i, j0 + j));
+      }
       continue;
     }
     const long long row = k * p.rp + i0 + i;
-    *reinterpret_cast<f32x4 *>(p.y + row * p.np + j0 + j) = v;
     store_split4(p.yp[0] + plane_at(row, j0 + j, p.np), v, kY);
   }
 }
@@ -259,162 +277,233 @@ enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 //   GRAM: P = Q = y      -> g and its planes
 //   POLY: P = Q = g      -> planes of b g + c g g
 //   APPLY: P = that, Q = y^T -> y = a y + C with its planes;  LAST: the same, result to the user's matrix
-// What becomes of four neighbouring elements (i, j..j+3) of the sum; returns the value (scale: of its planes).
+// What else goes into four neighbouring elements (i, j..j+3), y or g: parts loaded before the sums are needed.
+struct Parts {
+  f16x4 hi, lo;
+};
 template <int MODE>
-__device__ __forceinline__ f32x4 finish(const NsParams &p, int flip, long long k, int i, int j, f32x4 acc) {
-  const int cols = MODE >= APPLY ? p.np : p.rp;
-  const long long row = k * p.rp + i, at = row * cols + j;
+__device__ __forceinline__ Parts addend(const NsParams &p, int flip, long long k, int i, int j) {
+  if constexpr (MODE == GRAM) return Parts{};
+  const _Float16 *at = MODE == POLY ? p.gp + plane_at(k * p.rp + i, j, p.rp) : p.yp[flip] + plane_at(k * p.rp + i, j, p.np);
+  return Parts{*reinterpret_cast<const f16x4 *>(at), *reinterpret_cast<const f16x4 *>(at + 32)};
+}
+// The value of these elements, stored as planes (LAST: not stored).
+template <int MODE>
+__device__ __forceinline__ f32x4 finish(const NsParams &p, int flip, long long k, int i, int j, f32x4 acc, Parts add) {
+  const long long row = k * p.rp + i;
   f32x4 v;
-  if constexpr (MODE == GRAM) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = acc[e] * (1.f / (kY * kY));
-    *reinterpret_cast<f32x4 *>(p.g + at) = v;
-    store_split4(p.gp + plane_at(row, j, cols), v, kG);
-  } else if constexpr (MODE == POLY) {
-    const f32x4 g = *reinterpret_cast<const f32x4 *>(p.g + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = p.b * g[e] + p.c * (acc[e] * (1.f / (kG * kG)));
-    store_split4(p.bp + plane_at(row, j, cols), v, kG);
-  } else {
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(p.y + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
-    if constexpr (MODE == LAST) {
-      emit4(p, k, i, j, v);
-    } else {
-      *reinterpret_cast<f32x4 *>(p.y + at) = v;
-      store_split4(p.yp[1 - flip] + plane_at(row, j, cols), v, kY);
-    }
+  for (int e = 0; e < 4; ++e) {
+    const float x = (float)add.hi[e] + (float)add.lo[e];
+    if constexpr (MODE == GRAM)
+      v[e] = acc[e] * (1.f / (kY * kY));
+    else if constexpr (MODE == POLY)
+      v[e] = p.b * (x * (1.f / kG)) + p.c * (acc[e] * (1.f / (kG * kG)));
+    else
+      v[e] = p.a * (x * (1.f / kY)) + acc[e] * (1.f / (kG * kY));
   }
+  if constexpr (MODE == GRAM) store_split4(p.gp + plane_at(row, j, p.rp), v, kG);
+  if constexpr (MODE == POLY) store_split4(p.bp + plane_at(row, j, p.rp), v, kG);
+  if constexpr (MODE == APPLY) store_split4(p.yp[1 - flip] + plane_at(row, j, p.np), v, kY);
   return v;
 }
+// Four neighbouring elements (j, i..i+3) of the transposed tile: the mirrored part of a symmetric product, or the
+// result of a tall matrix.
+template <int MODE>
+__device__ __forceinline__ void finish_transposed(const NsParams &p, long long k, int j, int i, f32x4 v) {
+  if constexpr (MODE == LAST)
+    emit4(p, k, j, i, v, emit_old(p, k, j, i));
+  else
+    store_split4((MODE == GRAM ? p.gp : p.bp) + plane_at(k * p.rp + j, i, p.rp), v, kG);
+}
 
-// Tile t of a list: all tiles row by row, or those on and below the diagonal.
+// Tile t of a list: all tiles column by column (a column of tiles shares the long operand, and all of them the
+// short one), or those on and below the diagonal.
 template <bool LOWER>
-__device__ __forceinline__ void tile_of(int t, int tj, int &i, int &j) {
+__device__ __forceinline__ void tile_of(int t, int ti, int &i, int &j) {
   if constexpr (LOWER) {
     i = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (i * (i + 1) / 2 > t) --i;
     while ((i + 1) * (i + 2) / 2 <= t) ++i;
     j = t - i * (i + 1) / 2;
   } else {
-    i = t / tj;
-    j = t - i * tj;
+    j = t / ti;
+    i = t - j * ti;
   }
 }
 
-// T x T tiles, four waves of T/2 x T/2 each, slabs of 32 k double-buffered in LDS.
+// 16 bytes at base + voff + soff (bytes): a scalar base and offset, so that a thread keeps one address per operand.
+__device__ __forceinline__ f16x8 load_unit(const _Float16 *base, int voff, int soff) {
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16 *>(base), 0, 0x7fffffff, 0x00020000);
+  return __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+
+// T x T tiles, NW waves of T/2 x 2T/NW each, slabs of 32 k double-buffered in LDS and DIST more of them on
+// their way in registers: a slab is 768 cycles of matrix work at T = 128, what another XCD wrote is
+// 2000 to 3000 cycles away.
 // The workgroups of an XCD (every eighth) take neighbouring tiles, so that they share operands in its L2.
-template <int MODE, int T>
-__global__ __launch_bounds__(256, 2) void ns_tile_kernel(const NsParams p, int flip, int total) {
+template <int MODE, int T, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const NsParams p, int flip, int total) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
-  constexpr int NB = T / 64;                 // 32-wide blocks of a wave in each direction
-  constexpr int UNITS = T * 8;               // 16-byte units of an operand's slab
-  constexpr int LOADS = UNITS / 256;
-  __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][UNITS];
+  constexpr int NX = T / 64, NY = 2 * T / NW / 32;  // 32-wide blocks of a wave in each direction
+  constexpr int UNITS = T * 8;                      // 16-byte units of an operand's slab
+  constexpr int THREADS = 64 * NW, LOADS = UNITS / THREADS;
+  constexpr int DIST = T == 128 ? 2 : 4;
+  constexpr int SP = T + 4;  // pitch of the sums in the epilogue
+  constexpr int LDS_BYTES = T * SP * 4 > 4 * UNITS * 16 ? T * SP * 4 : 4 * UNITS * 16;
+  __shared__ __attribute__((aligned(16))) char lds_bytes[LDS_BYTES];
+  f16x8 (*lds)[2][UNITS] = reinterpret_cast<f16x8 (*)[2][UNITS]>(lds_bytes);  // [buffer][operand]
+  float *sums = reinterpret_cast<float *>(lds_bytes);
   const int per = (total + 7) / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (id >= total || (int)blockIdx.x / 8 >= per) return;
   const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
   const int ti = p.rp / T, tj = cols / T, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
   const long long k = id / tiles;
   int bi, bj;
-  tile_of<LOWER>(id % tiles, tj, bi, bj);
+  tile_of<LOWER>(id % tiles, ti, bi, bj);
   const int i0 = bi * T, j0 = bj * T;
-  const _Float16 *P = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.bp;
-  const _Float16 *Q = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.yp[flip];
   const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
-  const int wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2);
+  const int wi = (wave & 1) * (T / 2), wj = (wave >> 1) * (32 * NY);
 
-  // this thread's units of a slab: source (advancing by `psteps` / `qsteps` units per slab) and place in LDS
-  const f16x8 *ps[LOADS], *qs[LOADS];
-  int pd[LOADS], qd[LOADS];
-#pragma unroll
-  for (int u = 0; u < LOADS; ++u) {
-    const int id = threadIdx.x + 256 * u, row = id / 8, unit = id % 8;
-    ps[u] = reinterpret_cast<const f16x8 *>(P + (k * p.rp + i0 + row) * 2ll * depth) + unit;
-    pd[u] = row * 8 + (unit ^ swizzle(row));
-    if constexpr (TR) {  // 32 rows of T columns
-      const int qrow = id / (T / 4), qunit = id % (T / 4);
-      qs[u] = reinterpret_cast<const f16x8 *>(Q + (k * p.rp + qrow) * 2ll * cols + 2 * j0) + qunit;
-      qd[u] = qrow * (T / 4) + (qunit ^ swizzle(qrow));
-    } else {
-      qs[u] = reinterpret_cast<const f16x8 *>(Q + (k * p.rp + j0 + row) * 2ll * depth) + unit;
-      qd[u] = pd[u];
-    }
-  }
-  const long long qstep = TR ? 32ll * cols * 2 / 8 : 8;
+  // Operand slabs: THREADS / 8 rows of P (and Q) per pass, or, transposed, 4 THREADS / T rows of T columns.
+  // A unit's place in LDS is its own XOR a number of its row that spreads what one read touches over the banks:
+  // 16 rows of one unit, or, transposed, four rows of four neighbouring units.
+  const _Float16 *P = (MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.bp) + (k * p.rp + i0) * 2ll * depth;
+  const _Float16 *Q = MODE == POLY ? p.gp : p.yp[flip];
+  Q += TR ? k * p.rp * 2ll * cols + 2 * j0 : (k * p.rp + j0) * 2ll * depth;
+  const int prow = threadIdx.x / 8, punit = threadIdx.x % 8, qrow = threadIdx.x / (T / 4), qunit = threadIdx.x % (T / 4);
+  const int pv = (prow * 2 * depth + punit * 8) * 2, qv = TR ? (qrow * 2 * cols + qunit * 8) * 2 : pv;
+  const int ppass = (THREADS / 8) * 2 * depth * 2, qpass = TR ? (4 * THREADS / T) * 2 * cols * 2 : ppass;
+  auto row_swizzle = [](int row) { return (row >> 1) & 7; };
+  auto tr_swizzle = [](int row) { return (row & 3) * 4; };
+  const int pd = prow * 8 + (punit ^ row_swizzle(prow));
+  const int qd = TR ? qrow * (T / 4) + (qunit ^ tr_swizzle(qrow)) : pd;
+  const long long qslab = TR ? 32ll * 2 * cols : 64;
 
-  f32x16 acc[NB][NB];
+  f32x16 acc[NX][NY];
 #pragma unroll
-  for (int x = 0; x < NB; ++x)
+  for (int x = 0; x < NX; ++x)
 #pragma unroll
-    for (int y = 0; y < NB; ++y) acc[x][y] = zero16();
-  f16x8 pr[LOADS], qr[LOADS];
+    for (int y = 0; y < NY; ++y) acc[x][y] = zero16();
+  f16x8 pr[DIST][LOADS], qr[DIST][LOADS];
   const int slabs = depth / 32;
+  auto fetch = [&](int s, f16x8 (&x)[LOADS], f16x8 (&y)[LOADS]) {
+    s = min(s, slabs - 1);  // (behind the end: loaded and not used)
 #pragma unroll
-  for (int u = 0; u < LOADS; ++u) pr[u] = *ps[u], qr[u] = *qs[u];
+    for (int u = 0; u < LOADS; ++u) {
+      x[u] = load_unit(P + s * 64ll, pv, u * ppass);
+      y[u] = load_unit(Q + s * qslab, qv, u * qpass);
+    }
+  };
+  auto put = [&](int buf, const f16x8 (&x)[LOADS], const f16x8 (&y)[LOADS]) {
 #pragma unroll
-  for (int u = 0; u < LOADS; ++u) lds[0][0][pd[u]] = pr[u], lds[0][1][qd[u]] = qr[u];
+    for (int u = 0; u < LOADS; ++u) {
+      lds[buf][0][pd + THREADS * u] = x[u];
+      lds[buf][1][qd + THREADS * u] = y[u];
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DIST; ++d) fetch(d, pr[d], qr[d]);
+  put(0, pr[0], qr[0]);
+  fetch(DIST, pr[0], qr[0]);
   __syncthreads();
-  for (int s = 0; s < slabs; ++s) {
-    const bool more = s + 1 < slabs;
-    if (more) {
+  // slab s is in LDS, slabs s + 1 .. s + DIST are on their way, slab t in registers t % DIST.  The body has no
+  // branch: where loads may or may not have been issued the compiler waits for all of them.
+  auto multiply = [&](int s, int h) {
+    const f16x8 *lp = lds[s & 1][0], *lq = lds[s & 1][1];
+    f16x8 a[NX][2], b[NY][2];  // [block][part] of P (columns of the result tile's MFMA form) and Q
 #pragma unroll
-      for (int u = 0; u < LOADS; ++u) {
-        ps[u] += 8, qs[u] += qstep;
-        pr[u] = *ps[u], qr[u] = *qs[u];
+    for (int part = 0; part < 2; ++part) {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int row = wi + 32 * x + c;
+        a[x][part] = lp[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
+      }
+#pragma unroll
+      for (int y = 0; y < NY; ++y) {
+        if constexpr (TR) {
+          const int sub = (lane >> 4) & 1, k0 = 16 * h + 8 * g + ((lane & 15) >> 2);
+          const int unit = ((wj >> 5) + y) * 8 + 4 * part + 2 * sub + ((lane & 3) >> 1);
+          const _Float16 *base = reinterpret_cast<const _Float16 *>(lq) + 4 * (lane & 1);
+          b[y][part] = join(read_transposed(base + (k0 * (T / 4) + (unit ^ tr_swizzle(k0))) * 8),
+                            read_transposed(base + ((k0 + 4) * (T / 4) + (unit ^ tr_swizzle(k0 + 4))) * 8));
+        } else {
+          const int row = wj + 32 * y + c;
+          b[y][part] = lq[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
+        }
       }
     }
-    const f16x8 *lp = lds[s & 1][0], *lq = lds[s & 1][1];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f16x8 a[NB][2], b[NB][2];  // [block][part] of P (columns of the result tile's MFMA form) and Q
+    for (int x = 0; x < NX; ++x)
 #pragma unroll
-      for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          const int row = wi + 32 * x + c;
-          a[x][part] = lp[row * 8 + ((4 * part + 2 * h + g) ^ swizzle(row))];
-          if constexpr (TR) {
-            const int sub = (lane >> 4) & 1, k0 = 16 * h + 8 * g + ((lane & 15) >> 2);
-            const int unit = ((wj >> 5) + x) * 8 + 4 * part + 2 * sub + ((lane & 3) >> 1);
-            const _Float16 *base = reinterpret_cast<const _Float16 *>(lq) + 4 * (lane & 1);
-            b[x][part] = join(read_transposed(base + (k0 * (T / 4) + (unit ^ swizzle(k0))) * 8),
-                              read_transposed(base + ((k0 + 4) * (T / 4) + (unit ^ swizzle(k0 + 4))) * 8));
-          } else {
-            const int qrow = wj + 32 * x + c;
-            b[x][part] = lq[qrow * 8 + ((4 * part + 2 * h + g) ^ swizzle(qrow))];
-          }
-        }
-#pragma unroll
-      for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int y = 0; y < NB; ++y) acc[x][y] = product3(b[y][0], b[y][1], a[x][0], a[x][1], acc[x][y]);
-    }
-    if (more) {
-#pragma unroll
-      for (int u = 0; u < LOADS; ++u) lds[(s + 1) & 1][0][pd[u]] = pr[u], lds[(s + 1) & 1][1][qd[u]] = qr[u];
-    }
+      for (int y = 0; y < NY; ++y) acc[x][y] = product3(b[y][0], b[y][1], a[x][0], a[x][1], acc[x][y]);
+  };
+  auto step = [&](int s, f16x8 (&x)[LOADS], f16x8 (&y)[LOADS]) {
+    multiply(s, 0);
+    put((s + 1) & 1, x, y);
+    multiply(s, 1);
+    fetch(s + 1 + DIST, x, y);
     __syncthreads();
+  };
+  int s0 = 0;
+  for (; s0 + DIST <= slabs; s0 += DIST)
+#pragma unroll
+    for (int d = 0; d < DIST; ++d) step(s0 + d, pr[(d + 1) % DIST], qr[(d + 1) % DIST]);
+#pragma unroll
+  for (int d = 0; d + 1 < DIST; ++d)
+    if (s0 + d < slabs) step(s0 + d, pr[(d + 1) % DIST], qr[(d + 1) % DIST]);
+  // Epilogue by way of LDS, so that rows are read and written 512 bytes at a time.  Register 4 q + e of lane (c, g)
+  // is element (i = c, j = 8 q + 4 g + e) of a block.
+  constexpr int QUADS = T * T / 4 / THREADS, RQ = T / 4;  // quads of a thread, of a row
+  Parts add[QUADS];
+#pragma unroll
+  for (int u = 0; u < QUADS; ++u) {
+    const int quad = threadIdx.x + THREADS * u;
+    add[u] = addend<MODE>(p, flip, k, i0 + quad / RQ, j0 + quad % RQ * 4);
   }
-  // register 4 q + e of lane (c, g) is element (i = c, j = 8 q + 4 g + e) of a block
 #pragma unroll
-  for (int x = 0; x < NB; ++x)
+  for (int x = 0; x < NX; ++x)
 #pragma unroll
-    for (int y = 0; y < NB; ++y)
+    for (int y = 0; y < NY; ++y)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int i = i0 + wi + 32 * x + c, j = j0 + wj + 32 * y + 8 * q + 4 * g;
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * q + e];
-        v = finish<MODE>(p, flip, k, i, j, v);
-        if (LOWER && bi != bj) {
-          _Float16 *dst = MODE == GRAM ? p.gp : p.bp;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) store_split(dst + plane_at(k * p.rp + j + e, i, cols), v[e], kG);
-        }
+        *reinterpret_cast<f32x4 *>(sums + (wi + 32 * x + c) * SP + wj + 32 * y + 8 * q + 4 * g) = v;
       }
+  __syncthreads();
+  const bool turn = LOWER ? bi != bj : MODE == LAST && p.tall;  // (uniform)
+  f32x4 old[MODE == LAST ? QUADS : 1];
+  if constexpr (MODE == LAST) {
+#pragma unroll
+    for (int u = 0; u < QUADS; ++u) {
+      const int quad = threadIdx.x + THREADS * u;
+      if (!turn) old[u] = emit_old(p, k, i0 + quad / RQ, j0 + quad % RQ * 4);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < QUADS; ++u) {
+    const int quad = threadIdx.x + THREADS * u, i = quad / RQ, j = quad % RQ * 4;
+    f32x4 *at = reinterpret_cast<f32x4 *>(sums + i * SP + j);
+    const f32x4 v = finish<MODE>(p, flip, k, i0 + i, j0 + j, *at, add[u]);
+    if (turn)
+      *at = v;
+    else if constexpr (MODE == LAST)
+      emit4(p, k, i0 + i, j0 + j, v, old[u]);
+  }
+  if (!turn) return;
+  __syncthreads();
+  for (int block = threadIdx.x; block < RQ * RQ; block += THREADS) {  // 4 x 4 blocks, lanes along i
+    const int i = block % RQ * 4, j = block / RQ * 4;
+    f32x4 r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = *reinterpret_cast<const f32x4 *>(sums + (i + e) * SP + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      finish_transposed<MODE>(p, k, j0 + j + e, i0 + i, f32x4{r[0][e], r[1][e], r[2][e], r[3][e]});
+  }
 }
 
 // 32 x 32 tiles, a quarter of the contraction per wave, operands straight from memory.
@@ -430,7 +519,7 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
   const int ti = (p.r + 31) / 32, tj = TR ? (p.n + 31) / 32 : ti, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
   const long long k = blockIdx.x / tiles;
   int bi, bj;
-  tile_of<LOWER>(blockIdx.x % tiles, tj, bi, bj);
+  tile_of<LOWER>(blockIdx.x % tiles, ti, bi, bj);
   const int i0 = bi * 32, j0 = bj * 32;
   const _Float16 *P = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.bp;
   const _Float16 *Q = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.yp[flip];
@@ -441,6 +530,8 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
   const _Float16 *prow = P + (k * p.rp + i0 + c) * 2ll * depth + 8 * g;
   const _Float16 *qrow = TR ? Q + (k * p.rp + (lane >> 2)) * 2ll * cols + 2 * j0 + 8 * (lane & 3)
                             : Q + (k * p.rp + j0 + c) * 2ll * depth + 8 * g;
+  const int i = threadIdx.x >> 3, j = (threadIdx.x & 7) * 4;  // this thread's elements of the result
+  const Parts add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
   f32x16 acc = zero16();
   [[maybe_unused]] _Float16 *qt = reinterpret_cast<_Float16 *>(lds[wave]);
   for (int s = s0; s < s1; s += U) {
@@ -489,7 +580,6 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
     *reinterpret_cast<f32x4 *>(mine + c * SUM_PITCH + 8 * q + 4 * g) = v;
   }
   __syncthreads();
-  const int i = threadIdx.x >> 3, j = (threadIdx.x & 7) * 4;
   f32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -498,8 +588,8 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
     for (int x = 0; x < 4; ++x) w[x] = reinterpret_cast<const float *>(lds[x])[i * SUM_PITCH + j + e];
     v[e] = (w[0] + w[1]) + (w[2] + w[3]);
   }
-  v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v);
-  if (LOWER && bi != bj) {
+  v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v, add);
+  if (LOWER ? bi != bj : MODE == LAST && p.tall) {
     __syncthreads();
     float *turn = reinterpret_cast<float *>(lds[0]);
     *reinterpret_cast<f32x4 *>(turn + i * SUM_PITCH + j) = v;
@@ -507,7 +597,9 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
     f32x4 w;  // (j0 + i, i0 + j ..)
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = turn[(j + e) * SUM_PITCH + i];
-    store_split4((MODE == GRAM ? p.gp : p.bp) + plane_at(k * p.rp + j0 + i, i0 + j, cols), w, kG);
+    finish_transposed<MODE>(p, k, j0 + i, i0 + j, w);
+  } else if constexpr (MODE == LAST) {
+    emit4(p, k, i0 + i, j0 + j, v, emit_old(p, k, i0 + i, j0 + j));
   }
 }
 
@@ -633,7 +725,7 @@ int plan_form(int r, int n, int batch) {
   return FORM_SMALL;
 }
 
-// Workspace of one call: sums, then y, g (fp32), then the planes.
+// Workspace of one call: sums, then the planes (4 bytes an element).
 size_t plan(NsParams *p, float *workspace, int *form) {
   p->tall = p->rows > p->cols;
   p->r = p->tall ? p->cols : p->rows;
@@ -652,8 +744,6 @@ size_t plan(NsParams *p, float *workspace, int *form) {
     return r;
   };
   p->sums = reinterpret_cast<double *>(take(b * PARTS * sizeof(double)));
-  p->y = reinterpret_cast<float *>(take(yy * 4));
-  p->g = reinterpret_cast<float *>(take(gg * 4));
   for (auto *planes : {&p->yp[0], &p->yp[1]}) *planes = reinterpret_cast<_Float16 *>(take(yy * 4));
   for (auto *planes : {&p->gp, &p->bp}) *planes = reinterpret_cast<_Float16 *>(take(gg * 4));
   return used;
@@ -682,13 +772,13 @@ void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
   const int t = form == FORM_128 ? 128 : form == FORM_64 ? 64 : 32;
   const long long ti = (p.r + t - 1) / t, tj = (p.n + t - 1) / t;
   const long long total = p.batch * (MODE <= POLY ? ti * (ti + 1) / 2 : ti * tj);
-  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(256);
+  const dim3 grid((unsigned)((total + 7) / 8 * 8));
   if (form == FORM_128)
-    hipLaunchKernelGGL((ns_tile_kernel<MODE, 128>), grid, block, 0, st, p, flip, (int)total);
+    hipLaunchKernelGGL((ns_tile_kernel<MODE, 128, 8>), grid, dim3(512), 0, st, p, flip, (int)total);
   else if (form == FORM_64)
-    hipLaunchKernelGGL((ns_tile_kernel<MODE, 64>), grid, block, 0, st, p, flip, (int)total);
+    hipLaunchKernelGGL((ns_tile_kernel<MODE, 64, 4>), grid, dim3(256), 0, st, p, flip, (int)total);
   else
-    hipLaunchKernelGGL(ns_small_kernel<MODE>, dim3((unsigned)total), block, 0, st, p, flip);
+    hipLaunchKernelGGL(ns_small_kernel<MODE>, dim3((unsigned)total), dim3(256), 0, st, p, flip);
 }
 
 std::atomic<unsigned long long> g_one_lds{0};
