@@ -229,16 +229,18 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsParams p, int las
   const int t = blockIdx.x % tiles, i0 = t / tj * T, j0 = t % tj * T;
   const float norm = (float)sqrt(wave_sum(p.sums[k * PARTS + (threadIdx.x & 63)])) + p.eps;
   if (p.tall) {  // rows of the user's matrix are columns here
-    for (int u = threadIdx.x; u < T * T; u += 256) {
-      const int j = u / T, i = u % T;
+#pragma unroll
+    for (int w = 0; w < T * T / 256; ++w) {
+      const int u = threadIdx.x + 256 * w, j = u / T, i = u % T;
       float v = 0.f;
       if (i0 + i < p.r && j0 + j < p.n) v = update_value(p, k * p.stride_x + (j0 + j) * p.ld_x + i0 + i, false) / norm;
       tile[i][j] = v;
     }
     __syncthreads();
   }
-  for (int u = threadIdx.x; u < T * T / 4; u += 256) {
-    const int i = u / (T / 4), j = u % (T / 4) * 4;
+#pragma unroll
+  for (int w = 0; w < T * T / 4 / 256; ++w) {
+    const int u = threadIdx.x + 256 * w, i = u / (T / 4), j = u % (T / 4) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (p.tall) {
 #pragma unroll
@@ -506,15 +508,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const
   }
 }
 
-// 32 x 32 tiles, a quarter of the contraction per wave, operands straight from memory.
-template <int MODE>
-__global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int flip) {
+// 32 x 32 tiles, the contraction dealt to NW waves, operands straight from memory.
+template <int MODE, int NW>
+__global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int flip) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
   constexpr int U = TR ? 4 : 8;       // steps of 16 k in flight
   constexpr int PITCH = 80;           // fp16 pitch of a row of transposed operand (64 + a shift of 32 bytes)
   constexpr int SUM_PITCH = 36, REGION = TR ? U * 16 * PITCH * 2 : 32 * SUM_PITCH * 4;  // bytes of a wave
   static_assert(REGION >= 32 * SUM_PITCH * 4, "the wave's sums go where its operand was");
-  __shared__ __attribute__((aligned(16))) char lds[4][REGION];
+  __shared__ __attribute__((aligned(16))) char lds[NW][REGION];
   const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
   const int ti = (p.r + 31) / 32, tj = TR ? (p.n + 31) / 32 : ti, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
   const long long k = blockIdx.x / tiles;
@@ -525,13 +527,14 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
   const _Float16 *Q = MODE == GRAM ? p.yp[flip] : MODE == POLY ? p.gp : p.yp[flip];
   const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int steps = ((MODE == GRAM ? p.n : p.r) + 15) / 16, quarter = (steps + 3) / 4;  // k behind n / r is padding
-  const int s0 = min(wave * quarter, steps), s1 = min(s0 + quarter, steps);
+  const int steps = ((MODE == GRAM ? p.n : p.r) + 15) / 16, share = (steps + NW - 1) / NW;  // k behind n / r is padding
+  const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps);
   const _Float16 *prow = P + (k * p.rp + i0 + c) * 2ll * depth + 8 * g;
   const _Float16 *qrow = TR ? Q + (k * p.rp + (lane >> 2)) * 2ll * cols + 2 * j0 + 8 * (lane & 3)
                             : Q + (k * p.rp + j0 + c) * 2ll * depth + 8 * g;
   const int i = threadIdx.x >> 3, j = (threadIdx.x & 7) * 4;  // this thread's elements of the result
-  const Parts add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
+  Parts add = {};
+  if (threadIdx.x < 256) add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
   f32x16 acc = zero16();
   [[maybe_unused]] _Float16 *qt = reinterpret_cast<_Float16 *>(lds[wave]);
   for (int s = s0; s < s1; s += U) {
@@ -571,58 +574,79 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const NsParams p, int fli
 #pragma unroll
     for (int u = 0; u < U; ++u) acc = product3(b[u][0], b[u][1], a[u][0], a[u][1], acc);
   }
-  float *mine = reinterpret_cast<float *>(lds[wave]);
+  float *own = reinterpret_cast<float *>(lds[wave]);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     f32x4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e];
-    *reinterpret_cast<f32x4 *>(mine + c * SUM_PITCH + 8 * q + 4 * g) = v;
+    *reinterpret_cast<f32x4 *>(own + c * SUM_PITCH + 8 * q + 4 * g) = v;
   }
   __syncthreads();
-  f32x4 v;
+  const bool mine = threadIdx.x < 256;  // has elements of the result
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (mine) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float w[4];
+    for (int x = 0; x < NW; ++x) {
+      const f32x4 w = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds[x]) + i * SUM_PITCH + j);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) w[x] = reinterpret_cast<const float *>(lds[x])[i * SUM_PITCH + j + e];
-    v[e] = (w[0] + w[1]) + (w[2] + w[3]);
+      for (int e = 0; e < 4; ++e) v[e] += w[e];
+    }
+    v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v, add);
   }
-  v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v, add);
   if (LOWER ? bi != bj : MODE == LAST && p.tall) {
     __syncthreads();
     float *turn = reinterpret_cast<float *>(lds[0]);
-    *reinterpret_cast<f32x4 *>(turn + i * SUM_PITCH + j) = v;
+    if (mine) *reinterpret_cast<f32x4 *>(turn + i * SUM_PITCH + j) = v;
     __syncthreads();
+    if (!mine) return;
     f32x4 w;  // (j0 + i, i0 + j ..)
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = turn[(j + e) * SUM_PITCH + i];
     finish_transposed<MODE>(p, k, j0 + i, i0 + j, w);
   } else if constexpr (MODE == LAST) {
-    emit4(p, k, i0 + i, j0 + j, v, emit_old(p, k, i0 + i, j0 + j));
+    if (mine) emit4(p, k, i0 + i, j0 + j, v, emit_old(p, k, i0 + i, j0 + j));
   }
 }
 
-// Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; y stays in
-// registers, its planes and those of g and b g + c g g in LDS (64 KiB each).
+// Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of
+// y and of g, then b g + c g g, are in LDS (64 KiB each).
 __global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
   extern __shared__ __attribute__((aligned(16))) f16x8 one_lds[];
   __shared__ double red[16];
   const int tr = (p.r + 31) / 32, tn = (p.n + 31) / 32;  // blocks of 32 in use
   f16x8 *yl = one_lds, *gl = one_lds + tr * 32 * tn * 8;  // [row][column block][8 units]
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long k = blockIdx.x;
-  const int yi = wave / 4, yj = wave % 4;  // this wave's block of y and of g
-  const bool y_mine = yi < tr && yj < tn, g_mine = yi < tr && yj < tr;
-  float y[16];
+  // this wave's block of y, and of g on or below the diagonal
+  const int yi = wave / tn, yj = wave % tn;
+  const bool y_mine = yi < tr, g_mine = wave < tr * (tr + 1) / 2;
+  int gi, gj;
+  tile_of<true>(wave, tr, gi, gj);
+  float v[16];
   double s = 0.0;
+  {  // element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4 of the r x n form
+    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
+    const long long si = p.tall ? 1 : p.ld_x, sj = p.tall ? p.ld_x : 1, at = k * p.stride_x + i * si + j * sj;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int i = 32 * yi + c, j = 32 * yj + 8 * (e / 4) + 4 * g + e % 4;
-    y[e] = 0.f;
-    if (i < p.r && j < p.n) y[e] = update_value(p, k * p.stride_x + (p.tall ? j * p.ld_x + i : i * p.ld_x + j), true);
-    s += (double)y[e] * (double)y[e];
+    for (int e = 0; e < 16; ++e) {
+      const int d = 8 * (e / 4) + e % 4;
+      v[e] = i < p.r && j + d < p.n ? p.x[at + d * sj] : 0.f;
+    }
+    if (p.m) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = 8 * (e / 4) + e % 4;
+        if (i < p.r && j + d < p.n) {
+          const float gs = p.grad_scale * v[e], m = p.momentum * p.m[at + d * sj] + gs;
+          p.m[at + d * sj] = m;
+          v[e] = p.nesterov ? gs + p.momentum * m : m;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s += (double)v[e] * (double)v[e];
   }
   s = wave_sum(s);
   if (lane == 0) red[wave] = s;
@@ -634,12 +658,12 @@ __global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int i = 32 * yi + c, j = 32 * yj + 8 * (e / 4) + 4 * g + e % 4;
-    if (i < p.r && j < p.n) y[e] /= norm;
+    if (i < p.r && j < p.n) v[e] /= norm;
   }
-  // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout
-  auto store = [&](f16x8 *m, int blocks, const float (&v)[16], float scale) {
-    const int row = 32 * yi + c;
-    _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + yj) * 8);
+  // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout; and its mirror image
+  auto store = [&](f16x8 *m, int blocks, int bi, int bj, const float (&v)[16], float scale) {
+    const int row = 32 * bi + c;
+    _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + bj) * 8);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       f16x4 hi, lo;
@@ -653,63 +677,122 @@ __global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
       *reinterpret_cast<f16x4 *>(line + 8 * ((4 + q) ^ swizzle(row)) + 4 * g) = lo;
     }
   };
-  auto operand = [&](const f16x8 *m, int blocks, int block, int h, int part) {  // row `32 block + c`, k 16 h + 8 g ..
-    const int row = 32 * block + c;
-    return m[(row * blocks + (h >> 1)) * 8 + ((4 * part + 2 * (h & 1) + g) ^ swizzle(row))];
-  };
-  if (p.steps > 0 && y_mine) store(yl, tn, y, kY);
-  __syncthreads();
-  for (int step = 0; step < p.steps; ++step) {
-    float v[16], gv[16];
-    if (g_mine) {  // g = y y^T
-      f32x16 acc = zero16();
-#pragma unroll 1
-      for (int h = 0; h < 2 * tn; ++h)
-        acc = product3(operand(yl, tn, yj, h, 0), operand(yl, tn, yj, h, 1), operand(yl, tn, yi, h, 0),
-                       operand(yl, tn, yi, h, 1), acc);
+  auto store_mirrored = [&](f16x8 *m, int blocks, int bi, int bj, const float (&v)[16], float scale) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) gv[e] = acc[e] * (1.f / (kY * kY));
-      store(gl, tr, gv, kG);
+    for (int e = 0; e < 16; ++e) {
+      const int row = 32 * bj + 8 * (e / 4) + 4 * g + e % 4;
+      _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + bi) * 8);
+      _Float16 h, l;
+      split(v[e] * scale, h, l);
+      line[8 * ((c >> 3) ^ swizzle(row)) + (c & 7)] = h;
+      line[8 * ((4 + (c >> 3)) ^ swizzle(row)) + (c & 7)] = l;
+    }
+  };
+  // the elements of block (bi, bj) that the registers' layout gives this lane
+  auto load = [&](const f16x8 *m, int blocks, int bi, int bj, float scale, float (&v)[16]) {
+    const int row = 32 * bi + c;
+    const _Float16 *line = reinterpret_cast<const _Float16 *>(m + (row * blocks + bj) * 8);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f16x4 hi = *reinterpret_cast<const f16x4 *>(line + 8 * (q ^ swizzle(row)) + 4 * g);
+      const f16x4 lo = *reinterpret_cast<const f16x4 *>(line + 8 * ((4 + q) ^ swizzle(row)) + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = ((float)hi[e] + (float)lo[e]) * scale;
+    }
+  };
+  struct Operand {
+    f16x8 x[2][2];  // [16 k][part]
+  };
+  // row 32 block + c, columns of column block cb
+  auto rows = [&](const f16x8 *m, int blocks, int block, int cb) {
+    Operand o;
+    const int row = 32 * block + c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int part = 0; part < 2; ++part) o.x[h][part] = m[(row * blocks + cb) * 8 + ((4 * part + 2 * h + g) ^ swizzle(row))];
+    return o;
+  };
+  // columns 32 yj + c of y, rows of row block rb
+  auto columns = [&](int rb) {
+    Operand o;
+    const _Float16 *base = reinterpret_cast<const _Float16 *>(yl + yj * 8) + 4 * (lane & 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const int row = 32 * rb + 16 * h + 8 * g + ((lane & 15) >> 2);
+        const int unit = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        o.x[h][part] = join(read_transposed(base + (row * tn * 8 + (unit ^ swizzle(row))) * 8),
+                            read_transposed(base + ((row + 4) * tn * 8 + (unit ^ swizzle(row + 4))) * 8));
+      }
+    return o;
+  };
+  auto multiply = [&](const Operand &a, const Operand &b, f32x16 acc) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) acc = product3(a.x[h][0], a.x[h][1], b.x[h][0], b.x[h][1], acc);
+    return acc;
+  };
+  // sum over k of row blocks bi and bj of one matrix; the next operands are on their way behind each product
+  auto symmetric = [&](const f16x8 *m, int blocks, int bi, int bj) {
+    f32x16 acc = zero16();
+    Operand a = rows(m, blocks, bj, 0), b = rows(m, blocks, bi, 0);
+#pragma unroll 1
+    for (int cb = 1; cb < blocks; ++cb) {
+      const Operand na = rows(m, blocks, bj, cb), nb = rows(m, blocks, bi, cb);
+      acc = multiply(a, b, acc);
+      a = na, b = nb;
+    }
+    return multiply(a, b, acc);
+  };
+  if (p.steps > 0 && y_mine) store(yl, tn, yi, yj, v, kY);
+  __syncthreads();
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    // (the compiler would compute every address of the body before the loop and run out of registers)
+    asm volatile("" : "+v"(lane), "+v"(c), "+v"(g));
+    if (g_mine) {  // g = y y^T
+      const f32x16 acc = symmetric(yl, tn, gi, gj);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[e] * (1.f / (kY * kY));
+      store(gl, tr, gi, gj, v, kG);
+      if (gi != gj) store_mirrored(gl, tr, gi, gj, v, kG);
     }
     __syncthreads();
     if (g_mine) {  // b g + c g g
-      f32x16 acc = zero16();
-#pragma unroll 1
-      for (int h = 0; h < 2 * tr; ++h)
-        acc = product3(operand(gl, tr, yj, h, 0), operand(gl, tr, yj, h, 1), operand(gl, tr, yi, h, 0),
-                       operand(gl, tr, yi, h, 1), acc);
+      const f32x16 acc = symmetric(gl, tr, gi, gj);
+      load(gl, tr, gi, gj, 1.f / kG, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = p.b * gv[e] + p.c * (acc[e] * (1.f / (kG * kG)));
+      for (int e = 0; e < 16; ++e) v[e] = p.b * v[e] + p.c * (acc[e] * (1.f / (kG * kG)));
     }
     __syncthreads();
-    if (g_mine) store(gl, tr, v, kG);
+    if (g_mine) {
+      store(gl, tr, gi, gj, v, kG);
+      if (gi != gj) store_mirrored(gl, tr, gi, gj, v, kG);
+    }
     __syncthreads();
     if (y_mine) {  // y = a y + that y
       f32x16 acc = zero16();
-      const int sub = (lane >> 4) & 1, rr = (lane & 15) >> 2;
+      Operand a = columns(0), b = rows(gl, tr, yi, 0);
 #pragma unroll 1
-      for (int h = 0; h < 2 * tr; ++h) {
-        f16x8 b[2];
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          const int row = 16 * h + 8 * g + rr, unit = 4 * part + 2 * sub + ((lane & 3) >> 1);
-          const _Float16 *base = reinterpret_cast<const _Float16 *>(yl + yj * 8) + 4 * (lane & 1);
-          b[part] = join(read_transposed(base + (row * tn * 8 + (unit ^ swizzle(row))) * 8),
-                         read_transposed(base + ((row + 4) * tn * 8 + (unit ^ swizzle(row + 4))) * 8));
-        }
-        acc = product3(b[0], b[1], operand(gl, tr, yi, h, 0), operand(gl, tr, yi, h, 1), acc);
+      for (int rb = 1; rb < tr; ++rb) {
+        const Operand na = columns(rb), nb = rows(gl, tr, yi, rb);
+        acc = multiply(a, b, acc);
+        a = na, b = nb;
       }
+      acc = multiply(a, b, acc);
+      load(yl, tn, yi, yj, 1.f / kY, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) y[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
+      for (int e = 0; e < 16; ++e) v[e] = p.a * v[e] + acc[e] * (1.f / (kG * kY));
     }
-    __syncthreads();
     if (step + 1 < p.steps) {
-      if (y_mine) store(yl, tn, y, kY);
+      __syncthreads();
+      if (y_mine) store(yl, tn, yi, yj, v, kY);
       __syncthreads();
     }
   }
 #pragma unroll
-  for (int e = 0; e < 16; ++e) emit(p, k, 32 * yi + c, 32 * yj + 8 * (e / 4) + 4 * g + e % 4, y[e]);
+  for (int e = 0; e < 16; ++e) emit(p, k, 32 * yi + c, 32 * yj + 8 * (e / 4) + 4 * g + e % 4, v[e]);
 }
 
 // ------------------------------------------------------------------------------------------- plan
@@ -777,8 +860,10 @@ void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
     hipLaunchKernelGGL((ns_tile_kernel<MODE, 128, 8>), grid, dim3(512), 0, st, p, flip, (int)total);
   else if (form == FORM_64)
     hipLaunchKernelGGL((ns_tile_kernel<MODE, 64, 4>), grid, dim3(256), 0, st, p, flip, (int)total);
+  else if ((MODE == GRAM ? p.n : p.r) > (MODE >= APPLY ? 256 : 512))  // more than one batch of loads a wave with four
+    hipLaunchKernelGGL((ns_small_kernel<MODE, 8>), dim3((unsigned)total), dim3(512), 0, st, p, flip);
   else
-    hipLaunchKernelGGL(ns_small_kernel<MODE>, dim3((unsigned)total), dim3(256), 0, st, p, flip);
+    hipLaunchKernelGGL((ns_small_kernel<MODE, 4>), dim3((unsigned)total), dim3(256), 0, st, p, flip);
 }
 
 std::atomic<unsigned long long> g_one_lds{0};
