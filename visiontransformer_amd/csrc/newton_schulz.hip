@@ -59,9 +59,18 @@ struct NsParams {
 };
 
 // ------------------------------------------------------------------------------------- the planes
-__device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split4(f32x4 v, float scale, f16x4 &hi, f16x4 &lo) {  // two elements an instruction
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 x = {v[2 * h] * scale, v[2 * h + 1] * scale};
+    const f16x2 a = __builtin_convertvector(x, f16x2);
+    const f32x2 r = {x[0] - (float)a[0], x[1] - (float)a[1]};
+    const f16x2 b = __builtin_convertvector(r, f16x2);
+    hi[2 * h] = a[0], hi[2 * h + 1] = a[1];
+    lo[2 * h] = b[0], lo[2 * h + 1] = b[1];
+  }
 }
 // fp16 offset of the hi part of element (row, col) of a matrix of `cols` columns; the lo part lies 32 behind
 __device__ __forceinline__ long long plane_at(long long row, int col, int cols) {
@@ -69,25 +78,10 @@ __device__ __forceinline__ long long plane_at(long long row, int col, int cols) 
 }
 __device__ __forceinline__ void store_split4(_Float16 *at, f32x4 v, float scale) {
   f16x4 hi, lo;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    _Float16 h, l;
-    split(v[e] * scale, h, l);
-    hi[e] = h, lo[e] = l;
-  }
+  split4(v, scale, hi, lo);
   *reinterpret_cast<f16x4 *>(at) = hi;
   *reinterpret_cast<f16x4 *>(at + 32) = lo;
 }
-__device__ __forceinline__ void store_split(_Float16 *at, float v, float scale) {
-  _Float16 h, l;
-  split(v * scale, h, l);
-  at[0] = h;
-  at[32] = l;
-}
-// In LDS unit u of row `row` sits at u ^ swizzle(row): eight rows of one unit, and four rows of two
-// neighbouring units (a transposed read), then fall on different banks.
-__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
-
 // Transposed read: lane l of each 16 gets rows 0..3 of column l of the 4 x 16 block whose row l / 4,
 // columns 4 (l % 4) .. + 3, its address names.
 __device__ __forceinline__ f16x4 read_transposed(const _Float16 *at) {
@@ -609,123 +603,98 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   }
 }
 
-// Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of
-// y and of g, then b g + c g g, are in LDS (64 KiB each).
-__global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
+// Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of y
+// and of g, then b g + c g g, are in LDS (70 KiB each), what a wave adds to its products in registers.  All blocks of g are computed: writing a block's
+// mirror image, two bytes at a time, takes longer than its product.
+// A row of planes takes 3 mod 16 units of 16 bytes, so that 16 rows of one unit, and mostly four rows of four
+// neighbouring ones, are on different banks.
+constexpr int ONE_WAVES = 16;
+__host__ __device__ constexpr int one_pitch(int blocks) { return 8 * blocks + (blocks % 2 ? 11 : 3); }
+__global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p) {
   extern __shared__ __attribute__((aligned(16))) f16x8 one_lds[];
-  __shared__ double red[16];
+  __shared__ double red[ONE_WAVES];
   const int tr = (p.r + 31) / 32, tn = (p.n + 31) / 32;  // blocks of 32 in use
-  f16x8 *yl = one_lds, *gl = one_lds + tr * 32 * tn * 8;  // [row][column block][8 units]
+  const int yp = one_pitch(tn), gp = one_pitch(tr);
+  f16x8 *yl = one_lds, *gl = one_lds + tr * 32 * yp;  // [row][column block][8 units]
   int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long k = blockIdx.x;
-  // this wave's block of y, and of g on or below the diagonal
-  const int yi = wave / tn, yj = wave % tn;
-  const bool y_mine = yi < tr, g_mine = wave < tr * (tr + 1) / 2;
-  int gi, gj;
-  tile_of<true>(wave, tr, gi, gj);
-  float v[16];
+  // this wave's block of y and of g
+  const int yi = wave / tn, yj = wave % tn, gi = wave / tr, gj = wave % tr;
+  const bool y_mine = yi < tr, g_mine = gi < tr;
+  float y[16];
   double s = 0.0;
-  {  // element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4 of the r x n form
+  {  // element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4
     const int i = 32 * yi + c, j = 32 * yj + 4 * g;
     const long long si = p.tall ? 1 : p.ld_x, sj = p.tall ? p.ld_x : 1, at = k * p.stride_x + i * si + j * sj;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int d = 8 * (e / 4) + e % 4;
-      v[e] = i < p.r && j + d < p.n ? p.x[at + d * sj] : 0.f;
+      y[e] = i < p.r && j + d < p.n ? p.x[at + d * sj] : 0.f;
     }
     if (p.m) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int d = 8 * (e / 4) + e % 4;
         if (i < p.r && j + d < p.n) {
-          const float gs = p.grad_scale * v[e], m = p.momentum * p.m[at + d * sj] + gs;
+          const float gs = p.grad_scale * y[e], m = p.momentum * p.m[at + d * sj] + gs;
           p.m[at + d * sj] = m;
-          v[e] = p.nesterov ? gs + p.momentum * m : m;
+          y[e] = p.nesterov ? gs + p.momentum * m : m;
         }
       }
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s += (double)v[e] * (double)v[e];
+    for (int e = 0; e < 16; ++e) s += (double)y[e] * (double)y[e];
   }
   s = wave_sum(s);
   if (lane == 0) red[wave] = s;
   __syncthreads();
   s = 0.0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) s += red[w];
+  for (int w = 0; w < ONE_WAVES; ++w) s += red[w];
   const float norm = (float)sqrt(s) + p.eps;
+  {
+    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int i = 32 * yi + c, j = 32 * yj + 8 * (e / 4) + 4 * g + e % 4;
-    if (i < p.r && j < p.n) v[e] /= norm;
+    for (int e = 0; e < 16; ++e)
+      if (i < p.r && j + 8 * (e / 4) + e % 4 < p.n) y[e] /= norm;
   }
-  // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout; and its mirror image
-  auto store = [&](f16x8 *m, int blocks, int bi, int bj, const float (&v)[16], float scale) {
+  // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout
+  auto store = [&](f16x8 *m, int pitch, int bi, int bj, const float (&x)[16], float scale) {
     const int row = 32 * bi + c;
-    _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + bj) * 8);
+    _Float16 *line = reinterpret_cast<_Float16 *>(m + row * pitch + bj * 8);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       f16x4 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        _Float16 h, l;
-        split(v[4 * q + e] * scale, h, l);
-        hi[e] = h, lo[e] = l;
-      }
-      *reinterpret_cast<f16x4 *>(line + 8 * (q ^ swizzle(row)) + 4 * g) = hi;
-      *reinterpret_cast<f16x4 *>(line + 8 * ((4 + q) ^ swizzle(row)) + 4 * g) = lo;
-    }
-  };
-  auto store_mirrored = [&](f16x8 *m, int blocks, int bi, int bj, const float (&v)[16], float scale) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int row = 32 * bj + 8 * (e / 4) + 4 * g + e % 4;
-      _Float16 *line = reinterpret_cast<_Float16 *>(m + (row * blocks + bi) * 8);
-      _Float16 h, l;
-      split(v[e] * scale, h, l);
-      line[8 * ((c >> 3) ^ swizzle(row)) + (c & 7)] = h;
-      line[8 * ((4 + (c >> 3)) ^ swizzle(row)) + (c & 7)] = l;
-    }
-  };
-  // the elements of block (bi, bj) that the registers' layout gives this lane
-  auto load = [&](const f16x8 *m, int blocks, int bi, int bj, float scale, float (&v)[16]) {
-    const int row = 32 * bi + c;
-    const _Float16 *line = reinterpret_cast<const _Float16 *>(m + (row * blocks + bj) * 8);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f16x4 hi = *reinterpret_cast<const f16x4 *>(line + 8 * (q ^ swizzle(row)) + 4 * g);
-      const f16x4 lo = *reinterpret_cast<const f16x4 *>(line + 8 * ((4 + q) ^ swizzle(row)) + 4 * g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * q + e] = ((float)hi[e] + (float)lo[e]) * scale;
+      split4(f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, scale, hi, lo);
+      *reinterpret_cast<f16x4 *>(line + 8 * q + 4 * g) = hi;
+      *reinterpret_cast<f16x4 *>(line + 8 * (4 + q) + 4 * g) = lo;
     }
   };
   struct Operand {
     f16x8 x[2][2];  // [16 k][part]
   };
   // row 32 block + c, columns of column block cb
-  auto rows = [&](const f16x8 *m, int blocks, int block, int cb) {
+  auto rows = [&](const f16x8 *m, int pitch, int block, int cb) {
     Operand o;
-    const int row = 32 * block + c;
+    const f16x8 *at = m + (32 * block + c) * pitch + 8 * cb + g;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int part = 0; part < 2; ++part) o.x[h][part] = m[(row * blocks + cb) * 8 + ((4 * part + 2 * h + g) ^ swizzle(row))];
+      for (int part = 0; part < 2; ++part) o.x[h][part] = at[4 * part + 2 * h];
     return o;
   };
-  // columns 32 yj + c of y, rows of row block rb
-  auto columns = [&](int rb) {
+  // columns 32 cb + c of y, rows of row block rb
+  auto columns = [&](int rb, int cb) {
     Operand o;
-    const _Float16 *base = reinterpret_cast<const _Float16 *>(yl + yj * 8) + 4 * (lane & 1);
+    const _Float16 *at = reinterpret_cast<const _Float16 *>(yl + (32 * rb + 8 * g + ((lane & 15) >> 2)) * yp + 8 * cb) +
+                         16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const int row = 32 * rb + 16 * h + 8 * g + ((lane & 15) >> 2);
-        const int unit = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        o.x[h][part] = join(read_transposed(base + (row * tn * 8 + (unit ^ swizzle(row))) * 8),
-                            read_transposed(base + ((row + 4) * tn * 8 + (unit ^ swizzle(row + 4))) * 8));
-      }
+      for (int part = 0; part < 2; ++part)
+        o.x[h][part] = join(read_transposed(at + 16 * h * yp * 8 + 32 * part),
+                            read_transposed(at + (16 * h + 4) * yp * 8 + 32 * part));
     return o;
   };
   auto multiply = [&](const Operand &a, const Operand &b, f32x16 acc) {
@@ -734,65 +703,77 @@ __global__ __launch_bounds__(1024, 4) void ns_one_kernel(const NsParams p) {
     return acc;
   };
   // sum over k of row blocks bi and bj of one matrix; the next operands are on their way behind each product
-  auto symmetric = [&](const f16x8 *m, int blocks, int bi, int bj) {
+  auto symmetric = [&](const f16x8 *m, int pitch, int blocks, int bi, int bj) {
     f32x16 acc = zero16();
-    Operand a = rows(m, blocks, bj, 0), b = rows(m, blocks, bi, 0);
+    Operand a = rows(m, pitch, bj, 0), b = rows(m, pitch, bi, 0);
 #pragma unroll 1
     for (int cb = 1; cb < blocks; ++cb) {
-      const Operand na = rows(m, blocks, bj, cb), nb = rows(m, blocks, bi, cb);
+      const Operand na = rows(m, pitch, bj, cb), nb = rows(m, pitch, bi, cb);
       acc = multiply(a, b, acc);
       a = na, b = nb;
     }
     return multiply(a, b, acc);
   };
-  if (p.steps > 0 && y_mine) store(yl, tn, yi, yj, v, kY);
+  if (p.steps > 0) {
+      if (y_mine) store(yl, yp, yi, yj, y, kY);
+  }
   __syncthreads();
 #pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
     // (the compiler would compute every address of the body before the loop and run out of registers)
     asm volatile("" : "+v"(lane), "+v"(c), "+v"(g));
+    float v[16];
     if (g_mine) {  // g = y y^T
-      const f32x16 acc = symmetric(yl, tn, gi, gj);
+      const f32x16 acc = symmetric(yl, yp, tn, gi, gj);
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = acc[e] * (1.f / (kY * kY));
-      store(gl, tr, gi, gj, v, kG);
-      if (gi != gj) store_mirrored(gl, tr, gi, gj, v, kG);
+      store(gl, gp, gi, gj, v, kG);
     }
     __syncthreads();
     if (g_mine) {  // b g + c g g
-      const f32x16 acc = symmetric(gl, tr, gi, gj);
-      load(gl, tr, gi, gj, 1.f / kG, v);
+      const f32x16 acc = symmetric(gl, gp, tr, gi, gj);
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = p.b * v[e] + p.c * (acc[e] * (1.f / (kG * kG)));
     }
     __syncthreads();
-    if (g_mine) {
-      store(gl, tr, gi, gj, v, kG);
-      if (gi != gj) store_mirrored(gl, tr, gi, gj, v, kG);
-    }
+    if (g_mine) store(gl, gp, gi, gj, v, kG);
     __syncthreads();
     if (y_mine) {  // y = a y + that y
       f32x16 acc = zero16();
-      Operand a = columns(0), b = rows(gl, tr, yi, 0);
+      Operand x = columns(0, yj), w = rows(gl, gp, yi, 0);
 #pragma unroll 1
       for (int rb = 1; rb < tr; ++rb) {
-        const Operand na = columns(rb), nb = rows(gl, tr, yi, rb);
-        acc = multiply(a, b, acc);
-        a = na, b = nb;
+        const Operand nx = columns(rb, yj), nw = rows(gl, gp, yi, rb);
+        acc = multiply(x, w, acc);
+        x = nx, w = nw;
       }
-      acc = multiply(a, b, acc);
-      load(yl, tn, yi, yj, 1.f / kY, v);
+      acc = multiply(x, w, acc);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = p.a * v[e] + acc[e] * (1.f / (kG * kY));
+      for (int e = 0; e < 16; ++e) y[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
     }
     if (step + 1 < p.steps) {
       __syncthreads();
-      if (y_mine) store(yl, tn, yi, yj, v, kY);
+      if (y_mine) store(yl, yp, yi, yj, y, kY);
       __syncthreads();
     }
   }
+  {
+    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
+    const long long si = p.tall ? 1 : p.ld_out, sj = p.tall ? p.ld_out : 1, at = k * p.stride_out + i * si + j * sj;
+    if (p.p) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) emit(p, k, 32 * yi + c, 32 * yj + 8 * (e / 4) + 4 * g + e % 4, v[e]);
+      for (int e = 0; e < 16; ++e) {
+        const int d = 8 * (e / 4) + e % 4;
+        if (i < p.r && j + d < p.n) p.p[at + d * sj] = p.p[at + d * sj] * p.keep - p.step * y[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = 8 * (e / 4) + e % 4;
+        if (i < p.r && j + d < p.n) p.out[at + d * sj] = y[e];
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------- plan
@@ -874,13 +855,14 @@ int run(const char *who, NsParams *p, float *workspace, size_t bytes, hipStream_
   const dim3 block(256);
   if (form == FORM_ONE) {
     const int tr = (p->r + 31) / 32, tn = (p->n + 31) / 32;
-    const size_t lds = (size_t)tr * 32 * (tn + tr) * 128;
+    const size_t lds = (size_t)tr * 32 * (one_pitch(tn) + one_pitch(tr)) * 16;
     if (vitk::first_use_on_device(&g_one_lds)) {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(ns_one_kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 2 * ONE * ONE * 4);
+                                               hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               2 * ONE * one_pitch(ONE / 32) * 16);
       VITK_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(ns_one_kernel, dim3(p->batch), dim3(1024), lds, st, *p);
+    hipLaunchKernelGGL(ns_one_kernel, dim3(p->batch), dim3(64 * ONE_WAVES), lds, st, *p);
     return vitk::check_launch(who);
   }
   VITK_REQUIRE(workspace && bytes >= need, "%s: workspace of %zu bytes needed, %zu given", who, need,
