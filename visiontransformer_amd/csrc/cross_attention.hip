@@ -71,14 +71,28 @@ namespace {
 
 using namespace vitk::cross;
 
-constexpr int KT = 32;   // keys per tile
-constexpr int RB = 128;  // rows per workgroup
+// NW waves: RW groups of 32 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
+// stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
+// A stage is KT keys: loaded into registers one stage ahead, split and put into LDS between two barriers.
+template <int DH, int NW, int RW>
+struct Forward {
+  static constexpr int KW = NW / RW, KT = DH < 128 || KW > 1 ? 64 : 32, SUB = KT / 32 / KW;  // 32-key tiles of a wave
+  static constexpr int THREADS = 64 * NW, TASKS = KT * DH / 8 / THREADS;  // 8 columns of a key, per tensor and thread
+  static_assert(TASKS * THREADS * 8 == KT * DH, "a stage is dealt evenly");
+  static constexpr int UNITS = KT * Tile<DH>::ROW;
+  static constexpr int JOIN = KW > 1 ? RW * 64 * (DH / 2 + 2) * 4 : 0;  // bytes: o, m, l of the other key group
+  static constexpr int LDS = 2 * UNITS * 16 > JOIN ? 2 * UNITS * 16 : JOIN;
+};
 
-template <int DH>
-__global__ __launch_bounds__(256) void cross_fwd_kernel(const Params p) {
-  constexpr int LP = DH + 4, NB = DH / 32;
-  __shared__ __attribute__((aligned(16))) float kt[KT * LP], vt[KT * LP];
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
+template <int DH, int NW, int RW>
+__global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_fwd_kernel(const Params p) {
+  typedef Forward<DH, NW, RW> F;
+  typedef Tile<DH> T;
+  constexpr int NB = DH / 32, KS = DH / 16;
+  __shared__ __attribute__((aligned(16))) char lds[F::LDS];
+  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + F::UNITS;
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
   const int rb = (int)(wg % p.blocks);
   wg /= p.blocks;
@@ -87,73 +101,113 @@ __global__ __launch_bounds__(256) void cross_fwd_kernel(const Params p) {
   const int b = (int)(wg % p.B), split = (int)(wg / p.B);
   const int len = valid_keys(p, b);
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
-  const int row = rb * RB + wave * 32 + c;
+  const int row = (rb * RW + rg) * 32 + c;
   const bool row_ok = row < p.rows;
 
-  float qf[DH / 2];  // columns g*DH/2 .. of this lane's row
+  Split8 q[KS];  // this lane's row times scale log2(e), split
 #pragma unroll
-  for (int i = 0; i < DH / 2; i += 4) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (row_ok) x = load_quad(p.q.ptr + row_offset(p, p.q.ld, b, hk, row), g * (DH / 2) + i, p.dh, p.vec);
+  for (int i = 0; i < KS; ++i) {
+    float x[8] = {};
+    if (row_ok) load_eight(p.q.ptr + row_offset(p, p.q.ld, b, hk, row), 16 * i + 8 * g, p, x);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) qf[i + e] = x[e];
+    for (int e = 0; e < 8; ++e) x[e] *= p.c;
+    q[i] = split8(x);
   }
   f32x16 o[NB];
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  for (int n = 0; n < NB; ++n) o[n] = zero16();
   float m = -INFINITY, l = 0.f;
 
-  for (int t = k0; t < k1; t += KT) {
-    __syncthreads();
+  float kx[F::TASKS][8], vx[F::TASKS][8];
+  auto fetch = [&](int t) {
 #pragma unroll
-    for (int u = 0; u < DH / 32; ++u) {
-      const int quad = threadIdx.x + 256 * u, key = quad / (DH / 4), d = 4 * (quad % (DH / 4));
-      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-      if (t + key < k1) {
-        x = load_quad(p.k.ptr + key_offset(p, p.k.ld, b, hk, t + key), d, p.dh, p.vec);
-        y = load_quad(p.v.ptr + key_offset(p, p.v.ld, b, hk, t + key), d, p.dh, p.vec);
+    for (int u = 0; u < F::TASKS; ++u) {
+      const int task = threadIdx.x + F::THREADS * u, key = t + task / (DH / 8), d = task % (DH / 8) * 8;
+      if (key < k1) {
+        load_eight(p.k.ptr + key_offset(p, p.k.ld, b, hk, key), d, p, kx[u]);
+        load_eight(p.v.ptr + key_offset(p, p.v.ld, b, hk, key), d, p, vx[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) kx[u][e] = vx[u][e] = 0.f;
       }
-      *reinterpret_cast<f32x4 *>(kt + key * LP + d) = x;
-      *reinterpret_cast<f32x4 *>(vt + key * LP + d) = y;
+    }
+  };
+  if (k0 < k1) fetch(k0);
+  for (int t = k0; t < k1; t += F::KT) {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < F::TASKS; ++u) {
+      const int task = threadIdx.x + F::THREADS * u;
+      T::put(kt, task / (DH / 8), task % (DH / 8), split8(kx[u]));
+      T::put(vt, task / (DH / 8), task % (DH / 8), split8(vx[u]));
     }
     __syncthreads();
-    f32x16 s;
+    if (t + F::KT < k1) fetch(t + F::KT);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    for (int sub = 0; sub < F::SUB; ++sub) {
+      const int first = 32 * (kg * F::SUB + sub);  // of the stage
+      if (t + first >= k1) break;
+      f32x16 s = zero16();
 #pragma unroll
-    for (int i = 0; i < DH / 2; i += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4 *>(kt + c * LP + g * (DH / 2) + i);
+      for (int i = 0; i < KS; ++i) s = product6(T::rows(kt, first + c, i, g), q[i], s);
+      if (t + first + 32 > k1) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[i + e], s, 0, 0, 0);
+        for (int i = 0; i < 16; ++i)
+          if (t + first + 8 * (i / 4) + 4 * g + i % 4 >= k1) s[i] = -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m_new = fmaxf(m, top);
+      if (__any(m_new != m)) {  // (NaN scores: l and o become NaN below)
+        const float fall = __builtin_amdgcn_exp2f(m - m_new);
+        l *= fall;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[n][i] *= fall;
+        m = m_new;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(s[i] - m);
+        sum += s[i];
+      }
+      l += sum;  // of this lane's half of the keys
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Split8 x = split_half(s, h);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n] = product6(T::columns(vt, first + 16 * h, n, lane), x, o[n]);
+      }
     }
-    float top = -INFINITY;
+  }
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (F::KW > 1) {
+    static_assert(F::KW == 2, "two key groups");
+    float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 2 + 2) + lane;
+    __syncthreads();
+    if (kg == 1) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = t + 8 * (i / 4) + 4 * g + i % 4;
-      s[i] = key < k1 ? s[i] * p.c : -INFINITY;
-      top = fmaxf(top, s[i]);
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) box[(16 * n + i) * 64] = o[n][i];
+      box[(DH / 2) * 64] = m;
+      box[(DH / 2 + 1) * 64] = l;
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m_new = fmaxf(m, top);
-    const float fall = __builtin_amdgcn_exp2f(m - m_new);
-    float sum = 0.f;
+    __syncthreads();
+    if (kg == 1) return;
+    const float m2 = box[(DH / 2) * 64], l2 = box[(DH / 2 + 1) * 64], top = fmaxf(m, m2);
+    if (top > -INFINITY) {
+      const float f1 = __builtin_amdgcn_exp2f(m - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
+      l = l * f1 + l2 * f2;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] - m_new);
-      sum += s[i];
-    }
-    sum += __shfl_xor(sum, 32, 64);
-    l = l * fall + sum;
-    m = m_new;
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][i] *= fall;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vt[(8 * (i / 4) + 4 * g + i % 4) * LP + 32 * n + c], s[i], o[n], 0, 0, 0);
+        for (int i = 0; i < 16; ++i) o[n][i] = o[n][i] * f1 + box[(16 * n + i) * 64] * f2;
+      m = top;
     }
   }
   if (!row_ok) return;
@@ -167,7 +221,7 @@ __global__ __launch_bounds__(256) void cross_fwd_kernel(const Params p) {
   } else {
     dst = p.out.ptr + row_offset(p, p.out.ld, b, hk, row);
     st = p.stats ? p.stats + stat * 2 : nullptr;
-    f = l > 0.f || l != l ? 1.f / l : 0.f;
+    f = l == 0.f ? 0.f : 1.f / l;
     if (l == 0.f) m = 0.f;
   }
 #pragma unroll
@@ -214,20 +268,33 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
   }
 }
 
-// Row blocks, and over how many workgroups the keys of one block are split.
-void plan_fwd(Params *p) {
-  p->blocks = (p->rows + RB - 1) / RB;
+// Rows per workgroup, and over how many workgroups the keys of one block are split.
+constexpr int CHUNK = 64;  // key ranges of splits are whole stages
+int plan_fwd(Params *p) {
+  const int row_groups = p->rows > 64 ? 4 : p->rows > 32 ? 2 : 1;
+  p->blocks = (int)(((long long)p->rows + 32 * row_groups - 1) / (32 * row_groups));
   const long long groups = (long long)p->B * p->Hkv * p->blocks;
   long long splits = 1;
   if (groups > 0) splits = 2ll * vitk::cu_count() / groups;
-  const long long tiles = (p->Nk + KT - 1) / KT;
-  if (splits > tiles / 4) splits = tiles / 4;
+  const long long stages = ((long long)p->Nk + CHUNK - 1) / CHUNK;
+  if (splits > stages / 4) splits = stages / 4;
   if (splits > 64) splits = 64;
   if (splits < 1) splits = 1;
-  p->chunk = (int)((tiles + splits - 1) / splits) * KT;
-  if (p->chunk == 0) p->chunk = KT;
-  p->splits = (p->Nk + p->chunk - 1) / p->chunk;
+  p->chunk = (int)((stages + splits - 1) / splits) * CHUNK;
+  if (p->chunk == 0) p->chunk = CHUNK;
+  p->splits = (int)(((long long)p->Nk + p->chunk - 1) / p->chunk);
   if (p->splits < 1) p->splits = 1;
+  return row_groups;
+}
+
+template <int DH>
+void launch_fwd(const Params &p, int row_groups, unsigned wgs, hipStream_t st) {
+  if (row_groups == 4)
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
+  else if (row_groups == 2)
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
 }
 
 size_t fwd_bytes(const Params &p) {
@@ -250,7 +317,7 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   Params p = {};
   if (check_args("vitk_cross_sdpa_fwd", a, false, &p)) return 1;
   if (p.B == 0 || p.Nq == 0) return 0;
-  plan_fwd(&p);
+  const int row_groups = plan_fwd(&p);
   const size_t need = fwd_bytes(p);
   VITK_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
                "vitk_cross_sdpa_fwd: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
@@ -259,19 +326,18 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   const long long wgs = (long long)p.B * p.Hkv * p.blocks * p.splits;
   VITK_REQUIRE(wgs < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
   hipStream_t st = vitk::as_stream(stream);
-  const dim3 grid((unsigned)wgs), block(256);
   if (p.dh <= 32)
-    hipLaunchKernelGGL(cross_fwd_kernel<32>, grid, block, 0, st, p);
+    launch_fwd<32>(p, row_groups, (unsigned)wgs, st);
   else if (p.dh <= 64)
-    hipLaunchKernelGGL(cross_fwd_kernel<64>, grid, block, 0, st, p);
+    launch_fwd<64>(p, row_groups, (unsigned)wgs, st);
   else if (p.dh <= 96)
-    hipLaunchKernelGGL(cross_fwd_kernel<96>, grid, block, 0, st, p);
+    launch_fwd<96>(p, row_groups, (unsigned)wgs, st);
   else
-    hipLaunchKernelGGL(cross_fwd_kernel<128>, grid, block, 0, st, p);
+    launch_fwd<128>(p, row_groups, (unsigned)wgs, st);
   if (p.splits > 1) {
     const long long all = (long long)p.B * p.H * p.Nq;
     VITK_REQUIRE((all + 3) / 4 < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
-    hipLaunchKernelGGL(cross_join_kernel, dim3((unsigned)((all + 3) / 4)), block, 0, st, p);
+    hipLaunchKernelGGL(cross_join_kernel, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
   }
   return vitk::check_launch("vitk_cross_sdpa_fwd");
 }
