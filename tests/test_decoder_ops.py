@@ -104,6 +104,11 @@ ATTENTION = {
     "one_by_one": (1, 1, 1, 1, 1, 1, None, 0, 0),
     "token_over_197": (4, 12, 12, 1, 197, 64, None, 0, 0),
     "token_shared_heads_long": (3, 8, 2, 1, 5001, 128, [5001, 0, 1234], 0, 0),
+    "token_three_rows_dh_24": (2, 6, 2, 1, 700, 24, [700, 3], 0, 0),
+    "few_rows_of_two_tokens": (2, 8, 4, 3, 129, 96, [0, 129], 4, 0),
+    "eight_rows_split": (1, 8, 1, 1, 4000, 128, None, 0, 0),
+    "many_heads_no_split": (48, 12, 12, 1, 1500, 32, None, 0, 0),
+    "nine_rows": (2, 9, 1, 1, 2100, 64, [2100, 65], 0, 0),
     "token_all_heads_share_one": (2, 7, 1, 1, 333, 48, [1, 332], 4, 0),
     "prompt": (2, 3, 3, 33, 197, 64, None, 0, 0),
     "one_key": (3, 4, 4, 70, 1, 64, None, 0, 0),

@@ -8,7 +8,9 @@
 // keys with a running maximum and sum per row.
 #include "cross_attention.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace vitk {
 namespace cross {
@@ -239,52 +241,236 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_fwd_kernel(co
   }
 }
 
-// Joins the parts of a split row: one wave per row, lanes over the columns.
+// Joins the parts of a split row: one wave per row, a lane per part for the statistics, then lanes over the columns.
+constexpr int MAX_SPLITS = 64;
 __global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
   const long long all = (long long)p.B * p.H * p.Nq;
   const int lane = threadIdx.x & 63;
   const long long r = blockIdx.x * 4ll + (threadIdx.x >> 6);
   if (r >= all) return;
   const float *st = p.part + p.splits * all * p.dh;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, st[(s * all + r) * 2]);
-  if (m == -INFINITY) m = 0.f;  // no key at all
-  float l = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(st[(s * all + r) * 2] - m);
-    l += f * st[(s * all + r) * 2 + 1];
-    const float *src = p.part + (s * all + r) * p.dh;
-    if (lane < p.dh) x0 += f * src[lane];
-    if (lane + 64 < p.dh) x1 += f * src[lane + 64];
+  float m = -INFINITY, l = 0.f;
+  if (lane < p.splits) {
+    m = st[(lane * all + r) * 2];
+    l = st[(lane * all + r) * 2 + 1];
   }
-  const float f = l == 0.f ? 0.f : 1.f / l;
+  float top = vitk::wave_max(m);
+  if (top == -INFINITY) top = 0.f;  // no key at all
+  const float f = __builtin_amdgcn_exp2f(m - top);
+  l = vitk::wave_sum(l * f);
+  float x0 = 0.f, x1 = 0.f;
+  const float *src = p.part + r * p.dh + lane;
+  for (int s = 0; s < p.splits; s += 8) {  // eight parts in flight
+    float a[8], b[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool in = s + u < p.splits;
+      a[u] = in && lane < p.dh ? src[(s + u) * all * p.dh] : 0.f;
+      b[u] = in && lane + 64 < p.dh ? src[(s + u) * all * p.dh + 64] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float fs = __shfl(f, (s + u) & 63, 64);  // (parts behind the last one: 0 times something finite)
+      x0 += fs * a[u];
+      x1 += fs * b[u];
+    }
+  }
+  const float scale = l == 0.f ? 0.f : 1.f / l;
   const long long bh = r / p.Nq, n = r % p.Nq, b = bh / p.H, h = bh % p.H;
   float *dst = p.out.ptr + (b * p.Nq + n) * p.out.ld + h * p.dh;
-  if (lane < p.dh) dst[lane] = x0 * f;
-  if (lane + 64 < p.dh) dst[lane + 64] = x1 * f;
+  if (lane < p.dh) dst[lane] = x0 * scale;
+  if (lane + 64 < p.dh) dst[lane + 64] = x1 * scale;
   if (lane == 0 && p.stats) {
-    p.stats[2 * r] = m;
+    p.stats[2 * r] = top;
     p.stats[2 * r + 1] = l;
   }
 }
 
-// Rows per workgroup, and over how many workgroups the keys of one block are split.
-constexpr int CHUNK = 64;  // key ranges of splits are whole stages
-int plan_fwd(Params *p) {
-  const int row_groups = p->rows > 64 ? 4 : p->rows > 32 ? 2 : 1;
-  p->blocks = (int)(((long long)p->rows + 32 * row_groups - 1) / (32 * row_groups));
-  const long long groups = (long long)p->B * p->Hkv * p->blocks;
+// ------------------------------------------------------------------------------------- few rows
+// At most 8 rows per key head (single tokens): every key and value is read once and used for at most 8 dot
+// products, so memory bounds this and the vector ALU computes it.  LP lanes share a key, four columns each;
+// 64 / LP keys per wave and U of those in flight.  Each group of LP lanes keeps a running maximum and
+// sum per row of its own; groups, then waves, are joined at the end.
+template <int LP>
+__device__ __forceinline__ float group_sum(float x) {  // over LP neighbouring lanes, in all of them
+  auto add = [&](auto ctrl) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl.value, 0xf, 0xf, true));
+  };
+  add(std::integral_constant<int, 0xB1>());   // neighbours
+  add(std::integral_constant<int, 0x4E>());   // pairs
+  add(std::integral_constant<int, 0x141>());  // mirrored halves of a row of 16
+  if constexpr (LP >= 16) add(std::integral_constant<int, 0x140>());  // mirrored rows
+  if constexpr (LP >= 32)  // lane ^ 16
+    x += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), 0x401F));
+  return x;
+}
+
+// load_quad of what nobody reads again
+__device__ __forceinline__ f32x4 stream_quad(const float *row, int d, int dh, bool vec) {
+  if (!vec) return load_quad(row, d, dh, false);
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+  if (d < dh) r = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + d));
+  return r;
+}
+
+template <int LP, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
+  constexpr int U = 4, KEYS = 64 / LP, DP = 4 * LP;
+  __shared__ float box[NW][R][DP + 2];
+  const int lane = threadIdx.x & 63, li = lane % LP, lg = lane / LP, d = 4 * li;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  long long wg = blockIdx.x;
+  const int hk = (int)(wg % p.Hkv);
+  wg /= p.Hkv;
+  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int len = valid_keys(p, b);
+  const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
+  f32x4 q[R], o[R];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    q[r] = o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[r] = -INFINITY, l[r] = 0.f;
+    if (r < p.rows) {
+      q[r] = load_quad(p.q.ptr + row_offset(p, p.q.ld, b, hk, r), d, p.dh, p.vec);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[r][e] *= p.c;
+    }
+  }
+  const float *kp = p.k.ptr + key_offset(p, p.k.ld, b, hk, 0), *vp = p.v.ptr + key_offset(p, p.v.ld, b, hk, 0);
+  for (int t = k0 + wave * KEYS * U; t < k1; t += NW * KEYS * U) {
+    f32x4 k[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = t + u * KEYS + lg;
+      k[u] = v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (key < k1) {
+        k[u] = stream_quad(kp + key * p.k.ld, d, p.dh, p.vec);
+        v[u] = stream_quad(vp + key * p.v.ld, d, p.dh, p.vec);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float s[U], top = m[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = group_sum<LP>((q[r][0] * k[u][0] + q[r][1] * k[u][1]) + (q[r][2] * k[u][2] + q[r][3] * k[u][3]));
+        if (t + u * KEYS + lg >= k1) s[u] = -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      const float base = top == -INFINITY ? 0.f : top, fall = __builtin_amdgcn_exp2f(m[r] - base);
+      m[r] = top;
+      l[r] *= fall;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][e] *= fall;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float x = __builtin_amdgcn_exp2f(s[u] - base);
+        l[r] += x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][e] += x * v[u][e];
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int off = LP; off < 64; off <<= 1) {
+      const float m2 = __shfl_xor(m[r], off, 64), l2 = __shfl_xor(l[r], off, 64);
+      const float top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.f : top;
+      const float f1 = __builtin_amdgcn_exp2f(m[r] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+      l[r] = l[r] * f1 + l2 * f2;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][e] = o[r][e] * f1 + __shfl_xor(o[r][e], off, 64) * f2;
+      m[r] = top;
+    }
+    if (lg == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) box[wave][r][d + e] = o[r][e];
+      if (li == 0) box[wave][r][DP] = m[r], box[wave][r][DP + 1] = l[r];
+    }
+  }
+  __syncthreads();
+  const long long all = (long long)p.B * p.H * p.Nq;
+  for (int i = threadIdx.x; i < R * DP; i += 64 * NW) {
+    const int r = i / DP, col = i % DP;
+    if (r >= p.rows || col >= p.dh) continue;
+    float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, box[w][r][DP]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(box[w][r][DP] - base);
+      sum += f * box[w][r][DP + 1];
+      x += f * box[w][r][col];
+    }
+    const long long stat = row_stat(p, b, hk, r);
+    if (p.splits > 1) {
+      p.part[(split * all + stat) * p.dh + col] = x;
+      float *st = p.part + p.splits * all * p.dh + (split * all + stat) * 2;
+      if (col == 0) st[0] = top, st[1] = sum;
+    } else {
+      p.out.ptr[row_offset(p, p.out.ld, b, hk, r) + col] = sum == 0.f ? 0.f : x / sum;
+      if (col == 0 && p.stats) p.stats[2 * stat] = base, p.stats[2 * stat + 1] = sum;
+    }
+  }
+}
+
+// The kernel, the rows of a workgroup, and over how many workgroups the keys of a block are split.
+constexpr int CHUNK = 64;      // key ranges of splits are multiples of this
+constexpr int FEW_ROWS = 8;    // rows per key head up to which the vector kernel runs
+struct FwdPlan {
+  int row_groups;  // of 32 rows; 0 = the vector kernel
+  int waves;       // of the vector kernel
+};
+FwdPlan plan_fwd(Params *p) {
+  FwdPlan f = {};
+  const long long heads = (long long)p->B * p->Hkv, stages = ((long long)p->Nk + CHUNK - 1) / CHUNK;
   long long splits = 1;
-  if (groups > 0) splits = 2ll * vitk::cu_count() / groups;
-  const long long stages = ((long long)p->Nk + CHUNK - 1) / CHUNK;
-  if (splits > stages / 4) splits = stages / 4;
-  if (splits > 64) splits = 64;
+  if (p->rows <= FEW_ROWS) {
+    p->blocks = 1;
+    f.waves = 4;
+    const long long cus = vitk::cu_count();
+    if (heads < 2 * cus) {
+      if (p->Nk <= 1024)
+        f.waves = 16;  // one launch: a split's join costs more than it saves
+      else if (heads > 0)
+        splits = std::min((8 * cus + heads - 1) / heads, stages / 4);
+    }
+  } else {
+    f.row_groups = p->rows > 64 ? 4 : p->rows > 32 ? 2 : 1;
+    p->blocks = (int)(((long long)p->rows + 32 * f.row_groups - 1) / (32 * f.row_groups));
+    const long long groups = heads * p->blocks;
+    if (groups > 0) splits = std::min(2ll * vitk::cu_count() / groups, stages / 4);
+  }
+  if (splits > MAX_SPLITS) splits = MAX_SPLITS;
   if (splits < 1) splits = 1;
   p->chunk = (int)((stages + splits - 1) / splits) * CHUNK;
   if (p->chunk == 0) p->chunk = CHUNK;
   p->splits = (int)(((long long)p->Nk + p->chunk - 1) / p->chunk);
   if (p->splits < 1) p->splits = 1;
-  return row_groups;
+  return f;
+}
+
+template <int LP, int NW>
+void launch_rows(const Params &p, unsigned wgs, hipStream_t st) {
+  const dim3 grid(wgs), block(64 * NW);
+  if (p.rows == 1)
+    hipLaunchKernelGGL((cross_row_kernel<LP, 1, NW>), grid, block, 0, st, p);
+  else if (p.rows == 2)
+    hipLaunchKernelGGL((cross_row_kernel<LP, 2, NW>), grid, block, 0, st, p);
+  else if (p.rows <= 4)
+    hipLaunchKernelGGL((cross_row_kernel<LP, 4, NW>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((cross_row_kernel<LP, 8, NW>), grid, block, 0, st, p);
+}
+template <int LP>
+void launch_rows(const Params &p, int waves, unsigned wgs, hipStream_t st) {
+  if (waves == 4)
+    launch_rows<LP, 4>(p, wgs, st);
+  else
+    launch_rows<LP, 16>(p, wgs, st);
 }
 
 template <int DH>
@@ -317,7 +503,7 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   Params p = {};
   if (check_args("vitk_cross_sdpa_fwd", a, false, &p)) return 1;
   if (p.B == 0 || p.Nq == 0) return 0;
-  const int row_groups = plan_fwd(&p);
+  const FwdPlan plan = plan_fwd(&p);
   const size_t need = fwd_bytes(p);
   VITK_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
                "vitk_cross_sdpa_fwd: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
@@ -326,14 +512,24 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   const long long wgs = (long long)p.B * p.Hkv * p.blocks * p.splits;
   VITK_REQUIRE(wgs < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
   hipStream_t st = vitk::as_stream(stream);
-  if (p.dh <= 32)
-    launch_fwd<32>(p, row_groups, (unsigned)wgs, st);
-  else if (p.dh <= 64)
-    launch_fwd<64>(p, row_groups, (unsigned)wgs, st);
-  else if (p.dh <= 96)
-    launch_fwd<96>(p, row_groups, (unsigned)wgs, st);
-  else
-    launch_fwd<128>(p, row_groups, (unsigned)wgs, st);
+  const int rg = plan.row_groups;
+  const unsigned grid = (unsigned)wgs;
+  if (rg == 0) {
+    if (p.dh <= 32)
+      launch_rows<8>(p, plan.waves, grid, st);
+    else if (p.dh <= 64)
+      launch_rows<16>(p, plan.waves, grid, st);
+    else
+      launch_rows<32>(p, plan.waves, grid, st);
+  } else if (p.dh <= 32) {
+    launch_fwd<32>(p, rg, grid, st);
+  } else if (p.dh <= 64) {
+    launch_fwd<64>(p, rg, grid, st);
+  } else if (p.dh <= 96) {
+    launch_fwd<96>(p, rg, grid, st);
+  } else {
+    launch_fwd<128>(p, rg, grid, st);
+  }
   if (p.splits > 1) {
     const long long all = (long long)p.B * p.H * p.Nq;
     VITK_REQUIRE((all + 3) / 4 < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
