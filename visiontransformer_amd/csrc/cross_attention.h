@@ -31,7 +31,9 @@ struct Params {
   const int32_t *len;
   float *stats;  // [B*H][Nq][2]
   float *delta;  // backward: [B*H][Nq] dout . out
-  float *part;   // forward, keys split: [splits][B*H][Nq][dh] unnormalised sums, then [splits][B*H][Nq][2]
+  // forward, keys split: [splits][B*H][Nq][dh] unnormalised sums, then [splits][B*H][Nq][2];
+  // backward, keys or rows split: [splits][B][N][heads][dh] of one gradient (of dk, then of dv)
+  float *part;
   int B, H, Hkv, G, Nq, Nk, dh;
   int rows;      // G * Nq: the query rows that share one key head, head by head
   int blocks;    // row (or key) blocks per (batch, key head)

@@ -1,77 +1,106 @@
-// Cross attention backward, three launches without atomics:
-//   delta[row] = dout . out
-//   dK, dV: one workgroup per 128 keys of one (batch, key head), all rows that read them in order
-//   dQ:     one workgroup per 128 rows, all keys in order
-// Both main kernels rebuild the probabilities from the stored row statistics,
+// Cross attention backward without atomics:
+//   dQ (and delta[row] = dout . out): one workgroup per block of rows, all keys in order;
+//   dK, dV: one workgroup per block of keys of one (batch, key head), all rows that read them in order.
+// Both rebuild the probabilities from the stored row statistics,
 //   p = exp2(c s - m) / l,  ds = p (dout v^T - delta),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T dout,
-// with products on v_mfma_f32_32x32x2_f32 arranged as in the forward: the accumulator of the first
-// product is the operand of the next.
+// with fp32 products in three bf16 parts arranged as in the forward: the accumulator of the first
+// product is the operand of the next.  That is seven products where five would do (s and dp are formed
+// twice); one pass would have to add dQ (or dK and dV) up across workgroups.
+// Blocks of up to 128 rows (keys); with fewer, two waves share a 32-wide group and deal the tiles of the
+// other side.  Where the blocks are too few for the device, the other side is split over workgroups and
+// the parts are added in order by a second launch.
 #include "cross_attention.h"
+
+#include <algorithm>
 
 namespace {
 
 using namespace vitk::cross;
 
-constexpr int RB = 128;  // rows (dQ) or keys (dK, dV) per workgroup
+// NW waves, GROUPS of 32 rows (dQ) or keys (dK, dV); OTHER = waves that deal the tiles of a stage.
+template <int DH, int NW, int GROUPS>
+struct Shape {
+  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 128 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
+  static constexpr int THREADS = 64 * NW, TASKS = STAGE * DH / 8 / THREADS;  // 8 columns, per tensor and thread
+  static_assert(TASKS * THREADS * 8 == STAGE * DH, "a stage is dealt evenly");
+  static constexpr int UNITS = STAGE * Tile<DH>::ROW;
+};
 
-__global__ __launch_bounds__(256) void cross_delta_kernel(const Params p) {
-  const long long all = (long long)p.B * p.H * p.Nq;
-  const int lane = threadIdx.x & 63;
-  const long long r = blockIdx.x * 4ll + (threadIdx.x >> 6);
-  if (r >= all) return;
-  const long long bh = r / p.Nq, n = r % p.Nq, b = bh / p.H, h = bh % p.H;
-  const float *x = p.o.ptr + (b * p.Nq + n) * p.o.ld + h * p.dh;
-  const float *y = p.dout.ptr + (b * p.Nq + n) * p.dout.ld + h * p.dh;
-  float s = 0.f;
-  for (int d = lane; d < p.dh; d += 64) s += x[d] * y[d];
-  s = vitk::wave_sum(s);
-  if (lane == 0) p.delta[r] = s;
-}
+// Two tensors' next stage in registers, then split into LDS.
+template <int DH, int NW, int GROUPS>
+struct Stage {
+  typedef Shape<DH, NW, GROUPS> S;
+  float x[S::TASKS][8], y[S::TASKS][8];
+  template <class OffX, class OffY>
+  __device__ __forceinline__ void fetch(const Params &p, const float *px, const float *py, int first, int end, OffX offx,
+                                        OffY offy) {
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int task = threadIdx.x + S::THREADS * u, r = first + task / (DH / 8), d = task % (DH / 8) * 8;
+      if (r < end) {
+        load_eight(px + offx(r), d, p, x[u]);
+        load_eight(py + offy(r), d, p, y[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] = y[u][e] = 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(bf16x8 *tx, bf16x8 *ty) const {
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int task = threadIdx.x + S::THREADS * u;
+      Tile<DH>::put(tx, task / (DH / 8), task % (DH / 8), split8(x[u]));
+      Tile<DH>::put(ty, task / (DH / 8), task % (DH / 8), split8(y[u]));
+    }
+  }
+};
 
 template <int DH>
-__device__ __forceinline__ void zero(f32x16 (&x)[DH / 32]) {
+__device__ __forceinline__ void load_row(Split8 (&f)[DH / 16], const float *row, bool ok, int g, float scale, const Params &p) {
 #pragma unroll
-  for (int n = 0; n < DH / 32; ++n)
+  for (int i = 0; i < DH / 16; ++i) {
+    float x[8] = {};
+    if (ok) load_eight(row, 16 * i + 8 * g, p, x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[n][i] = 0.f;
-}
-// columns g*DH/2 .. of one row (zeros if it does not exist)
-template <int DH>
-__device__ __forceinline__ void load_half(float (&f)[DH / 2], const float *row, bool ok, int g, const Params &p) {
-#pragma unroll
-  for (int i = 0; i < DH / 2; i += 4) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (ok) x = load_quad(row, g * (DH / 2) + i, p.dh, p.vec);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[i + e] = x[e];
+    for (int e = 0; e < 8; ++e) x[e] *= scale;
+    f[i] = split8(x);
   }
 }
-// tile [32][DH+4] of rows in LDS times the lane's half row: one 32 x 32 product
 template <int DH>
-__device__ __forceinline__ f32x16 product(const float *tile, const float (&f)[DH / 2], int c, int g) {
-  f32x16 s;
+__device__ __forceinline__ f32x16 rows_times(const bf16x8 *tile, int row, int g, const Split8 (&f)[DH / 16]) {
+  f32x16 s = zero16();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < DH / 2; i += 4) {
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(tile + c * (DH + 4) + g * (DH / 2) + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], f[i + e], s, 0, 0, 0);
-  }
+  for (int i = 0; i < DH / 16; ++i) s = product6(Tile<DH>::rows(tile, row, i, g), f[i], s);
   return s;
 }
-// acc^T[d][col] += tile^T[d][r] x[r][col]
+// acc^T[d][col] += tile^T[d][r] x[r][col], r in first .. first + 31
 template <int DH>
-__device__ __forceinline__ void accumulate(f32x16 (&acc)[DH / 32], const float *tile, const f32x16 &x, int c, int g) {
+__device__ __forceinline__ void add_columns(f32x16 (&acc)[DH / 32], const bf16x8 *tile, int first, int lane, const f32x16 &x) {
 #pragma unroll
-  for (int n = 0; n < DH / 32; ++n)
+  for (int h = 0; h < 2; ++h) {
+    const Split8 f = split_half(x, h);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(tile[(8 * (i / 4) + 4 * g + i % 4) * (DH + 4) + 32 * n + c], x[i],
-                                                    acc[n], 0, 0, 0);
+    for (int n = 0; n < DH / 32; ++n) acc[n] = product6(Tile<DH>::columns(tile, first + 16 * h, n, lane), f, acc[n]);
+  }
+}
+// The other wave's sums of the same rows (keys) are added through LDS.
+template <int NB>
+__device__ __forceinline__ void give(float *box, const f32x16 (&acc)[NB]) {
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) box[(16 * n + i) * 64] = acc[n][i];
+}
+template <int NB>
+__device__ __forceinline__ void take(const float *box, f32x16 (&acc)[NB]) {
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[n][i] += box[(16 * n + i) * 64];
 }
 template <int DH>
-__device__ __forceinline__ void store(float *row, const f32x16 (&acc)[DH / 32], float f, int g, const Params &p) {
+__device__ __forceinline__ void store(float *row, const f32x16 (&acc)[DH / 32], float f, int g, const Params &p, bool vec) {
 #pragma unroll
   for (int n = 0; n < DH / 32; ++n)
 #pragma unroll
@@ -79,135 +108,283 @@ __device__ __forceinline__ void store(float *row, const f32x16 (&acc)[DH / 32], 
       f32x4 x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = acc[n][4 * j + e] * f;
-      store_quad(row, 32 * n + 8 * j + 4 * g, p.dh, p.vec, x);
+      store_quad(row, 32 * n + 8 * j + 4 * g, p.dh, vec, x);
     }
 }
 
-template <int DH>
-__global__ __launch_bounds__(256) void cross_dkv_kernel(const Params p) {
-  constexpr int LP = DH + 4;
-  __shared__ __attribute__((aligned(16))) float qt[32 * LP], gt[32 * LP];
-  __shared__ float rm[32], rl[32], rd[32];
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
-  long long wg = blockIdx.x;
-  const int kb = (int)(wg % p.blocks);
-  wg /= p.blocks;
-  const int hk = (int)(wg % p.Hkv), b = (int)(wg / p.Hkv);
-  const int len = valid_keys(p, b), key = kb * RB + wave * 32 + c;
-  const bool key_ok = key < len;
-  float kf[DH / 2], vf[DH / 2];
-  load_half<DH>(kf, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p);
-  load_half<DH>(vf, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, p);
-  f32x16 dk[DH / 32], dv[DH / 32];
-  zero<DH>(dk), zero<DH>(dv);
-  const int rows = kb * RB < len ? p.rows : 0;  // a block behind the length has nothing to add
-  for (int t = 0; t < rows; t += 32) {
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < DH / 32; ++u) {
-      const int quad = threadIdx.x + 256 * u, r = quad / (DH / 4), d = 4 * (quad % (DH / 4));
-      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-      if (t + r < rows) {
-        x = load_quad(p.q.ptr + row_offset(p, p.q.ld, b, hk, t + r), d, p.dh, p.vec);
-        y = load_quad(p.dout.ptr + row_offset(p, p.dout.ld, b, hk, t + r), d, p.dh, p.vec);
-      }
-      *reinterpret_cast<f32x4 *>(qt + r * LP + d) = x;
-      *reinterpret_cast<f32x4 *>(gt + r * LP + d) = y;
-    }
-    if (threadIdx.x < 32) {
-      const int r = t + threadIdx.x;
-      float m = 0.f, f = 0.f, d = 0.f;
-      if (r < rows) {
-        const long long st = row_stat(p, b, hk, r);
-        m = p.stats[2 * st];
-        const float l = p.stats[2 * st + 1];
-        f = l == 0.f ? 0.f : 1.f / l;
-        d = p.delta[st];
-      }
-      rm[threadIdx.x] = m, rl[threadIdx.x] = f, rd[threadIdx.x] = d;
-    }
-    __syncthreads();
-    f32x16 s = product<DH>(qt, kf, c, g), ds = product<DH>(gt, vf, c, g);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = 8 * (i / 4) + 4 * g + i % 4;
-      const float e = key_ok && t + r < rows ? __builtin_amdgcn_exp2f(s[i] * p.c - rm[r]) * rl[r] : 0.f;
-      s[i] = e;
-      ds[i] = e * (ds[i] - rd[r]);
-    }
-    accumulate<DH>(dv, gt, s, c, g);
-    accumulate<DH>(dk, qt, ds, c, g);
-  }
-  if (key < p.Nk) {
-    store<DH>(p.dk.ptr + key_offset(p, p.dk.ld, b, hk, key), dk, p.scale, g, p);
-    store<DH>(p.dv.ptr + key_offset(p, p.dv.ld, b, hk, key), dv, 1.f, g, p);
-  }
-}
-
-template <int DH>
-__global__ __launch_bounds__(256) void cross_dq_kernel(const Params p) {
-  constexpr int LP = DH + 4;
-  __shared__ __attribute__((aligned(16))) float kt[32 * LP], vt[32 * LP];
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
+template <int DH, int NW, int RW>
+__global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
+  typedef Shape<DH, NW, RW> S;
+  constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 2) * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
+  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + S::UNITS;
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
   const int rb = (int)(wg % p.blocks);
   wg /= p.blocks;
-  const int hk = (int)(wg % p.Hkv), b = (int)(wg / p.Hkv);
-  const int len = valid_keys(p, b), row = rb * RB + wave * 32 + c;
+  const int hk = (int)(wg % p.Hkv);
+  wg /= p.Hkv;
+  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int len = valid_keys(p, b), row = (rb * RW + rg) * 32 + c;
+  const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
   const bool row_ok = row < p.rows;
-  float qf[DH / 2], gf[DH / 2];
-  load_half<DH>(qf, p.q.ptr + row_offset(p, p.q.ld, b, hk, row_ok ? row : 0), row_ok, g, p);
-  load_half<DH>(gf, p.dout.ptr + row_offset(p, p.dout.ld, b, hk, row_ok ? row : 0), row_ok, g, p);
+  Split8 q[DH / 16], dout[DH / 16];
   float m = 0.f, f = 0.f, delta = 0.f;
-  if (row_ok) {
-    const long long st = row_stat(p, b, hk, row);
-    m = p.stats[2 * st];
-    const float l = p.stats[2 * st + 1];
-    f = l == 0.f ? 0.f : 1.f / l;
-    delta = p.delta[st];
+  {
+    const int r = row_ok ? row : 0;
+    load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, r), row_ok, g, p.c, p);
+    const float *gp = p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r), *op = p.o.ptr + row_offset(p, p.o.ld, b, hk, r);
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) {
+      float x[8] = {}, y[8] = {};
+      if (row_ok) {
+        load_eight(gp, 16 * i + 8 * g, p, x);
+        load_eight(op, 16 * i + 8 * g, p, y);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta += x[e] * y[e];
+      dout[i] = split8(x);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (row_ok) {
+      const long long st = row_stat(p, b, hk, row);
+      m = p.stats[2 * st];
+      const float l = p.stats[2 * st + 1];
+      f = l == 0.f ? 0.f : 1.f / l;
+      if (g == 0 && kg == 0 && split == 0) p.delta[st] = delta;
+    }
   }
   f32x16 dq[DH / 32];
-  zero<DH>(dq);
-  for (int t = 0; t < len; t += 32) {
-    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < DH / 32; ++u) {
-      const int quad = threadIdx.x + 256 * u, key = quad / (DH / 4), d = 4 * (quad % (DH / 4));
-      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-      if (t + key < len) {
-        x = load_quad(p.k.ptr + key_offset(p, p.k.ld, b, hk, t + key), d, p.dh, p.vec);
-        y = load_quad(p.v.ptr + key_offset(p, p.v.ld, b, hk, t + key), d, p.dh, p.vec);
+  for (int n = 0; n < DH / 32; ++n) dq[n] = zero16();
+  Stage<DH, NW, RW> next;
+  auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
+  auto offv = [&](int n) { return key_offset(p, p.v.ld, b, hk, n); };
+  if (k0 < k1) next.fetch(p, p.k.ptr, p.v.ptr, k0, k1, offk, offv);
+  for (int t = k0; t < k1; t += S::STAGE) {
+    __syncthreads();
+    next.put(kt, vt);
+    __syncthreads();
+    if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
+#pragma unroll
+    for (int sub = 0; sub < S::SUB; ++sub) {
+      const int first = 32 * (kg * S::SUB + sub);
+      if (t + first >= k1) break;
+      const f32x16 s = rows_times<DH>(kt, first + c, g, q);
+      f32x16 ds = rows_times<DH>(vt, first + c, g, dout);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(s[i] - m) * f * (ds[i] - delta);
+      if (t + first + 32 > k1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t + first + 8 * (i / 4) + 4 * g + i % 4 >= k1) ds[i] = 0.f;
       }
-      *reinterpret_cast<f32x4 *>(kt + key * LP + d) = x;
-      *reinterpret_cast<f32x4 *>(vt + key * LP + d) = y;
+      add_columns<DH>(dq, kt, first, lane, ds);
+    }
+  }
+  if constexpr (S::OTHER > 1) {
+    float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 2) + lane;
+    __syncthreads();
+    if (kg == 1) give<DH / 32>(box, dq);
+    __syncthreads();
+    if (kg == 1) return;
+    take<DH / 32>(box, dq);
+  }
+  if (!row_ok) return;
+  if (p.splits > 1) {
+    const long long pitch = (long long)p.H * p.dh, all = (long long)p.B * p.Nq * pitch;
+    store<DH>(p.part + split * all + row_offset(p, pitch, b, hk, row), dq, p.scale, g, p, p.dh % 4 == 0);
+  } else {
+    store<DH>(p.dq.ptr + row_offset(p, p.dq.ld, b, hk, row), dq, p.scale, g, p, p.vec);
+  }
+}
+
+template <int DH, int NW, int KG>
+__global__ __launch_bounds__(64 * NW, 1) void cross_dkv_kernel(const Params p) {
+  typedef Shape<DH, NW, KG> S;
+  constexpr int JOIN = S::OTHER > 1 ? KG * 64 * DH * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
+  __shared__ __attribute__((aligned(16))) float rm[S::STAGE], rl[S::STAGE], rd[S::STAGE];
+  bf16x8 *qt = reinterpret_cast<bf16x8 *>(lds), *gt = qt + S::UNITS;
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, rg = wave / KG;
+  long long wg = blockIdx.x;
+  const int kb = (int)(wg % p.blocks);
+  wg /= p.blocks;
+  const int hk = (int)(wg % p.Hkv);
+  wg /= p.Hkv;
+  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int len = valid_keys(p, b), key = (kb * KG + kg) * 32 + c;
+  const bool key_ok = key < len;
+  Split8 k[DH / 16], v[DH / 16];
+  load_row<DH>(k, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p.c, p);
+  load_row<DH>(v, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, 1.f, p);
+  f32x16 dk[DH / 32], dv[DH / 32];
+#pragma unroll
+  for (int n = 0; n < DH / 32; ++n) dk[n] = zero16(), dv[n] = zero16();
+  // a block behind the length has nothing to add
+  const int r0 = min((long long)split * p.chunk, (long long)p.rows);
+  const int r1 = kb * KG * 32 < len ? (int)min((long long)r0 + p.chunk, (long long)p.rows) : r0;
+  Stage<DH, NW, KG> next;
+  auto offq = [&](int r) { return row_offset(p, p.q.ld, b, hk, r); };
+  auto offg = [&](int r) { return row_offset(p, p.dout.ld, b, hk, r); };
+  float sm = 0.f, sl = 0.f, sd = 0.f;
+  auto fetch = [&](int t) {
+    next.fetch(p, p.q.ptr, p.dout.ptr, t, r1, offq, offg);
+    if (threadIdx.x < S::STAGE) {
+      sm = sl = sd = 0.f;  // a row that is not there: p = 1 * 0
+      const int r = t + threadIdx.x;
+      if (r < r1) {
+        const long long st = row_stat(p, b, hk, r);
+        sm = p.stats[2 * st], sl = p.stats[2 * st + 1], sd = p.delta[st];
+      }
+    }
+  };
+  if (r0 < r1) fetch(r0);
+  for (int t = r0; t < r1; t += S::STAGE) {
+    __syncthreads();
+    next.put(qt, gt);
+    if (threadIdx.x < S::STAGE) {
+      rm[threadIdx.x] = sm;
+      rl[threadIdx.x] = sl == 0.f ? 0.f : 1.f / sl;
+      rd[threadIdx.x] = sd;
     }
     __syncthreads();
-    const f32x16 s = product<DH>(kt, qf, c, g);
-    f32x16 ds = product<DH>(vt, gf, c, g);
+    if (t + S::STAGE < r1) fetch(t + S::STAGE);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = t + 8 * (i / 4) + 4 * g + i % 4;
-      ds[i] = key < len ? __builtin_amdgcn_exp2f(s[i] * p.c - m) * f * (ds[i] - delta) : 0.f;
+    for (int sub = 0; sub < S::SUB; ++sub) {
+      const int first = 32 * (rg * S::SUB + sub);
+      if (t + first >= r1) break;
+      f32x16 s = rows_times<DH>(qt, first + c, g, k);
+      f32x16 ds = rows_times<DH>(gt, first + c, g, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 m = *reinterpret_cast<const f32x4 *>(rm + first + 8 * j + 4 * g);
+        const f32x4 f = *reinterpret_cast<const f32x4 *>(rl + first + 8 * j + 4 * g);
+        const f32x4 d = *reinterpret_cast<const f32x4 *>(rd + first + 8 * j + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * j + e;
+          s[i] = __builtin_amdgcn_exp2f(s[i] - m[e]) * f[e];
+          ds[i] = s[i] * (ds[i] - d[e]);
+        }
+      }
+      add_columns<DH>(dv, gt, first, lane, s);
+      add_columns<DH>(dk, qt, first, lane, ds);
     }
-    accumulate<DH>(dq, kt, ds, c, g);
   }
-  if (row_ok) store<DH>(p.dq.ptr + row_offset(p, p.dq.ld, b, hk, row), dq, p.scale, g, p);
+  if constexpr (S::OTHER > 1) {
+    float *box = reinterpret_cast<float *>(lds) + kg * 64 * DH + lane;
+    __syncthreads();
+    if (rg == 1) give<DH / 32>(box, dk), give<DH / 32>(box + 64 * (DH / 2), dv);
+    __syncthreads();
+    if (rg == 1) return;
+    take<DH / 32>(box, dk), take<DH / 32>(box + 64 * (DH / 2), dv);
+  }
+  if (key >= p.Nk) return;
+  if (!key_ok) {  // (whatever its column held)
+#pragma unroll
+    for (int n = 0; n < DH / 32; ++n) dk[n] = zero16(), dv[n] = zero16();
+  }
+  if (p.splits > 1) {
+    const long long pitch = (long long)p.Hkv * p.dh, all = (long long)p.B * p.Nk * pitch;
+    const long long at = key_offset(p, pitch, b, hk, key);
+    store<DH>(p.part + split * all + at, dk, p.scale, g, p, p.dh % 4 == 0);
+    store<DH>(p.part + (p.splits + split) * all + at, dv, 1.f, g, p, p.dh % 4 == 0);
+  } else {
+    store<DH>(p.dk.ptr + key_offset(p, p.dk.ld, b, hk, key), dk, p.scale, g, p, p.vec);
+    store<DH>(p.dv.ptr + key_offset(p, p.dv.ld, b, hk, key), dv, 1.f, g, p, p.vec);
+  }
+}
+
+// out[row][col] = sum of the parts in order; `rows` rows of `width` columns
+__global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part, int splits, long long rows, int width,
+                                                              Result out) {
+  const long long all = rows * width;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int x = 0; x < splits; ++x) s += part[x * all + i];
+    const long long r = i / width;
+    out.ptr[r * out.ld + (i - r * width)] = s;
+  }
+}
+
+// Groups of 32 in a workgroup, blocks, and how the other side is split.
+struct Side {
+  int groups, blocks, splits, chunk;
+};
+Side plan_side(long long own, long long other, long long heads) {
+  Side s;
+  s.groups = own > 64 ? 4 : own > 32 ? 2 : 1;
+  s.blocks = (int)((own + 32 * s.groups - 1) / (32 * s.groups));
+  const long long stages = (other + 63) / 64, wgs = heads * s.blocks;
+  long long splits = 1;
+  if (wgs > 0) splits = std::min((long long)vitk::cu_count() / wgs, stages / 8);
+  splits = std::min(std::max(splits, 1ll), 64ll);
+  s.chunk = std::max((int)((stages + splits - 1) / splits) * 64, 64);
+  s.splits = std::max((int)((other + s.chunk - 1) / s.chunk), 1);
+  return s;
+}
+struct Plan {
+  Side rows, keys;
+  size_t delta, part;  // floats
+};
+Plan make_plan(const Params &p) {
+  Plan n;
+  const long long heads = (long long)p.B * p.Hkv;
+  n.rows = plan_side(p.rows, p.Nk, heads);
+  n.keys = plan_side(p.Nk, p.rows, heads);
+  n.delta = ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
+  const size_t q = n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
+  const size_t k = n.keys.splits > 1 ? (size_t)2 * n.keys.splits * p.B * p.Nk * p.Hkv * p.dh : 0;
+  n.part = std::max(q, k);  // one after the other
+  return n;
 }
 
 template <int DH>
-int launch(Params p, hipStream_t st) {
-  const long long heads = (long long)p.B * p.Hkv, all = (long long)p.B * p.H * p.Nq;
-  const long long qb = (p.rows + RB - 1) / RB, kb = (p.Nk + RB - 1) / RB;
-  VITK_REQUIRE((all + 3) / 4 < (1ll << 31) && heads * qb < (1ll << 31) && heads * kb < (1ll << 31),
-               "vitk_cross_sdpa_bwd: too many rows for one launch");
-  if (all) hipLaunchKernelGGL(cross_delta_kernel, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
-  if (kb) {
-    p.blocks = (int)kb;
-    hipLaunchKernelGGL(cross_dkv_kernel<DH>, dim3((unsigned)(heads * kb)), dim3(256), 0, st, p);
+void launch_dq(const Params &p, int groups, unsigned wgs, hipStream_t st) {
+  if (groups == 4)
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
+  else if (groups == 2)
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
+}
+template <int DH>
+void launch_dkv(const Params &p, int groups, unsigned wgs, hipStream_t st) {
+  if (groups == 4)
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
+  else if (groups == 2)
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
+}
+void add_parts(const float *part, int splits, long long rows, int width, Result out, hipStream_t st) {
+  hipLaunchKernelGGL(cross_add_parts_kernel, dim3(vitk::grid_for(rows * width, 256)), dim3(256), 0, st, part, splits, rows,
+                     width, out);
+}
+
+template <int DH>
+int launch(Params p, const Plan &n, hipStream_t st) {
+  const long long heads = (long long)p.B * p.Hkv;
+  const long long qw = heads * n.rows.blocks * n.rows.splits, kw = heads * n.keys.blocks * n.keys.splits;
+  VITK_REQUIRE(qw < (1ll << 31) && kw < (1ll << 31), "vitk_cross_sdpa_bwd: too many rows for one launch");
+  if (p.Nq > 0) {
+    p.blocks = n.rows.blocks, p.splits = n.rows.splits, p.chunk = n.rows.chunk;
+    launch_dq<DH>(p, n.rows.groups, (unsigned)qw, st);
+    if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nq, p.H * p.dh, p.dq, st);
   }
-  if (qb) {
-    p.blocks = (int)qb;
-    hipLaunchKernelGGL(cross_dq_kernel<DH>, dim3((unsigned)(heads * qb)), dim3(256), 0, st, p);
+  if (p.Nk > 0) {
+    p.blocks = n.keys.blocks, p.splits = n.keys.splits, p.chunk = n.keys.chunk;
+    launch_dkv<DH>(p, n.keys.groups, (unsigned)kw, st);
+    if (p.splits > 1) {
+      const long long rows = (long long)p.B * p.Nk;
+      const int width = p.Hkv * p.dh;
+      add_parts(p.part, p.splits, rows, width, p.dk, st);
+      add_parts(p.part + p.splits * rows * width, p.splits, rows, width, p.dv, st);
+    }
   }
   return vitk::check_launch("vitk_cross_sdpa_bwd");
 }
@@ -215,23 +392,28 @@ int launch(Params p, hipStream_t st) {
 }  // namespace
 
 extern "C" size_t vitk_cross_sdpa_bwd_workspace_bytes(const vitk_cross_sdpa_args *a) {
-  if (!a || a->B <= 0 || a->H <= 0 || a->Nq <= 0) return 0;
-  return (size_t)a->B * a->H * a->Nq * sizeof(float);
+  if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->Nq < 0 || a->Nk < 0 || a->dh < 1) return 0;
+  Params p = {};
+  p.B = a->B, p.H = a->H, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Nq = a->Nq, p.Nk = a->Nk, p.dh = a->dh;
+  p.rows = p.G * p.Nq;
+  const Plan n = make_plan(p);
+  return (n.delta + n.part) * sizeof(float);
 }
 
 extern "C" int vitk_cross_sdpa_bwd(const vitk_cross_sdpa_args *a, vitk_stream_t stream) {
   Params p = {};
   if (check_args("vitk_cross_sdpa_bwd", a, true, &p)) return 1;
   if (p.B == 0 || (p.Nq == 0 && p.Nk == 0)) return 0;
-  const size_t need = vitk_cross_sdpa_bwd_workspace_bytes(a);
+  const Plan n = make_plan(p);
+  const size_t need = (n.delta + n.part) * sizeof(float);
   VITK_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
                "vitk_cross_sdpa_bwd: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
   VITK_REQUIRE(need == 0 || vitk::aligned16(a->workspace), "vitk_cross_sdpa_bwd: workspace is not 16-byte aligned");
   p.delta = a->workspace;
-  p.splits = 1;
+  p.part = a->workspace + n.delta;
   hipStream_t st = vitk::as_stream(stream);
-  if (p.dh <= 32) return launch<32>(p, st);
-  if (p.dh <= 64) return launch<64>(p, st);
-  if (p.dh <= 96) return launch<96>(p, st);
-  return launch<128>(p, st);
+  if (p.dh <= 32) return launch<32>(p, n, st);
+  if (p.dh <= 64) return launch<64>(p, n, st);
+  if (p.dh <= 96) return launch<96>(p, n, st);
+  return launch<128>(p, n, st);
 }
