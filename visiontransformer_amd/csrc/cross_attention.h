@@ -7,7 +7,6 @@ namespace cross {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -83,7 +82,9 @@ __device__ __forceinline__ void store_quad(float *row, int d, int dh, bool vec, 
 // x = p0 + p1 + p2 exactly: each part the bf16 nearest to what is left (8 + 8 + 8 bits and two signs
 // cover the 24 of fp32).  A product of two such numbers to fp32 accuracy is the six part products
 // p0 p0', p0 p1', p1 p0', p0 p2', p2 p0', p1 p1' (the others are below 2^-26), summed in fp32 by
-// v_mfma_f32_32x32x16_bf16: 16 times the rate of the fp32 instruction, so 2.7 times with six.
+// v_mfma_f32_16x16x32_bf16: 16 times the rate of the fp32 instruction, so 2.7 times with six.  16 rows a wave
+// instead of 32 halve what a wave keeps in registers (its own operand and its sums), and with four
+// waves a SIMD instead of one or two the matrix cores work while other waves split and exponentiate.
 struct Split8 {
   bf16x8 p[3];
 };
@@ -109,55 +110,51 @@ __device__ __forceinline__ Split8 split8(const float (&x)[8]) {
   return r;
 }
 // acc += a b, the small products first
-__device__ __forceinline__ f32x16 product6(const Split8 &a, const Split8 &b, f32x16 acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
+__device__ __forceinline__ f32x4 product6(const Split8 &a, const Split8 &b, f32x4 acc) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 zero16() {
-  f32x16 z;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) z[i] = 0.f;
-  return z;
-}
+__device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
+// Lane (c = lane & 15, g = lane >> 4) of the instruction supplies A[i = c][k = 8 g ..] and B[k = 8 g ..][j = c] and
+// receives D[i = 4 g + r][j = c] in register r.  Two results for rows 0..15 and 16..31 are the operand
+// B of a contraction over those 32 rows if slot (g, e) stands for row 4 g + e, e < 4, and 16 + 4 g + e - 4:
+// the other operand is read in that order (Tile::columns).
 // A tile of rows x DH in LDS: per row three parts of DH bf16, in units of 16 bytes.  Unit u of a part sits at
-// u ^ spread(row), which puts 16 rows of one unit (a read along the columns) and four rows of four
+// u ^ spread(row), which puts 16 rows of one unit (a read along the columns) and eight rows of two
 // neighbouring units (a transposed read) on different banks.
 template <int DH>
 struct Tile {
   static constexpr int PART = DH / 8, ROW = 3 * PART;  // units
   __device__ static __forceinline__ int spread(int row) {
-    if constexpr (DH == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-    if constexpr (DH == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
-    return (row >> 2) & 3;
+    if constexpr (DH == 64) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+    if constexpr (DH == 128) return ((row & 7) << 1) | ((row >> 3) & 1);
+    return (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
   }
   __device__ static __forceinline__ void put(bf16x8 *tile, int row, int unit, const Split8 &x) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) tile[row * ROW + k * PART + (unit ^ spread(row))] = x.p[k];
   }
-  // operand of 16 columns: lane (c, g) takes columns 16 step + 8 g .. + 7 of row `row` (= first + c)
+  // columns 32 step + 8 g .. + 7 of row `row` (= first + c)
   __device__ static __forceinline__ Split8 rows(const bf16x8 *tile, int row, int step, int g) {
     Split8 r;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) r.p[k] = tile[row * ROW + k * PART + ((2 * step + g) ^ spread(row))];
+    for (int k = 0; k < 3; ++k) r.p[k] = tile[row * ROW + k * PART + ((4 * step + g) ^ spread(row))];
     return r;
   }
-  // operand of 16 rows of the transposed tile: lane (c, g) takes column 32 block + c of rows
-  // first + 4 g .. + 3 and first + 8 + 4 g .. + 3, the rows whose products registers 8 s .. 8 s + 7 of a
-  // 32 x 32 result hold (first = 16 s)
+  // column 16 block + c of rows first + 4 g .. + 3 and first + 16 + 4 g .. + 3
   __device__ static __forceinline__ Split8 columns(const bf16x8 *tile, int first, int block, int lane) {
     Split8 r;
-    const int row = first + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int unit = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const int row = first + 4 * (lane >> 4) + ((lane & 15) >> 2), unit = 2 * block + ((lane & 3) >> 1);
     const __bf16 *base = reinterpret_cast<const __bf16 *>(tile) + 4 * (lane & 1);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const bf16x4 x = transposed(base + (row * ROW + k * PART + (unit ^ spread(row))) * 8);
-      const bf16x4 y = transposed(base + ((row + 8) * ROW + k * PART + (unit ^ spread(row + 8))) * 8);
+      const bf16x4 y = transposed(base + ((row + 16) * ROW + k * PART + (unit ^ spread(row + 16))) * 8);
       r.p[k] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return r;
@@ -169,19 +166,113 @@ struct Tile {
     return __builtin_bit_cast(bf16x4, r);
   }
 };
-// registers 8 s .. 8 s + 7 of a 32 x 32 result as an operand
-__device__ __forceinline__ Split8 split_half(const f32x16 &x, int s) {
+// two results (rows 0..15 and 16..31) as an operand
+__device__ __forceinline__ Split8 split_pair(const f32x4 (&x)[2]) {
   float v[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = x[8 * s + e];
+  for (int e = 0; e < 4; ++e) v[e] = x[0][e], v[4 + e] = x[1][e];
   return split8(v);
 }
+// rows first .. first + 31 of a tile times this lane's row f (DH / 32 steps)
+template <int DH>
+__device__ __forceinline__ void rows_times(const bf16x8 *tile, int first, int c, int g, const Split8 (&f)[DH / 32],
+                                           f32x4 (&s)[2]) {
+  s[0] = s[1] = zero4();
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[h] = product6(Tile<DH>::rows(tile, first + 16 * h + c, i, g), f[i], s[h]);
+}
+// acc^T[d][col] += tile^T[d][r] x[r][col], r in first .. first + 31
+template <int DH>
+__device__ __forceinline__ void add_columns(f32x4 (&acc)[DH / 16], const bf16x8 *tile, int first, int lane, const Split8 &x) {
+#pragma unroll
+  for (int n = 0; n < DH / 16; ++n) acc[n] = product6(Tile<DH>::columns(tile, first, n, lane), x, acc[n]);
+}
+// over the four lanes that hold one column: exchanging the upper half of one copy with the lower half of another
+// leaves {own, other} in the two; then the same with neighbouring rows of 16 lanes.  (Written out: of the
+// builtin's two results this compiler keeps one.  The wait is the one it puts before the exchange.)
+__device__ __forceinline__ float column_max(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = y = fmaxf(x, y);
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
 // columns d .. d + 7 of a row; zeros behind dh
 __device__ __forceinline__ void load_eight(const float *row, int d, const Params &p, float (&x)[8]) {
   const f32x4 a = load_quad(row, d, p.dh, p.vec), b = load_quad(row, d + 4, p.dh, p.vec);
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
 }
+
+// this lane's row (columns 32 i + 8 g ..) times `scale`, split
+template <int DH>
+__device__ __forceinline__ void load_row(Split8 (&f)[DH / 32], const float *row, bool ok, int g, float scale, const Params &p) {
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i) {
+    float x[8] = {};
+    if (ok) load_eight(row, 32 * i + 8 * g, p, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= scale;
+    f[i] = split8(x);
+  }
+}
+// column c of acc^T to a row
+template <int DH>
+__device__ __forceinline__ void store_row(float *row, const f32x4 (&acc)[DH / 16], float f, int g, int dh, bool vec) {
+#pragma unroll
+  for (int n = 0; n < DH / 16; ++n) {
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = acc[n][e] * f;
+    store_quad(row, 16 * n + 4 * g, dh, vec, x);
+  }
+}
+
+// NW waves, GROUPS of 16 rows (or keys); OTHER = waves that share a group and deal the 32-row tiles of a stage of
+// the other side.
+template <int DH, int NW, int GROUPS>
+struct Shape {
+  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 128 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
+  static constexpr int THREADS = 64 * NW, ALL = STAGE * DH / 8, TASKS = (ALL + THREADS - 1) / THREADS;
+  static constexpr int UNITS = STAGE * Tile<DH>::ROW;
+};
+// Two tensors' next stage in registers (8 columns of a row, per tensor and task), then split into LDS.
+template <int DH, int NW, int GROUPS>
+struct Stage {
+  typedef Shape<DH, NW, GROUPS> S;
+  float x[S::TASKS][8], y[S::TASKS][8];
+  template <class OffX, class OffY>
+  __device__ __forceinline__ void fetch(const Params &p, const float *px, const float *py, int first, int end, OffX offx,
+                                        OffY offy) {
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int task = threadIdx.x + S::THREADS * u, r = first + task / (DH / 8), d = task % (DH / 8) * 8;
+      if (r < end && (S::ALL % S::THREADS == 0 || task < S::ALL)) {
+        load_eight(px + offx(r), d, p, x[u]);
+        load_eight(py + offy(r), d, p, y[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] = y[u][e] = 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(bf16x8 *tx, bf16x8 *ty) const {
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int task = threadIdx.x + S::THREADS * u;
+      if (S::ALL % S::THREADS != 0 && task >= S::ALL) continue;
+      Tile<DH>::put(tx, task / (DH / 8), task % (DH / 8), split8(x[u]));
+      Tile<DH>::put(ty, task / (DH / 8), task % (DH / 8), split8(y[u]));
+    }
+  }
+};
 
 // Argument checks both directions share; fills everything but the launch plan.
 int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Params *p);

@@ -1,10 +1,9 @@
 // Cross attention forward: softmax(scale * q k^T) v with queries and keys of different sequences.
 //
-// One workgroup = 128 query rows of one (batch, key head); the query heads that share the key head are
-// rows of the same block, so shared keys are read once per block.  A wave holds 32 rows as the columns of
-// S^T[key][row] = K Q^T on v_mfma_f32_32x32x2_f32; register i of lane (c = lane & 31, g = lane >> 5) is key
-// 8 (i / 4) + 4 g + i % 4 of row c, which is the operand the second product O^T[d][row] += V^T P^T
-// wants for contraction index g, so probabilities never leave their registers.  One pass over the
+// One workgroup = up to 128 query rows of one (batch, key head); the query heads that share the key head are
+// rows of the same block, so shared keys are read once per block.  A wave holds 16 rows as the columns of
+// S^T[key][row] = K Q^T; what a lane receives of 32 keys is the operand that the second product
+// O^T[d][row] += V^T P^T wants from it, so probabilities never leave their registers.  One pass over the
 // keys with a running maximum and sum per row.
 #include "cross_attention.h"
 
@@ -73,27 +72,17 @@ namespace {
 
 using namespace vitk::cross;
 
-// NW waves: RW groups of 32 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
+// NW waves: RW groups of 16 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
-// A stage is KT keys: loaded into registers one stage ahead, split and put into LDS between two barriers.
+// A stage of keys is loaded into registers one stage ahead, split and put into LDS between two barriers.
 template <int DH, int NW, int RW>
-struct Forward {
-  static constexpr int KW = NW / RW, KT = DH < 128 || KW > 1 ? 64 : 32, SUB = KT / 32 / KW;  // 32-key tiles of a wave
-  static constexpr int THREADS = 64 * NW, TASKS = KT * DH / 8 / THREADS;  // 8 columns of a key, per tensor and thread
-  static_assert(TASKS * THREADS * 8 == KT * DH, "a stage is dealt evenly");
-  static constexpr int UNITS = KT * Tile<DH>::ROW;
-  static constexpr int JOIN = KW > 1 ? RW * 64 * (DH / 2 + 2) * 4 : 0;  // bytes: o, m, l of the other key group
-  static constexpr int LDS = 2 * UNITS * 16 > JOIN ? 2 * UNITS * 16 : JOIN;
-};
-
-template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_fwd_kernel(const Params p) {
-  typedef Forward<DH, NW, RW> F;
-  typedef Tile<DH> T;
-  constexpr int NB = DH / 32, KS = DH / 16;
-  __shared__ __attribute__((aligned(16))) char lds[F::LDS];
-  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + F::UNITS;
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+__global__ __launch_bounds__(64 * NW, NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ? 2 : 1)) void cross_fwd_kernel(const Params p) {
+  typedef Shape<DH, NW, RW> S;
+  constexpr int NB = DH / 16, BOX = DH / 4 + 2;  // words a lane passes on: o, m, l
+  constexpr int JOIN = S::OTHER > 1 ? RW * 64 * BOX * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
+  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + S::UNITS;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
   const int rb = (int)(wg % p.blocks);
@@ -103,112 +92,84 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_fwd_kernel(co
   const int b = (int)(wg % p.B), split = (int)(wg / p.B);
   const int len = valid_keys(p, b);
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
-  const int row = (rb * RW + rg) * 32 + c;
+  const int row = (rb * RW + rg) * 16 + c;
   const bool row_ok = row < p.rows;
 
-  Split8 q[KS];  // this lane's row times scale log2(e), split
+  Split8 q[DH / 32];  // times scale log2(e)
+  load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, row_ok ? row : 0), row_ok, g, p.c, p);
+  f32x4 o[NB];
 #pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    float x[8] = {};
-    if (row_ok) load_eight(p.q.ptr + row_offset(p, p.q.ld, b, hk, row), 16 * i + 8 * g, p, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= p.c;
-    q[i] = split8(x);
-  }
-  f32x16 o[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) o[n] = zero16();
+  for (int n = 0; n < NB; ++n) o[n] = zero4();
   float m = -INFINITY, l = 0.f;
 
-  float kx[F::TASKS][8], vx[F::TASKS][8];
-  auto fetch = [&](int t) {
-#pragma unroll
-    for (int u = 0; u < F::TASKS; ++u) {
-      const int task = threadIdx.x + F::THREADS * u, key = t + task / (DH / 8), d = task % (DH / 8) * 8;
-      if (key < k1) {
-        load_eight(p.k.ptr + key_offset(p, p.k.ld, b, hk, key), d, p, kx[u]);
-        load_eight(p.v.ptr + key_offset(p, p.v.ld, b, hk, key), d, p, vx[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) kx[u][e] = vx[u][e] = 0.f;
-      }
-    }
-  };
-  if (k0 < k1) fetch(k0);
-  for (int t = k0; t < k1; t += F::KT) {
+  Stage<DH, NW, RW> next;
+  auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
+  auto offv = [&](int n) { return key_offset(p, p.v.ld, b, hk, n); };
+  if (k0 < k1) next.fetch(p, p.k.ptr, p.v.ptr, k0, k1, offk, offv);
+  for (int t = k0; t < k1; t += S::STAGE) {
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < F::TASKS; ++u) {
-      const int task = threadIdx.x + F::THREADS * u;
-      T::put(kt, task / (DH / 8), task % (DH / 8), split8(kx[u]));
-      T::put(vt, task / (DH / 8), task % (DH / 8), split8(vx[u]));
-    }
+    next.put(kt, vt);
     __syncthreads();
-    if (t + F::KT < k1) fetch(t + F::KT);
+    if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
 #pragma unroll
-    for (int sub = 0; sub < F::SUB; ++sub) {
-      const int first = 32 * (kg * F::SUB + sub);  // of the stage
+    for (int sub = 0; sub < S::SUB; ++sub) {
+      const int first = 32 * (kg * S::SUB + sub);  // of the stage
       if (t + first >= k1) break;
-      f32x16 s = zero16();
-#pragma unroll
-      for (int i = 0; i < KS; ++i) s = product6(T::rows(kt, first + c, i, g), q[i], s);
+      f32x4 s[2];
+      rows_times<DH>(kt, first, c, g, q, s);
       if (t + first + 32 > k1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t + first + 8 * (i / 4) + 4 * g + i % 4 >= k1) s[i] = -INFINITY;
-      }
-      float top = s[0];
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float m_new = fmaxf(m, top);
+          for (int e = 0; e < 4; ++e)
+            if (t + first + 16 * h + 4 * g + e >= k1) s[h][e] = -INFINITY;
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+      const float m_new = fmaxf(m, column_max(top));
       if (__any(m_new != m)) {  // (NaN scores: l and o become NaN below)
         const float fall = __builtin_amdgcn_exp2f(m - m_new);
         l *= fall;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[n][i] *= fall;
+          for (int e = 0; e < 4; ++e) o[n][e] *= fall;
         m = m_new;
       }
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(s[i] - m);
-        sum += s[i];
-      }
-      l += sum;  // of this lane's half of the keys
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Split8 x = split_half(s, h);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) o[n] = product6(T::columns(vt, first + 16 * h, n, lane), x, o[n]);
-      }
+        for (int e = 0; e < 4; ++e) {
+          s[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m);
+          l += s[h][e];  // of this lane's quarter of the keys
+        }
+      add_columns<DH>(o, vt, first, lane, split_pair(s));
     }
   }
-  l += __shfl_xor(l, 32, 64);
-  if constexpr (F::KW > 1) {
-    static_assert(F::KW == 2, "two key groups");
-    float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 2 + 2) + lane;
+  l = column_sum(l);
+  if constexpr (S::OTHER > 1) {
+    static_assert(S::OTHER == 2, "two key groups");
+    float *box = reinterpret_cast<float *>(lds) + rg * 64 * BOX + lane;
     __syncthreads();
     if (kg == 1) {
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) box[(16 * n + i) * 64] = o[n][i];
-      box[(DH / 2) * 64] = m;
-      box[(DH / 2 + 1) * 64] = l;
+        for (int e = 0; e < 4; ++e) box[(4 * n + e) * 64] = o[n][e];
+      box[(BOX - 2) * 64] = m;
+      box[(BOX - 1) * 64] = l;
     }
     __syncthreads();
     if (kg == 1) return;
-    const float m2 = box[(DH / 2) * 64], l2 = box[(DH / 2 + 1) * 64], top = fmaxf(m, m2);
+    const float m2 = box[(BOX - 2) * 64], l2 = box[(BOX - 1) * 64], top = fmaxf(m, m2);
     if (top > -INFINITY) {
       const float f1 = __builtin_amdgcn_exp2f(m - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
       l = l * f1 + l2 * f2;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][i] = o[n][i] * f1 + box[(16 * n + i) * 64] * f2;
+        for (int e = 0; e < 4; ++e) o[n][e] = o[n][e] * f1 + box[(4 * n + e) * 64] * f2;
       m = top;
     }
   }
@@ -216,25 +177,19 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_fwd_kernel(co
   const long long stat = row_stat(p, b, hk, row);
   float *dst, *st;
   float f = 1.f;
+  bool vec = p.vec;
   if (p.splits > 1) {
     const long long all = (long long)p.B * p.H * p.Nq;
     dst = p.part + (split * all + stat) * p.dh;
     st = p.part + p.splits * all * p.dh + (split * all + stat) * 2;
+    vec = p.dh % 4 == 0;
   } else {
     dst = p.out.ptr + row_offset(p, p.out.ld, b, hk, row);
     st = p.stats ? p.stats + stat * 2 : nullptr;
     f = l == 0.f ? 0.f : 1.f / l;
     if (l == 0.f) m = 0.f;
   }
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = o[n][4 * j + e] * f;
-      store_quad(dst, 32 * n + 8 * j + 4 * g, p.dh, p.vec, x);
-    }
+  store_row<DH>(dst, o, f, g, p.dh, vec);
   if (st && g == 0) {
     st[0] = m;
     st[1] = l;
@@ -423,7 +378,7 @@ __global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
 constexpr int CHUNK = 64;      // key ranges of splits are multiples of this
 constexpr int FEW_ROWS = 8;    // rows per key head up to which the vector kernel runs
 struct FwdPlan {
-  int row_groups;  // of 32 rows; 0 = the vector kernel
+  int row_groups;  // of 16 rows; 0 = the vector kernel
   int waves;       // of the vector kernel
 };
 FwdPlan plan_fwd(Params *p) {
@@ -441,8 +396,8 @@ FwdPlan plan_fwd(Params *p) {
         splits = std::min((12 * cus + heads - 1) / heads, stages / 4);
     }
   } else {
-    f.row_groups = p->rows > 64 ? 4 : p->rows > 32 ? 2 : 1;
-    p->blocks = (int)(((long long)p->rows + 32 * f.row_groups - 1) / (32 * f.row_groups));
+    f.row_groups = p->rows > 64 ? 8 : p->rows > 32 ? 4 : 2;
+    p->blocks = (int)(((long long)p->rows + 16 * f.row_groups - 1) / (16 * f.row_groups));
     const long long groups = heads * p->blocks;
     if (groups > 0) splits = std::min(2ll * vitk::cu_count() / groups, stages / 4);
   }
@@ -477,12 +432,12 @@ void launch_rows(const Params &p, int waves, unsigned wgs, hipStream_t st) {
 
 template <int DH>
 void launch_fwd(const Params &p, int row_groups, unsigned wgs, hipStream_t st) {
-  if (row_groups == 4)
-    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
-  else if (row_groups == 2)
-    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  if (row_groups == 8)
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
+  else if (row_groups == 4)
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((cross_fwd_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
 
 size_t fwd_bytes(const Params &p) {

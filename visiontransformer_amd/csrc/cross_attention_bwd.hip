@@ -6,7 +6,7 @@
 // with fp32 products in three bf16 parts arranged as in the forward: the accumulator of the first
 // product is the operand of the next.  That is seven products where five would do (s and dp are formed
 // twice); one pass would have to add dQ (or dK and dV) up across workgroups.
-// Blocks of up to 128 rows (keys); with fewer, two waves share a 32-wide group and deal the tiles of the
+// Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves share a group and deal the tiles of the
 // other side.  Where the blocks are too few for the device, the other side is split over workgroups and
 // the parts are added in order by a second launch.
 #include "cross_attention.h"
@@ -17,108 +17,29 @@ namespace {
 
 using namespace vitk::cross;
 
-// NW waves, GROUPS of 32 rows (dQ) or keys (dK, dV); OTHER = waves that deal the tiles of a stage.
-template <int DH, int NW, int GROUPS>
-struct Shape {
-  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 128 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
-  static constexpr int THREADS = 64 * NW, TASKS = STAGE * DH / 8 / THREADS;  // 8 columns, per tensor and thread
-  static_assert(TASKS * THREADS * 8 == STAGE * DH, "a stage is dealt evenly");
-  static constexpr int UNITS = STAGE * Tile<DH>::ROW;
-};
-
-// Two tensors' next stage in registers, then split into LDS.
-template <int DH, int NW, int GROUPS>
-struct Stage {
-  typedef Shape<DH, NW, GROUPS> S;
-  float x[S::TASKS][8], y[S::TASKS][8];
-  template <class OffX, class OffY>
-  __device__ __forceinline__ void fetch(const Params &p, const float *px, const float *py, int first, int end, OffX offx,
-                                        OffY offy) {
-#pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {
-      const int task = threadIdx.x + S::THREADS * u, r = first + task / (DH / 8), d = task % (DH / 8) * 8;
-      if (r < end) {
-        load_eight(px + offx(r), d, p, x[u]);
-        load_eight(py + offy(r), d, p, y[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = y[u][e] = 0.f;
-      }
-    }
-  }
-  __device__ __forceinline__ void put(bf16x8 *tx, bf16x8 *ty) const {
-#pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {
-      const int task = threadIdx.x + S::THREADS * u;
-      Tile<DH>::put(tx, task / (DH / 8), task % (DH / 8), split8(x[u]));
-      Tile<DH>::put(ty, task / (DH / 8), task % (DH / 8), split8(y[u]));
-    }
-  }
-};
-
-template <int DH>
-__device__ __forceinline__ void load_row(Split8 (&f)[DH / 16], const float *row, bool ok, int g, float scale, const Params &p) {
-#pragma unroll
-  for (int i = 0; i < DH / 16; ++i) {
-    float x[8] = {};
-    if (ok) load_eight(row, 16 * i + 8 * g, p, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= scale;
-    f[i] = split8(x);
-  }
-}
-template <int DH>
-__device__ __forceinline__ f32x16 rows_times(const bf16x8 *tile, int row, int g, const Split8 (&f)[DH / 16]) {
-  f32x16 s = zero16();
-#pragma unroll
-  for (int i = 0; i < DH / 16; ++i) s = product6(Tile<DH>::rows(tile, row, i, g), f[i], s);
-  return s;
-}
-// acc^T[d][col] += tile^T[d][r] x[r][col], r in first .. first + 31
-template <int DH>
-__device__ __forceinline__ void add_columns(f32x16 (&acc)[DH / 32], const bf16x8 *tile, int first, int lane, const f32x16 &x) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const Split8 f = split_half(x, h);
-#pragma unroll
-    for (int n = 0; n < DH / 32; ++n) acc[n] = product6(Tile<DH>::columns(tile, first + 16 * h, n, lane), f, acc[n]);
-  }
-}
 // The other wave's sums of the same rows (keys) are added through LDS.
 template <int NB>
-__device__ __forceinline__ void give(float *box, const f32x16 (&acc)[NB]) {
+__device__ __forceinline__ void give(float *box, const f32x4 (&acc)[NB]) {
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) box[(16 * n + i) * 64] = acc[n][i];
+    for (int e = 0; e < 4; ++e) box[(4 * n + e) * 64] = acc[n][e];
 }
 template <int NB>
-__device__ __forceinline__ void take(const float *box, f32x16 (&acc)[NB]) {
+__device__ __forceinline__ void take(const float *box, f32x4 (&acc)[NB]) {
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[n][i] += box[(16 * n + i) * 64];
-}
-template <int DH>
-__device__ __forceinline__ void store(float *row, const f32x16 (&acc)[DH / 32], float f, int g, const Params &p, bool vec) {
-#pragma unroll
-  for (int n = 0; n < DH / 32; ++n)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = acc[n][4 * j + e] * f;
-      store_quad(row, 32 * n + 8 * j + 4 * g, p.dh, vec, x);
-    }
+    for (int e = 0; e < 4; ++e) acc[n][e] += box[(4 * n + e) * 64];
 }
 
 template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
-  constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 2) * 4 : 0;
+  constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 4) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
   bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + S::UNITS;
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
   const int rb = (int)(wg % p.blocks);
@@ -126,27 +47,27 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_dq_kernel(con
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
   const int b = (int)(wg % p.B), split = (int)(wg / p.B);
-  const int len = valid_keys(p, b), row = (rb * RW + rg) * 32 + c;
+  const int len = valid_keys(p, b), row = (rb * RW + rg) * 16 + c;
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
   const bool row_ok = row < p.rows;
-  Split8 q[DH / 16], dout[DH / 16];
+  Split8 q[DH / 32], dout[DH / 32];
   float m = 0.f, f = 0.f, delta = 0.f;
   {
     const int r = row_ok ? row : 0;
     load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, r), row_ok, g, p.c, p);
     const float *gp = p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r), *op = p.o.ptr + row_offset(p, p.o.ld, b, hk, r);
 #pragma unroll
-    for (int i = 0; i < DH / 16; ++i) {
+    for (int i = 0; i < DH / 32; ++i) {
       float x[8] = {}, y[8] = {};
       if (row_ok) {
-        load_eight(gp, 16 * i + 8 * g, p, x);
-        load_eight(op, 16 * i + 8 * g, p, y);
+        load_eight(gp, 32 * i + 8 * g, p, x);
+        load_eight(op, 32 * i + 8 * g, p, y);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += x[e] * y[e];
       dout[i] = split8(x);
     }
-    delta += __shfl_xor(delta, 32, 64);
+    delta = column_sum(delta);
     if (row_ok) {
       const long long st = row_stat(p, b, hk, row);
       m = p.stats[2 * st];
@@ -155,9 +76,9 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_dq_kernel(con
       if (g == 0 && kg == 0 && split == 0) p.delta[st] = delta;
     }
   }
-  f32x16 dq[DH / 32];
+  f32x4 dq[DH / 16];
 #pragma unroll
-  for (int n = 0; n < DH / 32; ++n) dq[n] = zero16();
+  for (int n = 0; n < DH / 16; ++n) dq[n] = zero4();
   Stage<DH, NW, RW> next;
   auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
   auto offv = [&](int n) { return key_offset(p, p.v.ld, b, hk, n); };
@@ -171,43 +92,48 @@ __global__ __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) void cross_dq_kernel(con
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (kg * S::SUB + sub);
       if (t + first >= k1) break;
-      const f32x16 s = rows_times<DH>(kt, first + c, g, q);
-      f32x16 ds = rows_times<DH>(vt, first + c, g, dout);
+      f32x4 s[2], ds[2];
+      rows_times<DH>(kt, first, c, g, q, s);
+      rows_times<DH>(vt, first, c, g, dout, ds);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(s[i] - m) * f * (ds[i] - delta);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m) * f * (ds[h][e] - delta);
       if (t + first + 32 > k1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t + first + 8 * (i / 4) + 4 * g + i % 4 >= k1) ds[i] = 0.f;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t + first + 16 * h + 4 * g + e >= k1) ds[h][e] = 0.f;
       }
-      add_columns<DH>(dq, kt, first, lane, ds);
+      add_columns<DH>(dq, kt, first, lane, split_pair(ds));
     }
   }
   if constexpr (S::OTHER > 1) {
-    float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 2) + lane;
+    float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 4) + lane;
     __syncthreads();
-    if (kg == 1) give<DH / 32>(box, dq);
+    if (kg == 1) give<DH / 16>(box, dq);
     __syncthreads();
     if (kg == 1) return;
-    take<DH / 32>(box, dq);
+    take<DH / 16>(box, dq);
   }
   if (!row_ok) return;
   if (p.splits > 1) {
     const long long pitch = (long long)p.H * p.dh, all = (long long)p.B * p.Nq * pitch;
-    store<DH>(p.part + split * all + row_offset(p, pitch, b, hk, row), dq, p.scale, g, p, p.dh % 4 == 0);
+    store_row<DH>(p.part + split * all + row_offset(p, pitch, b, hk, row), dq, p.scale, g, p.dh, p.dh % 4 == 0);
   } else {
-    store<DH>(p.dq.ptr + row_offset(p, p.dq.ld, b, hk, row), dq, p.scale, g, p, p.vec);
+    store_row<DH>(p.dq.ptr + row_offset(p, p.dq.ld, b, hk, row), dq, p.scale, g, p.dh, p.vec);
   }
 }
 
 template <int DH, int NW, int KG>
-__global__ __launch_bounds__(64 * NW, 1) void cross_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
-  constexpr int JOIN = S::OTHER > 1 ? KG * 64 * DH * 4 : 0;
+  constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
   __shared__ __attribute__((aligned(16))) float rm[S::STAGE], rl[S::STAGE], rd[S::STAGE];
   bf16x8 *qt = reinterpret_cast<bf16x8 *>(lds), *gt = qt + S::UNITS;
-  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, rg = wave / KG;
   long long wg = blockIdx.x;
   const int kb = (int)(wg % p.blocks);
@@ -215,17 +141,17 @@ __global__ __launch_bounds__(64 * NW, 1) void cross_dkv_kernel(const Params p) {
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
   const int b = (int)(wg % p.B), split = (int)(wg / p.B);
-  const int len = valid_keys(p, b), key = (kb * KG + kg) * 32 + c;
+  const int len = valid_keys(p, b), key = (kb * KG + kg) * 16 + c;
   const bool key_ok = key < len;
-  Split8 k[DH / 16], v[DH / 16];
+  Split8 k[DH / 32], v[DH / 32];
   load_row<DH>(k, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p.c, p);
   load_row<DH>(v, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, 1.f, p);
-  f32x16 dk[DH / 32], dv[DH / 32];
+  f32x4 dk[DH / 16], dv[DH / 16];
 #pragma unroll
-  for (int n = 0; n < DH / 32; ++n) dk[n] = zero16(), dv[n] = zero16();
+  for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
   // a block behind the length has nothing to add
   const int r0 = min((long long)split * p.chunk, (long long)p.rows);
-  const int r1 = kb * KG * 32 < len ? (int)min((long long)r0 + p.chunk, (long long)p.rows) : r0;
+  const int r1 = kb * KG * 16 < len ? (int)min((long long)r0 + p.chunk, (long long)p.rows) : r0;
   Stage<DH, NW, KG> next;
   auto offq = [&](int r) { return row_offset(p, p.q.ld, b, hk, r); };
   auto offg = [&](int r) { return row_offset(p, p.dout.ld, b, hk, r); };
@@ -256,45 +182,45 @@ __global__ __launch_bounds__(64 * NW, 1) void cross_dkv_kernel(const Params p) {
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (rg * S::SUB + sub);
       if (t + first >= r1) break;
-      f32x16 s = rows_times<DH>(qt, first + c, g, k);
-      f32x16 ds = rows_times<DH>(gt, first + c, g, v);
+      f32x4 s[2], ds[2];
+      rows_times<DH>(qt, first, c, g, k, s);
+      rows_times<DH>(gt, first, c, g, v, ds);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 m = *reinterpret_cast<const f32x4 *>(rm + first + 8 * j + 4 * g);
-        const f32x4 f = *reinterpret_cast<const f32x4 *>(rl + first + 8 * j + 4 * g);
-        const f32x4 d = *reinterpret_cast<const f32x4 *>(rd + first + 8 * j + 4 * g);
+      for (int h = 0; h < 2; ++h) {
+        const int r = first + 16 * h + 4 * g;
+        const f32x4 m = *reinterpret_cast<const f32x4 *>(rm + r), f = *reinterpret_cast<const f32x4 *>(rl + r);
+        const f32x4 d = *reinterpret_cast<const f32x4 *>(rd + r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = 4 * j + e;
-          s[i] = __builtin_amdgcn_exp2f(s[i] - m[e]) * f[e];
-          ds[i] = s[i] * (ds[i] - d[e]);
+          s[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m[e]) * f[e];
+          ds[h][e] = s[h][e] * (ds[h][e] - d[e]);
         }
       }
-      add_columns<DH>(dv, gt, first, lane, s);
-      add_columns<DH>(dk, qt, first, lane, ds);
+      add_columns<DH>(dv, gt, first, lane, split_pair(s));
+      add_columns<DH>(dk, qt, first, lane, split_pair(ds));
     }
   }
   if constexpr (S::OTHER > 1) {
-    float *box = reinterpret_cast<float *>(lds) + kg * 64 * DH + lane;
+    float *box = reinterpret_cast<float *>(lds) + kg * 64 * (DH / 2) + lane;
     __syncthreads();
-    if (rg == 1) give<DH / 32>(box, dk), give<DH / 32>(box + 64 * (DH / 2), dv);
+    if (rg == 1) give<DH / 16>(box, dk), give<DH / 16>(box + 64 * (DH / 4), dv);
     __syncthreads();
     if (rg == 1) return;
-    take<DH / 32>(box, dk), take<DH / 32>(box + 64 * (DH / 2), dv);
+    take<DH / 16>(box, dk), take<DH / 16>(box + 64 * (DH / 4), dv);
   }
   if (key >= p.Nk) return;
   if (!key_ok) {  // (whatever its column held)
 #pragma unroll
-    for (int n = 0; n < DH / 32; ++n) dk[n] = zero16(), dv[n] = zero16();
+    for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
   }
   if (p.splits > 1) {
     const long long pitch = (long long)p.Hkv * p.dh, all = (long long)p.B * p.Nk * pitch;
     const long long at = key_offset(p, pitch, b, hk, key);
-    store<DH>(p.part + split * all + at, dk, p.scale, g, p, p.dh % 4 == 0);
-    store<DH>(p.part + (p.splits + split) * all + at, dv, 1.f, g, p, p.dh % 4 == 0);
+    store_row<DH>(p.part + split * all + at, dk, p.scale, g, p.dh, p.dh % 4 == 0);
+    store_row<DH>(p.part + (p.splits + split) * all + at, dv, 1.f, g, p.dh, p.dh % 4 == 0);
   } else {
-    store<DH>(p.dk.ptr + key_offset(p, p.dk.ld, b, hk, key), dk, p.scale, g, p, p.vec);
-    store<DH>(p.dv.ptr + key_offset(p, p.dv.ld, b, hk, key), dv, 1.f, g, p, p.vec);
+    store_row<DH>(p.dk.ptr + key_offset(p, p.dk.ld, b, hk, key), dk, p.scale, g, p.dh, p.vec);
+    store_row<DH>(p.dv.ptr + key_offset(p, p.dv.ld, b, hk, key), dv, 1.f, g, p.dh, p.vec);
   }
 }
 
@@ -311,14 +237,14 @@ __global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part,
   }
 }
 
-// Groups of 32 in a workgroup, blocks, and how the other side is split.
+// Groups of 16 in a workgroup, blocks, and how the other side is split.
 struct Side {
   int groups, blocks, splits, chunk;
 };
 Side plan_side(long long own, long long other, long long heads) {
   Side s;
-  s.groups = own > 64 ? 4 : own > 32 ? 2 : 1;
-  s.blocks = (int)((own + 32 * s.groups - 1) / (32 * s.groups));
+  s.groups = own > 64 ? 8 : own > 32 ? 4 : 2;
+  s.blocks = (int)((own + 16 * s.groups - 1) / (16 * s.groups));
   const long long stages = (other + 63) / 64, wgs = heads * s.blocks;
   long long splits = 1;
   if (wgs > 0) splits = std::min((long long)vitk::cu_count() / wgs, stages / 8);
@@ -345,21 +271,21 @@ Plan make_plan(const Params &p) {
 
 template <int DH>
 void launch_dq(const Params &p, int groups, unsigned wgs, hipStream_t st) {
-  if (groups == 4)
-    hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
-  else if (groups == 2)
-    hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  if (groups == 8)
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
+  else if (groups == 4)
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((cross_dq_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
+    hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
 template <int DH>
 void launch_dkv(const Params &p, int groups, unsigned wgs, hipStream_t st) {
-  if (groups == 4)
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
-  else if (groups == 2)
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  if (groups == 8)
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
+  else if (groups == 4)
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 2, 1>), dim3(wgs), dim3(128), 0, st, p);
+    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
 void add_parts(const float *part, int splits, long long rows, int width, Result out, hipStream_t st) {
   hipLaunchKernelGGL(cross_add_parts_kernel, dim3(vitk::grid_for(rows * width, 256)), dim3(256), 0, st, part, splits, rows,
