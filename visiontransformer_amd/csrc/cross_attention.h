@@ -29,7 +29,7 @@ struct Params {
   Result out, dq, dk, dv;
   const int32_t *len;
   float *stats;  // [B*H][Nq][2]
-  float *delta;  // backward: [B*H][Nq] dout . out
+  float *delta;  // backward: [B*H][Nq] dout . out / l
   // forward, keys split: [splits][B*H][Nq][dh] unnormalised sums, then [splits][B*H][Nq][2];
   // backward, keys or rows split: [splits][B][N][heads][dh] of one gradient (of dk, then of dv)
   float *part;
@@ -118,22 +118,25 @@ __device__ __forceinline__ f32x4 product6(const Split8 &a, const Split8 &b, f32x
   acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ f32x4 all4(float x) { return f32x4{x, x, x, x}; }
+__device__ __forceinline__ f32x4 zero4() { return all4(0.f); }
 
 // Lane (c = lane & 15, g = lane >> 4) of the instruction supplies A[i = c][k = 8 g ..] and B[k = 8 g ..][j = c] and
 // receives D[i = 4 g + r][j = c] in register r.  Two results for rows 0..15 and 16..31 are the operand
 // B of a contraction over those 32 rows if slot (g, e) stands for row 4 g + e, e < 4, and 16 + 4 g + e - 4:
 // the other operand is read in that order (Tile::columns).
 // A tile of rows x DH in LDS: per row three parts of DH bf16, in units of 16 bytes.  Unit u of a part sits at
-// u ^ spread(row), which puts 16 rows of one unit (a read along the columns) and eight rows of two
-// neighbouring units (a transposed read) on different banks.
+// u ^ spread(row), so that what is accessed together lies on different banks (64 of 4 bytes).  16 bytes a lane:
+// lanes 0-3, 12-15, 20-27 go together, then the other 16 of 32, so a read along the columns takes unit u of
+// rows 0-3 and 12-15 with unit u ^ 1 of rows 4-11.  A transposed read: eight rows of two neighbouring units.
 template <int DH>
 struct Tile {
   static constexpr int PART = DH / 8, ROW = 3 * PART;  // units
   __device__ static __forceinline__ int spread(int row) {
-    if constexpr (DH == 64) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
-    if constexpr (DH == 128) return ((row & 7) << 1) | ((row >> 3) & 1);
-    return (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+    const int high = (row >> 2) & 1;
+    if constexpr (DH == 64) return (((row >> 1) & 3) << 1) | high;
+    if constexpr (DH == 128) return ((row & 7) << 1) | high;
+    return 3 * high;
   }
   __device__ static __forceinline__ void put(bf16x8 *tile, int row, int unit, const Split8 &x) {
 #pragma unroll
@@ -173,11 +176,10 @@ __device__ __forceinline__ Split8 split_pair(const f32x4 (&x)[2]) {
   for (int e = 0; e < 4; ++e) v[e] = x[0][e], v[4 + e] = x[1][e];
   return split8(v);
 }
-// rows first .. first + 31 of a tile times this lane's row f (DH / 32 steps)
+// s += rows first .. first + 31 of a tile times this lane's row f (DH / 32 steps)
 template <int DH>
 __device__ __forceinline__ void rows_times(const bf16x8 *tile, int first, int c, int g, const Split8 (&f)[DH / 32],
                                            f32x4 (&s)[2]) {
-  s[0] = s[1] = zero4();
 #pragma unroll
   for (int i = 0; i < DH / 32; ++i)
 #pragma unroll
@@ -239,7 +241,7 @@ __device__ __forceinline__ void store_row(float *row, const f32x4 (&acc)[DH / 16
 // the other side.
 template <int DH, int NW, int GROUPS>
 struct Shape {
-  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 128 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
+  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 96 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
   static constexpr int THREADS = 64 * NW, ALL = STAGE * DH / 8, TASKS = (ALL + THREADS - 1) / THREADS;
   static constexpr int UNITS = STAGE * Tile<DH>::ROW;
 };
@@ -273,6 +275,19 @@ struct Stage {
     }
   }
 };
+
+// Over how many workgroups the other side of a block is split: the least of whole rounds over the device's
+// places for workgroups (a last round that is hardly filled costs as much as a full one) plus writing and
+// adding the parts.  `us`: time of a whole block; `part_us`: of one part of the results.
+inline int plan_splits(long long wgs, long long places, long long stages, double us, double part_us) {
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 16 && (s == 1 || s * 4 <= stages); ++s) {
+    const double t = (double)((wgs * s + places - 1) / places) / s * us + (s > 1 ? 5.0 + s * part_us : 0.0);
+    if (s == 1 || t < least) best = s, least = t;
+  }
+  return best;
+}
 
 // Argument checks both directions share; fills everything but the launch plan.
 int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Params *p);

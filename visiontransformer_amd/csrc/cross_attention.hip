@@ -76,7 +76,7 @@ using namespace vitk::cross;
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
 // A stage of keys is loaded into registers one stage ahead, split and put into LDS between two barriers.
 template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ? 2 : 1)) void cross_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ? 2 : 1)) void cross_fwd_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int NB = DH / 16, BOX = DH / 4 + 2;  // words a lane passes on: o, m, l
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * BOX * 4 : 0;
@@ -100,7 +100,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ?
   f32x4 o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = zero4();
-  float m = -INFINITY, l = 0.f;
+  float m = 0.f, l = 0.f;
+  bool started = false;  // (uniform)
 
   Stage<DH, NW, RW> next;
   auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ?
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (kg * S::SUB + sub);  // of the stage
       if (t + first >= k1) break;
-      f32x4 s[2];
+      f32x4 s[2] = {all4(-m), all4(-m)};  // the products are added to this: what the exponent wants
       rows_times<DH>(kt, first, c, g, q, s);
       if (t + first + 32 > k1) {
 #pragma unroll
@@ -127,27 +128,33 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ?
       float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
       for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
-      const float m_new = fmaxf(m, column_max(top));
-      if (__any(m_new != m)) {  // (NaN scores: l and o become NaN below)
-        const float fall = __builtin_amdgcn_exp2f(m - m_new);
+      top = column_max(top);
+      if (!started || __any(top > 0.f)) {
+        const float up = started ? fmaxf(top, 0.f) : top, fall = started ? __builtin_amdgcn_exp2f(-up) : 0.f;
+        m += up;
         l *= fall;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[n][e] *= fall;
-        m = m_new;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][e] -= up;
+        started = true;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m);
+          s[h][e] = __builtin_amdgcn_exp2f(s[h][e]);
           l += s[h][e];  // of this lane's quarter of the keys
         }
       add_columns<DH>(o, vt, first, lane, split_pair(s));
     }
   }
   l = column_sum(l);
+  if (!started) m = -INFINITY;
   if constexpr (S::OTHER > 1) {
     static_assert(S::OTHER == 2, "two key groups");
     float *box = reinterpret_cast<float *>(lds) + rg * 64 * BOX + lane;
@@ -398,8 +405,12 @@ FwdPlan plan_fwd(Params *p) {
   } else {
     f.row_groups = p->rows > 64 ? 8 : p->rows > 32 ? 4 : 2;
     p->blocks = (int)(((long long)p->rows + 16 * f.row_groups - 1) / (16 * f.row_groups));
-    const long long groups = heads * p->blocks;
-    if (groups > 0) splits = std::min(2ll * vitk::cu_count() / groups, stages / 4);
+    const int wide = p->dh <= 32 ? 32 : p->dh <= 64 ? 64 : p->dh <= 96 ? 96 : 128;
+    const int resident = (f.row_groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);  // workgroups a CU
+    const double flop = 64.0 * f.row_groups * p->Nk * wide;                   // of a block; 0.6 TFLOP/s a CU
+    const double part = 2.0 * p->B * p->H * p->Nq * p->dh * 4 / 4e6;          // written and read at 4 TB/s
+    splits = vitk::cross::plan_splits(heads * p->blocks, resident * (long long)vitk::cu_count(), stages,
+                                      flop / (0.6e6 / resident), part);
   }
   if (splits > MAX_SPLITS) splits = MAX_SPLITS;
   if (splits < 1) splits = 1;

@@ -1,9 +1,11 @@
 // Cross attention backward without atomics:
-//   dQ (and delta[row] = dout . out): one workgroup per block of rows, all keys in order;
+//   dQ (and delta[row] = dout . out / l): one workgroup per block of rows, all keys in order;
 //   dK, dV: one workgroup per block of keys of one (batch, key head), all rows that read them in order.
 // Both rebuild the probabilities from the stored row statistics,
-//   p = exp2(c s - m) / l,  ds = p (dout v^T - delta),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T dout,
-// with fp32 products in three bf16 parts arranged as in the forward: the accumulator of the first
+//   e = exp2(c s - m),  p = e / l,  ds = p (dout v^T - delta),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T dout,
+// with dout / l and delta / l in the place of dout and delta, so that e needs no factor, and with -m and
+// -delta / l as what the products are added to;
+// the products are fp32 in three bf16 parts, arranged as in the forward: the accumulator of the first
 // product is the operand of the next.  That is seven products where five would do (s and dp are formed
 // twice); one pass would have to add dQ (or dK and dV) up across workgroups.
 // Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves share a group and deal the tiles of the
@@ -50,10 +52,17 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
   const int len = valid_keys(p, b), row = (rb * RW + rg) * 16 + c;
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
   const bool row_ok = row < p.rows;
-  Split8 q[DH / 32], dout[DH / 32];
-  float m = 0.f, f = 0.f, delta = 0.f;
+  Split8 q[DH / 32], dout[DH / 32];  // q times scale log2(e); dout / l
+  float m = 0.f, delta = 0.f;        // delta / l
   {
     const int r = row_ok ? row : 0;
+    float f = 0.f;
+    const long long st = row_stat(p, b, hk, r);
+    if (row_ok) {
+      m = p.stats[2 * st];
+      const float l = p.stats[2 * st + 1];
+      f = l == 0.f ? 0.f : 1.f / l;
+    }
     load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, r), row_ok, g, p.c, p);
     const float *gp = p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r), *op = p.o.ptr + row_offset(p, p.o.ld, b, hk, r);
 #pragma unroll
@@ -64,17 +73,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
         load_eight(op, 32 * i + 8 * g, p, y);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta += x[e] * y[e];
+      for (int e = 0; e < 8; ++e) {
+        delta += x[e] * y[e];
+        x[e] *= f;
+      }
       dout[i] = split8(x);
     }
-    delta = column_sum(delta);
-    if (row_ok) {
-      const long long st = row_stat(p, b, hk, row);
-      m = p.stats[2 * st];
-      const float l = p.stats[2 * st + 1];
-      f = l == 0.f ? 0.f : 1.f / l;
-      if (g == 0 && kg == 0 && split == 0) p.delta[st] = delta;
-    }
+    delta = column_sum(delta) * f;
+    if (row_ok && g == 0 && kg == 0 && split == 0) p.delta[st] = delta;
   }
   f32x4 dq[DH / 16];
 #pragma unroll
@@ -92,13 +98,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (kg * S::SUB + sub);
       if (t + first >= k1) break;
-      f32x4 s[2], ds[2];
+      f32x4 s[2] = {all4(-m), all4(-m)}, ds[2] = {all4(-delta), all4(-delta)};
       rows_times<DH>(kt, first, c, g, q, s);
       rows_times<DH>(vt, first, c, g, dout, ds);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ds[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m) * f * (ds[h][e] - delta);
+        for (int e = 0; e < 4; ++e) ds[h][e] *= __builtin_amdgcn_exp2f(s[h][e]);
       if (t + first + 32 > k1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -131,7 +137,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
-  __shared__ __attribute__((aligned(16))) float rm[S::STAGE], rl[S::STAGE], rd[S::STAGE];
+  __shared__ __attribute__((aligned(16))) float rm[S::STAGE], rd[S::STAGE];
   bf16x8 *qt = reinterpret_cast<bf16x8 *>(lds), *gt = qt + S::UNITS;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, rg = wave / KG;
@@ -155,47 +161,52 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
   Stage<DH, NW, KG> next;
   auto offq = [&](int r) { return row_offset(p, p.q.ld, b, hk, r); };
   auto offg = [&](int r) { return row_offset(p, p.dout.ld, b, hk, r); };
-  float sm = 0.f, sl = 0.f, sd = 0.f;
+  float sm = 0.f, sd = 0.f, sl[S::TASKS];
   auto fetch = [&](int t) {
     next.fetch(p, p.q.ptr, p.dout.ptr, t, r1, offq, offg);
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {  // l of the task's row
+      const int r = t + (threadIdx.x + S::THREADS * u) / (DH / 8);
+      sl[u] = r < r1 ? p.stats[2 * row_stat(p, b, hk, r) + 1] : 0.f;
+    }
     if (threadIdx.x < S::STAGE) {
-      sm = sl = sd = 0.f;  // a row that is not there: p = 1 * 0
+      sm = sd = 0.f;  // a row that is not there: exp2(0) times zeros
       const int r = t + threadIdx.x;
-      if (r < r1) {
-        const long long st = row_stat(p, b, hk, r);
-        sm = p.stats[2 * st], sl = p.stats[2 * st + 1], sd = p.delta[st];
-      }
+      if (r < r1) sm = -p.stats[2 * row_stat(p, b, hk, r)], sd = -p.delta[row_stat(p, b, hk, r)];
     }
   };
   if (r0 < r1) fetch(r0);
   for (int t = r0; t < r1; t += S::STAGE) {
     __syncthreads();
-    next.put(qt, gt);
-    if (threadIdx.x < S::STAGE) {
-      rm[threadIdx.x] = sm;
-      rl[threadIdx.x] = sl == 0.f ? 0.f : 1.f / sl;
-      rd[threadIdx.x] = sd;
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {  // dout / l
+      const float f = sl[u] == 0.f ? 0.f : 1.f / sl[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) next.y[u][e] *= f;
     }
+    next.put(qt, gt);
+    if (threadIdx.x < S::STAGE) rm[threadIdx.x] = sm, rd[threadIdx.x] = sd;
     __syncthreads();
     if (t + S::STAGE < r1) fetch(t + S::STAGE);
 #pragma unroll
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (rg * S::SUB + sub);
       if (t + first >= r1) break;
-      f32x4 s[2], ds[2];
+      f32x4 s[2], ds[2];  // start from -m and -delta / l of their rows
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = *reinterpret_cast<const f32x4 *>(rm + first + 16 * h + 4 * g);
+        ds[h] = *reinterpret_cast<const f32x4 *>(rd + first + 16 * h + 4 * g);
+      }
       rows_times<DH>(qt, first, c, g, k, s);
       rows_times<DH>(gt, first, c, g, v, ds);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = first + 16 * h + 4 * g;
-        const f32x4 m = *reinterpret_cast<const f32x4 *>(rm + r), f = *reinterpret_cast<const f32x4 *>(rl + r);
-        const f32x4 d = *reinterpret_cast<const f32x4 *>(rd + r);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[h][e] = __builtin_amdgcn_exp2f(s[h][e] - m[e]) * f[e];
-          ds[h][e] = s[h][e] * (ds[h][e] - d[e]);
+          s[h][e] = __builtin_amdgcn_exp2f(s[h][e]);
+          ds[h][e] *= s[h][e];
         }
-      }
       add_columns<DH>(dv, gt, first, lane, split_pair(s));
       add_columns<DH>(dk, qt, first, lane, split_pair(ds));
     }
@@ -241,14 +252,16 @@ __global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part,
 struct Side {
   int groups, blocks, splits, chunk;
 };
-Side plan_side(long long own, long long other, long long heads) {
+Side plan_side(long long own, long long other, long long heads, int dh, int products, double part_us) {
   Side s;
   s.groups = own > 64 ? 8 : own > 32 ? 4 : 2;
   s.blocks = (int)((own + 16 * s.groups - 1) / (16 * s.groups));
-  const long long stages = (other + 63) / 64, wgs = heads * s.blocks;
-  long long splits = 1;
-  if (wgs > 0) splits = std::min((long long)vitk::cu_count() / wgs, stages / 8);
-  splits = std::min(std::max(splits, 1ll), 64ll);
+  const long long stages = (other + 63) / 64;
+  const int wide = dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128;
+  const int resident = s.groups == 2 ? 2 : 1;  // workgroups a CU
+  const double flop = 32.0 * products * s.groups * other * wide;  // of a block; 0.5 TFLOP/s a CU
+  const int splits = plan_splits(heads * s.blocks, resident * (long long)vitk::cu_count(), stages,
+                                 flop / (0.5e6 / resident), part_us);
   s.chunk = std::max((int)((stages + splits - 1) / splits) * 64, 64);
   s.splits = std::max((int)((other + s.chunk - 1) / s.chunk), 1);
   return s;
@@ -260,8 +273,9 @@ struct Plan {
 Plan make_plan(const Params &p) {
   Plan n;
   const long long heads = (long long)p.B * p.Hkv;
-  n.rows = plan_side(p.rows, p.Nk, heads);
-  n.keys = plan_side(p.Nk, p.rows, heads);
+  // one part of the results, written and read at 4 TB/s
+  n.rows = plan_side(p.rows, p.Nk, heads, p.dh, 3, 2.0 * p.B * p.H * p.Nq * p.dh * 4 / 4e6);
+  n.keys = plan_side(p.Nk, p.rows, heads, p.dh, 4, 4.0 * p.B * p.Hkv * p.Nk * p.dh * 4 / 4e6);
   n.delta = ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
   const size_t q = n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
   const size_t k = n.keys.splits > 1 ? (size_t)2 * n.keys.splits * p.B * p.Nk * p.Hkv * p.dh : 0;
