@@ -55,6 +55,19 @@ __device__ __forceinline__ long long key_offset(const Params &p, long long ld, i
 __device__ __forceinline__ int valid_keys(const Params &p, int b) {
   return p.len ? min(max(p.len[b], 0), p.Nk) : p.Nk;
 }
+// The batch entry whose workgroups come `place`-th: the longest first, so that the last ones to start are short
+// (only an order of work: every entry has one place).  Up to 64 entries, a lane each.
+__device__ __forceinline__ int by_length(const Params &p, int place) {
+  if (!p.len || p.B > 64) return place;
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < p.B ? valid_keys(p, lane) : -1;
+  int rank = 0;
+  for (int j = 0; j < p.B; ++j) {
+    const int other = __builtin_amdgcn_readlane(mine, j);
+    rank += other > mine || (other == mine && j < lane);
+  }
+  return __builtin_ctzll(__ballot(lane < p.B && rank == place));
+}
 
 // Columns d .. d+3 of a row; zeros behind dh.
 __device__ __forceinline__ f32x4 load_quad(const float *row, int d, int dh, bool vec) {
@@ -275,6 +288,10 @@ struct Stage {
     }
   }
 };
+
+// Groups of 16 rows in a workgroup.  (Smaller blocks where they leave fewer empty rows do not pay: 147 rows of 64
+// over 50 keys in blocks of 128, 64 and 32: 22.7, 25.0 and 30.8 us.)
+inline int plan_groups(long long rows) { return rows > 64 ? 8 : rows > 32 ? 4 : 2; }
 
 // Over how many workgroups the other side of a block is split: the least of whole rounds over the device's
 // places for workgroups (a last round that is hardly filled costs as much as a full one) plus writing and

@@ -112,6 +112,7 @@ __global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <
     next.put(kt, vt);
     __syncthreads();
     if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
+    if ((rb * RW + rg) * 16 >= p.rows) continue;  // no row in this wave
 #pragma unroll
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (kg * S::SUB + sub);  // of the stage
@@ -403,7 +404,7 @@ FwdPlan plan_fwd(Params *p) {
         splits = std::min((12 * cus + heads - 1) / heads, stages / 4);
     }
   } else {
-    f.row_groups = p->rows > 64 ? 8 : p->rows > 32 ? 4 : 2;
+    f.row_groups = plan_groups(p->rows);
     p->blocks = (int)(((long long)p->rows + 16 * f.row_groups - 1) / (16 * f.row_groups));
     const int wide = p->dh <= 32 ? 32 : p->dh <= 64 ? 64 : p->dh <= 96 ? 96 : 128;
     const int resident = (f.row_groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);  // workgroups a CU

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
   wg /= p.blocks;
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
-  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int b = by_length(p, (int)(wg % p.B)), split = (int)(wg / p.B);
   const int len = valid_keys(p, b), row = (rb * RW + rg) * 16 + c;
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
   const bool row_ok = row < p.rows;
@@ -94,6 +94,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
     next.put(kt, vt);
     __syncthreads();
     if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
+    if ((rb * RW + rg) * 16 >= p.rows) continue;  // no row in this wave
 #pragma unroll
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (kg * S::SUB + sub);
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
   wg /= p.blocks;
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
-  const int b = (int)(wg % p.B), split = (int)(wg / p.B);
+  const int b = by_length(p, (int)(wg % p.B)), split = (int)(wg / p.B);
   const int len = valid_keys(p, b), key = (kb * KG + kg) * 16 + c;
   const bool key_ok = key < len;
   Split8 k[DH / 32], v[DH / 32];
@@ -188,6 +189,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
     if (threadIdx.x < S::STAGE) rm[threadIdx.x] = sm, rd[threadIdx.x] = sd;
     __syncthreads();
     if (t + S::STAGE < r1) fetch(t + S::STAGE);
+    if ((kb * KG + kg) * 16 >= len) continue;  // no key in this wave
 #pragma unroll
     for (int sub = 0; sub < S::SUB; ++sub) {
       const int first = 32 * (rg * S::SUB + sub);
@@ -254,7 +256,7 @@ struct Side {
 };
 Side plan_side(long long own, long long other, long long heads, int dh, int products, double part_us) {
   Side s;
-  s.groups = own > 64 ? 8 : own > 32 ? 4 : 2;
+  s.groups = plan_groups(own);
   s.blocks = (int)((own + 16 * s.groups - 1) / (16 * s.groups));
   const long long stages = (other + 63) / 64;
   const int wide = dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128;
