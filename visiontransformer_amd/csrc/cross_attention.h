@@ -251,41 +251,43 @@ __device__ __forceinline__ void store_row(float *row, const f32x4 (&acc)[DH / 16
 }
 
 // NW waves, GROUPS of 16 rows (or keys); OTHER = waves that share a group and deal the 32-row tiles of a stage of
-// the other side.
+// the other side.  A stage (two tensors) is loaded into registers, split and put into one of two buffers while
+// the waves work on the other one: half of the waves before their products, half after them, so that on each
+// SIMD one wave splits while the other multiplies.  (With OTHER = 2 a stage is twice as long and has one buffer:
+// two would leave room for one workgroup a CU.)
 template <int DH, int NW, int GROUPS>
 struct Shape {
-  static constexpr int OTHER = NW / GROUPS, STAGE = DH < 96 || OTHER > 1 ? 64 : 32, SUB = STAGE / 32 / OTHER;
-  static constexpr int THREADS = 64 * NW, ALL = STAGE * DH / 8, TASKS = (ALL + THREADS - 1) / THREADS;
-  static constexpr int UNITS = STAGE * Tile<DH>::ROW;
+  static constexpr int OTHER = NW / GROUPS, STAGE = 32 * OTHER, BUFFERS = OTHER == 1 ? 2 : 1;
+  static constexpr int THREADS = 64 * NW, HALF = STAGE * DH / 8, TASKS = (2 * HALF + THREADS - 1) / THREADS;
+  static constexpr int UNITS = STAGE * Tile<DH>::ROW;  // of a tensor; a buffer holds two
 };
-// Two tensors' next stage in registers (8 columns of a row, per tensor and task), then split into LDS.
+// Eight columns of a row per task: first those of x, then those of y.
 template <int DH, int NW, int GROUPS>
 struct Stage {
   typedef Shape<DH, NW, GROUPS> S;
-  float x[S::TASKS][8], y[S::TASKS][8];
-  template <class OffX, class OffY>
-  __device__ __forceinline__ void fetch(const Params &p, const float *px, const float *py, int first, int end, OffX offx,
-                                        OffY offy) {
+  float v[S::TASKS][8];
+  __device__ static __forceinline__ int task(int u) { return threadIdx.x + S::THREADS * u; }
+  __device__ static __forceinline__ bool any(int u) { return 2 * S::HALF % S::THREADS == 0 || task(u) < 2 * S::HALF; }
+  __device__ static __forceinline__ bool is_y(int u) { return task(u) >= S::HALF; }
+  __device__ static __forceinline__ int row(int u) { return (task(u) - (is_y(u) ? S::HALF : 0)) / (DH / 8); }
+  __device__ static __forceinline__ int unit(int u) { return task(u) % (DH / 8); }
+  // at(y, row): the row's first element
+  template <class At>
+  __device__ __forceinline__ void fetch(const Params &p, int first, int end, At at) {
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {
-      const int task = threadIdx.x + S::THREADS * u, r = first + task / (DH / 8), d = task % (DH / 8) * 8;
-      if (r < end && (S::ALL % S::THREADS == 0 || task < S::ALL)) {
-        load_eight(px + offx(r), d, p, x[u]);
-        load_eight(py + offy(r), d, p, y[u]);
+      if (any(u) && first + row(u) < end) {
+        load_eight(at(is_y(u), first + row(u)), unit(u) * 8, p, v[u]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = y[u][e] = 0.f;
+        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
       }
     }
   }
-  __device__ __forceinline__ void put(bf16x8 *tx, bf16x8 *ty) const {
+  __device__ __forceinline__ void put(bf16x8 *buffer) const {
 #pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {
-      const int task = threadIdx.x + S::THREADS * u;
-      if (S::ALL % S::THREADS != 0 && task >= S::ALL) continue;
-      Tile<DH>::put(tx, task / (DH / 8), task % (DH / 8), split8(x[u]));
-      Tile<DH>::put(ty, task / (DH / 8), task % (DH / 8), split8(y[u]));
-    }
+    for (int u = 0; u < S::TASKS; ++u)
+      if (any(u)) Tile<DH>::put(buffer + (is_y(u) ? S::UNITS : 0), row(u), unit(u), split8(v[u]));
   }
 };
 

@@ -74,14 +74,13 @@ using namespace vitk::cross;
 
 // NW waves: RW groups of 16 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
-// A stage of keys is loaded into registers one stage ahead, split and put into LDS between two barriers.
 template <int DH, int NW, int RW>
 __global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ? 2 : 1)) void cross_fwd_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int NB = DH / 16, BOX = DH / 4 + 2;  // words a lane passes on: o, m, l
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * BOX * 4 : 0;
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
-  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + S::UNITS;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
+  bf16x8 *buffers = reinterpret_cast<bf16x8 *>(lds);
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
@@ -104,19 +103,26 @@ __global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <
   bool started = false;  // (uniform)
 
   Stage<DH, NW, RW> next;
-  auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
-  auto offv = [&](int n) { return key_offset(p, p.v.ld, b, hk, n); };
-  if (k0 < k1) next.fetch(p, p.k.ptr, p.v.ptr, k0, k1, offk, offv);
-  for (int t = k0; t < k1; t += S::STAGE) {
+  auto at = [&](bool y, int n) {
+    return y ? p.v.ptr + key_offset(p, p.v.ld, b, hk, n) : p.k.ptr + key_offset(p, p.k.ld, b, hk, n);
+  };
+  const bool early = wave < NW / 2, empty = (rb * RW + rg) * 16 >= p.rows;
+  next.fetch(p, k0, k1, at);
+  if constexpr (S::BUFFERS == 2) {
+    next.put(buffers);
+    next.fetch(p, k0 + S::STAGE, k1, at);
     __syncthreads();
-    next.put(kt, vt);
-    __syncthreads();
-    if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
-    if ((rb * RW + rg) * 16 >= p.rows) continue;  // no row in this wave
-#pragma unroll
-    for (int sub = 0; sub < S::SUB; ++sub) {
-      const int first = 32 * (kg * S::SUB + sub);  // of the stage
-      if (t + first >= k1) break;
+  }
+  for (int t = k0, n = 0; t < k1; t += S::STAGE, n ^= S::BUFFERS - 1) {
+    const bf16x8 *kt = buffers + n * 2 * S::UNITS, *vt = kt + S::UNITS;
+    auto advance = [&] {
+      next.put(buffers + (S::BUFFERS - 1 - n) * 2 * S::UNITS);
+      if constexpr (S::BUFFERS == 1) __syncthreads();
+      next.fetch(p, t + S::BUFFERS * S::STAGE, k1, at);
+    };
+    if (S::BUFFERS == 1 || early) advance();
+    const int first = 32 * kg;  // of the stage
+    if (!empty && t + first < k1) {
       f32x4 s[2] = {all4(-m), all4(-m)};  // the products are added to this: what the exponent wants
       rows_times<DH>(kt, first, c, g, q, s);
       if (t + first + 32 > k1) {
@@ -153,6 +159,8 @@ __global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <
         }
       add_columns<DH>(o, vt, first, lane, split_pair(s));
     }
+    if (S::BUFFERS == 2 && !early) advance();
+    __syncthreads();
   }
   l = column_sum(l);
   if (!started) m = -INFINITY;

@@ -39,8 +39,8 @@ template <int DH, int NW, int RW>
 __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 4) * 4 : 0;
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
-  bf16x8 *kt = reinterpret_cast<bf16x8 *>(lds), *vt = kt + S::UNITS;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
+  bf16x8 *buffers = reinterpret_cast<bf16x8 *>(lds);
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RW, kg = wave / RW;
   long long wg = blockIdx.x;
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
   wg /= p.blocks;
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
-  const int b = by_length(p, (int)(wg % p.B)), split = (int)(wg / p.B);
+  const int split = (int)(wg % p.splits), b = by_length(p, (int)(wg / p.splits));
   const int len = valid_keys(p, b), row = (rb * RW + rg) * 16 + c;
   const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
   const bool row_ok = row < p.rows;
@@ -86,19 +86,26 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
 #pragma unroll
   for (int n = 0; n < DH / 16; ++n) dq[n] = zero4();
   Stage<DH, NW, RW> next;
-  auto offk = [&](int n) { return key_offset(p, p.k.ld, b, hk, n); };
-  auto offv = [&](int n) { return key_offset(p, p.v.ld, b, hk, n); };
-  if (k0 < k1) next.fetch(p, p.k.ptr, p.v.ptr, k0, k1, offk, offv);
-  for (int t = k0; t < k1; t += S::STAGE) {
+  auto at = [&](bool y, int n) {
+    return y ? p.v.ptr + key_offset(p, p.v.ld, b, hk, n) : p.k.ptr + key_offset(p, p.k.ld, b, hk, n);
+  };
+  const bool early = wave < NW / 2, empty = (rb * RW + rg) * 16 >= p.rows;
+  next.fetch(p, k0, k1, at);
+  if constexpr (S::BUFFERS == 2) {
+    next.put(buffers);
+    next.fetch(p, k0 + S::STAGE, k1, at);
     __syncthreads();
-    next.put(kt, vt);
-    __syncthreads();
-    if (t + S::STAGE < k1) next.fetch(p, p.k.ptr, p.v.ptr, t + S::STAGE, k1, offk, offv);
-    if ((rb * RW + rg) * 16 >= p.rows) continue;  // no row in this wave
-#pragma unroll
-    for (int sub = 0; sub < S::SUB; ++sub) {
-      const int first = 32 * (kg * S::SUB + sub);
-      if (t + first >= k1) break;
+  }
+  for (int t = k0, n = 0; t < k1; t += S::STAGE, n ^= S::BUFFERS - 1) {
+    const bf16x8 *kt = buffers + n * 2 * S::UNITS, *vt = kt + S::UNITS;
+    auto advance = [&] {
+      next.put(buffers + (S::BUFFERS - 1 - n) * 2 * S::UNITS);
+      if constexpr (S::BUFFERS == 1) __syncthreads();
+      next.fetch(p, t + S::BUFFERS * S::STAGE, k1, at);
+    };
+    if (S::BUFFERS == 1 || early) advance();
+    const int first = 32 * kg;
+    if (!empty && t + first < k1) {
       f32x4 s[2] = {all4(-m), all4(-m)}, ds[2] = {all4(-delta), all4(-delta)};
       rows_times<DH>(kt, first, c, g, q, s);
       rows_times<DH>(vt, first, c, g, dout, ds);
@@ -115,6 +122,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
       }
       add_columns<DH>(dq, kt, first, lane, split_pair(ds));
     }
+    if (S::BUFFERS == 2 && !early) advance();
+    __syncthreads();
   }
   if constexpr (S::OTHER > 1) {
     float *box = reinterpret_cast<float *>(lds) + rg * 64 * (DH / 4) + lane;
@@ -137,9 +146,9 @@ template <int DH, int NW, int KG>
 __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::UNITS * 16 > JOIN ? 2 * S::UNITS * 16 : JOIN];
-  __shared__ __attribute__((aligned(16))) float rm[S::STAGE], rd[S::STAGE];
-  bf16x8 *qt = reinterpret_cast<bf16x8 *>(lds), *gt = qt + S::UNITS;
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
+  __shared__ __attribute__((aligned(16))) float rm[S::BUFFERS][S::STAGE], rd[S::BUFFERS][S::STAGE];
+  bf16x8 *buffers = reinterpret_cast<bf16x8 *>(lds);
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, rg = wave / KG;
   long long wg = blockIdx.x;
@@ -147,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
   wg /= p.blocks;
   const int hk = (int)(wg % p.Hkv);
   wg /= p.Hkv;
-  const int b = by_length(p, (int)(wg % p.B)), split = (int)(wg / p.B);
+  const int split = (int)(wg % p.splits), b = by_length(p, (int)(wg / p.splits));
   const int len = valid_keys(p, b), key = (kb * KG + kg) * 16 + c;
   const bool key_ok = key < len;
   Split8 k[DH / 32], v[DH / 32];
@@ -160,15 +169,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
   const int r0 = min((long long)split * p.chunk, (long long)p.rows);
   const int r1 = kb * KG * 16 < len ? (int)min((long long)r0 + p.chunk, (long long)p.rows) : r0;
   Stage<DH, NW, KG> next;
-  auto offq = [&](int r) { return row_offset(p, p.q.ld, b, hk, r); };
-  auto offg = [&](int r) { return row_offset(p, p.dout.ld, b, hk, r); };
+  auto at = [&](bool y, int r) {
+    return y ? p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r) : p.q.ptr + row_offset(p, p.q.ld, b, hk, r);
+  };
   float sm = 0.f, sd = 0.f, sl[S::TASKS];
   auto fetch = [&](int t) {
-    next.fetch(p, p.q.ptr, p.dout.ptr, t, r1, offq, offg);
+    next.fetch(p, t, r1, at);
 #pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {  // l of the task's row
-      const int r = t + (threadIdx.x + S::THREADS * u) / (DH / 8);
-      sl[u] = r < r1 ? p.stats[2 * row_stat(p, b, hk, r) + 1] : 0.f;
+    for (int u = 0; u < S::TASKS; ++u) {  // l of a task's row of dout
+      const int r = t + next.row(u);
+      sl[u] = next.any(u) && next.is_y(u) && r < r1 ? p.stats[2 * row_stat(p, b, hk, r) + 1] : 1.f;
     }
     if (threadIdx.x < S::STAGE) {
       sm = sd = 0.f;  // a row that is not there: exp2(0) times zeros
@@ -176,29 +186,38 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
       if (r < r1) sm = -p.stats[2 * row_stat(p, b, hk, r)], sd = -p.delta[row_stat(p, b, hk, r)];
     }
   };
-  if (r0 < r1) fetch(r0);
-  for (int t = r0; t < r1; t += S::STAGE) {
-    __syncthreads();
+  auto put = [&](int n) {
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {  // dout / l
       const float f = sl[u] == 0.f ? 0.f : 1.f / sl[u];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) next.y[u][e] *= f;
+      for (int e = 0; e < 8; ++e) next.v[u][e] *= f;
     }
-    next.put(qt, gt);
-    if (threadIdx.x < S::STAGE) rm[threadIdx.x] = sm, rd[threadIdx.x] = sd;
+    next.put(buffers + n * 2 * S::UNITS);
+    if (threadIdx.x < S::STAGE) rm[n][threadIdx.x] = sm, rd[n][threadIdx.x] = sd;
+  };
+  const bool early = wave < NW / 2, empty = (kb * KG + kg) * 16 >= len;
+  fetch(r0);
+  if constexpr (S::BUFFERS == 2) {
+    put(0);
+    fetch(r0 + S::STAGE);
     __syncthreads();
-    if (t + S::STAGE < r1) fetch(t + S::STAGE);
-    if ((kb * KG + kg) * 16 >= len) continue;  // no key in this wave
-#pragma unroll
-    for (int sub = 0; sub < S::SUB; ++sub) {
-      const int first = 32 * (rg * S::SUB + sub);
-      if (t + first >= r1) break;
+  }
+  for (int t = r0, n = 0; t < r1; t += S::STAGE, n ^= S::BUFFERS - 1) {
+    const bf16x8 *qt = buffers + n * 2 * S::UNITS, *gt = qt + S::UNITS;
+    auto advance = [&] {
+      put(S::BUFFERS - 1 - n);
+      if constexpr (S::BUFFERS == 1) __syncthreads();
+      fetch(t + S::BUFFERS * S::STAGE);
+    };
+    if (S::BUFFERS == 1 || early) advance();
+    const int first = 32 * rg;
+    if (!empty && t + first < r1) {
       f32x4 s[2], ds[2];  // start from -m and -delta / l of their rows
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s[h] = *reinterpret_cast<const f32x4 *>(rm + first + 16 * h + 4 * g);
-        ds[h] = *reinterpret_cast<const f32x4 *>(rd + first + 16 * h + 4 * g);
+        s[h] = *reinterpret_cast<const f32x4 *>(rm[n] + first + 16 * h + 4 * g);
+        ds[h] = *reinterpret_cast<const f32x4 *>(rd[n] + first + 16 * h + 4 * g);
       }
       rows_times<DH>(qt, first, c, g, k, s);
       rows_times<DH>(gt, first, c, g, v, ds);
@@ -212,6 +231,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dk
       add_columns<DH>(dv, gt, first, lane, split_pair(s));
       add_columns<DH>(dk, qt, first, lane, split_pair(ds));
     }
+    if (S::BUFFERS == 2 && !early) advance();
+    __syncthreads();
   }
   if constexpr (S::OTHER > 1) {
     float *box = reinterpret_cast<float *>(lds) + kg * 64 * (DH / 2) + lane;
