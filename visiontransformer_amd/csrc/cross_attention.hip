@@ -212,9 +212,50 @@ __global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <
   }
 }
 
-// Joins the parts of a split row: one wave per row, a lane per part for the statistics, then lanes over the columns.
-constexpr int MAX_SPLITS = 64;
+constexpr int MAX_SPLITS = 64, JOIN_FEW = 8;
+// Joins up to eight parts of split rows: LP lanes per row, four columns each, all parts in flight.
+template <int LP>
 __global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
+  const long long all = (long long)p.B * p.H * p.Nq;
+  const long long r = (blockIdx.x * 256ll + threadIdx.x) / LP;
+  if (r >= all) return;
+  const int d = threadIdx.x % LP * 4;
+  const bool vec = p.dh % 4 == 0;
+  const float *st = p.part + p.splits * all * p.dh + 2 * r, *src = p.part + r * p.dh;
+  float ms[JOIN_FEW], ls[JOIN_FEW], m = -INFINITY, l = 0.f;
+  f32x4 x[JOIN_FEW], o = zero4();
+#pragma unroll
+  for (int s = 0; s < JOIN_FEW; ++s) {
+    ms[s] = -INFINITY, ls[s] = 0.f, x[s] = zero4();
+    if (s < p.splits) {
+      ms[s] = st[s * all * 2], ls[s] = st[s * all * 2 + 1];
+      x[s] = load_quad(src + s * all * p.dh, d, p.dh, vec);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < JOIN_FEW; ++s) m = fmaxf(m, ms[s]);
+  if (m == -INFINITY) m = 0.f;  // no key at all
+#pragma unroll
+  for (int s = 0; s < JOIN_FEW; ++s) {
+    const float f = __builtin_amdgcn_exp2f(ms[s] - m);
+    l += f * ls[s];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * x[s][e];
+  }
+  const float scale = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= scale;
+  const long long bh = r / p.Nq, n = r % p.Nq, b = bh / p.H, h = bh % p.H;
+  store_quad(p.out.ptr + (b * p.Nq + n) * p.out.ld + h * p.dh, d, p.dh, p.vec, o);
+  if (d == 0 && p.stats) {
+    p.stats[2 * r] = m;
+    p.stats[2 * r + 1] = l;
+  }
+}
+
+// More than eight parts (few rows): one wave per row, a lane per part for the statistics, then lanes over the
+// columns; every part's statistics arrive in one round trip (49 parts of 256 rows: 4.8 us, in batches of eight 23).
+__global__ __launch_bounds__(256) void cross_join_many_kernel(const Params p) {
   const long long all = (long long)p.B * p.H * p.Nq;
   const int lane = threadIdx.x & 63;
   const long long r = blockIdx.x * 4ll + (threadIdx.x >> 6);
@@ -508,9 +549,17 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
     launch_fwd<128>(p, rg, grid, st);
   }
   if (p.splits > 1) {
-    const long long all = (long long)p.B * p.H * p.Nq;
-    VITK_REQUIRE((all + 3) / 4 < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
-    hipLaunchKernelGGL(cross_join_kernel, dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
+    const int lp = p.splits > JOIN_FEW ? 64 : p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32;
+    const long long blocks = ((long long)p.B * p.H * p.Nq * lp + 255) / 256;
+    VITK_REQUIRE(blocks < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
+    if (lp == 64)
+      hipLaunchKernelGGL(cross_join_many_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else if (lp == 8)
+      hipLaunchKernelGGL(cross_join_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else if (lp == 16)
+      hipLaunchKernelGGL(cross_join_kernel<16>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL(cross_join_kernel<32>, dim3((unsigned)blocks), dim3(256), 0, st, p);
   }
   return vitk::check_launch("vitk_cross_sdpa_fwd");
 }
