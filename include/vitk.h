@@ -307,9 +307,10 @@ int vitk_sdpa_row_bwd(const float *q, int64_t ld_q, const float *k, const float 
  * written as 0.  A row without a key gives out = 0, stats = {0, 0} and no gradient.
  * stats (optional in the forward, required by the backward; [B*H][Nq][2]): {row maximum of the
  * scaled scores times log2(e), row sum of exp(score - maximum)}.
- * Any Nq, Nk >= 0, 1 <= dh <= 128, any alignment.  Operands are finite fp32 numbers below 3.38e38 (an infinity
- * among them gives NaN).  Outputs must not overlap inputs.  The sum over a row's
- * keys may be split over workgroups, a rule on the sizes; every result has a fixed order of sums.
+ * Any Nq, Nk >= 0, 1 <= dh <= 128, any alignment.  Products are formed to fp32 accuracy from three
+ * bf16 parts of each operand: finite numbers below 3.38e38 (an infinity among them gives NaN);
+ * numbers below 2^-100 keep fewer than 24 bits.  Outputs must not overlap inputs or each other.  The sum over
+ * a row's keys may be split over workgroups, a rule on the sizes; every result has a fixed order of sums.
  * workspace: vitk_cross_sdpa_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments (0 =
  * none needed); one call at a time may use it (two captured graphs replayed at once need two). */
 typedef struct vitk_cross_sdpa_args {
@@ -352,7 +353,8 @@ int vitk_cross_sdpa_bwd(const vitk_cross_sdpa_args *args, vitk_stream_t stream);
  * index: device array of `rows` int32 values; a value outside [0, V) (padding) gives a row of zeros
  * and adds to no gradient.  table / dtable are [V][D], out / dout [rows][D].  The backward sorts
  * the tokens (stable) and adds each token's rows in a fixed order: no floating-point atomics, the
- * same bits on every call.  accumulate == 0 writes every row of dtable. */
+ * same bits on every call.  accumulate == 0 writes every row of dtable.  Outputs must not overlap inputs.
+ * workspace: vitk_embedding_bwd_workspace_bytes (0 = none needed), 16-byte aligned, one call at a time. */
 int vitk_embedding_fwd(const float *table, int64_t V, const int32_t *index, int64_t rows, int64_t D, float scale,
                        float *out, vitk_stream_t stream);
 size_t vitk_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D);
@@ -446,14 +448,15 @@ int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float 
  * ptr[k*stride + i*ld + j]):
  *   y = x / (|x|_F + eps);  `steps` times: g = y y^T, y = a y + (b g + c g g) y;  out = y
  * (y^T y on the other side where rows > cols: the same polynomial of the singular values.)  The
- * Frobenius norm is summed in double precision; products take fp32 operands as two fp16 parts each
- * (22 significant bits, three matrix products, fp32 sums), the iterate y itself stays in fp32.
- * out may be x.  0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1]
+ * Frobenius norm is summed in double precision; between products y and g are pairs of fp16 numbers, 32
+ * bits within 2^-23 of the value, and a product is three matrix products of parts with fp32 sums: as
+ * close to the exact result as the same steps in fp32.  A zero matrix gives zeros (NaN with eps = 0).
+ * out may be x, with one layout for both; no other overlap.  0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1]
  * within [-4, 4], with |b t^2 + c t^4| below 31 (checked on 65 points), which every useful triple does.
  * vitk_muon_f32 (p, g, m share ld and stride, as arenas of one layout do):
  *   m = momentum*m + grad_scale*g;  u = nesterov ? grad_scale*g + momentum*m : m
  *   p = p * (1 - lr*weight_decay) - lr*update_scale * NS(u)
- * workspace: *_workspace_bytes of the same arguments, 16-byte aligned, one call at a time. */
+ * workspace: *_workspace_bytes of the same sizes (0 = none needed), 16-byte aligned, one call at a time. */
 typedef struct vitk_newton_schulz_args {
   int32_t rows, cols, batch, steps;
   const float *x;

@@ -163,6 +163,56 @@ def test_cross_attention_forward_and_backward(K, name):
 
 
 @gpu
+@pytest.mark.parametrize("dh", [20, 64, 88, 128])
+def test_cross_attention_every_block_size(K, dh):
+    """Rows and keys of each count of 16-row groups (2, 4, 8, more than one block) against each other."""
+    for Nq in (17, 40, 100, 131):
+        for Nk in (13, 33, 70, 140):
+            g = rng(1000 * Nq + Nk)
+            q, k, v, dout = randn(g, 2, Nq, 2, dh), randn(g, 2, Nk, 2, dh), randn(g, 2, Nk, 2, dh), randn(g, 2, Nq, 2, dh)
+            lens = [Nk, Nk - 7]
+            want, tol, _ = attention64(q, k, v, lens, dh ** -0.5, dout)
+            out, dq, dk, dv = (torch.full_like(x, 7.0) for x in (q, q, k, v))
+            a = K.cross_sdpa_args(q, k, v, out, key_len=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                  stats=torch.empty(4, Nq, 2, device="cuda"), dout=dout, dq=dq, dk=dk, dv=dv)
+            K.cross_sdpa_fwd(a)
+            K.cross_sdpa_bwd(a)
+            for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+                within(t, want[n], tol[n], f"{n} {Nq} x {Nk}")
+
+
+@gpu
+@pytest.mark.parametrize("dh", [8, 60, 100])
+def test_cross_attention_few_rows_of_every_count(K, dh):
+    for rows in range(1, 9):
+        for Nk in (3, 300, 2500):  # one launch of sixteen waves; split and joined
+            g = rng(10 * rows + Nk)
+            q, k, v = randn(g, 2, 1, rows, dh), randn(g, 2, Nk, 1, dh), randn(g, 2, Nk, 1, dh)
+            lens = [Nk - 2, Nk]
+            want, tol, wst = attention64(q, k, v, lens, -dh ** -0.5)
+            out, st = torch.full_like(q, 7.0), torch.empty(2 * rows, 1, 2, device="cuda")
+            K.cross_sdpa_fwd(K.cross_sdpa_args(q, k, v, out, key_len=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                               stats=st, scale=-dh ** -0.5))
+            within(out, want["out"], tol["out"], f"{rows} rows, {Nk} keys")
+            l = st.double().cpu().view(2, rows, 1, 2)[..., 1]
+            assert ((l - wst[..., 1]).abs() <= 1e-4 * (1 + wst[..., 1])).all()
+
+
+@gpu
+def test_cross_attention_splits_where_blocks_are_few(K):
+    """The forms with parts really run at the sizes that the tests above use for them."""
+    def need(fn, **kw):
+        return fn(C.byref(_xargs(K, **kw)))
+    d = K.dll()
+    long_keys = dict(B=1, H=2, Hkv=1, Nq=40, Nk=3001, dh=64, ld_q=128, ld_k=64, ld_v=64, ld_out=128, ld_dout=128, ld_dq=128,
+                     ld_dk=64, ld_dv=64)
+    assert need(d.vitk_cross_sdpa_fwd_workspace_bytes, **long_keys) > 0
+    assert need(d.vitk_cross_sdpa_bwd_workspace_bytes, **long_keys) > 4096
+    long_rows = dict(long_keys, Nq=1500, Nk=70)
+    assert need(d.vitk_cross_sdpa_bwd_workspace_bytes, **long_rows) > 4 * 2 * 1500 + 4096
+
+
+@gpu
 def test_cross_attention_leaves_what_is_between_the_rows(K):
     g = rng(5)
     B, H, N, dh = 2, 3, 11, 20
@@ -556,9 +606,9 @@ def test_muon_captured_and_replayed(K):
 # ------------------------------------------------------------------------------------- refusals
 def _xargs(vitk, **kw):
     a = vitk.CrossSdpaArgs()
-    d = dict(B=2, H=4, Hkv=2, Nq=3, Nk=5, dh=8, scale=1.0, q=4096, ld_q=32, k=4096, ld_k=16, v=4096, ld_v=16, out=4096,
-             ld_out=32, stats=4096, dout=4096, ld_dout=32, dq=4096, ld_dq=32, dk=4096, ld_dk=16, dv=4096, ld_dv=16,
-             workspace=4096, workspace_bytes=1 << 20)
+    d = dict(B=2, H=4, Hkv=2, Nq=3, Nk=5, dh=8, scale=1.0, q=4096, ld_q=32, k=8192, ld_k=16, v=12288, ld_v=16, out=16384,
+             ld_out=32, stats=20480, dout=24576, ld_dout=32, dq=28672, ld_dq=32, dk=32768, ld_dk=16, dv=36864, ld_dv=16,
+             workspace=40960, workspace_bytes=1 << 20)
     d.update(kw)
     for n, x in d.items():
         setattr(a, n, x)
@@ -570,7 +620,7 @@ def _xargs(vitk, **kw):
     (dict(H=0), "query heads over"), (dict(dh=0), "outside"), (dict(dh=129), "outside"),
     (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(q=0), "null pointer"),
     (dict(k=0), "null pointer"), (dict(out=0), "null pointer"), (dict(ld_q=31), "pitch"), (dict(ld_k=15), "pitch"),
-    (dict(ld_out=1), "pitch"), (dict(reserved=1), "reserved"), (dict(Nq=2 ** 30, H=8), "too many rows")])
+    (dict(ld_out=1), "pitch"), (dict(out=4096), "one of the inputs"), (dict(reserved=1), "reserved"), (dict(Nq=2 ** 30, H=8), "too many rows")])
 def test_cross_attention_refuses(change, message):
     from visiontransformer_amd import vitk
     d = vitk.dll()
@@ -581,8 +631,9 @@ def test_cross_attention_refuses(change, message):
 
 @pytest.mark.parametrize("change, message", [
     (dict(dout=0), "null pointer"), (dict(dq=0), "null pointer"), (dict(dk=0), "null pointer"), (dict(dv=0), "null pointer"),
-    (dict(stats=0), "null pointer"), (dict(ld_dq=31), "pitch"), (dict(ld_dv=15), "pitch"),
-    (dict(workspace=0), "workspace"), (dict(workspace_bytes=4), "workspace"), (dict(workspace=4100), "aligned")])
+    (dict(stats=0), "null pointer"), (dict(dq=24576), "one of the inputs"), (dict(dk=8192), "one of the inputs"),
+    (dict(dv=16384), "one of the inputs"), (dict(dv=32768), "share"), (dict(dq=36864), "share"), (dict(ld_dq=31), "pitch"), (dict(ld_dv=15), "pitch"),
+    (dict(workspace=0), "workspace"), (dict(workspace_bytes=4), "workspace"), (dict(workspace=40964), "aligned")])
 def test_cross_attention_backward_refuses(change, message):
     from visiontransformer_amd import vitk
     d = vitk.dll()
@@ -602,17 +653,19 @@ def test_cross_attention_refuses_null_arguments_and_a_missing_workspace():
 
 
 @pytest.mark.parametrize("name, args, message", [
-    ("vitk_embedding_fwd", (4096, 10, 4096, -1, 8, 1.0, 4096, None), "bad shape"),
+    ("vitk_embedding_fwd", (4096, 10, 4096, -1, 8, 1.0, 8192, None), "bad shape"),
+    ("vitk_embedding_fwd", (4096, 10, 8192, 3, 8, 1.0, 4096, None), "is the table"),
+    ("vitk_embedding_bwd", (4096, 8192, 3, 10, 8, 1.0, 0, 4096, 12288, 1 << 20, None), "is dout"),
     ("vitk_embedding_fwd", (None, 10, 4096, 3, 8, 1.0, 4096, None), "null pointer"),
     ("vitk_embedding_fwd", (4096, 10, None, 3, 8, 1.0, 4096, None), "null pointer"),
-    ("vitk_embedding_fwd", (4096, 2 ** 31, 4096, 3, 8, 1.0, 4096, None), "table of"),
+    ("vitk_embedding_fwd", (4096, 2 ** 31, 4096, 3, 8, 1.0, 8192, None), "table of"),
     ("vitk_embedding_bwd", (4096, 4096, 3, -10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "bad shape"),
     ("vitk_embedding_bwd", (None, 4096, 3, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "null pointer"),
     ("vitk_embedding_bwd", (4096, 4096, 3, 10, 8, 1.0, 0, None, 4096, 1 << 20, None), "null pointer"),
-    ("vitk_embedding_bwd", (4096, 4096, 3, 5000, 8, 1.0, 0, 4096, None, 1 << 20, None), "workspace"),
-    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 4096, 4096, 16, None), "workspace"),
-    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 4096, 4100, 1 << 20, None), "aligned"),
-    ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "tokens over"),
+    ("vitk_embedding_bwd", (4096, 4096, 3, 5000, 8, 1.0, 0, 8192, None, 1 << 20, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4096, 16, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4100, 1 << 20, None), "aligned"),
+    ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 8192, 4096, 1 << 20, None), "tokens over"),
 ])
 def test_embedding_refuses(name, args, message):
     from visiontransformer_amd import vitk
@@ -647,7 +700,8 @@ def test_newton_schulz_and_muon_refuse(change, message):
 
 @pytest.mark.parametrize("cls, change, message", [
     ("NewtonSchulzArgs", dict(x=0), "null pointer"), ("NewtonSchulzArgs", dict(out=0), "null pointer"),
-    ("NewtonSchulzArgs", dict(ld_x=7), "pitch"), ("NewtonSchulzArgs", dict(stride_out=63), "overlap"),
+    ("NewtonSchulzArgs", dict(ld_x=7), "pitch"), ("NewtonSchulzArgs", dict(ld_x=201, stride_x=40200), "one layout"),
+    ("NewtonSchulzArgs", dict(stride_x=0), "one layout"), ("NewtonSchulzArgs", dict(stride_out=63), "overlap"),
     ("MuonArgs", dict(p=0), "null pointer"), ("MuonArgs", dict(m=8192), "different buffers"),
     ("MuonArgs", dict(ld=7), "pitch"), ("MuonArgs", dict(stride=63), "overlap")])
 def test_newton_schulz_and_muon_refuse_their_own(cls, change, message):
@@ -669,3 +723,88 @@ def test_bindings_refuse_wrong_tensors():
         vitk.newton_schulz_args(torch.zeros(4, 4), torch.zeros(4, 4))
     with pytest.raises(vitk.VitkError, match="CUDA"):
         vitk.muon_args(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), lr=0.1)
+
+
+# ---------------------------------------------------------------------------- the run together
+@gpu
+def test_decoder_step_on_the_encoders_states(K):
+    """One training step of a small decoder on a ViT encoder, every piece by the library: token embeddings, query
+    projection, cross attention to the encoder's final states (ragged: one image has none), output
+    projection to a vocabulary, softmax cross-entropy, the way back, the gradient of the embedding
+    table and a Muon step on the two projections -- against float64 autograd on the CPU."""
+    import vitlibs as V
+    from visiontransformer_amd import host
+    host.init(0)
+    host.use_torch_stream()
+    cfgd = V.TINY
+    model = host.Model(host.Config.make(**cfgd))
+    model.set_params(V.init_params(V.Cfg.make(**cfgd), 3))
+    B, T, vocab, D, H = 4, 7, 50, cfgd["embedding_dim"], cfgd["num_heads"]
+    dh, g = D // H, rng(400)
+    acts, _ = model.forward_trace(torch.from_numpy(V.rng_normal(4, B, cfgd["in_channels"], cfgd["image_size"],
+                                                                cfgd["image_size"])).cuda())
+    states = acts[-1].contiguous()  # [B, N, D] behind the final norm
+    N = states.shape[1]
+    klen = torch.tensor([N, 0, N - 1, 2], dtype=torch.int32, device="cuda")
+    index = torch.randint(0, vocab, (B * T,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    index[5:7] = -1  # padding
+    target = torch.randint(0, vocab, (B * T,), generator=torch.Generator().manual_seed(2))
+    onehot = torch.nn.functional.one_hot(target, vocab).float().cuda()
+    index = index.cuda()
+    table, wq, wk, wv, wo = (randn(g, *s) * 0.3 for s in ((vocab, D), (D, D), (D, D), (D, D), (D, vocab)))
+    rows, keys = B * T, B * N
+    e = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
+    emb, q, k, v, ctx, logits = e(rows, D), e(rows, D), e(keys, D), e(keys, D), e(rows, D), e(rows, vocab)
+    scale = D ** 0.5
+    K.embedding_fwd(table, index, emb, scale=scale)
+    K.gemm(emb, wq, q, rows, D, D)
+    K.gemm(states, wk, k, keys, D, D)
+    K.gemm(states, wv, v, keys, D, D)
+    dctx, dq, dk, dv = e(rows, D), e(rows, D), e(keys, D), e(keys, D)
+    shape = lambda t, n: t.view(B, n, H, dh)  # noqa: E731
+    args = K.cross_sdpa_args(shape(q, T), shape(k, N), shape(v, N), shape(ctx, T), key_len=klen, stats=e(B * H, T, 2),
+                             dout=shape(dctx, T), dq=shape(dq, T), dk=shape(dk, N), dv=shape(dv, N))
+    K.cross_sdpa_fwd(args)
+    K.gemm(ctx, wo, logits, rows, vocab, D)
+    dlogits, probs, out2, ws = e(rows, vocab), e(rows, vocab), e(2), e(2 * rows)
+    K.call("vitk_softmax_ce", logits, onehot, rows, vocab, None, float(rows), dlogits, probs, out2, ws, ws.numel() * 4,
+           K.stream())
+    dwo, dwq, demb, dtable = e(D, vocab), e(D, D), e(rows, D), e(vocab, D)
+    K.gemm(ctx, dlogits, dwo, D, vocab, rows, trans_a=True)
+    K.gemm(dlogits, wo, dctx, rows, D, vocab, trans_b=True)
+    K.cross_sdpa_bwd(args)
+    K.gemm(emb, dq, dwq, D, D, rows, trans_a=True)
+    K.gemm(dq, wq, demb, rows, D, D, trans_b=True)
+    K.embedding_bwd(demb, index, dtable, scale=scale)
+    # the same in float64
+    leaf = {n: t.double().cpu().requires_grad_() for n, t in (("table", table), ("wq", wq), ("wo", wo), ("k", k), ("v", v))}
+    idx = index.long().cpu()
+    there = (idx >= 0)[:, None]
+    emb64 = torch.where(there, leaf["table"][idx.clamp(min=0)] * scale, 0.0)
+    q64 = (emb64 @ leaf["wq"]).view(B, T, H, dh)
+    k64, v64 = (leaf[n].view(B, N, H, dh) for n in ("k", "v"))
+    out = []
+    for b in range(B):
+        n = int(klen[b])
+        if n == 0:
+            out.append(torch.zeros(T, D, dtype=torch.float64))
+            continue
+        s = torch.einsum("qhd,khd->hqk", q64[b], k64[b, :n]) * dh ** -0.5
+        out.append(torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), v64[b, :n]).reshape(T, D))
+    ctx64 = torch.cat(out)
+    loss = torch.nn.functional.cross_entropy(ctx64 @ leaf["wo"], target)
+    loss.backward()
+    assert abs(out2[0].item() - loss.item()) <= 1e-5 * abs(loss.item())
+    # sums of at most B T vocab = 1400 terms in fp32, five products deep: LAM sqrt(1400) u = 1.3e-5 of the largest entry each
+    for name, got in (("wo", dwo), ("wq", dwq), ("table", dtable), ("k", dk), ("v", dv)):
+        want = leaf[name].grad.reshape(got.shape)
+        assert (got.double().cpu() - want).abs().max() <= 5 * 1.3e-5 * want.abs().max(), name
+    # and the step on both projections
+    for p, grad in ((wq, dwq), (wo, dwo)):
+        before, m = p.double().cpu(), torch.zeros_like(p)
+        K.muon(K.muon_args(p, grad, m, lr=0.05, momentum=0.9, nesterov=False))
+        h = grad.cpu().numpy()
+        o = newton_schulz(h, 5, COEF, 1e-7, np.float64)
+        err = np.linalg.norm(p.double().cpu().numpy() - (before.numpy() - 0.05 * o))
+        assert err <= 0.05 * ns_tolerance(h, o, 5, COEF, 1e-7) + 4 * U * np.linalg.norm(before.numpy())
+    model.close()

@@ -33,6 +33,13 @@ int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Pa
     VITK_REQUIRE(a->k && a->v, "%s: null pointer", who);
     VITK_REQUIRE(a->ld_k >= wk && a->ld_v >= wk, "%s: row pitch below Hkv*dh", who);
   }
+  const float *in[] = {a->q, a->k, a->v};
+  auto fresh = [&](const float *out) {  // not one of the inputs
+    bool ok = true;
+    for (const float *x : in) ok = ok && (out == nullptr || out != x);
+    return ok;
+  };
+  VITK_REQUIRE(fresh(a->out), "%s: out is one of the inputs", who);
   p->q = {a->q, a->ld_q};
   p->k = {a->k, a->ld_k};
   p->v = {a->v, a->ld_v};
@@ -55,6 +62,10 @@ int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Pa
       VITK_REQUIRE(a->dk && a->dv, "%s: null pointer", who);
       VITK_REQUIRE(a->ld_dk >= wk && a->ld_dv >= wk, "%s: row pitch below Hkv*dh", who);
     }
+    for (const float *x : {a->dq, a->dk, a->dv})
+      VITK_REQUIRE(fresh(x) && (x == nullptr || (x != a->out && x != a->dout)), "%s: a gradient is one of the inputs", who);
+    VITK_REQUIRE(!a->dk || (a->dk != a->dv && a->dk != a->dq), "%s: two gradients share a buffer", who);
+    VITK_REQUIRE(!a->dq || a->dq != a->dv, "%s: two gradients share a buffer", who);
     p->dout = {a->dout, a->ld_dout};
     p->dq = {a->dq, a->ld_dq};
     p->dk = {a->dk, a->ld_dk};

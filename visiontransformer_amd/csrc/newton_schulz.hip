@@ -919,6 +919,8 @@ extern "C" int vitk_newton_schulz_f32(const vitk_newton_schulz_args *a, vitk_str
   VITK_REQUIRE(a->ld_x >= a->cols && a->ld_out >= a->cols, "%s: row pitch below the columns", who);
   VITK_REQUIRE(a->batch == 1 || (a->stride_x >= 0 && a->stride_out >= (a->rows - 1) * a->ld_out + a->cols),
                "%s: matrices overlap", who);
+  VITK_REQUIRE(a->x != a->out || ((a->rows == 1 || a->ld_x == a->ld_out) && (a->batch == 1 || a->stride_x == a->stride_out)),
+               "%s: in place, x and out have to have one layout", who);
   NsParams p = {};
   p.x = a->x, p.out = a->out;
   p.ld_x = a->ld_x, p.stride_x = a->stride_x, p.ld_out = a->ld_out, p.stride_out = a->stride_out;

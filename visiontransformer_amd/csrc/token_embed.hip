@@ -449,6 +449,7 @@ extern "C" int vitk_embedding_fwd(const float *table, int64_t V, const int32_t *
   VITK_REQUIRE(shape_ok(rows, V, D), "vitk_embedding_fwd: bad shape");
   if (rows == 0 || D == 0) return 0;
   VITK_REQUIRE(index && out && (table || V == 0), "vitk_embedding_fwd: null pointer");
+  VITK_REQUIRE(out != table, "vitk_embedding_fwd: out is the table");
   VITK_REQUIRE(V <= INT32_MAX, "vitk_embedding_fwd: table of %lld rows", (long long)V);
   const bool vec = D % 4 == 0 && vitk::aligned16(table) && vitk::aligned16(out);
   hipStream_t st = vitk::as_stream(stream);
@@ -477,6 +478,7 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
   VITK_REQUIRE(shape_ok(rows, V, D), "vitk_embedding_bwd: bad shape");
   if (V == 0 || D == 0) return 0;
   VITK_REQUIRE(dtable && (rows == 0 || (dout && index)), "vitk_embedding_bwd: null pointer");
+  VITK_REQUIRE(dtable != dout, "vitk_embedding_bwd: dtable is dout");
   VITK_REQUIRE(V <= INT32_MAX && rows <= kMaxTokens && D <= kMaxWidth,
                "vitk_embedding_bwd: %lld tokens over a table of %lld rows of %lld", (long long)rows, (long long)V,
                (long long)D);

@@ -355,6 +355,7 @@ def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace
     if workspace is None:
         import torch
         need = dll().vitk_embedding_bwd_workspace_bytes(rows, V, D)
+        _need(need == 0 or st is None, "embedding_bwd: another stream than the current one needs a workspace of its own")
         workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=dout.device)
     check(dll().vitk_embedding_bwd(ptr(dout), ptr(index), rows, V, D, scale, int(bool(accumulate)), ptr(dtable),
                                    ptr(workspace), workspace.numel() * workspace.element_size(),
