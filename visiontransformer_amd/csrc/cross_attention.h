@@ -254,10 +254,10 @@ __device__ __forceinline__ void store_row(float *row, const f32x4 (&acc)[DH / 16
 // the other side.  A stage (two tensors) is loaded into registers, split and put into one of two buffers while
 // the waves work on the other one: half of the waves before their products, half after them, so that on each
 // SIMD one wave splits while the other multiplies.  (With OTHER = 2 a stage is twice as long and has one buffer:
-// two would leave room for one workgroup a CU.)
+// two would leave room for one workgroup a CU.  So have four waves of OTHER = 1, for more workgroups a CU.)
 template <int DH, int NW, int GROUPS>
 struct Shape {
-  static constexpr int OTHER = NW / GROUPS, STAGE = 32 * OTHER, BUFFERS = OTHER == 1 ? 2 : 1;
+  static constexpr int OTHER = NW / GROUPS, STAGE = 32 * OTHER, BUFFERS = OTHER == 1 && NW == 8 ? 2 : 1;
   static constexpr int THREADS = 64 * NW, HALF = STAGE * DH / 8, TASKS = (2 * HALF + THREADS - 1) / THREADS;
   static constexpr int UNITS = STAGE * Tile<DH>::ROW;  // of a tensor; a buffer holds two
 };

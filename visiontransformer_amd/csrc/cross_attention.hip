@@ -85,8 +85,15 @@ using namespace vitk::cross;
 
 // NW waves: RW groups of 16 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
+// Blocks of 64 rows are four waves of 16, whose keys no waves share: with one buffer four such workgroups are on a
+// CU and hide each other's loads and barriers.  48 rows x 197 keys x 64, 768 heads: 29.4 us; eight waves that
+// share the keys 33.6.
+constexpr int waves_a_simd(int dh, int nw, int rw) {
+  if (nw == rw) return dh <= 64 ? 4 : nw == 8 ? (dh <= 96 ? 4 : 2) : dh <= 96 ? 3 : 2;
+  return dh <= 64 ? 2 : 1;
+}
 template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, NW == RW && DH <= 96 ? 4 : NW == 8 ? (DH <= 64 ? 4 : 2) : (DH <= 64 ? 2 : 1)) void cross_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int NB = DH / 16, BOX = DH / 4 + 2;  // words a lane passes on: o, m, l
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * BOX * 4 : 0;
@@ -467,7 +474,8 @@ FwdPlan plan_fwd(Params *p) {
     f.row_groups = plan_groups(p->rows);
     p->blocks = (int)(((long long)p->rows + 16 * f.row_groups - 1) / (16 * f.row_groups));
     const int wide = p->dh <= 32 ? 32 : p->dh <= 64 ? 64 : p->dh <= 96 ? 96 : 128;
-    const int resident = (f.row_groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);  // workgroups a CU
+    const int resident = f.row_groups == 4 ? (wide <= 64 ? 4 : wide <= 96 ? 3 : 2)  // workgroups a CU
+                                           : (f.row_groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);
     const double flop = 64.0 * f.row_groups * p->Nk * wide;                   // of a block; 0.6 TFLOP/s a CU
     const double part = 2.0 * p->B * p->H * p->Nq * p->dh * 4 / 4e6;          // written and read at 4 TB/s
     splits = vitk::cross::plan_splits(heads * p->blocks, resident * (long long)vitk::cu_count(), stages,
@@ -507,7 +515,7 @@ void launch_fwd(const Params &p, int row_groups, unsigned wgs, hipStream_t st) {
   if (row_groups == 8)
     hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
   else if (row_groups == 4)
-    hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
