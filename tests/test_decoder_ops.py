@@ -182,6 +182,27 @@ def test_cross_attention_every_block_size(K, dh):
 
 
 @gpu
+@pytest.mark.parametrize("dh", [20, 64, 88, 128])
+def test_cross_attention_every_block_size_with_many_heads(K, dh):
+    """Blocks of 64 as four waves, which at least one workgroup a CU takes: alone, as 3 and 5 blocks, over keys of
+    every kind of count."""
+    for Nq, Nk in ((40, 33), (60, 130), (131, 50), (190, 200), (120, 64), (259, 20)):
+        g = rng(1000 * Nq + Nk)
+        B, Hkv = 40, 8  # 320 workgroups
+        q, k, v, dout = (randn(g, B, n, Hkv, dh) for n in (Nq, Nk, Nk, Nq))
+        lens = [Nk - b if b % 8 else Nk for b in range(B)]
+        lens[3] = 0
+        want, tol, _ = attention64(q, k, v, lens, dh ** -0.5, dout)
+        out, dq, dk, dv = (torch.full_like(x, 7.0) for x in (q, q, k, v))
+        a = K.cross_sdpa_args(q, k, v, out, key_len=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                              stats=torch.empty(B * Hkv, Nq, 2, device="cuda"), dout=dout, dq=dq, dk=dk, dv=dv)
+        K.cross_sdpa_fwd(a)
+        K.cross_sdpa_bwd(a)
+        for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+            within(t, want[n], tol[n], f"{n} {Nq} x {Nk}")
+
+
+@gpu
 @pytest.mark.parametrize("dh", [8, 60, 100])
 def test_cross_attention_few_rows_of_every_count(K, dh):
     for rows in range(1, 9):

@@ -291,10 +291,24 @@ struct Stage {
   }
 };
 
-// Groups of 16 rows in a workgroup.  (Smaller blocks where they leave fewer empty rows do not pay: 147 rows of 64
-// over 50 keys in blocks of 128, 64 and 32: 22.7, 25.0 and 30.8 us.)
-inline int plan_groups(long long rows) { return rows > 64 ? 8 : rows > 32 ? 4 : 2; }
-
+// Groups of 16 rows (or keys) in a workgroup, and its waves.  Eight groups split the other side's tiles for 128
+// rows at once.  Four groups are four waves, of which several workgroups are on a CU, if there are at least as
+// many such workgroups as CUs; otherwise eight, so that two share a group's other side (64 columns, forward and
+// backward, eight waves -> four: 64 x 64, 2048 heads: 207 -> 140 us; 900 x 50, 24 heads: 52 -> 65).  More than 64
+// rows are cut into blocks of 64 where the last block of 128 were half empty and that is a sixth of the rows or more
+// (147 x 197, 320 heads: forward 42 -> 33, row gradient 19 less), up to `half` on the other side, and up to
+// `any` on the other side always (row gradient of 512 x 50, 192 heads: 7 less; 512 x 197: 2 more).
+struct Block {
+  int groups, waves;
+};
+inline Block plan_block(long long own, long long other, long long heads, bool small, int half, int any) {
+  if (own <= 32) return {2, 4};
+  const long long blocks = (own + 63) / 64;
+  small = small && heads * blocks >= vitk::cu_count();
+  if (own <= 64) return {4, small ? 4 : 8};
+  const bool halves = blocks % 2 == 1 && blocks <= 5;
+  return small && ((halves && other <= half) || other <= any) ? Block{4, 4} : Block{8, 8};
+}
 // Over how many workgroups the other side of a block is split: the least of whole rounds over the device's
 // places for workgroups (a last round that is hardly filled costs as much as a full one) plus writing and
 // adding the parts.  `us`: time of a whole block; `part_us`: of one part of the results.

@@ -85,12 +85,12 @@ using namespace vitk::cross;
 
 // NW waves: RW groups of 16 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
-// Blocks of 64 rows are four waves of 16, whose keys no waves share: with one buffer four such workgroups are on a
-// CU and hide each other's loads and barriers.  48 rows x 197 keys x 64, 768 heads: 29.4 us; eight waves that
-// share the keys 33.6.
+// Blocks of 64 rows as four waves of 16, whose keys no waves share: with one buffer up to four such workgroups are
+// on a CU and hide each other's loads and barriers.  48 rows x 197 keys x 64, 768 heads: 29.4 us; eight waves
+// that share the keys 33.6.
 constexpr int waves_a_simd(int dh, int nw, int rw) {
   if (nw == rw) return dh <= 64 ? 4 : nw == 8 ? (dh <= 96 ? 4 : 2) : dh <= 96 ? 3 : 2;
-  return dh <= 64 ? 2 : 1;
+  return nw == 8 ? (dh <= 64 ? 4 : 2) : dh <= 64 ? 2 : 1;
 }
 template <int DH, int NW, int RW>
 __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_kernel(const Params p) {
@@ -453,8 +453,7 @@ __global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
 constexpr int CHUNK = 64;      // key ranges of splits are multiples of this
 constexpr int FEW_ROWS = 8;    // rows per key head up to which the vector kernel runs
 struct FwdPlan {
-  int row_groups;  // of 16 rows; 0 = the vector kernel
-  int waves;       // of the vector kernel
+  Block block;  // no groups = the vector kernel
 };
 FwdPlan plan_fwd(Params *p) {
   FwdPlan f = {};
@@ -462,22 +461,23 @@ FwdPlan plan_fwd(Params *p) {
   long long splits = 1;
   if (p->rows <= FEW_ROWS) {
     p->blocks = 1;
-    f.waves = 4;
+    f.block.waves = 4;
     const long long cus = vitk::cu_count();
     if (heads < 2 * cus) {
       if (p->Nk <= 1024)
-        f.waves = 16;  // one launch: a split's join costs more than it saves
+        f.block.waves = 16;  // one launch: a split's join costs more than it saves
       else if (heads > 0)
         splits = std::min((12 * cus + heads - 1) / heads, stages / 4);
     }
   } else {
-    f.row_groups = plan_groups(p->rows);
-    p->blocks = (int)(((long long)p->rows + 16 * f.row_groups - 1) / (16 * f.row_groups));
+    f.block = plan_block(p->rows, p->Nk, heads, true, 256, 0);
+    const int groups = f.block.groups;
+    p->blocks = (int)(((long long)p->rows + 16 * groups - 1) / (16 * groups));
     const int wide = p->dh <= 32 ? 32 : p->dh <= 64 ? 64 : p->dh <= 96 ? 96 : 128;
-    const int resident = f.row_groups == 4 ? (wide <= 64 ? 4 : wide <= 96 ? 3 : 2)  // workgroups a CU
-                                           : (f.row_groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);
-    const double flop = 64.0 * f.row_groups * p->Nk * wide;                   // of a block; 0.6 TFLOP/s a CU
-    const double part = 2.0 * p->B * p->H * p->Nq * p->dh * 4 / 4e6;          // written and read at 4 TB/s
+    const int resident = groups == 4 && f.block.waves == 4 ? waves_a_simd(wide, 4, 4)  // workgroups a CU
+                                                           : (groups == 2 ? 2 : 1) * (wide <= 96 ? 2 : 1);
+    const double flop = 64.0 * groups * p->Nk * wide;                 // of a block; 0.6 TFLOP/s a CU
+    const double part = 2.0 * p->B * p->H * p->Nq * p->dh * 4 / 4e6;  // written and read at 4 TB/s
     splits = vitk::cross::plan_splits(heads * p->blocks, resident * (long long)vitk::cu_count(), stages,
                                       flop / (0.6e6 / resident), part);
   }
@@ -511,10 +511,12 @@ void launch_rows(const Params &p, int waves, unsigned wgs, hipStream_t st) {
 }
 
 template <int DH>
-void launch_fwd(const Params &p, int row_groups, unsigned wgs, hipStream_t st) {
-  if (row_groups == 8)
+void launch_fwd(const Params &p, Block block, unsigned wgs, hipStream_t st) {
+  if (block.groups == 8)
     hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
-  else if (row_groups == 4)
+  else if (block.groups == 4 && block.waves == 8)
+    hipLaunchKernelGGL((cross_fwd_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
+  else if (block.groups == 4)
     hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((cross_fwd_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
@@ -549,23 +551,22 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   const long long wgs = (long long)p.B * p.Hkv * p.blocks * p.splits;
   VITK_REQUIRE(wgs < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
   hipStream_t st = vitk::as_stream(stream);
-  const int rg = plan.row_groups;
   const unsigned grid = (unsigned)wgs;
-  if (rg == 0) {
+  if (plan.block.groups == 0) {
     if (p.dh <= 32)
-      launch_rows<8>(p, plan.waves, grid, st);
+      launch_rows<8>(p, plan.block.waves, grid, st);
     else if (p.dh <= 64)
-      launch_rows<16>(p, plan.waves, grid, st);
+      launch_rows<16>(p, plan.block.waves, grid, st);
     else
-      launch_rows<32>(p, plan.waves, grid, st);
+      launch_rows<32>(p, plan.block.waves, grid, st);
   } else if (p.dh <= 32) {
-    launch_fwd<32>(p, rg, grid, st);
+    launch_fwd<32>(p, plan.block, grid, st);
   } else if (p.dh <= 64) {
-    launch_fwd<64>(p, rg, grid, st);
+    launch_fwd<64>(p, plan.block, grid, st);
   } else if (p.dh <= 96) {
-    launch_fwd<96>(p, rg, grid, st);
+    launch_fwd<96>(p, plan.block, grid, st);
   } else {
-    launch_fwd<128>(p, rg, grid, st);
+    launch_fwd<128>(p, plan.block, grid, st);
   }
   if (p.splits > 1) {
     const int lp = p.splits > JOIN_FEW ? 64 : p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32;

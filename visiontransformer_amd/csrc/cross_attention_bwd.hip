@@ -35,8 +35,13 @@ __device__ __forceinline__ void take(const float *box, f32x4 (&acc)[NB]) {
     for (int e = 0; e < 4; ++e) acc[n][e] += box[(4 * n + e) * 64];
 }
 
+// Workgroups of four waves that a CU holds, with one group of rows or keys a wave.  (Of 128 columns one, which is
+// slower than eight waves that share the groups: 64 x 64, 2048 heads, forward and backward 455 -> 490 us.)
+constexpr int dq_resident(int dh) { return dh <= 32 ? 4 : dh <= 64 ? 3 : 2; }
+constexpr int dkv_resident(int dh) { return dh <= 32 ? 4 : 2; }
+
 template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && RW == 4 ? dq_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 4) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
@@ -143,7 +148,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dq
 }
 
 template <int DH, int NW, int KG>
-__global__ __launch_bounds__(64 * NW, NW == 8 || DH <= 64 ? 2 : 1) void cross_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && KG == 4 ? dkv_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1) void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
@@ -273,16 +278,19 @@ __global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part,
 
 // Groups of 16 in a workgroup, blocks, and how the other side is split.
 struct Side {
-  int groups, blocks, splits, chunk;
+  Block block;
+  int blocks, splits, chunk;
 };
-Side plan_side(long long own, long long other, long long heads, int dh, int products, double part_us) {
+Side plan_side(long long own, long long other, long long heads, int dh, bool keys, double part_us) {
   Side s;
-  s.groups = plan_groups(own);
-  s.blocks = (int)((own + 16 * s.groups - 1) / (16 * s.groups));
+  s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 256, keys ? 0 : 128);
+  const int groups = s.block.groups;
+  s.blocks = (int)((own + 16 * groups - 1) / (16 * groups));
   const long long stages = (other + 63) / 64;
   const int wide = dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128;
-  const int resident = s.groups == 2 ? 2 : 1;  // workgroups a CU
-  const double flop = 32.0 * products * s.groups * other * wide;  // of a block; 0.5 TFLOP/s a CU
+  const int four = keys ? dkv_resident(dh) : dq_resident(dh);
+  const int resident = groups == 4 && s.block.waves == 4 ? four : groups == 2 ? 2 : 1;  // workgroups a CU
+  const double flop = 32.0 * (keys ? 4 : 3) * groups * other * wide;  // of a block; 0.5 TFLOP/s a CU
   const int splits = plan_splits(heads * s.blocks, resident * (long long)vitk::cu_count(), stages,
                                  flop / (0.5e6 / resident), part_us);
   s.chunk = std::max((int)((stages + splits - 1) / splits) * 64, 64);
@@ -297,8 +305,8 @@ Plan make_plan(const Params &p) {
   Plan n;
   const long long heads = (long long)p.B * p.Hkv;
   // one part of the results, written and read at 4 TB/s
-  n.rows = plan_side(p.rows, p.Nk, heads, p.dh, 3, 2.0 * p.B * p.H * p.Nq * p.dh * 4 / 4e6);
-  n.keys = plan_side(p.Nk, p.rows, heads, p.dh, 4, 4.0 * p.B * p.Hkv * p.Nk * p.dh * 4 / 4e6);
+  n.rows = plan_side(p.rows, p.Nk, heads, p.dh, false, 2.0 * p.B * p.H * p.Nq * p.dh * 4 / 4e6);
+  n.keys = plan_side(p.Nk, p.rows, heads, p.dh, true, 4.0 * p.B * p.Hkv * p.Nk * p.dh * 4 / 4e6);
   n.delta = ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
   const size_t q = n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
   const size_t k = n.keys.splits > 1 ? (size_t)2 * n.keys.splits * p.B * p.Nk * p.Hkv * p.dh : 0;
@@ -307,19 +315,31 @@ Plan make_plan(const Params &p) {
 }
 
 template <int DH>
-void launch_dq(const Params &p, int groups, unsigned wgs, hipStream_t st) {
-  if (groups == 8)
+void launch_dq(const Params &p, Block block, unsigned wgs, hipStream_t st) {
+  if constexpr (DH <= 96) {
+    if (block.groups == 4 && block.waves == 4) {
+      hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
+      return;
+    }
+  }
+  if (block.groups == 8)
     hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
-  else if (groups == 4)
+  else if (block.groups == 4)
     hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
   else
     hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
 template <int DH>
-void launch_dkv(const Params &p, int groups, unsigned wgs, hipStream_t st) {
-  if (groups == 8)
+void launch_dkv(const Params &p, Block block, unsigned wgs, hipStream_t st) {
+  if constexpr (DH <= 96) {
+    if (block.groups == 4 && block.waves == 4) {
+      hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
+      return;
+    }
+  }
+  if (block.groups == 8)
     hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
-  else if (groups == 4)
+  else if (block.groups == 4)
     hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
   else
     hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
@@ -336,12 +356,12 @@ int launch(Params p, const Plan &n, hipStream_t st) {
   VITK_REQUIRE(qw < (1ll << 31) && kw < (1ll << 31), "vitk_cross_sdpa_bwd: too many rows for one launch");
   if (p.Nq > 0) {
     p.blocks = n.rows.blocks, p.splits = n.rows.splits, p.chunk = n.rows.chunk;
-    launch_dq<DH>(p, n.rows.groups, (unsigned)qw, st);
+    launch_dq<DH>(p, n.rows.block, (unsigned)qw, st);
     if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nq, p.H * p.dh, p.dq, st);
   }
   if (p.Nk > 0) {
     p.blocks = n.keys.blocks, p.splits = n.keys.splits, p.chunk = n.keys.chunk;
-    launch_dkv<DH>(p, n.keys.groups, (unsigned)kw, st);
+    launch_dkv<DH>(p, n.keys.block, (unsigned)kw, st);
     if (p.splits > 1) {
       const long long rows = (long long)p.B * p.Nk;
       const int width = p.Hkv * p.dh;
