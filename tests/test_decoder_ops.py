@@ -748,6 +748,15 @@ def test_bindings_refuse_wrong_tensors():
 
 # ---------------------------------------------------------------------------- the run together
 @gpu
+def test_the_bindings_follow_the_current_stream(K):
+    assert K.stream() == torch.cuda.current_stream().cuda_stream
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        assert K.stream() == torch.cuda.current_stream().cuda_stream != 0
+    assert K.stream() == torch.cuda.current_stream().cuda_stream
+
+
+@gpu
 def test_decoder_step_on_the_encoders_states(K):
     """One training step of a small decoder on a ViT encoder, every piece by the library: token embeddings, query
     projection, cross attention to the encoder's final states (ragged: one image has none), output

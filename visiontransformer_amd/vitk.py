@@ -172,9 +172,18 @@ def ptr(t):
     return t.data_ptr()
 
 
+_raw_stream = None
+
+
 def stream():
+    """Handle of torch's current stream on the current device.  (Building the Stream object for it takes 2.5 us, as
+    much as the smallest kernels here, so the handle is asked for by itself where torch offers that: 0.3 us.)"""
+    global _raw_stream
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(torch.cuda.current_device())
 
 
 def check(rc):
