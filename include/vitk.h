@@ -451,8 +451,9 @@ int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float 
  * Frobenius norm is summed in double precision; between products y and g are pairs of fp16 numbers, 32
  * bits within 2^-23 of the value, and a product is three matrix products of parts with fp32 sums: as
  * close to the exact result as the same steps in fp32.  A zero matrix gives zeros (NaN with eps = 0).
- * out may be x, with one layout for both; no other overlap.  0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1]
- * within [-4, 4], with |b t^2 + c t^4| below 31 (checked on 65 points), which every useful triple does.
+ * out may be x, with one layout for both; no other overlap.
+ * 0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1] within [-4, 4], with
+ * |b t^2 + c t^4| below 31 (checked on 65 points), which every useful triple does.
  * vitk_muon_f32 (p, g, m share ld and stride, as arenas of one layout do):
  *   m = momentum*m + grad_scale*g;  u = nesterov ? grad_scale*g + momentum*m : m
  *   p = p * (1 - lr*weight_decay) - lr*update_scale * NS(u)

