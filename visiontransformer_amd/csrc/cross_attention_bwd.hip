@@ -268,6 +268,143 @@ void cross_dkv_kernel(const Params p) {
   }
 }
 
+// Few keys: all of a (batch, key head) in one workgroup of four waves, so dQ is complete here too: five products
+// instead of seven, and each row is read once.  Each wave forms p and ds of its 16 keys with a stage of 32 rows
+// and adds to dK and dV; ds goes through LDS as [key][row], and dQ^T[d][row] += K^T ds is dealt to the waves by
+// blocks of 16 x 16.  K is there times scale log2(e), for the scores.
+template <int DH>
+__global__ __launch_bounds__(256, 2) void cross_short_kernel(const Params p) {
+  typedef Shape<DH, 4, 4> S;
+  typedef Tile<32> Turn;
+  constexpr int UNITS = DH / 8;  // of a row of a stage: that many lanes load it
+  static_assert(DH <= 64 && 64 % UNITS == 0, "the lanes of a row are neighbours in a wave");
+  __shared__ __attribute__((aligned(16))) bf16x8 stage[2 * S::UNITS], kt[64 * Tile<DH>::ROW], turn[64 * Turn::ROW];
+  __shared__ __attribute__((aligned(16))) float rm[32], rd[32];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  long long wg = blockIdx.x;
+  const int hk = (int)(wg % p.Hkv);
+  wg /= p.Hkv;
+  const int split = (int)(wg % p.splits), b = (int)(wg / p.splits);
+  const int len = valid_keys(p, b), key = wave * 16 + c;
+  const bool key_ok = key < len, empty = wave * 16 >= len;
+  Split8 k[DH / 32], v[DH / 32];
+  load_row<DH>(k, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p.c, p);
+  load_row<DH>(v, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, 1.f, p);
+  f32x4 dk[DH / 16], dv[DH / 16];
+#pragma unroll
+  for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
+  const int r0 = min((long long)split * p.chunk, (long long)p.rows), r1 = min((long long)r0 + p.chunk, (long long)p.rows);
+  Stage<DH, 4, 4> next;
+  float o[S::TASKS][8], m[S::TASKS], l[S::TASKS];  // of a task's row of dout
+  auto at = [&](bool y, int r) {
+    return y ? p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r) : p.q.ptr + row_offset(p, p.q.ld, b, hk, r);
+  };
+  auto fetch = [&](int t) {
+    next.fetch(p, t, r1, at);
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int r = t + next.row(u);
+      m[u] = l[u] = 0.f;  // a row that is not there: exp2(0) times zeros
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[u][e] = 0.f;
+      if (next.any(u) && next.is_y(u) && r < r1) {
+        const long long st = 2 * row_stat(p, b, hk, r);
+        m[u] = p.stats[st], l[u] = p.stats[st + 1];
+        load_eight(p.o.ptr + row_offset(p, p.o.ld, b, hk, r), next.unit(u) * 8, p, o[u]);
+      }
+    }
+  };
+  auto put = [&] {
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      if (!next.any(u) || !next.is_y(u)) continue;
+      const float f = l[u] == 0.f ? 0.f : 1.f / l[u];
+      float delta = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        delta += next.v[u][e] * o[u][e];
+        next.v[u][e] *= f;
+      }
+#pragma unroll
+      for (int x = 1; x < UNITS; x *= 2) delta += __shfl_xor(delta, x, 64);
+      if (next.unit(u) == 0) rm[next.row(u)] = -m[u], rd[next.row(u)] = -(delta * f);
+    }
+    next.put(stage);
+  };
+  fetch(r0);
+  bf16x4 *half = reinterpret_cast<bf16x4 *>(turn);
+  auto turn_at = [&](int part, int h) {  // rows 16 h + 4 g .. + 3 of this lane's key
+    return 2 * (key * Turn::ROW + part * Turn::PART + ((2 * h + (g >> 1)) ^ Turn::spread(key))) + (g & 1);
+  };
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i) Tile<DH>::put(kt, key, 4 * i + g, k[i]);
+#pragma unroll
+  for (int part = 0; part < 3; ++part)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) half[turn_at(part, h)] = bf16x4{};  // keys that are not there
+  const bf16x8 *qt = stage, *gt = stage + S::UNITS;
+  for (int t = r0; t < r1; t += 32) {
+    put();
+    __syncthreads();
+    fetch(t + 32);
+    if (!empty) {
+      f32x4 s[2], ds[2];  // start from -m and -delta / l of their rows
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = *reinterpret_cast<const f32x4 *>(rm + 16 * h + 4 * g);
+        ds[h] = *reinterpret_cast<const f32x4 *>(rd + 16 * h + 4 * g);
+      }
+      rows_times<DH>(qt, 0, c, g, k, s);
+      rows_times<DH>(gt, 0, c, g, v, ds);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[h][e] = __builtin_amdgcn_exp2f(s[h][e]);
+          ds[h][e] = key_ok ? ds[h][e] * s[h][e] : 0.f;
+        }
+      const Split8 x = split_pair(ds);
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        half[turn_at(part, 0)] = __builtin_shufflevector(x.p[part], x.p[part], 0, 1, 2, 3);
+        half[turn_at(part, 1)] = __builtin_shufflevector(x.p[part], x.p[part], 4, 5, 6, 7);
+      }
+      add_columns<DH>(dv, gt, 0, lane, split_pair(s));
+      add_columns<DH>(dk, qt, 0, lane, x);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) {
+      const int n = (wave * (DH / 32) + i) / 2, h = (wave * (DH / 32) + i) % 2;
+      f32x4 dq[1] = {zero4()};
+#pragma unroll 1
+      for (int first = 0; first < len; first += 32)
+        dq[0] = product6(Tile<DH>::columns(kt, first, n, lane), Turn::columns(turn, first, h, lane), dq[0]);
+      const int row = t + 16 * h + c;
+      if (row < r1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dq[0][e] *= kLn2;
+        store_quad(p.dq.ptr + row_offset(p, p.dq.ld, b, hk, row), 16 * n + 4 * g, p.dh, p.vec, dq[0]);
+      }
+    }
+  }
+  if (key >= p.Nk) return;
+  if (!key_ok) {  // (whatever its column held)
+#pragma unroll
+    for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
+  }
+  if (p.splits > 1) {
+    const long long pitch = (long long)p.Hkv * p.dh, all = (long long)p.B * p.Nk * pitch;
+    const long long at = key_offset(p, pitch, b, hk, key);
+    store_row<DH>(p.part + split * all + at, dk, p.scale, g, p.dh, p.dh % 4 == 0);
+    store_row<DH>(p.part + (p.splits + split) * all + at, dv, 1.f, g, p.dh, p.dh % 4 == 0);
+  } else {
+    store_row<DH>(p.dk.ptr + key_offset(p, p.dk.ld, b, hk, key), dk, p.scale, g, p.dh, p.vec);
+    store_row<DH>(p.dv.ptr + key_offset(p, p.dv.ld, b, hk, key), dv, 1.f, g, p.dh, p.vec);
+  }
+}
+
 // out[row][col] = sum of the parts in order; `rows` rows of `width` columns
 __global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part, int splits, long long rows, int width,
                                                               Result out) {
@@ -304,6 +441,7 @@ Side plan_side(long long own, long long other, long long heads, int dh, bool key
 }
 struct Plan {
   Side rows, keys;
+  bool few_keys;       // one kernel for all gradients
   size_t delta, part;  // floats
 };
 Plan make_plan(const Params &p) {
@@ -312,8 +450,9 @@ Plan make_plan(const Params &p) {
   // one part of the results, written and read at 4 TB/s
   n.rows = plan_side(p.rows, p.Nk, heads, p.dh, false, 2.0 * p.B * p.H * p.Nq * p.dh * 4 / 4e6);
   n.keys = plan_side(p.Nk, p.rows, heads, p.dh, true, 4.0 * p.B * p.Hkv * p.Nk * p.dh * 4 / 4e6);
-  n.delta = ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
-  const size_t q = n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
+  n.few_keys = p.Nk <= 64 && p.dh <= 64 && n.keys.block.groups == 4 && n.keys.block.waves == 4;
+  n.delta = n.few_keys ? 0 : ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
+  const size_t q = !n.few_keys && n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
   const size_t k = n.keys.splits > 1 ? (size_t)2 * n.keys.splits * p.B * p.Nk * p.Hkv * p.dh : 0;
   n.part = std::max(q, k);  // one after the other
   return n;
@@ -359,14 +498,18 @@ int launch(Params p, const Plan &n, hipStream_t st) {
   const long long heads = (long long)p.B * p.Hkv;
   const long long qw = heads * n.rows.blocks * n.rows.splits, kw = heads * n.keys.blocks * n.keys.splits;
   VITK_REQUIRE(qw < (1ll << 31) && kw < (1ll << 31), "vitk_cross_sdpa_bwd: too many rows for one launch");
-  if (p.Nq > 0) {
+  if (p.Nq > 0 && !n.few_keys) {
     p.blocks = n.rows.blocks, p.splits = n.rows.splits, p.chunk = n.rows.chunk;
     launch_dq<DH>(p, n.rows.block, (unsigned)qw, st);
     if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nq, p.H * p.dh, p.dq, st);
   }
   if (p.Nk > 0) {
     p.blocks = n.keys.blocks, p.splits = n.keys.splits, p.chunk = n.keys.chunk;
-    launch_dkv<DH>(p, n.keys.block, (unsigned)kw, st);
+    if (n.few_keys) {
+      if constexpr (DH <= 64) hipLaunchKernelGGL(cross_short_kernel<DH>, dim3((unsigned)kw), dim3(256), 0, st, p);
+    } else {
+      launch_dkv<DH>(p, n.keys.block, (unsigned)kw, st);
+    }
     if (p.splits > 1) {
       const long long rows = (long long)p.B * p.Nk;
       const int width = p.Hkv * p.dh;
