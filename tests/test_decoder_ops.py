@@ -121,6 +121,12 @@ ATTENTION = {
     "few_keys_many_rows": (2, 6, 6, 147, 50, 64, None, 0, 0),
     "long_keys_split": (1, 2, 1, 40, 3001, 64, [2999], 0, 0),
     "long_rows": (1, 2, 1, 1500, 70, 80, None, 0, 0),
+    # all keys of a head in one workgroup of the backward: rows of shared heads, split; lengths; alignment
+    "few_keys_shared_split": (3, 6, 2, 333, 64, 64, [64, 0, 33], 0, 0),
+    "few_keys_narrow": (2, 4, 1, 700, 31, 32, [31, 16], 4, 0),
+    "few_keys_unaligned": (2, 3, 1, 95, 49, 35, [49, 17], 1, 1),
+    "one_key_many_rows": (2, 2, 2, 1000, 1, 8, None, 0, 0),
+    "few_keys_full_device": (64, 8, 8, 45, 40, 60, None, 4, 0),
 }
 
 
@@ -654,7 +660,8 @@ def test_cross_attention_refuses(change, message):
     (dict(dout=0), "null pointer"), (dict(dq=0), "null pointer"), (dict(dk=0), "null pointer"), (dict(dv=0), "null pointer"),
     (dict(stats=0), "null pointer"), (dict(dq=24576), "one of the inputs"), (dict(dk=8192), "one of the inputs"),
     (dict(dv=16384), "one of the inputs"), (dict(dv=32768), "share"), (dict(dq=36864), "share"), (dict(ld_dq=31), "pitch"), (dict(ld_dv=15), "pitch"),
-    (dict(workspace=0), "workspace"), (dict(workspace_bytes=4), "workspace"), (dict(workspace=40964), "aligned")])
+    (dict(Nk=70, workspace=0), "workspace"), (dict(Nk=70, workspace_bytes=4), "workspace"),
+    (dict(Nk=70, workspace=40964), "aligned"), (dict(Nq=1000, workspace=0), "workspace")])
 def test_cross_attention_backward_refuses(change, message):
     from visiontransformer_amd import vitk
     d = vitk.dll()

@@ -294,11 +294,11 @@ struct Stage {
 
 // Groups of 16 rows (or keys) in a workgroup, and its waves.  Eight groups split the other side's tiles for 128
 // rows at once.  Four groups are four waves, of which several workgroups are on a CU, if there are at least as
-// many such workgroups as CUs; otherwise eight, so that two share a group's other side (64 columns, forward and
-// backward, eight waves -> four: 64 x 64, 2048 heads: 207 -> 140 us; 900 x 50, 24 heads: 52 -> 65).  More than 64
-// rows are cut into blocks of 64 where the last block of 128 were half empty and that is a sixth of the rows or more
-// (147 x 197, 320 heads: forward 42 -> 33, row gradient 19 less), up to `half` on the other side, and up to
-// `any` on the other side always (row gradient of 512 x 50, 192 heads: 7 less; 512 x 197: 2 more).
+// many such workgroups as CUs; otherwise eight, so that two share a group's other side (64 columns, forward, eight
+// waves -> four: 64 x 64, 2048 heads: 40 -> 33 us; 50 x 900, 24 heads: 18 -> 23).  More than 64 rows are cut into
+// blocks of 64 where the last block of 128 were half empty and that is a sixth of the rows or more (147 x 197, 320
+// heads: forward 42 -> 33, row gradient 19 less), up to `half` on the other side, and up to `any` on the other
+// side always (row gradient of 512 x 128, 192 heads: 5 less; 512 x 197: 2 more).
 struct Block {
   int groups, waves;
 };

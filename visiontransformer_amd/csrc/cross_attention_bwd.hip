@@ -12,8 +12,8 @@
 // other side.  Where the blocks are too few for the device, the other side is split over workgroups and
 // the parts are added in order by a second launch.
 // Bound by the matrix cores (512 x 1536 x 96, 128 heads of which 4 share a key head: dQ 330 us, dK and dV 461, 1054
-// and 1006 TFLOP/s of bf16 products; 16 entries of 1024 keys: 522, 1185); short keys by the start and the end of
-// a workgroup (147 x 50 x 64, 384 heads: 28.5 and 27.4 us, twice what they move at the rate of a copy).
+// and 1006 TFLOP/s of bf16 products; 16 entries of 1024 keys: 522, 1185); few keys by the start and the
+// end of a workgroup.
 #include "cross_attention.h"
 
 #include <algorithm>
@@ -38,10 +38,9 @@ __device__ __forceinline__ void take(const float *box, f32x4 (&acc)[NB]) {
     for (int e = 0; e < 4; ++e) acc[n][e] += box[(4 * n + e) * 64];
 }
 
-// Workgroups of four waves that a CU holds, with one group of rows or keys a wave.  (Of 128 columns one, which is
-// slower than eight waves that share the groups: 64 x 64, 2048 heads, both together 370 -> 386 us.)
+// Workgroups of four waves that a CU holds, with one group of rows (or keys: 2) a wave.  (Of 128 columns one,
+// which is slower than eight waves that share the groups: 64 x 64, 2048 heads, both together 370 -> 386 us.)
 constexpr int dq_resident(int dh) { return dh <= 32 ? 4 : dh <= 64 ? 3 : 2; }
-constexpr int dkv_resident(int dh) { return dh <= 32 ? 4 : 2; }
 
 template <int DH, int NW, int RW>
 __global__ __launch_bounds__(64 * NW, NW == 4 && RW == 4 ? dq_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1)
@@ -152,7 +151,7 @@ void cross_dq_kernel(const Params p) {
 }
 
 template <int DH, int NW, int KG>
-__global__ __launch_bounds__(64 * NW, NW == 4 && KG == 4 ? dkv_resident(DH) : NW == 8 || DH <= 64 ? 2 : 1)
+__global__ __launch_bounds__(64 * NW, NW == 8 || KG == 4 ? 2 : 1)
 void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
@@ -271,14 +270,18 @@ void cross_dkv_kernel(const Params p) {
 // Few keys: all of a (batch, key head) in one workgroup of four waves, so dQ is complete here too: five products
 // instead of seven, and each row is read once.  Each wave forms p and ds of its 16 keys with a stage of 32 rows
 // and adds to dK and dV; ds goes through LDS as [key][row], and dQ^T[d][row] += K^T ds is dealt to the waves by
-// blocks of 16 x 16.  K is there times scale log2(e), for the scores.
+// blocks of 16 x 16.  K is there times scale log2(e), for the scores.  With fewer heads than places, rows are split.
+// 147 x 50 x 64, 384 heads: 37 us (dQ, then dK and dV: 56); 50 x 50, 512 heads 21 (28); 900 x 50, 24 heads, split
+// 28 (43).  (64 columns fill the registers of two workgroups a CU.)
+constexpr int FEW_KEYS = 64;
+constexpr int short_resident(int dh) { return dh <= 32 ? 3 : 2; }
 template <int DH>
-__global__ __launch_bounds__(256, 2) void cross_short_kernel(const Params p) {
+__global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(const Params p) {
   typedef Shape<DH, 4, 4> S;
   typedef Tile<32> Turn;
   constexpr int UNITS = DH / 8;  // of a row of a stage: that many lanes load it
   static_assert(DH <= 64 && 64 % UNITS == 0, "the lanes of a row are neighbours in a wave");
-  __shared__ __attribute__((aligned(16))) bf16x8 stage[2 * S::UNITS], kt[64 * Tile<DH>::ROW], turn[64 * Turn::ROW];
+  __shared__ __attribute__((aligned(16))) bf16x8 stage[2 * S::UNITS], kt[FEW_KEYS * Tile<DH>::ROW], turn[FEW_KEYS * Turn::ROW];
   __shared__ __attribute__((aligned(16))) float rm[32], rd[32];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -405,10 +408,12 @@ __global__ __launch_bounds__(256, 2) void cross_short_kernel(const Params p) {
   }
 }
 
-// out[row][col] = sum of the parts in order; `rows` rows of `width` columns
+// out[row][col] = sum of the parts in order; `rows` rows of `width` columns; of two gradients at once: y
 __global__ __launch_bounds__(256) void cross_add_parts_kernel(const float *part, int splits, long long rows, int width,
-                                                              Result out) {
+                                                              Result x, Result y) {
   const long long all = rows * width;
+  const Result out = blockIdx.y == 0 ? x : y;
+  part += blockIdx.y * splits * all;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
     float s = 0.f;
 #pragma unroll 4
@@ -430,7 +435,7 @@ Side plan_side(long long own, long long other, long long heads, int dh, bool key
   s.blocks = (int)((own + 16 * groups - 1) / (16 * groups));
   const long long stages = (other + 63) / 64;
   const int wide = dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128;
-  const int four = keys ? dkv_resident(dh) : dq_resident(dh);
+  const int four = keys ? 2 : dq_resident(dh);
   const int resident = groups == 4 && s.block.waves == 4 ? four : groups == 2 ? 2 : 1;  // workgroups a CU
   const double flop = 32.0 * (keys ? 4 : 3) * groups * other * wide;  // of a block; 0.5 TFLOP/s a CU
   const int splits = plan_splits(heads * s.blocks, resident * (long long)vitk::cu_count(), stages,
@@ -450,7 +455,15 @@ Plan make_plan(const Params &p) {
   // one part of the results, written and read at 4 TB/s
   n.rows = plan_side(p.rows, p.Nk, heads, p.dh, false, 2.0 * p.B * p.H * p.Nq * p.dh * 4 / 4e6);
   n.keys = plan_side(p.Nk, p.rows, heads, p.dh, true, 4.0 * p.B * p.Hkv * p.Nk * p.dh * 4 / 4e6);
-  n.few_keys = p.Nk <= 64 && p.dh <= 64 && n.keys.block.groups == 4 && n.keys.block.waves == 4;
+  n.few_keys = p.Nk > 0 && p.Nk <= FEW_KEYS && p.dh <= 64;
+  if (n.few_keys) {  // one round of workgroups, and two stages of rows or more in each
+    const long long stages = ((long long)p.rows + 31) / 32;
+    const long long places = short_resident(p.dh) * (long long)vitk::cu_count();
+    const int splits = (int)std::max(std::min({places / heads, (stages + 1) / 2, (long long)16}), 1ll);
+    n.keys.blocks = 1;
+    n.keys.chunk = std::max((int)((stages + splits - 1) / splits) * 32, 32);
+    n.keys.splits = std::max((int)(((long long)p.rows + n.keys.chunk - 1) / n.keys.chunk), 1);
+  }
   n.delta = n.few_keys ? 0 : ((size_t)p.B * p.H * p.Nq + 63) / 64 * 64;
   const size_t q = !n.few_keys && n.rows.splits > 1 ? (size_t)n.rows.splits * p.B * p.Nq * p.H * p.dh : 0;
   const size_t k = n.keys.splits > 1 ? (size_t)2 * n.keys.splits * p.B * p.Nk * p.Hkv * p.dh : 0;
@@ -475,22 +488,27 @@ void launch_dq(const Params &p, Block block, unsigned wgs, hipStream_t st) {
 }
 template <int DH>
 void launch_dkv(const Params &p, Block block, unsigned wgs, hipStream_t st) {
-  if constexpr (DH <= 96) {
-    if (block.groups == 4 && block.waves == 4) {
+  if constexpr (DH > 64) {  // others are not here with so few keys
+    if (block.groups == 2) {
+      hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+      return;
+    }
+    if (block.groups == 4 && block.waves == 8) {
+      hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
+      return;
+    }
+  }
+  if constexpr (DH == 96) {
+    if (block.groups == 4) {
       hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
       return;
     }
   }
-  if (block.groups == 8)
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
-  else if (block.groups == 4)
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
-  else
-    hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
 }
-void add_parts(const float *part, int splits, long long rows, int width, Result out, hipStream_t st) {
-  hipLaunchKernelGGL(cross_add_parts_kernel, dim3(vitk::grid_for(rows * width, 256)), dim3(256), 0, st, part, splits, rows,
-                     width, out);
+void add_parts(const float *part, int splits, long long rows, int width, Result x, const Result *y, hipStream_t st) {
+  hipLaunchKernelGGL(cross_add_parts_kernel, dim3(vitk::grid_for(rows * width, 256), y ? 2 : 1), dim3(256), 0, st, part,
+                     splits, rows, width, x, y ? *y : x);
 }
 
 template <int DH>
@@ -501,7 +519,7 @@ int launch(Params p, const Plan &n, hipStream_t st) {
   if (p.Nq > 0 && !n.few_keys) {
     p.blocks = n.rows.blocks, p.splits = n.rows.splits, p.chunk = n.rows.chunk;
     launch_dq<DH>(p, n.rows.block, (unsigned)qw, st);
-    if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nq, p.H * p.dh, p.dq, st);
+    if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nq, p.H * p.dh, p.dq, nullptr, st);
   }
   if (p.Nk > 0) {
     p.blocks = n.keys.blocks, p.splits = n.keys.splits, p.chunk = n.keys.chunk;
@@ -510,12 +528,7 @@ int launch(Params p, const Plan &n, hipStream_t st) {
     } else {
       launch_dkv<DH>(p, n.keys.block, (unsigned)kw, st);
     }
-    if (p.splits > 1) {
-      const long long rows = (long long)p.B * p.Nk;
-      const int width = p.Hkv * p.dh;
-      add_parts(p.part, p.splits, rows, width, p.dk, st);
-      add_parts(p.part + p.splits * rows * width, p.splits, rows, width, p.dv, st);
-    }
+    if (p.splits > 1) add_parts(p.part, p.splits, (long long)p.B * p.Nk, p.Hkv * p.dh, p.dk, &p.dv, st);
   }
   return vitk::check_launch("vitk_cross_sdpa_bwd");
 }
