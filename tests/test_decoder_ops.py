@@ -382,6 +382,16 @@ EMBED = {
     "one_token_takes_all_long": (5000, 20, 200003, "same"),
     "two_levels": (20000, 12, 40000, "rank"),
     "large_table_few_tokens": (100003, 32, 9, "uniform"),
+    # placed by counting (up to 8192 tokens; 4096 over a table of one digit), by digits behind that
+    "counted_most": (20000, 40, 8192, "rank"),
+    "counted_odd": (70001, 36, 8191, "padded"),
+    "counted_outside": (20000, 32, 3333, "outside"),
+    "counted_one_chunk": (20000, 48, 31, "rank"),
+    "counted_small_table": (200, 64, 4096, "rank"),
+    "digits_two": (3000, 64, 8193, "rank"),
+    "digits_one": (200, 64, 4097, "padded"),
+    "digits_three": (70001, 36, 9001, "rank"),
+    "direct_largest_table": (16384, 36, 1024, "rank"),
 }
 
 
@@ -690,7 +700,7 @@ def test_cross_attention_refuses_null_arguments_and_a_missing_workspace():
     ("vitk_embedding_bwd", (4096, 4096, 3, -10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "bad shape"),
     ("vitk_embedding_bwd", (None, 4096, 3, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "null pointer"),
     ("vitk_embedding_bwd", (4096, 4096, 3, 10, 8, 1.0, 0, None, 4096, 1 << 20, None), "null pointer"),
-    ("vitk_embedding_bwd", (4096, 4096, 3, 5000, 8, 1.0, 0, 8192, None, 1 << 20, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 3, 50000, 8, 1.0, 0, 8192, None, 1 << 20, None), "workspace"),
     ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4096, 16, None), "workspace"),
     ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4100, 1 << 20, None), "aligned"),
     ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 8192, 4096, 1 << 20, None), "tokens over"),

@@ -4,9 +4,9 @@
 //
 // Both are bound by memory.  The backward reads dout once and writes the table once; what decides is
 // that a few tokens make up most of a batch, so the work is cut by tokens, not by table rows:
-//   1. a stable radix sort of (token, position), 8 bits a pass: counts per block and digit, then the scatter.
-//      The launches also clear the table: the clearing is most of their
-//      traffic and hides the latency of the sort;
+//   1. a stable sort of (token, position).  Up to 8192 tokens by counting the smaller ones, one launch; more by
+//      digits of 8 bits: counts per block and digit, then the scatter.  The launches also clear the table: the
+//      clearing is most of their traffic and hides the latency of the sort;
 //   2. sums over chunks of 32 sorted positions.  A token that lies inside one chunk is finished; one
 //      that crosses a border leaves partial rows (at most one at each end of a chunk), which are
 //      again a sorted list, 1/16 as long, summed the same way in chunks of 64 until at most
@@ -16,9 +16,12 @@
 // Every sum has a fixed order (positions, then chunks); integer counts are the only atomics, in LDS.
 #include "common.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
 
@@ -103,8 +106,8 @@ __device__ __forceinline__ int token(const Sort &s, int i) {
 // Workgroups behind the sort's clear the table.
 __device__ __forceinline__ bool clear_part(const Sort &s) {
   if ((int)blockIdx.x < s.blocks) return false;
-  const long long stride = (long long)(gridDim.x - s.blocks) * TPB;
-  const long long first = (long long)(blockIdx.x - s.blocks) * TPB + threadIdx.x;
+  const long long stride = (long long)(gridDim.x - s.blocks) * blockDim.x;
+  const long long first = (long long)(blockIdx.x - s.blocks) * blockDim.x + threadIdx.x;
   // scalar stores up to the first 16-byte border, then quads, then what is left
   const long long lead = min((long long)((16 - ((uintptr_t)s.fill & 15)) & 15) / 4, s.fill_n);
   const long long quads = (s.fill_n - lead) / 4;
@@ -188,6 +191,51 @@ __global__ __launch_bounds__(TPB) void embedding_scatter_kernel(const Sort s) {
       s.pos_out[to] = s.pos ? s.pos[i] : i;
     }
   }
+}
+
+// Up to RANK_TOKENS tokens in one launch instead of two a digit (8000 tokens x 192 over 4000 rows, all launches:
+// 21.8 us instead of 28; over a table of one digit up to half as many, where it takes 15.8 and digits 16): a token's place is the number of tokens before it
+// in the order (token, position).  A workgroup places 32, each counted by 32 threads; all tokens are in LDS.
+constexpr int RANK_TOKENS = 8192, RANK_THREADS = 1024, RANK_TILE = 32, RANK_PARTS = RANK_THREADS / RANK_TILE;
+__global__ __launch_bounds__(RANK_THREADS) void embedding_rank_kernel(const Sort s) {
+  __shared__ __attribute__((aligned(16))) int32_t keys[RANK_TOKENS];
+  __shared__ int part[RANK_PARTS][RANK_TILE];
+  if (clear_part(s)) return;
+  const int size = (s.n + 4 * RANK_PARTS - 1) / (4 * RANK_PARTS) * 4;  // of a part; all of them fit `keys`
+#pragma unroll
+  for (int u = 0; u < RANK_TOKENS / RANK_THREADS; ++u) {
+    const int i = threadIdx.x + RANK_THREADS * u, k = token(s, min(i, s.n - 1));
+    keys[i] = i < s.n ? k : INT32_MAX;
+  }
+  __syncthreads();
+  const int i0 = blockIdx.x * RANK_TILE, t = threadIdx.x % RANK_TILE, i = i0 + t, own = threadIdx.x / RANK_TILE;
+  const int mine = keys[i], j0 = own * size, j1 = j0 + size;
+  int count = 0;
+  auto four = [&](int j) { return *reinterpret_cast<const i32x4 *>(keys + j); };
+#pragma unroll 4
+  for (int j = j0; j < min(j1, i0); j += 4) {  // before the tile: equal ones too
+    const i32x4 k = four(j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) count += k[e] <= mine;
+  }
+  for (int j = max(j0, i0); j < min(j1, i0 + RANK_TILE); j += 4) {
+    const i32x4 k = four(j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) count += k[e] < mine || (k[e] == mine && j + e < i);
+  }
+#pragma unroll 4
+  for (int j = max(j0, i0 + RANK_TILE); j < j1; j += 4) {
+    const i32x4 k = four(j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) count += k[e] < mine;
+  }
+  part[own][t] = count;
+  __syncthreads();
+  if (own > 0 || i >= s.n) return;
+#pragma unroll
+  for (int w = 1; w < RANK_PARTS; ++w) count += part[w][t];
+  s.key_out[count] = mine;
+  s.pos_out[count] = i;
 }
 
 // ------------------------------------------------------------------------------------------ sums
@@ -322,10 +370,10 @@ __global__ __launch_bounds__(TPB) void embedding_join_kernel(const Sums s) {
   store_cols<W>(dst, acc);
 }
 
-// Few tokens, small table: no sort (528 tokens x 192 over 1000 rows: 4 us; the sort's five launches 20).  One
-// workgroup per table row; each wave looks through a quarter of the tokens and adds the rows of its own in their
-// order, the four sums are added in order.
-constexpr int DIRECT_TOKENS = 1024, DIRECT_TABLE = 4096;
+// Few tokens, not too large a table: no sort (528 tokens x 192 over 1000 rows: 4 us; 1000 over 6000 and 16000
+// rows 6 and 12.7, by counting 15 and 15.6).  One workgroup per table row; each wave looks through a quarter of the
+// tokens and adds the rows of its own in their order, the four sums are added in order.
+constexpr int DIRECT_TOKENS = 1024, DIRECT_TABLE = 16384;
 template <int W>
 __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__restrict__ dout,
                                                                const int32_t *__restrict__ index, int n, long long D,
@@ -389,7 +437,7 @@ __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__re
 bool direct(long long n, long long V) { return n <= DIRECT_TOKENS && V <= DIRECT_TABLE; }
 
 struct Plan {
-  int passes, blocks, chunk;
+  int passes, blocks, chunk;  // no passes: by rank
   int levels;
   long long chunks[8];
   // offsets in the workspace, in 4-byte units
@@ -401,6 +449,7 @@ Plan make_plan(long long n, long long V, long long D) {
   int bits = 1;
   while ((V >> bits) != 0) ++bits;  // V itself is the key of padding
   p.passes = (bits + 7) / 8;
+  if (n <= (p.passes > 1 ? RANK_TOKENS : RANK_TOKENS / 2)) p.passes = 0;
   long long blocks = (n + BLOCK_MIN - 1) / BLOCK_MIN;
   if (blocks > MAX_BLOCKS) blocks = MAX_BLOCKS;
   p.chunk = (int)(((n + blocks - 1) / blocks + TPB - 1) / TPB * TPB);
@@ -411,8 +460,8 @@ Plan make_plan(long long n, long long V, long long D) {
     at += (count + 63) / 64 * 64;
     return r;
   };
-  for (int i = 0; i < 2; ++i) p.key[i] = take(n), p.pos[i] = take(n);
-  p.hist = take((long long)DIGITS * p.blocks);
+  for (int i = 0; i < (p.passes > 0 ? 2 : 1); ++i) p.key[i] = take(n), p.pos[i] = take(n);
+  p.hist = take(p.passes > 0 ? (long long)DIGITS * p.blocks : 0);
   long long entries = n, size = CHUNK1;
   do {
     const long long c = (entries + size - 1) / size;
@@ -506,25 +555,27 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
   // the clearing, a tenth to each count and the rest to the scatters, which take longer (multiples of 4 floats)
   const long long all = accumulate ? 0 : V * D;
   long long cleared = 0;
-  auto sort_launch = [&](bool scatter, bool last) {
-    const long long share = (all / p.passes * (scatter ? 4 : 1) / 5 + 3) / 4 * 4;
+  auto sort_launch = [&](void (*kernel)(Sort), unsigned threads, long long share, bool last) {
+    share = (share + 3) / 4 * 4;
     s.fill = dtable + cleared;
-    s.fill_n = last ? all - cleared : (share < all - cleared ? share : all - cleared);
+    s.fill_n = last ? all - cleared : std::min(share, all - cleared);
     cleared += s.fill_n;
-    const long long want = (s.fill_n / 4 + TPB * 4 - 1) / (TPB * 4);
-    const unsigned grid = (unsigned)(s.blocks + (want < 2048 ? want : 2048) + (s.fill_n > 0 && want == 0));
-    if (scatter)
-      hipLaunchKernelGGL(embedding_scatter_kernel, dim3(grid), dim3(TPB), 0, st, s);
-    else
-      hipLaunchKernelGGL(embedding_count_kernel, dim3(grid), dim3(TPB), 0, st, s);
+    const long long want = (s.fill_n / 4 + threads * 4 - 1) / (threads * 4);
+    const unsigned grid = (unsigned)(s.blocks + std::min(want, (long long)(2048 * TPB / threads)) + (s.fill_n > 0 && want == 0));
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, s);
   };
+  if (p.passes == 0) {
+    s.blocks = (int)((rows + RANK_TILE - 1) / RANK_TILE);
+    s.key = index, s.key_out = iw + p.key[0], s.pos_out = iw + p.pos[0];
+    sort_launch(embedding_rank_kernel, RANK_THREADS, all, true);
+  }
   for (int pass = 0; pass < p.passes; ++pass) {
     s.key = pass == 0 ? index : iw + p.key[1 - (pass & 1)];
     s.pos = pass == 0 ? nullptr : iw + p.pos[1 - (pass & 1)];
     s.key_out = iw + p.key[pass & 1], s.pos_out = iw + p.pos[pass & 1];
     s.shift = 8 * pass;
-    sort_launch(false, false);
-    sort_launch(true, pass + 1 == p.passes);
+    sort_launch(embedding_count_kernel, TPB, all / p.passes / 5, false);
+    sort_launch(embedding_scatter_kernel, TPB, all / p.passes * 4 / 5, pass + 1 == p.passes);
   }
   Sums q = {};
   q.key = s.key_out, q.pos = s.pos_out, q.src = dout;
