@@ -607,6 +607,69 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   }
 }
 
+// The symmetric products where 32 x 32 tiles leave CUs without work: 16 x 16 tiles, half as much for each to read.
+// The contraction is dealt to the waves, 32 k a step, a line of planes for 16 rows; the first wave adds the sums.
+template <int MODE, int NW>
+__global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int flip) {
+  static_assert(MODE <= POLY, "the symmetric products");
+  constexpr int U = 4, PITCH = 20;  // steps in flight
+  __shared__ __attribute__((aligned(16))) float lds[NW][16 * PITCH];
+  const int depth = MODE == GRAM ? p.np : p.rp, ti = (p.r + 31) / 32 * 2, tiles = ti * (ti + 1) / 2;
+  const long long k = blockIdx.x / tiles;
+  int bi, bj;
+  tile_of<true>(blockIdx.x % tiles, ti, bi, bj);
+  const int i0 = bi * 16, j0 = bj * 16;
+  const _Float16 *P = MODE == GRAM ? p.yp[flip] : p.gp;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int steps = ((MODE == GRAM ? p.n : p.r) + 31) / 32, share = (steps + NW - 1) / NW;  // what is behind is zero
+  const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps);
+  const _Float16 *prow = P + (k * p.rp + i0 + c) * 2ll * depth + 8 * g;
+  const _Float16 *qrow = P + (k * p.rp + j0 + c) * 2ll * depth + 8 * g;
+  const int i = lane >> 2, j = (lane & 3) * 4;  // the first wave's elements of the result
+  Parts add = {};
+  if (wave == 0) add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = s0; s < s1; s += U) {
+    f16x8 a[U][2], b[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const int at = min(s + u, s1 - 1) * 64 + 32 * part;
+        a[u][part] = *reinterpret_cast<const f16x8 *>(prow + at);
+        b[u][part] = *reinterpret_cast<const f16x8 *>(qrow + at);
+      }
+    __builtin_amdgcn_sched_barrier(0);  // keep them all in flight
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= s1) a[u][0] = a[u][1] = f16x8{};  // (a step that was loaded twice adds nothing)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][0], a[u][1], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][1], a[u][0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][0], a[u][0], acc, 0, 0, 0);
+    }
+  }
+  *reinterpret_cast<f32x4 *>(lds[wave] + c * PITCH + 4 * g) = acc;
+  __syncthreads();
+  if (wave > 0) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < NW; ++x) {
+    const f32x4 w = *reinterpret_cast<const f32x4 *>(lds[x] + i * PITCH + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += w[e];
+  }
+  v = finish<MODE>(p, flip, k, i0 + i, j0 + j, v, add);
+  if (bi == bj) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  *reinterpret_cast<f32x4 *>(lds[0] + i * PITCH + j) = v;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  f32x4 w;  // (j0 + i, i0 + j ..)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = lds[0][(j + e) * PITCH + i];
+  finish_transposed<MODE>(p, k, j0 + i, i0 + j, w);
+}
+
 // Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of
 // y and of g, then b g + c g g, are in LDS (70 KiB each), what a wave adds to its products in registers.  All
 // blocks of g are computed: writing a block's mirror image, two bytes at a time, takes longer than its product.
@@ -842,6 +905,16 @@ void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
   const long long ti = (p.r + t - 1) / t, tj = (p.n + t - 1) / t;
   const long long total = p.batch * (MODE <= POLY ? ti * (ti + 1) / 2 : ti * tj);
   const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  if constexpr (MODE <= POLY) {
+    if (form == FORM_SMALL && total < vitk::cu_count()) {
+      const unsigned wgs = (unsigned)(p.batch * ti * (2 * ti + 1));  // twice the tiles a side
+      if ((MODE == GRAM ? p.n : p.r) > 512)
+        hipLaunchKernelGGL((ns_lower_kernel<MODE, 8>), dim3(wgs), dim3(512), 0, st, p, flip);
+      else
+        hipLaunchKernelGGL((ns_lower_kernel<MODE, 4>), dim3(wgs), dim3(256), 0, st, p, flip);
+      return;
+    }
+  }
   if (form == FORM_128)
     hipLaunchKernelGGL((ns_tile_kernel<MODE, 128, 8>), grid, dim3(512), 0, st, p, flip, (int)total);
   else if (form == FORM_64)
