@@ -226,12 +226,16 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsParams p, int las
   const int t = blockIdx.x % tiles, i0 = t / tj * T, j0 = t % tj * T;
   const float norm = (float)sqrt(wave_sum(p.sums[k * PARTS + (threadIdx.x & 63)])) + p.eps;
   if (p.tall) {  // rows of the user's matrix are columns here
+    float x[T * T / 256];
+#pragma unroll
+    for (int w = 0; w < T * T / 256; ++w) {
+      const int u = threadIdx.x + 256 * w, j = min(j0 + u / T, p.n - 1), i = min(i0 + u % T, p.r - 1);
+      x[w] = update_value(p, k * p.stride_x + j * p.ld_x + i, false);
+    }
 #pragma unroll
     for (int w = 0; w < T * T / 256; ++w) {
       const int u = threadIdx.x + 256 * w, j = u / T, i = u % T;
-      float v = 0.f;
-      if (i0 + i < p.r && j0 + j < p.n) v = update_value(p, k * p.stride_x + (j0 + j) * p.ld_x + i0 + i, false) / norm;
-      tile[i][j] = v;
+      tile[i][j] = i0 + i < p.r && j0 + j < p.n ? x[w] / norm : 0.f;
     }
     __syncthreads();
   }
@@ -512,7 +516,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
   constexpr int U = TR ? 4 : 8;       // steps of 16 k in flight
   constexpr int PITCH = 80;           // fp16 pitch of a row of transposed operand (64 + a shift of 32 bytes)
-  constexpr int SUM_PITCH = 36, REGION = TR ? U * 16 * PITCH * 2 : 32 * SUM_PITCH * 4;  // bytes of a wave
+  constexpr int SUM_PITCH = 36, REGION = TR ? 2 * 16 * PITCH * 2 : 32 * SUM_PITCH * 4;  // bytes of a wave
   static_assert(REGION >= 32 * SUM_PITCH * 4, "the wave's sums go where its operand was");
   __shared__ __attribute__((aligned(16))) char lds[NW][REGION];
   const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
@@ -553,21 +557,24 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s + u >= s1) a[u][0] = a[u][1] = f16x8{};  // (a step that was loaded twice adds nothing)
-    if constexpr (TR) {  // through the wave's own part of LDS
+    if constexpr (TR) {  // through the wave's own part of LDS, two steps at a time (so that three workgroups fit a CU)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; u += 2) {
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-          *reinterpret_cast<f16x8 *>(qt + (u * 16 + (lane >> 2)) * PITCH + 32 * part + 8 * (lane & 3)) = b[u][part];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+          for (int part = 0; part < 2; ++part)
+            *reinterpret_cast<f16x8 *>(qt + (x * 16 + (lane >> 2)) * PITCH + 32 * part + 8 * (lane & 3)) = b[u + x][part];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          const int row = u * 16 + 8 * g + ((lane & 15) >> 2), col = 32 * part + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          b[u][part] = join(read_transposed(qt + row * PITCH + col), read_transposed(qt + (row + 4) * PITCH + col));
-        }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const int row = x * 16 + 8 * g + ((lane & 15) >> 2), col = 32 * part + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            b[u + x][part] = join(read_transposed(qt + row * PITCH + col), read_transposed(qt + (row + 4) * PITCH + col));
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) acc = product3(b[u][0], b[u][1], a[u][0], a[u][1], acc);
