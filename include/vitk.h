@@ -308,7 +308,8 @@ int vitk_sdpa_row_bwd(const float *q, int64_t ld_q, const float *k, const float 
  * stats (optional in the forward, required by the backward; [B*H][Nq][2]): {row maximum of the
  * scaled scores times log2(e), row sum of exp(score - maximum)}.
  * Any Nq, Nk >= 0, 1 <= dh <= 128, any alignment.  Products are formed to fp32 accuracy from three
- * bf16 parts of each operand: finite numbers below 3.38e38 (an infinity among them gives NaN);
+ * bf16 parts of each operand: finite numbers below 3.38e38 (an infinity among them gives NaN), and
+ * scores that are finite in fp32;
  * numbers below 2^-100 keep fewer than 24 bits.  Outputs must not overlap inputs or each other.  The sum over
  * a row's keys may be split over workgroups, a rule on the sizes; every result has a fixed order of sums.
  * workspace: vitk_cross_sdpa_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments (0 =
@@ -453,7 +454,7 @@ int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float 
  * close to the exact result as the same steps in fp32.  A zero matrix gives zeros (NaN with eps = 0).
  * out may be x, with one layout for both; no other overlap.
  * 0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1] within [-4, 4], with
- * |b t^2 + c t^4| below 31 (checked on 65 points), which every useful triple does.
+ * |b t^2 + c t^4| below 31 (checked from the largest values of each step), which every useful triple does.
  * vitk_muon_f32 (p, g, m share ld and stride, as arenas of one layout do):
  *   m = momentum*m + grad_scale*g;  u = nesterov ? grad_scale*g + momentum*m : m
  *   p = p * (1 - lr*weight_decay) - lr*update_scale * NS(u)

@@ -763,7 +763,88 @@ def test_bindings_refuse_wrong_tensors():
         vitk.muon_args(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), lr=0.1)
 
 
+@gpu
+def test_the_bindings_refuse_another_device(K):
+    g = rng(5)
+    x, out = randn(g, 16, 16), torch.empty(16, 16, device="cuda")
+    args = K.newton_schulz_args(x, out)
+    assert args.device == torch.cuda.current_device()
+    args.device += 1  # as if its tensors were there
+    with pytest.raises(K.VitkError, match="current one"):
+        K.newton_schulz(args)
+    with pytest.raises(K.VitkError, match="current one"):
+        K.stream(torch.cuda.current_device() + 1)
+    with pytest.raises(K.VitkError, match="different devices"):
+        K._one_device(x, torch.empty(2))
+
+
+def test_newton_schulz_takes_every_triple_that_stays_and_no_other():
+    """A coarse search over triples: what is accepted stays within the bounds on a fine grid."""
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    r = np.random.default_rng(9)
+    t0 = np.linspace(0.0, 1.0, 20001)
+    seen = set()
+    for _ in range(400):
+        a, b, c = (np.float32(x) for x in r.uniform((0.0, -12.0, -2.0), (6.0, 6.0, 8.0)))
+        if r.random() < 0.2:
+            c = np.float32(0.0)
+        if r.random() < 0.1:
+            b = np.float32(0.0)
+        steps = int(r.integers(1, 9))
+        args = _nargs(vitk, vitk.NewtonSchulzArgs, a=a, b=b, c=c, steps=steps, workspace=0)  # refused either way
+        assert d.vitk_newton_schulz_f32(C.byref(args), None) != 0
+        taken = "bounded" not in d.vitk_last_error().decode()
+        seen.add(taken)
+        if taken:
+            t = t0.copy()
+            for _ in range(steps):
+                poly = float(b) * t ** 2 + float(c) * t ** 4
+                assert (np.abs(poly) < 31.0).all()
+                t = float(a) * t + poly * t
+                assert (np.abs(t) <= 4.0 + 1e-9).all(), (a, b, c, steps)
+    assert seen == {True, False}
+
+
 # ---------------------------------------------------------------------------- the run together
+@gpu
+def test_all_of_them_captured_in_one_graph(K):
+    """Few keys (one kernel in the backward), tokens placed by counting, one launch of Newton-Schulz."""
+    g = rng(77)
+    x, out = randn(g, 96, 96), torch.empty(96, 96, device="cuda")
+    q, k, v, dout = randn(g, 2, 70, 4, 64), randn(g, 2, 40, 4, 64), randn(g, 2, 40, 4, 64), randn(g, 2, 70, 4, 64)
+    o, dq, dk, dv = (torch.empty_like(t) for t in (q, q, k, v))
+    ns = K.newton_schulz_args(x, out)
+    attn = K.cross_sdpa_args(q, k, v, o, stats=torch.empty(8, 70, 2, device="cuda"), dout=dout, dq=dq, dk=dk, dv=dv)
+    index = tokens("rank", 20000, 3000, 4)
+    d, dtable = randn(g, 3000, 64), torch.empty(20000, 64, device="cuda")
+    workspace = torch.empty(K.dll().vitk_embedding_bwd_workspace_bytes(3000, 20000, 64) // 4 + 1, device="cuda")
+
+    def run():
+        K.newton_schulz(ns)
+        K.cross_sdpa_fwd(attn)
+        K.cross_sdpa_bwd(attn)
+        K.embedding_bwd(d, index, dtable, workspace=workspace)
+
+    results = (out, o, dq, dk, dv, dtable)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(3):
+        for t in (x, q, k, v, dout, d):
+            t.mul_(1.25)
+        for t in results:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in results]
+        run()
+        for a, b in zip(replayed, results):
+            assert torch.equal(a, b), i
+
+
 @gpu
 def test_the_bindings_follow_the_current_stream(K):
     assert K.stream() == torch.cuda.current_stream().cuda_stream

@@ -29,6 +29,7 @@
 // 131 us, the latency of 15 dependent products.
 #include "common.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -892,16 +893,24 @@ bool size_ok(int64_t rows, int64_t cols, int64_t batch) {
   return rows >= 0 && cols >= 0 && batch >= 0 && rows <= (1 << 20) && cols <= (1 << 20);
 }
 
-// Does the iteration t -> a t + b t^3 + c t^5 stay where the fixed scales hold?
-bool bounded(float a, float b, float c, int steps) {
-  for (int i = 0; i <= 64; ++i) {
-    double t = i / 64.0;
-    for (int s = 0; s < steps; ++s) {
-      const double q = t * t, poly = b * q + c * q * q;
+// Does the iteration t -> a t + b t^3 + c t^5 stay where the fixed scales hold?  From |t| <= top, the largest values
+// of the odd polynomial, and of b q + c q^2 with q = t^2, are at the ends or where their derivatives vanish.
+bool bounded(double a, double b, double c, int steps) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  double top = 1.0;
+  for (int s = 0; s < steps; ++s) {
+    const double end = top * top, root = std::sqrt(std::max(9.0 * b * b - 20.0 * a * c, 0.0));
+    const double at[] = {end, c != 0.0 ? -b / (2.0 * c) : end, c != 0.0 ? (-3.0 * b + root) / (10.0 * c) : -a / (3.0 * b),
+                         c != 0.0 ? (-3.0 * b - root) / (10.0 * c) : end};
+    double next = 0.0;
+    for (const double x : at) {
+      if (!(x >= 0.0)) continue;
+      const double q = std::min(x, end), poly = b * q + c * q * q;
       if (!(std::fabs(poly) < 31.0)) return false;
-      t = a * t + poly * t;
-      if (!(std::fabs(t) <= 4.0)) return false;
+      next = std::max(next, std::fabs(std::sqrt(q) * (a + poly)));
     }
+    if (!(next <= 4.0)) return false;
+    top = next;
   }
   return true;
 }

@@ -175,15 +175,32 @@ def ptr(t):
 _raw_stream = None
 
 
-def stream():
-    """Handle of torch's current stream on the current device.  (Building the Stream object for it takes 2.5 us, as
-    much as the smallest kernels here, so the handle is asked for by itself where torch offers that: 0.3 us.)"""
+def stream(device=None):
+    """Handle of torch's current stream on the current device, which has to be `device` if one is named.  (Building
+    the Stream object for it takes 2.5 us, as much as the smallest kernels here, so the handle is asked for by itself
+    where torch offers that: 0.3 us.)"""
     global _raw_stream
     import torch
     if _raw_stream is None:
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda device: torch.cuda.current_stream(device).cuda_stream)
-    return _raw_stream(torch.cuda.current_device())
+    current = torch.cuda.current_device()
+    if device is not None and device != current:
+        raise VitkError(f"the tensors are on device {device}, the current one is {current}")
+    return _raw_stream(current)
+
+
+def _stream_for(args, st):
+    """`st`, or the current stream; arguments made from tensors know their device."""
+    current = stream(getattr(args, "device", None))
+    return current if st is None else st
+
+
+def _one_device(*tensors):
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise VitkError(f"tensors on different devices: {sorted(devices)}")
+    return devices.pop()
 
 
 def check(rc):
@@ -328,16 +345,17 @@ def cross_sdpa_args(q, k, v, out, *, key_len=None, scale=None, stats=None, dout=
     if workspace is not None:
         a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
     a.keep = (q, k, v, out, key_len, stats, dout, dq, dk, dv, workspace)
+    a.device = _one_device(*a.keep)
     return a
 
 
 def cross_sdpa_fwd(args, st=None):
     """Softmax attention of args.q over args.k / args.v; see include/vitk.h."""
-    check(dll().vitk_cross_sdpa_fwd(C.byref(args), st if st is not None else stream()))
+    check(dll().vitk_cross_sdpa_fwd(C.byref(args), _stream_for(args, st)))
 
 
 def cross_sdpa_bwd(args, st=None):
-    check(dll().vitk_cross_sdpa_bwd(C.byref(args), st if st is not None else stream()))
+    check(dll().vitk_cross_sdpa_bwd(C.byref(args), _stream_for(args, st)))
 
 
 def _rows_2d(name, t, dtype="float32"):
@@ -351,8 +369,8 @@ def embedding_fwd(table, index, out, *, scale=1.0, st=None):
     V, D = table.shape
     rows = index.numel()
     _need(out.numel() == rows * D, f"out: {rows} rows of {D} are needed")
-    check(dll().vitk_embedding_fwd(ptr(table), V, ptr(index), rows, D, scale, ptr(out),
-                                   st if st is not None else stream()))
+    current = stream(_one_device(table, index, out))
+    check(dll().vitk_embedding_fwd(ptr(table), V, ptr(index), rows, D, scale, ptr(out), current if st is None else st))
 
 
 def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace=None, st=None):
@@ -366,9 +384,10 @@ def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace
         need = dll().vitk_embedding_bwd_workspace_bytes(rows, V, D)
         _need(need == 0 or st is None, "embedding_bwd: another stream than the current one needs a workspace of its own")
         workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=dout.device)
+    current = stream(_one_device(dout, index, dtable, workspace))
     check(dll().vitk_embedding_bwd(ptr(dout), ptr(index), rows, V, D, scale, int(bool(accumulate)), ptr(dtable),
                                    ptr(workspace), workspace.numel() * workspace.element_size(),
-                                   st if st is not None else stream()))
+                                   current if st is None else st))
     return workspace
 
 
@@ -420,15 +439,16 @@ def _with_workspace(a, need, workspace, like, keep):
     if workspace is not None:
         a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
     a.keep = keep + (workspace,)
+    a.device = _one_device(*a.keep)
     return a
 
 
 def newton_schulz(args, st=None):
-    check(dll().vitk_newton_schulz_f32(C.byref(args), st if st is not None else stream()))
+    check(dll().vitk_newton_schulz_f32(C.byref(args), _stream_for(args, st)))
 
 
 def muon(args, st=None):
-    check(dll().vitk_muon_f32(C.byref(args), st if st is not None else stream()))
+    check(dll().vitk_muon_f32(C.byref(args), _stream_for(args, st)))
 
 
 def planning_cu_count(cus):
