@@ -20,13 +20,13 @@
 //
 // Three ways to run the products, by size:
 //   both sides <= 128: the whole iteration in one launch, a workgroup per matrix, planes in LDS;
-//   few tiles: 32 x 32 tiles, the contraction split over the waves of a workgroup, operands straight
-//     from memory (every load of a wave in flight: the time is a few round trips);
+//   few tiles: 32 x 32 tiles (symmetric products: 16 x 16), the contraction split over the waves of a
+//     workgroup, operands straight from memory (every load of a wave in flight: a few round trips);
 //   otherwise: 64 x 64 or 128 x 128 tiles staged through LDS.
 // y y^T and g g are symmetric: only tiles on and below the diagonal are computed, and mirrored.
 // Twelve 768 x 2304 (272 GFLOP): 1050 us, matrix cores: y y^T 66 us, the polynomial 29, the step of y 118, which is 860,
 // 650 and 830 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 31 us, 1000 x 257:
-// 131 us, the latency of 15 dependent products.
+// 96 us, the latency of 15 dependent products.
 #include "common.h"
 
 #include <algorithm>
@@ -510,8 +510,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const
   }
 }
 
-// 32 x 32 tiles, the contraction dealt to NW waves, operands straight from memory: 257 x 1000 takes 10.8 us for
-// y y^T (45 workgroups), 6.2 for the polynomial, 7.6 for the step of y (288), mostly round trips to memory.
+// 32 x 32 tiles, the contraction dealt to NW waves, operands straight from memory: the step of y of 257 x 1000 takes
+// 7.7 us (288 workgroups), mostly round trips to memory.
 template <int MODE, int NW>
 __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int flip) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
@@ -617,6 +617,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
 
 // The symmetric products where 32 x 32 tiles leave CUs without work: 16 x 16 tiles, half as much for each to read.
 // The contraction is dealt to the waves, 32 k a step, a line of planes for 16 rows; the first wave adds the sums.
+// 257 x 1000: y y^T 6.7 us, the polynomial 4.4 (32 x 32 tiles: 10.8 and 6.2).
 template <int MODE, int NW>
 __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int flip) {
   static_assert(MODE <= POLY, "the symmetric products");
