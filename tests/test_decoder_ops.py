@@ -536,6 +536,9 @@ ORTHO = {
     "tiles_64_tall": (700, 190, 9, 3, 1),
     "tiles_128": (300, 900, 9, 5, 0),
     "tiles_128_tall": (1001, 385, 7, 2, 0),
+    "small_tiles_many": (200, 201, 11, 5, 0),
+    "small_tiles_many_long": (777, 801, 1, 3, 0),
+    "small_tiles_16": (513, 514, 1, 4, 2),
 }
 
 
