@@ -127,6 +127,10 @@ ATTENTION = {
     "few_keys_unaligned": (2, 3, 1, 95, 49, 35, [49, 17], 1, 1),
     "one_key_many_rows": (2, 2, 2, 1000, 1, 8, None, 0, 0),
     "few_keys_full_device": (64, 8, 8, 45, 40, 60, None, 4, 0),
+    # single tokens: more than 64 parts, lengths far below the longest, more heads than CUs
+    "token_many_parts": (1, 2, 1, 1, 30011, 72, None, 0, 0),
+    "token_many_parts_ragged": (3, 4, 1, 1, 20000, 40, [20000, 3, 70], 0, 0),
+    "token_heads_over_cus": (70, 8, 8, 1, 130, 20, [130 - b for b in range(70)], 0, 0),
 }
 
 

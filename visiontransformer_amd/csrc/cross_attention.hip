@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_k
   }
 }
 
-constexpr int MAX_SPLITS = 64, JOIN_FEW = 8;
+constexpr int JOIN_FEW = 8, JOIN_WAVES = 16, MAX_SPLITS = 64 * JOIN_WAVES;
 // Joins up to eight parts of split rows: LP lanes per row, four columns each, all parts in flight.
 template <int LP>
 __global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
@@ -275,39 +275,58 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Params p) {
   }
 }
 
-// More than eight parts (few rows): one wave per row, a lane per part for the statistics, then lanes over the
-// columns; every part's statistics arrive in one round trip (49 parts of 256 rows: 4.8 us, in batches of eight 23).
-__global__ __launch_bounds__(256) void cross_join_many_kernel(const Params p) {
+// More than eight parts (few rows): W waves per row, each joins up to 64 parts, a lane per part for the statistics,
+// then lanes over the columns; every part's statistics arrive in one round trip (49 parts of 256 rows: 4.8 us, in
+// batches of eight 23).
+template <int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void cross_join_many_kernel(const Params p) {
+  __shared__ float box[W][130];
   const long long all = (long long)p.B * p.H * p.Nq;
-  const int lane = threadIdx.x & 63;
-  const long long r = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long r = W == 1 ? blockIdx.x * 4ll + wave : blockIdx.x;
   if (r >= all) return;
+  const int per = (p.splits + W - 1) / W, s0 = W == 1 ? 0 : min(wave * per, p.splits), s1 = min(s0 + per, p.splits);
   const float *st = p.part + p.splits * all * p.dh;
   float m = -INFINITY, l = 0.f;
-  if (lane < p.splits) {
-    m = st[(lane * all + r) * 2];
-    l = st[(lane * all + r) * 2 + 1];
+  if (s0 + lane < s1) {
+    m = st[((s0 + lane) * all + r) * 2];
+    l = st[((s0 + lane) * all + r) * 2 + 1];
   }
   float top = vitk::wave_max(m);
+  if constexpr (W > 1) {
+    if (lane == 0) box[wave][0] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, box[w][0]);
+    __syncthreads();
+  }
   if (top == -INFINITY) top = 0.f;  // no key at all
   const float f = __builtin_amdgcn_exp2f(m - top);
   l = vitk::wave_sum(l * f);
   float x0 = 0.f, x1 = 0.f;
   const float *src = p.part + r * p.dh + lane;
-  for (int s = 0; s < p.splits; s += 8) {  // eight parts in flight
+  for (int s = s0; s < s1; s += 8) {  // eight parts in flight
     float a[8], b[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const bool in = s + u < p.splits;
+      const bool in = s + u < s1;
       a[u] = in && lane < p.dh ? src[(s + u) * all * p.dh] : 0.f;
       b[u] = in && lane + 64 < p.dh ? src[(s + u) * all * p.dh + 64] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const float fs = __shfl(f, (s + u) & 63, 64);  // (parts behind the last one: 0 times something finite)
+      const float fs = __shfl(f, (s - s0 + u) & 63, 64);  // (parts behind the last one: 0 times something finite)
       x0 += fs * a[u];
       x1 += fs * b[u];
     }
+  }
+  if constexpr (W > 1) {
+    box[wave][lane] = x0, box[wave][64 + lane] = x1;
+    if (lane == 0) box[wave][128] = l;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) x0 += box[w][lane], x1 += box[w][64 + lane], l += box[w][128];
   }
   const float scale = l == 0.f ? 0.f : 1.f / l;
   const long long bh = r / p.Nq, n = r % p.Nq, b = bh / p.H, h = bh % p.H;
@@ -325,8 +344,8 @@ __global__ __launch_bounds__(256) void cross_join_many_kernel(const Params p) {
 // products, so memory bounds this and the vector ALU computes it.  LP lanes share a key, four columns each;
 // 64 / LP keys per wave and U of those in flight: fewer for more rows, since eight waves a SIMD read faster
 // than more loads in fewer waves (16 x 12345 keys x 4 heads x 128, four rows: 6.0 TB/s with U = 2, 4.9 with
-// 4).  About twelve workgroups a CU also even out ragged lengths.  Each group of LP lanes keeps a running maximum and
-// sum per row of its own; groups, then waves, are joined at the end.
+// 4).  Each batch entry is cut into equal parts, so ragged lengths leave no workgroup without work.  Each group of
+// LP lanes keeps a running maximum and sum per row of its own; groups, then waves, are joined at the end.
 template <int LP>
 __device__ __forceinline__ float group_sum(float x) {  // over LP neighbouring lanes, in all of them
   auto add = [&](auto ctrl) {
@@ -360,7 +379,8 @@ __global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
   wg /= p.Hkv;
   const int b = (int)(wg % p.B), split = (int)(wg / p.B);
   const int len = valid_keys(p, b);
-  const int k0 = min((long long)split * p.chunk, (long long)len), k1 = min((long long)k0 + p.chunk, (long long)len);
+  const int chunk = (len / p.splits + 16) / 16 * 16;  // each batch entry in equal parts
+  const int k0 = min((long long)split * chunk, (long long)len), k1 = min((long long)k0 + chunk, (long long)len);
   f32x4 q[R], o[R];
   float m[R], l[R];
 #pragma unroll
@@ -466,13 +486,15 @@ FwdPlan plan_fwd(Params *p) {
   if (p->rows <= FEW_ROWS) {
     p->blocks = 1;
     f.block.waves = 4;
-    const long long cus = vitk::cu_count();
-    if (heads < 2 * cus) {
-      if (p->Nk <= 1024)
-        f.block.waves = 16;  // one launch: a split's join costs more than it saves
-      else if (heads > 0)
-        splits = std::min((12 * cus + heads - 1) / heads, stages / 4);
-    }
+    // One round of the workgroups that fit the device by their registers, 64 keys or more each (16 x 12345 keys x 4
+    // heads x 128, four rows: 135 us with 6 a CU, 168 with 8; one row 123, without regard to a round 147; 2 x 100000
+    // keys x 2 heads 70, in at most 64 parts 209; one batch entry of 4000 keys x 8 heads x 64: 15 us in parts of 64
+    // keys, 20 in parts of 256).
+    const long long cus = vitk::cu_count(), places = cus * (p->rows <= 2 ? 7 : p->rows <= 4 ? 6 : 4);
+    if (heads < 2 * cus && p->Nk <= 1024)
+      f.block.waves = 16;  // one launch: a split's join costs more than it saves
+    else if (heads > 0)
+      splits = std::min(places / heads, stages);
   } else {
     f.block = plan_block(p->rows, p->Nk, heads, true, 256, 0);
     const int groups = f.block.groups;
@@ -487,6 +509,10 @@ FwdPlan plan_fwd(Params *p) {
   }
   if (splits > MAX_SPLITS) splits = MAX_SPLITS;
   if (splits < 1) splits = 1;
+  if (f.block.groups == 0) {
+    p->splits = (int)splits;  // each batch entry in that many equal parts
+    return f;
+  }
   p->chunk = (int)((stages + splits - 1) / splits) * CHUNK;
   if (p->chunk == 0) p->chunk = CHUNK;
   p->splits = (int)(((long long)p->Nk + p->chunk - 1) / p->chunk);
@@ -576,8 +602,10 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
     const int lp = p.splits > JOIN_FEW ? 64 : p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32;
     const long long blocks = ((long long)p.B * p.H * p.Nq * lp + 255) / 256;
     VITK_REQUIRE(blocks < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
-    if (lp == 64)
-      hipLaunchKernelGGL(cross_join_many_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    if (p.splits > 64)
+      hipLaunchKernelGGL(cross_join_many_kernel<JOIN_WAVES>, dim3((unsigned)(p.B * p.H * p.Nq)), dim3(64 * JOIN_WAVES), 0, st, p);
+    else if (lp == 64)
+      hipLaunchKernelGGL(cross_join_many_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     else if (lp == 8)
       hipLaunchKernelGGL(cross_join_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     else if (lp == 16)
