@@ -2,6 +2,8 @@
 #pragma once
 #include "common.h"
 
+#include <algorithm>
+
 namespace vitk {
 namespace cross {
 
@@ -298,7 +300,8 @@ struct Stage {
 // waves -> four: 64 x 64, 2048 heads: 40 -> 33 us; 50 x 900, 24 heads: 18 -> 23).  More than 64 rows are cut into
 // blocks of 64 where the last block of 128 were half empty and that is a sixth of the rows or more (147 x 197, 320
 // heads: forward 42 -> 33, row gradient 19 less), up to `half` on the other side, and up to `any` on the other
-// side always (row gradient of 512 x 128, 192 heads: 5 less; 512 x 197: 2 more).
+// side always (row gradient of 512 x 128, 192 heads: 5 less; 512 x 197: 2 more; key gradients of 16 rows x 1000, 128
+// heads of 96: 7 less).
 struct Block {
   int groups, waves;
 };
@@ -312,12 +315,15 @@ inline Block plan_block(long long own, long long other, long long heads, bool sm
 }
 // Over how many workgroups the other side of a block is split: the least of whole rounds over the device's
 // places for workgroups (a last round that is hardly filled costs as much as a full one) plus writing and
-// adding the parts.  `us`: time of a whole block; `part_us`: of one part of the results.
-inline int plan_splits(long long wgs, long long places, long long stages, double us, double part_us) {
+// adding the parts.  `us`: time of a whole block by its products; `stage_us`: of the loads, products and barriers of 64
+// on the other side, one after the other; `part_us`: of one part of the results.  (10 x 814 x 64, 42 heads: forward
+// 25 us in three parts, 13 in thirteen.)
+inline int plan_splits(long long wgs, long long places, long long stages, double us, double stage_us, double part_us) {
   int best = 1;
   double least = 0;
-  for (int s = 1; s <= 16 && (s == 1 || s * 4 <= stages); ++s) {
-    const double t = (double)((wgs * s + places - 1) / places) / s * us + (s > 1 ? 5.0 + s * part_us : 0.0);
+  for (int s = 1; s <= 16 && (s == 1 || s <= stages); ++s) {
+    const double block = std::max(us / s, (double)((stages + s - 1) / s) * stage_us);
+    const double t = (double)((wgs * s + places - 1) / places) * block + (s > 1 ? 5.0 + s * part_us : 0.0);
     if (s == 1 || t < least) best = s, least = t;
   }
   return best;

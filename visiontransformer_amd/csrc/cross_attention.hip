@@ -8,7 +8,7 @@
 //
 // Bounds: the matrix cores where keys are many (1021 x 4099 x 64, 48 heads: 200 - 220 us for 38.6 GFLOP, six bf16
 // products each, 1050 - 1160 TFLOP/s of them; 512 x 1536 x 96, 128 heads: 230 us, 1010), the loads and splits of
-// a stage where they are few (48 x 197 x 64, 768 heads: 29.4 us), memory for up to eight rows.
+// a stage where they are few (48 x 197 x 64, 768 heads: 29.4 us), memory for a few rows.
 #include "cross_attention.h"
 
 #include <algorithm>
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void cross_join_many_kernel(
 }
 
 // ------------------------------------------------------------------------------------- few rows
-// At most 8 rows per key head (single tokens): every key and value is read once and used for at most 8 dot
+// At most 4 rows per key head, 8 of wide heads (single tokens): every key and value is read once and used for at most 8 dot
 // products, so memory bounds this and the vector ALU computes it.  LP lanes share a key, four columns each;
 // 64 / LP keys per wave and U of those in flight: fewer for more rows, since eight waves a SIMD read faster
 // than more loads in fewer waves (16 x 12345 keys x 4 heads x 128, four rows: 6.0 TB/s with U = 2, 4.9 with
@@ -475,7 +475,9 @@ __global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
 
 // The kernel, the rows of a workgroup, and over how many workgroups the keys of a block are split.
 constexpr int CHUNK = 64;      // key ranges of splits are multiples of this
-constexpr int FEW_ROWS = 8;    // rows per key head up to which the vector kernel runs
+// Rows per key head up to which the vector kernel runs (eight rows, 320 heads x 1000 keys: of 64 columns 53 us, the
+// matrix kernel 38; of 128 columns 100 and 133).
+constexpr int few_rows(int dh) { return dh <= 96 ? 4 : 8; }
 struct FwdPlan {
   Block block;  // no groups = the vector kernel
 };
@@ -483,7 +485,7 @@ FwdPlan plan_fwd(Params *p) {
   FwdPlan f = {};
   const long long heads = (long long)p->B * p->Hkv, stages = ((long long)p->Nk + CHUNK - 1) / CHUNK;
   long long splits = 1;
-  if (p->rows <= FEW_ROWS) {
+  if (p->rows <= few_rows(p->dh)) {
     p->blocks = 1;
     f.block.waves = 4;
     // One round of the workgroups that fit the device by their registers, 64 keys or more each (16 x 12345 keys x 4
@@ -491,12 +493,17 @@ FwdPlan plan_fwd(Params *p) {
     // keys x 2 heads 70, in at most 64 parts 209; one batch entry of 4000 keys x 8 heads x 64: 15 us in parts of 64
     // keys, 20 in parts of 256).
     const long long cus = vitk::cu_count(), places = cus * (p->rows <= 2 ? 7 : p->rows <= 4 ? 6 : 4);
-    if (heads < 2 * cus && p->Nk <= 1024)
-      f.block.waves = 16;  // one launch: a split's join costs more than it saves
+    const int few = p->rows == 1 ? 448 : p->rows <= 4 ? 320 : 192;  // keys
+    if (p->Nk <= few && heads <= (p->rows == 1 ? 2 * cus : cus))
+      f.block.waves = 16;  // one launch (515 keys, 40 heads of 80, one row: 18 us, in parts 15; 260 keys: 7 and 9)
     else if (heads > 0)
       splits = std::min(places / heads, stages);
   } else {
+    // A workgroup of 64 rows with one buffer is worth its empty waves even for 9 to 32 rows: more of them are on a
+    // CU (16 x 1000, 320 heads of 64: 49 -> 38 us, of 128: 220 -> 133; of 32 no difference).
     f.block = plan_block(p->rows, p->Nk, heads, true, 256, 0);
+    const long long cus = vitk::cu_count();
+    if (p->rows <= 32 && p->dh > 32 && 4 * heads >= cus && heads * stages >= cus) f.block = {4, 4};
     const int groups = f.block.groups;
     p->blocks = (int)(((long long)p->rows + 16 * groups - 1) / (16 * groups));
     const int wide = p->dh <= 32 ? 32 : p->dh <= 64 ? 64 : p->dh <= 96 ? 96 : 128;
@@ -505,7 +512,7 @@ FwdPlan plan_fwd(Params *p) {
     const double flop = 64.0 * groups * p->Nk * wide;                 // of a block; 0.6 TFLOP/s a CU
     const double part = 2.0 * p->B * p->H * p->Nq * p->dh * 4 / 4e6;  // written and read at 4 TB/s
     splits = vitk::cross::plan_splits(heads * p->blocks, resident * (long long)vitk::cu_count(), stages,
-                                      flop / (0.6e6 / resident), part);
+                                      flop / (0.6e6 / resident), 3.0 * wide / 64, part);
   }
   if (splits > MAX_SPLITS) splits = MAX_SPLITS;
   if (splits < 1) splits = 1;
@@ -529,7 +536,7 @@ void launch_rows(const Params &p, unsigned wgs, hipStream_t st) {
     hipLaunchKernelGGL((cross_row_kernel<LP, 2, NW>), grid, block, 0, st, p);
   else if (p.rows <= 4)
     hipLaunchKernelGGL((cross_row_kernel<LP, 4, NW>), grid, block, 0, st, p);
-  else
+  else if constexpr (LP == 32)  // (narrower heads are not here with more)
     hipLaunchKernelGGL((cross_row_kernel<LP, 8, NW>), grid, block, 0, st, p);
 }
 template <int LP>

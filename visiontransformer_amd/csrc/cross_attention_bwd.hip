@@ -430,7 +430,7 @@ struct Side {
 };
 Side plan_side(long long own, long long other, long long heads, int dh, bool keys, double part_us) {
   Side s;
-  s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 256, keys ? 0 : 128);
+  s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 256, keys ? 64 : 128);
   const int groups = s.block.groups;
   s.blocks = (int)((own + 16 * groups - 1) / (16 * groups));
   const long long stages = (other + 63) / 64;
@@ -439,7 +439,7 @@ Side plan_side(long long own, long long other, long long heads, int dh, bool key
   const int resident = groups == 4 && s.block.waves == 4 ? four : groups == 2 ? 2 : 1;  // workgroups a CU
   const double flop = 32.0 * (keys ? 4 : 3) * groups * other * wide;  // of a block; 0.5 TFLOP/s a CU
   const int splits = plan_splits(heads * s.blocks, resident * (long long)vitk::cu_count(), stages,
-                                 flop / (0.5e6 / resident), part_us);
+                                 flop / (0.5e6 / resident), 3.0 * wide / 64, part_us);
   s.chunk = std::max((int)((stages + splits - 1) / splits) * 64, 64);
   s.splits = std::max((int)((other + s.chunk - 1) / s.chunk), 1);
   return s;
@@ -498,7 +498,7 @@ void launch_dkv(const Params &p, Block block, unsigned wgs, hipStream_t st) {
       return;
     }
   }
-  if constexpr (DH == 96) {
+  if constexpr (DH <= 96) {
     if (block.groups == 4) {
       hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 4>), dim3(wgs), dim3(256), 0, st, p);
       return;

@@ -391,7 +391,7 @@ __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__re
     any |= mine[u];
   }
   if (lane == 0) found[wave] = any != 0;
-  for (long long c0 = 0; c0 < D; c0 += 64 * W) {
+  for (long long c0 = blockIdx.y * 64ll * W; c0 < D; c0 += gridDim.y * 64ll * W) {
     const long long col = c0 + lane * W;
     Cols<W> acc = {};
 #pragma unroll
@@ -536,12 +536,15 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
   if (rows == 0) return accumulate ? 0 : vitk_fill_f32(dtable, 0.f, V * D, stream);
   const bool vec = D % 4 == 0 && vitk::aligned16(dout) && vitk::aligned16(dtable);
   if (direct(rows, V)) {
+    // few table rows: a workgroup for each block of their columns (756 tokens x 1024 over 51 rows: 14 -> 6 us)
+    const int width = vec ? 256 : 64;
+    const dim3 grid((unsigned)V, V < 1024 ? (unsigned)((D + width - 1) / width) : 1);
     if (vec)
-      hipLaunchKernelGGL(embedding_direct_kernel<4>, dim3((unsigned)V), dim3(TPB), 0, st, dout, index, (int)rows,
-                         (long long)D, scale, (int)accumulate, dtable);
+      hipLaunchKernelGGL(embedding_direct_kernel<4>, grid, dim3(TPB), 0, st, dout, index, (int)rows, (long long)D, scale,
+                         (int)accumulate, dtable);
     else
-      hipLaunchKernelGGL(embedding_direct_kernel<1>, dim3((unsigned)V), dim3(TPB), 0, st, dout, index, (int)rows,
-                         (long long)D, scale, (int)accumulate, dtable);
+      hipLaunchKernelGGL(embedding_direct_kernel<1>, grid, dim3(TPB), 0, st, dout, index, (int)rows, (long long)D, scale,
+                         (int)accumulate, dtable);
     return vitk::check_launch("vitk_embedding_bwd");
   }
   const Plan p = make_plan(rows, V, D);
