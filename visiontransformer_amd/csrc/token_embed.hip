@@ -536,9 +536,11 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
   if (rows == 0) return accumulate ? 0 : vitk_fill_f32(dtable, 0.f, V * D, stream);
   const bool vec = D % 4 == 0 && vitk::aligned16(dout) && vitk::aligned16(dtable);
   if (direct(rows, V)) {
-    // few table rows: a workgroup for each block of their columns (756 tokens x 1024 over 51 rows: 14 -> 6 us)
+    // few table rows: a workgroup for each block of their columns (756 tokens x 1024 over 51 rows: 14 -> 6 us, 1000
+    // over 2000 rows 10 -> 8, over 4000 11 -> 14)
     const int width = vec ? 256 : 64;
-    const dim3 grid((unsigned)V, V < 1024 ? (unsigned)((D + width - 1) / width) : 1);
+    const long long blocks = (D + width - 1) / width;
+    const dim3 grid((unsigned)V, V * blocks <= 8192 ? (unsigned)blocks : 1);
     if (vec)
       hipLaunchKernelGGL(embedding_direct_kernel<4>, grid, dim3(TPB), 0, st, dout, index, (int)rows, (long long)D, scale,
                          (int)accumulate, dtable);
