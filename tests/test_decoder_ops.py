@@ -545,6 +545,8 @@ ORTHO = {
     "small_tiles_many": (200, 201, 11, 5, 0),
     "small_tiles_many_long": (777, 801, 1, 3, 0),
     "small_tiles_16": (513, 514, 1, 4, 2),
+    "small_tiles_batch": (190, 192, 5, 5, 0),
+    "small_tiles_tall_batch": (300, 130, 6, 5, 1),
 }
 
 

@@ -8,7 +8,7 @@
 // the products are fp32 in three bf16 parts, arranged as in the forward: the accumulator of the first
 // product is the operand of the next.  That is seven products where five would do (s and dp are formed
 // twice); one pass would have to add dQ (or dK and dV) up across workgroups.
-// Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves share a group and deal the tiles of the
+// Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves may share a group and deal the tiles of the
 // other side.  Where the blocks are too few for the device, the other side is split over workgroups and
 // the parts are added in order by a second launch.
 // Bound by the matrix cores (512 x 1536 x 96, 128 heads of which 4 share a key head: dQ 330 us, dK and dV 461, 1054
@@ -151,7 +151,7 @@ void cross_dq_kernel(const Params p) {
 }
 
 template <int DH, int NW, int KG>
-__global__ __launch_bounds__(64 * NW, NW == 8 || KG == 4 ? 2 : 1)
+__global__ __launch_bounds__(64 * NW, 2)
 void cross_dkv_kernel(const Params p) {
   typedef Shape<DH, NW, KG> S;
   constexpr int JOIN = S::OTHER > 1 ? KG * 64 * (DH / 2) * 4 : 0;
@@ -431,6 +431,9 @@ struct Side {
 Side plan_side(long long own, long long other, long long heads, int dh, bool keys, double part_us) {
   Side s;
   s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 256, keys ? 64 : 128);
+  // Up to 32 keys, or rows of wide heads: eight waves, half of which only load (668 x 14 x 128, 24 key heads: 109 -> 88 us,
+  // 98 x 24 x 80, 128: 49 -> 41; rows: 10 x 814 x 128, 42 heads: 94 -> 74; of 80 columns no difference).
+  if (own <= 32 && (keys || dh > 96)) s.block = {4, 8};
   const int groups = s.block.groups;
   s.blocks = (int)((own + 16 * groups - 1) / (16 * groups));
   const long long stages = (other + 63) / 64;
@@ -481,18 +484,14 @@ void launch_dq(const Params &p, Block block, unsigned wgs, hipStream_t st) {
   }
   if (block.groups == 8)
     hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 8>), dim3(wgs), dim3(512), 0, st, p);
-  else if (block.groups == 4)
+  else if (DH > 96 || block.groups == 4)
     hipLaunchKernelGGL((cross_dq_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
-  else
+  else if constexpr (DH <= 96)
     hipLaunchKernelGGL((cross_dq_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
 }
 template <int DH>
 void launch_dkv(const Params &p, Block block, unsigned wgs, hipStream_t st) {
   if constexpr (DH > 64) {  // others are not here with so few keys
-    if (block.groups == 2) {
-      hipLaunchKernelGGL((cross_dkv_kernel<DH, 4, 2>), dim3(wgs), dim3(256), 0, st, p);
-      return;
-    }
     if (block.groups == 4 && block.waves == 8) {
       hipLaunchKernelGGL((cross_dkv_kernel<DH, 8, 4>), dim3(wgs), dim3(512), 0, st, p);
       return;

@@ -615,7 +615,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   }
 }
 
-// The symmetric products where 32 x 32 tiles leave CUs without work: 16 x 16 tiles, half as much for each to read.
+// The symmetric products where 32 x 32 tiles leave half of the CUs without work: 16 x 16 tiles, half as much for each to read.
 // The contraction is dealt to the waves, 32 k a step, a line of planes for 16 rows; the first wave adds the sums.
 // 257 x 1000: y y^T 6.7 us, the polynomial 4.4 (32 x 32 tiles: 10.8 and 6.2).
 template <int MODE, int NW>
@@ -923,12 +923,14 @@ void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
   const long long total = p.batch * (MODE <= POLY ? ti * (ti + 1) / 2 : ti * tj);
   const dim3 grid((unsigned)((total + 7) / 8 * 8));
   if constexpr (MODE <= POLY) {
-    if (form == FORM_SMALL && total < vitk::cu_count()) {
+    // (1000 x 257, 45 tiles of 32: 129 -> 98 us; five of 192 x 192, 105: 98 -> 90; eight of 172 x 214, 168: 114 -> 125)
+    if (form == FORM_SMALL && 2 * total <= vitk::cu_count()) {
       const unsigned wgs = (unsigned)(p.batch * ti * (2 * ti + 1));  // twice the tiles a side
-      if ((MODE == GRAM ? p.n : p.r) > 512)
-        hipLaunchKernelGGL((ns_lower_kernel<MODE, 8>), dim3(wgs), dim3(512), 0, st, p, flip);
-      else
+      if (MODE == GRAM && p.n > 512) {
+        if constexpr (MODE == GRAM) hipLaunchKernelGGL((ns_lower_kernel<MODE, 8>), dim3(wgs), dim3(512), 0, st, p, flip);
+      } else {
         hipLaunchKernelGGL((ns_lower_kernel<MODE, 4>), dim3(wgs), dim3(256), 0, st, p, flip);
+      }
       return;
     }
   }
