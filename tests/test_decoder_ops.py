@@ -546,6 +546,8 @@ ORTHO = {
     "small_tiles_many_long": (777, 801, 1, 3, 0),
     "small_tiles_16": (513, 514, 1, 4, 2),
     "small_tiles_batch": (190, 192, 5, 5, 0),
+    "thin_long": (100, 3300, 2, 5, 0),
+    "thin_tall_padded": (3301, 70, 2, 3, 3),
     "small_tiles_tall_batch": (300, 130, 6, 5, 1),
 }
 

@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const
 // 32 x 32 tiles, the contraction dealt to NW waves, operands straight from memory: the step of y of 257 x 1000 takes
 // 7.7 us (288 workgroups), mostly round trips to memory.
 template <int MODE, int NW>
-__global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int flip) {
+__global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int flip, int ti) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
   constexpr int U = TR ? 4 : 8;       // steps of 16 k in flight
   constexpr int PITCH = 80;           // fp16 pitch of a row of transposed operand (64 + a shift of 32 bytes)
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   static_assert(REGION >= 32 * SUM_PITCH * 4, "the wave's sums go where its operand was");
   __shared__ __attribute__((aligned(16))) char lds[NW][REGION];
   const int cols = TR ? p.np : p.rp, depth = MODE == GRAM ? p.np : p.rp;
-  const int ti = (p.r + 31) / 32, tj = TR ? (p.n + 31) / 32 : ti, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
+  const int tj = TR ? (p.n + 31) / 32 : ti, tiles = LOWER ? ti * (ti + 1) / 2 : ti * tj;
   const long long k = blockIdx.x / tiles;
   int bi, bj;
   tile_of<LOWER>(blockIdx.x % tiles, ti, bi, bj);
@@ -619,11 +619,11 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
 // The contraction is dealt to the waves, 32 k a step, a line of planes for 16 rows; the first wave adds the sums.
 // 257 x 1000: y y^T 6.7 us, the polynomial 4.4 (32 x 32 tiles: 10.8 and 6.2).
 template <int MODE, int NW>
-__global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int flip) {
+__global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int flip, int ti) {
   static_assert(MODE <= POLY, "the symmetric products");
   constexpr int U = 4, PITCH = 20;  // steps in flight
   __shared__ __attribute__((aligned(16))) float lds[NW][16 * PITCH];
-  const int depth = MODE == GRAM ? p.np : p.rp, ti = (p.r + 31) / 32 * 2, tiles = ti * (ti + 1) / 2;
+  const int depth = MODE == GRAM ? p.np : p.rp, tiles = ti * (ti + 1) / 2;
   const long long k = blockIdx.x / tiles;
   int bi, bj;
   tile_of<true>(blockIdx.x % tiles, ti, bi, bj);
@@ -919,29 +919,36 @@ bool bounded(double a, double b, double c, int steps) {
 template <int MODE>
 void launch_product(const NsParams &p, int form, int flip, hipStream_t st) {
   const int t = form == FORM_128 ? 128 : form == FORM_64 ? 64 : 32;
-  const long long ti = (p.r + t - 1) / t, tj = (p.n + t - 1) / t;
-  const long long total = p.batch * (MODE <= POLY ? ti * (ti + 1) / 2 : ti * tj);
-  const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  // what the next product reads: whole tiles of its own
+  int ti = form == FORM_SMALL ? (p.r + 31) / 32 : p.rp / t;
+  const long long tj = (p.n + t - 1) / t, cus = vitk::cu_count();
+  long long total = p.batch * (MODE <= POLY ? (long long)ti * (ti + 1) / 2 : ti * tj);
   if constexpr (MODE <= POLY) {
+    // (two of 100 x 6500, 6 tiles: 317 -> 199 us; three of 128 x 3000, 9 tiles: 197 -> 131; nine of 70 x 2225, 27: 184 -> 204)
+    if (form != FORM_SMALL && 16 * total <= cus) {
+      form = FORM_SMALL;
+      ti = p.rp / 32;
+      total = p.batch * (long long)ti * (ti + 1) / 2;
+    }
     // (1000 x 257, 45 tiles of 32: 129 -> 98 us; five of 192 x 192, 105: 98 -> 90; eight of 172 x 214, 168: 114 -> 125)
-    if (form == FORM_SMALL && 2 * total <= vitk::cu_count()) {
+    if (form == FORM_SMALL && 2 * total <= cus) {
       const unsigned wgs = (unsigned)(p.batch * ti * (2 * ti + 1));  // twice the tiles a side
-      if (MODE == GRAM && p.n > 512) {
-        if constexpr (MODE == GRAM) hipLaunchKernelGGL((ns_lower_kernel<MODE, 8>), dim3(wgs), dim3(512), 0, st, p, flip);
-      } else {
-        hipLaunchKernelGGL((ns_lower_kernel<MODE, 4>), dim3(wgs), dim3(256), 0, st, p, flip);
-      }
+      if (MODE == GRAM && p.n > 512)
+        hipLaunchKernelGGL((ns_lower_kernel<GRAM, 8>), dim3(wgs), dim3(512), 0, st, p, flip, 2 * ti);
+      else
+        hipLaunchKernelGGL((ns_lower_kernel<MODE, 4>), dim3(wgs), dim3(256), 0, st, p, flip, 2 * ti);
       return;
     }
   }
+  const dim3 grid((unsigned)((total + 7) / 8 * 8));
   if (form == FORM_128)
     hipLaunchKernelGGL((ns_tile_kernel<MODE, 128, 8>), grid, dim3(512), 0, st, p, flip, (int)total);
   else if (form == FORM_64)
     hipLaunchKernelGGL((ns_tile_kernel<MODE, 64, 4>), grid, dim3(256), 0, st, p, flip, (int)total);
   else if ((MODE == GRAM ? p.n : p.r) > (MODE >= APPLY ? 256 : 512))  // more than one batch of loads a wave with four
-    hipLaunchKernelGGL((ns_small_kernel<MODE, 8>), dim3((unsigned)total), dim3(512), 0, st, p, flip);
+    hipLaunchKernelGGL((ns_small_kernel<MODE, 8>), dim3((unsigned)total), dim3(512), 0, st, p, flip, ti);
   else
-    hipLaunchKernelGGL((ns_small_kernel<MODE, 4>), dim3((unsigned)total), dim3(256), 0, st, p, flip);
+    hipLaunchKernelGGL((ns_small_kernel<MODE, 4>), dim3((unsigned)total), dim3(256), 0, st, p, flip, ti);
 }
 
 std::atomic<unsigned long long> g_one_lds{0};
