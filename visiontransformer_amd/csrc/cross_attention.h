@@ -229,16 +229,40 @@ __device__ __forceinline__ void load_eight(const float *row, int d, const Params
   for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
 }
 
-// this lane's row (columns 32 i + 8 g ..) times `scale`, split
+// this lane's part of a row (columns 32 i + 8 g ..), which has to be there; every load in flight at once (a branch
+// around each, as for columns behind dh, would wait for one after the other)
 template <int DH>
-__device__ __forceinline__ void load_row(Split8 (&f)[DH / 32], const float *row, bool ok, int g, float scale, const Params &p) {
+__device__ __forceinline__ void load_raw(float (&x)[DH / 32][8], const float *row, int g, const Params &p) {
+  if (p.vec) {
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 32 * i + 8 * g + 4 * h;
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(row + (d < p.dh ? d : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][4 * h + e] = v[e];
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = row[min(32 * i + 8 * g + e, p.dh - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (32 * i + 8 * g + e >= p.dh) x[i][e] = 0.f;
+}
+// that times `scale`, split; zeros for a row that is not there
+template <int DH>
+__device__ __forceinline__ void split_row(Split8 (&f)[DH / 32], float (&x)[DH / 32][8], bool ok, float scale) {
 #pragma unroll
   for (int i = 0; i < DH / 32; ++i) {
-    float x[8] = {};
-    if (ok) load_eight(row, 32 * i + 8 * g, p, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= scale;
-    f[i] = split8(x);
+    for (int e = 0; e < 8; ++e) x[i][e] = ok ? x[i][e] * scale : 0.f;
+    f[i] = split8(x[i]);
   }
 }
 // column c of acc^T to a row

@@ -117,7 +117,8 @@ __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_k
   const bool row_ok = row < p.rows;
 
   Split8 q[DH / 32];  // times scale log2(e)
-  load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, row_ok ? row : 0), row_ok, g, p.c, p);
+  float raw[DH / 32][8];
+  load_raw<DH>(raw, p.q.ptr + row_offset(p, p.q.ld, b, hk, row_ok ? row : 0), g, p);
   f32x4 o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = zero4();
@@ -130,6 +131,7 @@ __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_k
   };
   const bool early = wave < NW / 2, empty = (rb * RW + rg) * 16 >= p.rows;
   next.fetch(p, k0, k1, at);
+  split_row<DH>(q, raw, row_ok, p.c);
   if constexpr (S::BUFFERS == 2) {
     next.put(buffers);
     next.fetch(p, k0 + S::STAGE, k1, at);

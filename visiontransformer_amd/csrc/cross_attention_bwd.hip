@@ -71,22 +71,16 @@ void cross_dq_kernel(const Params p) {
       const float l = p.stats[2 * st + 1];
       f = l == 0.f ? 0.f : 1.f / l;
     }
-    load_row<DH>(q, p.q.ptr + row_offset(p, p.q.ld, b, hk, r), row_ok, g, p.c, p);
-    const float *gp = p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r), *op = p.o.ptr + row_offset(p, p.o.ld, b, hk, r);
+    float x[DH / 32][8], y[DH / 32][8], z[DH / 32][8];
+    load_raw<DH>(x, p.q.ptr + row_offset(p, p.q.ld, b, hk, r), g, p);
+    load_raw<DH>(y, p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r), g, p);
+    load_raw<DH>(z, p.o.ptr + row_offset(p, p.o.ld, b, hk, r), g, p);
+    split_row<DH>(q, x, row_ok, p.c);
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) {
-      float x[8] = {}, y[8] = {};
-      if (row_ok) {
-        load_eight(gp, 32 * i + 8 * g, p, x);
-        load_eight(op, 32 * i + 8 * g, p, y);
-      }
+    for (int i = 0; i < DH / 32; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        delta += x[e] * y[e];
-        x[e] *= f;
-      }
-      dout[i] = split8(x);
-    }
+      for (int e = 0; e < 8; ++e) delta += row_ok ? y[i][e] * z[i][e] : 0.f;
+    split_row<DH>(dout, y, row_ok, f);
     delta = column_sum(delta) * f;
     if (row_ok && g == 0 && kg == 0 && split == 0) p.delta[st] = delta;
   }
@@ -169,8 +163,13 @@ void cross_dkv_kernel(const Params p) {
   const int len = valid_keys(p, b), key = (kb * KG + kg) * 16 + c;
   const bool key_ok = key < len;
   Split8 k[DH / 32], v[DH / 32];
-  load_row<DH>(k, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p.c, p);
-  load_row<DH>(v, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, 1.f, p);
+  if (kb * KG * 16 < len) {
+    float x[DH / 32][8], y[DH / 32][8];
+    load_raw<DH>(x, p.k.ptr + key_offset(p, p.k.ld, b, hk, key_ok ? key : 0), g, p);
+    load_raw<DH>(y, p.v.ptr + key_offset(p, p.v.ld, b, hk, key_ok ? key : 0), g, p);
+    split_row<DH>(k, x, key_ok, p.c);
+    split_row<DH>(v, y, key_ok, 1.f);
+  }
   f32x4 dk[DH / 16], dv[DH / 16];
 #pragma unroll
   for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
@@ -292,8 +291,15 @@ __global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(co
   const int len = valid_keys(p, b), key = wave * 16 + c;
   const bool key_ok = key < len, empty = wave * 16 >= len;
   Split8 k[DH / 32], v[DH / 32];
-  load_row<DH>(k, p.k.ptr + key_offset(p, p.k.ld, b, hk, key), key_ok, g, p.c, p);
-  load_row<DH>(v, p.v.ptr + key_offset(p, p.v.ld, b, hk, key), key_ok, g, 1.f, p);
+  {
+    float x[DH / 32][8] = {}, y[DH / 32][8] = {};
+    if (len > 0) {
+      load_raw<DH>(x, p.k.ptr + key_offset(p, p.k.ld, b, hk, key_ok ? key : 0), g, p);
+      load_raw<DH>(y, p.v.ptr + key_offset(p, p.v.ld, b, hk, key_ok ? key : 0), g, p);
+    }
+    split_row<DH>(k, x, key_ok, p.c);
+    split_row<DH>(v, y, key_ok, 1.f);
+  }
   f32x4 dk[DH / 16], dv[DH / 16];
 #pragma unroll
   for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
