@@ -244,6 +244,32 @@ def test_cross_attention_splits_where_blocks_are_few(K):
 
 
 @gpu
+@pytest.mark.parametrize("cus", [8, 64, 1024])
+def test_cross_attention_on_the_routes_of_other_devices(K, cus):
+    """Kernels, blocks and splits follow the number of CUs; every one of them is right for every size."""
+    shapes = ((2, 4, 2, 1, 500, 64), (3, 8, 8, 1, 2000, 128), (2, 8, 4, 3, 700, 80), (4, 4, 4, 20, 300, 64),
+              (4, 8, 8, 40, 100, 64), (2, 4, 2, 70, 330, 96), (1, 2, 2, 300, 500, 128), (5, 6, 6, 147, 50, 32),
+              (1, 1, 1, 9, 2000, 33))
+    K.planning_cu_count(cus)
+    try:
+        for B, H, Hkv, Nq, Nk, dh in shapes:
+            g = rng(Nq + Nk + dh)
+            q, dout = randn(g, B, Nq, H, dh), randn(g, B, Nq, H, dh)
+            k, v = randn(g, B, Nk, Hkv, dh), randn(g, B, Nk, Hkv, dh)
+            lens = [Nk - 13 * b for b in range(B)]
+            want, tol, _ = attention64(q, k, v, lens, dh ** -0.5, dout)
+            out, dq, dk, dv = (torch.full_like(x, 7.0) for x in (q, q, k, v))
+            a = K.cross_sdpa_args(q, k, v, out, key_len=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                  stats=torch.empty(B * H, Nq, 2, device="cuda"), dout=dout, dq=dq, dk=dk, dv=dv)
+            K.cross_sdpa_fwd(a)
+            K.cross_sdpa_bwd(a)
+            for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+                within(t, want[n], tol[n], f"{n} {Nq} x {Nk} x {dh}")
+    finally:
+        K.planning_cu_count(0)
+
+
+@gpu
 def test_cross_attention_leaves_what_is_between_the_rows(K):
     g = rng(5)
     B, H, N, dh = 2, 3, 11, 20
@@ -571,6 +597,23 @@ def test_newton_schulz(K, name):
     inplace = full.clone()
     K.newton_schulz(K.newton_schulz_args(inplace[:, :, :c], inplace[:, :, :c], steps=steps, coefficients=COEF, eps=1e-7))
     assert torch.equal(inplace[:, :, :c], out[:, :, :c])
+
+
+@gpu
+@pytest.mark.parametrize("cus", [8, 64, 1024])
+def test_newton_schulz_on_the_routes_of_other_devices(K, cus):
+    K.planning_cu_count(cus)
+    try:
+        for i, (batch, r, c) in enumerate(((1, 257, 500), (3, 200, 300), (4, 130, 320), (2, 90, 700), (2, 300, 200))):
+            x = randn(rng(900 + i), batch, r, c)
+            out = torch.full_like(x, 7.0)
+            K.newton_schulz(K.newton_schulz_args(x, out, steps=5, coefficients=COEF, eps=1e-7))
+            for b in range(batch):
+                want = newton_schulz(x[b].cpu().numpy(), 5, COEF, 1e-7, np.float64)
+                err = np.linalg.norm(out[b].double().cpu().numpy() - want)
+                assert err <= ns_tolerance(x[b].cpu().numpy(), want, 5, COEF, 1e-7), (batch, r, c, err)
+    finally:
+        K.planning_cu_count(0)
 
 
 @gpu

@@ -315,7 +315,8 @@ def cross_sdpa_args(q, k, v, out, *, key_len=None, scale=None, stats=None, dout=
                     workspace=None):
     """Arguments of cross_sdpa_fwd / cross_sdpa_bwd for q, out [B, Nq, H, dh] and k, v [B, Nk, Hkv, dh] (rows may be
     pitched, e.g. slices of a packed projection); the object keeps its tensors and, unless one is passed, a
-    workspace.  Build it once and call as often as the same buffers are used."""
+    workspace.  Build it once and call as often as the same buffers are used.  Work that was put on another stream
+    than torch's current one needs the object until it has ended, as any tensor there."""
     _need(q.dim() == 4 and k.dim() == 4, "cross_sdpa: q and k have four dimensions [B, N, heads, dh]")
     B, Nq, H, dh = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
