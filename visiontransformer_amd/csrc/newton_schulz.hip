@@ -25,7 +25,7 @@
 //   otherwise: 64 x 64 or 128 x 128 tiles staged through LDS.
 // y y^T and g g are symmetric: only tiles on and below the diagonal are computed, and mirrored.
 // Twelve 768 x 2304 (272 GFLOP): 1050 us, matrix cores: y y^T 66 us, the polynomial 29, the step of y 118, which is 860,
-// 650 and 830 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 31 us, 1000 x 257:
+// 650 and 830 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 26 us, 1000 x 257:
 // 96 us, the latency of 15 dependent products.
 #include "common.h"
 
@@ -682,7 +682,7 @@ __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int
 // Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of
 // y and of g, then b g + c g g, are in LDS (70 KiB each), what a wave adds to its products in registers.  All
 // blocks of g are computed: writing a block's mirror image, two bytes at a time, takes longer than its product.
-// 96 x 96, five steps: 31 us, 2 a product: operands from LDS 0.7, matrix cores 0.7, one after the other.
+// 96 x 96, five steps: 26 us, 1.3 a product: operands from LDS 0.7, matrix cores 0.7, one after the other.
 // A row of planes takes 3 mod 16 units of 16 bytes, so that 16 rows of one unit, and mostly four rows of four
 // neighbouring ones, are on different banks.
 constexpr int ONE_WAVES = 16;
@@ -701,27 +701,47 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
   const bool y_mine = yi < tr, g_mine = gi < tr;
   float y[16];
   double s = 0.0;
-  {  // element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4
-    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
-    const long long si = p.tall ? 1 : p.ld_x, sj = p.tall ? p.ld_x : 1, at = k * p.stride_x + i * si + j * sj;
+  // Element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4.  Every load is issued, its place
+// clamped: a branch around each would wait for one after the other (96 x 96 without a step: 11 us instead of 6).
+  const int row = 32 * yi + c, col = 32 * yj + 4 * g;
+  const bool quads = p.flat && !p.tall && p.cols % 4 == 0;
+  {
+    const long long si = p.tall ? 1 : p.ld_x, sj = p.tall ? p.ld_x : 1;
+    const long long line = k * p.stride_x + min(row, p.r - 1) * si;
+    auto load = [&](const float *x, float (&v)[16]) {
+      if (quads) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int d = 8 * (e / 4) + e % 4;
-      y[e] = i < p.r && j + d < p.n ? p.x[at + d * sj] : 0.f;
-    }
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 w = *reinterpret_cast<const f32x4 *>(x + line + min(col + 8 * q, p.n - 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = w[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = x[line + min(col + 8 * (e / 4) + e % 4, p.n - 1) * sj];
+      }
+    };
+    load(p.x, y);
     if (p.m) {
+      float m[16];
+      load(p.m, m);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int d = 8 * (e / 4) + e % 4;
-        if (i < p.r && j + d < p.n) {
-          const float gs = p.grad_scale * y[e], m = p.momentum * p.m[at + d * sj] + gs;
-          p.m[at + d * sj] = m;
-          y[e] = p.nesterov ? gs + p.momentum * m : m;
-        }
+        const float gs = p.grad_scale * y[e];
+        m[e] = p.momentum * m[e] + gs;
+        y[e] = p.nesterov ? gs + p.momentum * m[e] : m[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = col + 8 * (e / 4) + e % 4;
+        if (row < p.r && j < p.n) p.m[line + j * sj] = m[e];
       }
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s += (double)y[e] * (double)y[e];
+    for (int e = 0; e < 16; ++e) {
+      if (row >= p.r || col + 8 * (e / 4) + e % 4 >= p.n) y[e] = 0.f;
+      s += (double)y[e] * (double)y[e];
+    }
   }
   s = wave_sum(s);
   if (lane == 0) red[wave] = s;
@@ -730,12 +750,9 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
 #pragma unroll
   for (int w = 0; w < ONE_WAVES; ++w) s += red[w];
   const float norm = (float)sqrt(s) + p.eps;
-  {
-    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (i < p.r && j + 8 * (e / 4) + e % 4 < p.n) y[e] /= norm;
-  }
+  for (int e = 0; e < 16; ++e)
+    if (row < p.r && col + 8 * (e / 4) + e % 4 < p.n) y[e] /= norm;
   // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout
   auto store = [&](f16x8 *m, int pitch, int bi, int bj, const float (&x)[16], float scale) {
     const int row = 32 * bi + c;
@@ -834,22 +851,34 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
       __syncthreads();
     }
   }
-  {
-    const int i = 32 * yi + c, j = 32 * yj + 4 * g;
-    const long long si = p.tall ? 1 : p.ld_out, sj = p.tall ? p.ld_out : 1, at = k * p.stride_out + i * si + j * sj;
-    if (p.p) {
+  if (row >= p.r) return;
+  const long long si = p.tall ? 1 : p.ld_out, sj = p.tall ? p.ld_out : 1, line = k * p.stride_out + row * si;
+  if (p.vec && !p.tall && p.cols % 4 == 0) {
+    f32x4 old[4];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = 8 * (e / 4) + e % 4;
-        if (i < p.r && j + d < p.n) p.p[at + d * sj] = p.p[at + d * sj] * p.keep - p.step * y[e];
-      }
-    } else {
+    for (int q = 0; q < 4; ++q)
+      if (p.p) old[q] = *reinterpret_cast<const f32x4 *>(p.p + line + min(col + 8 * q, p.n - 4));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = 8 * (e / 4) + e % 4;
-        if (i < p.r && j + d < p.n) p.out[at + d * sj] = y[e];
-      }
+    for (int q = 0; q < 4; ++q) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = p.p ? old[q][e] * p.keep - p.step * y[4 * q + e] : y[4 * q + e];
+      if (col + 8 * q < p.n) *reinterpret_cast<f32x4 *>((p.p ? p.p : p.out) + line + col + 8 * q) = v;
     }
+    return;
+  }
+  if (p.p) {
+    float old[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) old[e] = p.p[line + min(col + 8 * (e / 4) + e % 4, p.n - 1) * sj];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = old[e] * p.keep - p.step * y[e];
+  }
+  float *to = p.p ? p.p : p.out;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int j = col + 8 * (e / 4) + e % 4;
+    if (j < p.n) to[line + j * sj] = y[e];
   }
 }
 
