@@ -298,17 +298,49 @@ struct Stage {
   __device__ static __forceinline__ bool is_y(int u) { return task(u) >= S::HALF; }
   __device__ static __forceinline__ int row(int u) { return (task(u) - (is_y(u) ? S::HALF : 0)) / (DH / 8); }
   __device__ static __forceinline__ int unit(int u) { return task(u) % (DH / 8); }
-  // at(y, row): the row's first element
+  // at(y, row): the row's first element.  Every load is issued, its place clamped (see load_raw); `clean` before
+  // the values are used.
   template <class At>
   __device__ __forceinline__ void fetch(const Params &p, int first, int end, At at) {
+    if (first >= end) {
 #pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {
-      if (any(u) && first + row(u) < end) {
-        load_eight(at(is_y(u), first + row(u)), unit(u) * 8, p, v[u]);
-      } else {
+      for (int u = 0; u < S::TASKS; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+      return;
+    }
+    if (p.vec) {
+#pragma unroll
+      for (int u = 0; u < S::TASKS; ++u) {
+        const float *from = at(is_y(u), min(first + row(u), end - 1));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = unit(u) * 8 + 4 * h;
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < p.dh ? d : 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][4 * h + e] = x[e];
+        }
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < S::TASKS; ++u) {
+        const float *from = at(is_y(u), min(first + row(u), end - 1));
+        int d = unit(u) * 8;
+        asm volatile("" : "+v"(d));  // (the compiler would keep eight places a task in registers for the whole loop)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[u][e] = from[min(d + e, p.dh - 1)];
+      }
+    }
+  }
+  // what was fetched: zeros for rows behind the end and columns behind dh
+  __device__ __forceinline__ void clean(const Params &p, int first, int end) {
+    if (first + S::STAGE <= end && p.dh == DH) return;
+#pragma unroll
+    for (int u = 0; u < S::TASKS; ++u) {
+      const int columns = first + row(u) < end ? p.dh - unit(u) * 8 : 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= columns) v[u][e] = 0.f;
     }
   }
   __device__ __forceinline__ void put(bf16x8 *buffer) const {

@@ -133,6 +133,7 @@ __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_k
   next.fetch(p, k0, k1, at);
   split_row<DH>(q, raw, row_ok, p.c);
   if constexpr (S::BUFFERS == 2) {
+    next.clean(p, k0, k1);
     next.put(buffers);
     next.fetch(p, k0 + S::STAGE, k1, at);
     __syncthreads();
@@ -140,6 +141,7 @@ __global__ __launch_bounds__(64 * NW, waves_a_simd(DH, NW, RW)) void cross_fwd_k
   for (int t = k0, n = 0; t < k1; t += S::STAGE, n ^= S::BUFFERS - 1) {
     const bf16x8 *kt = buffers + n * 2 * S::UNITS, *vt = kt + S::UNITS;
     auto advance = [&] {
+      next.clean(p, t + (S::BUFFERS - 1) * S::STAGE, k1);
       next.put(buffers + (S::BUFFERS - 1 - n) * 2 * S::UNITS);
       if constexpr (S::BUFFERS == 1) __syncthreads();
       next.fetch(p, t + S::BUFFERS * S::STAGE, k1, at);

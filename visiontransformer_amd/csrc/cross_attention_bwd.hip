@@ -94,6 +94,7 @@ void cross_dq_kernel(const Params p) {
   const bool early = wave < NW / 2, empty = (rb * RW + rg) * 16 >= p.rows;
   next.fetch(p, k0, k1, at);
   if constexpr (S::BUFFERS == 2) {
+    next.clean(p, k0, k1);
     next.put(buffers);
     next.fetch(p, k0 + S::STAGE, k1, at);
     __syncthreads();
@@ -101,6 +102,7 @@ void cross_dq_kernel(const Params p) {
   for (int t = k0, n = 0; t < k1; t += S::STAGE, n ^= S::BUFFERS - 1) {
     const bf16x8 *kt = buffers + n * 2 * S::UNITS, *vt = kt + S::UNITS;
     auto advance = [&] {
+      next.clean(p, t + (S::BUFFERS - 1) * S::STAGE, k1);
       next.put(buffers + (S::BUFFERS - 1 - n) * 2 * S::UNITS);
       if constexpr (S::BUFFERS == 1) __syncthreads();
       next.fetch(p, t + S::BUFFERS * S::STAGE, k1, at);
@@ -194,7 +196,8 @@ void cross_dkv_kernel(const Params p) {
       if (r < r1) sm = -p.stats[2 * row_stat(p, b, hk, r)], sd = -p.delta[row_stat(p, b, hk, r)];
     }
   };
-  auto put = [&](int n) {
+  auto put = [&](int n, int t) {
+    next.clean(p, t, r1);
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {  // dout / l
       const float f = sl[u] == 0.f ? 0.f : 1.f / sl[u];
@@ -207,14 +210,14 @@ void cross_dkv_kernel(const Params p) {
   const bool early = wave < NW / 2, empty = (kb * KG + kg) * 16 >= len;
   fetch(r0);
   if constexpr (S::BUFFERS == 2) {
-    put(0);
+    put(0, r0);
     fetch(r0 + S::STAGE);
     __syncthreads();
   }
   for (int t = r0, n = 0; t < r1; t += S::STAGE, n ^= S::BUFFERS - 1) {
     const bf16x8 *qt = buffers + n * 2 * S::UNITS, *gt = qt + S::UNITS;
     auto advance = [&] {
-      put(S::BUFFERS - 1 - n);
+      put(S::BUFFERS - 1 - n, t + (S::BUFFERS - 1) * S::STAGE);
       if constexpr (S::BUFFERS == 1) __syncthreads();
       fetch(t + S::BUFFERS * S::STAGE);
     };
@@ -324,7 +327,8 @@ __global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(co
       }
     }
   };
-  auto put = [&] {
+  auto put = [&](int t) {
+    next.clean(p, t, r1);
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {
       if (!next.any(u) || !next.is_y(u)) continue;
@@ -354,7 +358,7 @@ __global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(co
     for (int h = 0; h < 2; ++h) half[turn_at(part, h)] = bf16x4{};  // keys that are not there
   const bf16x8 *qt = stage, *gt = stage + S::UNITS;
   for (int t = r0; t < r1; t += 32) {
-    put();
+    put(t);
     __syncthreads();
     fetch(t + 32);
     if (!empty) {
