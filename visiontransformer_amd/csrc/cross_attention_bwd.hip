@@ -182,30 +182,31 @@ void cross_dkv_kernel(const Params p) {
   auto at = [&](bool y, int r) {
     return y ? p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r) : p.q.ptr + row_offset(p, p.q.ld, b, hk, r);
   };
-  float sm = 0.f, sd = 0.f, sl[S::TASKS];
+  float sm = 0.f, sd = 0.f, sl[S::TASKS] = {};
   auto fetch = [&](int t) {
     next.fetch(p, t, r1, at);
+    if (t >= r1) return;
 #pragma unroll
-    for (int u = 0; u < S::TASKS; ++u) {  // l of a task's row of dout
-      const int r = t + next.row(u);
-      sl[u] = next.any(u) && next.is_y(u) && r < r1 ? p.stats[2 * row_stat(p, b, hk, r) + 1] : 1.f;
-    }
+    for (int u = 0; u < S::TASKS; ++u)  // l of a task's row
+      sl[u] = p.stats[2 * row_stat(p, b, hk, min(t + next.row(u), r1 - 1)) + 1];
     if (threadIdx.x < S::STAGE) {
-      sm = sd = 0.f;  // a row that is not there: exp2(0) times zeros
-      const int r = t + threadIdx.x;
-      if (r < r1) sm = -p.stats[2 * row_stat(p, b, hk, r)], sd = -p.delta[row_stat(p, b, hk, r)];
+      const long long st = row_stat(p, b, hk, min(t + (int)threadIdx.x, r1 - 1));
+      sm = p.stats[2 * st], sd = p.delta[st];
     }
   };
   auto put = [&](int n, int t) {
     next.clean(p, t, r1);
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {  // dout / l
-      const float f = sl[u] == 0.f ? 0.f : 1.f / sl[u];
+      const float f = !next.is_y(u) ? 1.f : sl[u] == 0.f ? 0.f : 1.f / sl[u];
 #pragma unroll
       for (int e = 0; e < 8; ++e) next.v[u][e] *= f;
     }
     next.put(buffers + n * 2 * S::UNITS);
-    if (threadIdx.x < S::STAGE) rm[n][threadIdx.x] = sm, rd[n][threadIdx.x] = sd;
+    if (threadIdx.x < S::STAGE) {  // a row that is not there: exp2(0) times zeros
+      const bool there = t + (int)threadIdx.x < r1;
+      rm[n][threadIdx.x] = there ? -sm : 0.f, rd[n][threadIdx.x] = there ? -sd : 0.f;
+    }
   };
   const bool early = wave < NW / 2, empty = (kb * KG + kg) * 16 >= len;
   fetch(r0);
@@ -308,22 +309,30 @@ __global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(co
   for (int n = 0; n < DH / 16; ++n) dk[n] = zero4(), dv[n] = zero4();
   const int r0 = min((long long)split * p.chunk, (long long)p.rows), r1 = min((long long)r0 + p.chunk, (long long)p.rows);
   Stage<DH, 4, 4> next;
-  float o[S::TASKS][8], m[S::TASKS], l[S::TASKS];  // of a task's row of dout
+  float o[S::TASKS][8] = {}, m[S::TASKS] = {}, l[S::TASKS] = {};  // of a task's row of dout
   auto at = [&](bool y, int r) {
     return y ? p.dout.ptr + row_offset(p, p.dout.ld, b, hk, r) : p.q.ptr + row_offset(p, p.q.ld, b, hk, r);
   };
   auto fetch = [&](int t) {
     next.fetch(p, t, r1, at);
+    if (t >= r1) return;
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {
-      const int r = t + next.row(u);
-      m[u] = l[u] = 0.f;  // a row that is not there: exp2(0) times zeros
+      if (!next.any(u) || !next.is_y(u)) continue;
+      const int r = min(t + next.row(u), r1 - 1);
+      const long long st = 2 * row_stat(p, b, hk, r);
+      m[u] = p.stats[st], l[u] = p.stats[st + 1];
+      const float *from = p.o.ptr + row_offset(p, p.o.ld, b, hk, r);
+      int d = next.unit(u) * 8;
+      if (p.vec) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < p.dh ? d : 0)),
+                    y = *reinterpret_cast<const f32x4 *>(from + (d + 4 < p.dh ? d + 4 : 0));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[u][e] = 0.f;
-      if (next.any(u) && next.is_y(u) && r < r1) {
-        const long long st = 2 * row_stat(p, b, hk, r);
-        m[u] = p.stats[st], l[u] = p.stats[st + 1];
-        load_eight(p.o.ptr + row_offset(p, p.o.ld, b, hk, r), next.unit(u) * 8, p, o[u]);
+        for (int e = 0; e < 4; ++e) o[u][e] = x[e], o[u][4 + e] = y[e];
+      } else {
+        asm volatile("" : "+v"(d));  // (as in Stage::fetch)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[u][e] = from[min(d + e, p.dh - 1)];
       }
     }
   };
@@ -332,16 +341,17 @@ __global__ __launch_bounds__(256, short_resident(DH)) void cross_short_kernel(co
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {
       if (!next.any(u) || !next.is_y(u)) continue;
-      const float f = l[u] == 0.f ? 0.f : 1.f / l[u];
+      const bool there = t + next.row(u) < r1;  // if not: exp2(0) times zeros
+      const float f = !there || l[u] == 0.f ? 0.f : 1.f / l[u];
       float delta = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        delta += next.v[u][e] * o[u][e];
+        delta += there && next.unit(u) * 8 + e < p.dh ? next.v[u][e] * o[u][e] : 0.f;
         next.v[u][e] *= f;
       }
 #pragma unroll
       for (int x = 1; x < UNITS; x *= 2) delta += __shfl_xor(delta, x, 64);
-      if (next.unit(u) == 0) rm[next.row(u)] = -m[u], rd[next.row(u)] = -(delta * f);
+      if (next.unit(u) == 0) rm[next.row(u)] = there ? -m[u] : 0.f, rd[next.row(u)] = -(delta * f);
     }
     next.put(stage);
   };
