@@ -312,10 +312,12 @@ struct Stage {
     if (p.vec) {
 #pragma unroll
       for (int u = 0; u < S::TASKS; ++u) {
-        const float *from = at(is_y(u), min(first + row(u), end - 1));
+        int r = row(u), d0 = unit(u) * 8;
+        if constexpr (DH == 96) asm volatile("" : "+v"(r), "+v"(d0));  // (no place to keep what follows from them)
+        const float *from = at(is_y(u), min(first + r, end - 1));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int d = unit(u) * 8 + 4 * h;
+          const int d = d0 + 4 * h;
           const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < p.dh ? d : 0));
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[u][4 * h + e] = x[e];
@@ -337,7 +339,9 @@ struct Stage {
     if (first + S::STAGE <= end && p.dh == DH) return;
 #pragma unroll
     for (int u = 0; u < S::TASKS; ++u) {
-      const int columns = first + row(u) < end ? p.dh - unit(u) * 8 : 0;
+      int r = row(u), d0 = unit(u) * 8;
+      if constexpr (DH == 96) asm volatile("" : "+v"(r), "+v"(d0));
+      const int columns = first + r < end ? p.dh - d0 : 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e >= columns) v[u][e] = 0.f;
