@@ -344,11 +344,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void cross_join_many_kernel(
 }
 
 // ------------------------------------------------------------------------------------- few rows
-// At most 4 rows per key head, 8 of wide heads (single tokens): every key and value is read once and used for at most 8 dot
-// products, so memory bounds this and the vector ALU computes it.  LP lanes share a key, four columns each;
-// 64 / LP keys per wave and U of those in flight: fewer for more rows, since eight waves a SIMD read faster
-// than more loads in fewer waves (16 x 12345 keys x 4 heads x 128, four rows: 6.0 TB/s with U = 2, 4.9 with
-// 4).  Each batch entry is cut into equal parts, so ragged lengths leave no workgroup without work.  Each group of
+// At most 4 rows per key head, 8 of wide heads (single tokens): every key and value is read once and used for a few
+// dot products, so memory bounds this and the vector ALU computes it.  LP lanes share a key, four columns each;
+// 64 / LP keys per wave and U of those in flight: fewer for more rows, since more waves a SIMD read faster than more
+// loads in fewer waves.  16 x 12345 keys x 4 heads x 128, 809 MB: one row 121 us = 6.7 TB/s, four rows 131.
+// Each batch entry is cut into equal parts, so ragged lengths leave no workgroup without work.  Each group of
 // LP lanes keeps a running maximum and sum per row of its own; groups, then waves, are joined at the end.
 template <int LP>
 __device__ __forceinline__ float group_sum(float x) {  // over LP neighbouring lanes, in all of them
@@ -362,14 +362,6 @@ __device__ __forceinline__ float group_sum(float x) {  // over LP neighbouring l
   if constexpr (LP >= 32)  // lane ^ 16
     x += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), 0x401F));
   return x;
-}
-
-// load_quad of what nobody reads again
-__device__ __forceinline__ f32x4 stream_quad(const float *row, int d, int dh, bool vec) {
-  if (!vec) return load_quad(row, d, dh, false);
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (d < dh) r = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + d));
-  return r;
 }
 
 template <int LP, int R, int NW>
@@ -398,15 +390,29 @@ __global__ __launch_bounds__(64 * NW) void cross_row_kernel(const Params p) {
     }
   }
   const float *kp = p.k.ptr + key_offset(p, p.k.ld, b, hk, 0), *vp = p.v.ptr + key_offset(p, p.v.ld, b, hk, 0);
+  const int first = d < p.dh ? d : 0;
   for (int t = k0 + wave * KEYS * U; t < k1; t += NW * KEYS * U) {
+    // Keys behind the end stand for the last one, with a score of -inf; columns behind dh meet zeros of q, and
+    // nobody reads their sums.  (Nontemporal: nobody reads a key again.)
     f32x4 k[U], v[U];
+    if (p.vec) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int key = t + u * KEYS + lg;
-      k[u] = v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (key < k1) {
-        k[u] = stream_quad(kp + key * p.k.ld, d, p.dh, p.vec);
-        v[u] = stream_quad(vp + key * p.v.ld, d, p.dh, p.vec);
+      for (int u = 0; u < U; ++u) {
+        const int key = min(t + u * KEYS + lg, k1 - 1);
+        k[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(kp + key * p.k.ld + first));
+        v[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(vp + key * p.v.ld + first));
+      }
+    } else {
+      int from = d;
+      asm volatile("" : "+v"(from));  // (the compiler would keep these places in registers for the whole loop)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int key = min(t + u * KEYS + lg, k1 - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          k[u][e] = kp[key * p.k.ld + min(from + e, p.dh - 1)];
+          v[u][e] = vp[key * p.v.ld + min(from + e, p.dh - 1)];
+        }
       }
     }
 #pragma unroll
@@ -493,10 +499,10 @@ FwdPlan plan_fwd(Params *p) {
     p->blocks = 1;
     f.block.waves = 4;
     // One round of the workgroups that fit the device by their registers, 64 keys or more each (16 x 12345 keys x 4
-    // heads x 128, four rows: 135 us with 6 a CU, 168 with 8; one row 123, without regard to a round 147; 2 x 100000
-    // keys x 2 heads 70, in at most 64 parts 209; one batch entry of 4000 keys x 8 heads x 64: 15 us in parts of 64
-    // keys, 20 in parts of 256).
-    const long long cus = vitk::cu_count(), places = cus * (p->rows <= 2 ? 7 : p->rows <= 4 ? 6 : 4);
+    // heads x 128, four rows, ragged: 117 us with 5 a CU, 126 in 39 parts whatever fits; 48 x 12 heads x 3000 x 64, one
+    // row: 142 us in three parts, 223 in one; 2 x 100000 keys x 2 heads 67, in at most 64 parts 209; one batch entry
+    // of 4000 keys x 8 heads x 64: 15 us in parts of 64 keys, 20 in parts of 256).
+    const long long cus = vitk::cu_count(), places = cus * (p->rows <= 2 ? 7 : p->rows <= 4 ? 5 : 4);
     const int few = p->rows == 1 ? 448 : p->rows <= 4 ? 320 : 192;  // keys
     if (p->Nk <= few && heads <= (p->rows == 1 ? 2 * cus : cus))
       f.block.waves = 16;  // one launch (515 keys, 40 heads of 80, one row: 18 us, in parts 15; 260 keys: 7 and 9)
