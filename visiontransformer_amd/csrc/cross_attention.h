@@ -222,13 +222,6 @@ __device__ __forceinline__ float column_sum(float x) {
   return x + __shfl_xor(x, 32, 64);
 }
 
-// columns d .. d + 7 of a row; zeros behind dh
-__device__ __forceinline__ void load_eight(const float *row, int d, const Params &p, float (&x)[8]) {
-  const f32x4 a = load_quad(row, d, p.dh, p.vec), b = load_quad(row, d + 4, p.dh, p.vec);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-}
-
 // this lane's part of a row (columns 32 i + 8 g ..), which has to be there; every load in flight at once (a branch
 // around each, as for columns behind dh, would wait for one after the other)
 template <int DH>
