@@ -7,8 +7,8 @@
 // keys with a running maximum and sum per row.
 //
 // Bounds: the matrix cores where keys are many (1021 x 4099 x 64, 48 heads: 200 - 220 us for 38.6 GFLOP, six bf16
-// products each, 1050 - 1160 TFLOP/s of them; 512 x 1536 x 96, 128 heads: 230 us, 1010), the loads and splits of
-// a stage where they are few (48 x 197 x 64, 768 heads: 29.4 us), memory for a few rows.
+// products each, 1050 - 1160 TFLOP/s of them; 512 x 1536 x 96, 128 heads: 239 us, 970), the loads and splits of
+// a stage where they are few (48 x 197 x 64, 768 heads: 24.7 us, 3.9 TB/s), memory for a few rows.
 #include "cross_attention.h"
 
 #include <algorithm>
@@ -90,8 +90,8 @@ using namespace vitk::cross;
 // NW waves: RW groups of 16 rows, and NW / RW waves that share such a group's keys (few rows: the keys of a
 // stage are dealt to the waves instead of leaving them idle; their results are joined in LDS).
 // Blocks of 64 rows as four waves of 16, whose keys no waves share: with one buffer up to four such workgroups are
-// on a CU and hide each other's loads and barriers.  48 rows x 197 keys x 64, 768 heads: 29.4 us; eight waves
-// that share the keys 33.6.
+// on a CU and hide each other's loads and barriers.  48 rows x 197 keys x 64, 768 heads: 24.7 us; eight waves
+// that share the keys took 4 us more.
 constexpr int waves_a_simd(int dh, int nw, int rw) {
   if (nw == rw) return dh <= 64 ? 4 : nw == 8 ? (dh <= 96 ? 4 : 2) : dh <= 96 ? 3 : 2;
   return nw == 8 ? (dh <= 64 ? 4 : 2) : dh <= 64 ? 2 : 1;

@@ -11,9 +11,8 @@
 // Blocks of up to 128 rows (keys), 16 a wave; with fewer, two waves may share a group and deal the tiles of the
 // other side.  Where the blocks are too few for the device, the other side is split over workgroups and
 // the parts are added in order by a second launch.
-// Bound by the matrix cores (512 x 1536 x 96, 128 heads of which 4 share a key head: dQ 330 us, dK and dV 461, 1054
-// and 1006 TFLOP/s of bf16 products; 16 entries of 1024 keys: 522, 1185); few keys by the start and the
-// end of a workgroup.
+// Bound by the matrix cores (512 x 1536 x 96, 128 heads of which 4 share a key head: dQ 328 us, dK and dV 437, 1060
+// TFLOP/s of bf16 products each); few keys by the start and the end of a workgroup.
 #include "cross_attention.h"
 
 #include <algorithm>
@@ -274,8 +273,8 @@ void cross_dkv_kernel(const Params p) {
 // instead of seven, and each row is read once.  Each wave forms p and ds of its 16 keys with a stage of 32 rows
 // and adds to dK and dV; ds goes through LDS as [key][row], and dQ^T[d][row] += K^T ds is dealt to the waves by
 // blocks of 16 x 16.  K is there times scale log2(e), for the scores.  With fewer heads than places, rows are split.
-// 147 x 50 x 64, 384 heads: 37 us (dQ, then dK and dV: 56); 50 x 50, 512 heads 21 (28); 900 x 50, 24 heads, split
-// 28 (43).  (64 columns fill the registers of two workgroups a CU.)
+// 147 x 50 x 64, 384 heads: 33 us, 50 x 50, 512 heads 18, 900 x 50, 24 heads, split, 24 (dQ, then dK and dV took 56,
+// 28 and 43).  (64 columns fill the registers of two workgroups a CU.)
 constexpr int FEW_KEYS = 64;
 constexpr int short_resident(int dh) { return dh <= 32 ? 3 : 2; }
 template <int DH>
