@@ -423,6 +423,11 @@ EMBED = {
     "digits_three": (70001, 36, 9001, "rank"),
     "direct_largest_table": (16384, 36, 1024, "rank"),
     "direct_small_table_wide": (51, 1024, 756, "rank"),
+    "direct_sixteen_waves": (300, 768, 4096, "rank"),
+    "direct_sixteen_waves_same": (12, 192, 4001, "same"),
+    "direct_sixteen_waves_odd": (1000, 33, 1500, "padded"),
+    "counted_small_wide_table": (255, 2304, 1500, "rank"),
+    "counted_above_the_direct_form": (3000, 64, 1025, "outside"),
     "direct_small_table_odd_width": (51, 333, 256, "padded"),
 }
 
@@ -757,8 +762,8 @@ def test_cross_attention_refuses_null_arguments_and_a_missing_workspace():
     ("vitk_embedding_bwd", (None, 4096, 3, 10, 8, 1.0, 0, 4096, 4096, 1 << 20, None), "null pointer"),
     ("vitk_embedding_bwd", (4096, 4096, 3, 10, 8, 1.0, 0, None, 4096, 1 << 20, None), "null pointer"),
     ("vitk_embedding_bwd", (4096, 4096, 3, 50000, 8, 1.0, 0, 8192, None, 1 << 20, None), "workspace"),
-    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4096, 16, None), "workspace"),
-    ("vitk_embedding_bwd", (4096, 4096, 2000, 10, 8, 1.0, 0, 8192, 4100, 1 << 20, None), "aligned"),
+    ("vitk_embedding_bwd", (4096, 4096, 20000, 10, 8, 1.0, 0, 8192, 4096, 16, None), "workspace"),
+    ("vitk_embedding_bwd", (4096, 4096, 20000, 10, 8, 1.0, 0, 8192, 4100, 1 << 20, None), "aligned"),
     ("vitk_embedding_bwd", (4096, 4096, 2 ** 31, 10, 8, 1.0, 0, 8192, 4096, 1 << 20, None), "tokens over"),
 ])
 def test_embedding_refuses(name, args, message):

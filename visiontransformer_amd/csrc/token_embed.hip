@@ -371,22 +371,22 @@ __global__ __launch_bounds__(TPB) void embedding_join_kernel(const Sums s) {
 }
 
 // Few tokens, not too large a table: no sort (528 tokens x 192 over 1000 rows: 4 us; 1000 over 6000 and 16000
-// rows 6 and 12.7, by counting 15 and 15.6).  One workgroup per table row; each wave looks through a quarter of the
-// tokens and adds the rows of its own in their order, the four sums are added in order.
-constexpr int DIRECT_TOKENS = 1024, DIRECT_TABLE = 16384;
-template <int W>
-__global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__restrict__ dout,
+// rows 6 and 12.7, by counting 15 and 15.6).  One workgroup per table row; each wave looks through its share of the
+// tokens and adds the rows of its own in their order, the waves' sums are added in order.
+constexpr int DIRECT_STEPS = 4;  // of 64 tokens a wave
+template <int W, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void embedding_direct_kernel(const float *__restrict__ dout,
                                                                const int32_t *__restrict__ index, int n, long long D,
                                                                float scale, int accumulate, float *__restrict__ dtable) {
-  constexpr int WAVES = TPB / 64, U = 8;
+  constexpr int U = 8;
   __shared__ Cols<W> part[WAVES][64];
   __shared__ int found[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x;
-  unsigned long long mine[DIRECT_TOKENS / TPB];
+  unsigned long long mine[DIRECT_STEPS];
   unsigned long long any = 0;
 #pragma unroll
-  for (int u = 0; u < DIRECT_TOKENS / TPB; ++u) {
-    const int i = (wave * (DIRECT_TOKENS / TPB) + u) * 64 + lane;
+  for (int u = 0; u < DIRECT_STEPS; ++u) {
+    const int i = (wave * (DIRECT_STEPS) + u) * 64 + lane;
     mine[u] = __ballot(i < n && index[i] == t);
     any |= mine[u];
   }
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__re
     const long long col = c0 + lane * W;
     Cols<W> acc = {};
 #pragma unroll
-    for (int u = 0; u < DIRECT_TOKENS / TPB; ++u) {
-      const float *src = dout + (long long)(wave * (DIRECT_TOKENS / TPB) + u) * 64 * D + col;
+    for (int u = 0; u < DIRECT_STEPS; ++u) {
+      const float *src = dout + (long long)(wave * (DIRECT_STEPS) + u) * 64 * D + col;
       unsigned long long left = mine[u];
       while (left) {
         Cols<W> x[U];
@@ -416,7 +416,9 @@ __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__re
     }
     part[wave][lane] = acc;
     __syncthreads();
-    const int hit = found[0] | found[1] | found[2] | found[3];
+    int hit = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) hit |= found[w];
     if (wave == 0 && col < D && (hit || !accumulate)) {
       float *dst = dtable + (long long)t * D + col;
       Cols<W> r = part[0][lane];
@@ -434,7 +436,13 @@ __global__ __launch_bounds__(TPB) void embedding_direct_kernel(const float *__re
   }
 }
 
-bool direct(long long n, long long V) { return n <= DIRECT_TOKENS && V <= DIRECT_TABLE; }
+// Waves of the direct form, 0 = sorted.  Four for up to 1024 tokens and 16384 rows; sixteen, for up to 4096 tokens, if
+// the table is small enough for a few rounds of such workgroups (2000 tokens over 89 x 768: 6.2 us, sorted 13.8; 1671 x 192:
+// 10.8 and 16; 3000 x 192: 17 and 16).
+int direct_waves(long long n, long long V, long long D) {
+  if (n <= 64 * DIRECT_STEPS * 4 && V <= 16384) return 4;
+  return n <= 64 * DIRECT_STEPS * 16 && V * ((D + 255) / 256) <= 2048 ? 16 : 0;
+}
 
 struct Plan {
   int passes, blocks, chunk;  // no passes: by rank
@@ -518,7 +526,7 @@ extern "C" int vitk_embedding_fwd(const float *table, int64_t V, const int32_t *
 }
 
 extern "C" size_t vitk_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D) {
-  if (!shape_ok(rows, V, D) || rows == 0 || V == 0 || D == 0 || rows > kMaxTokens || direct(rows, V)) return 0;
+  if (!shape_ok(rows, V, D) || rows == 0 || V == 0 || D == 0 || rows > kMaxTokens || direct_waves(rows, V, D) > 0) return 0;
   return (size_t)make_plan(rows, V, D).total * 4;
 }
 
@@ -535,18 +543,19 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
   hipStream_t st = vitk::as_stream(stream);
   if (rows == 0) return accumulate ? 0 : vitk_fill_f32(dtable, 0.f, V * D, stream);
   const bool vec = D % 4 == 0 && vitk::aligned16(dout) && vitk::aligned16(dtable);
-  if (direct(rows, V)) {
+  if (const int waves = direct_waves(rows, V, D)) {
     // few table rows: a workgroup for each block of their columns (756 tokens x 1024 over 51 rows: 14 -> 6 us, 1000
     // over 2000 rows 10 -> 8, over 4000 11 -> 14)
     const int width = vec ? 256 : 64;
     const long long blocks = (D + width - 1) / width;
-    const dim3 grid((unsigned)V, V * blocks <= 8192 ? (unsigned)blocks : 1);
-    if (vec)
-      hipLaunchKernelGGL(embedding_direct_kernel<4>, grid, dim3(TPB), 0, st, dout, index, (int)rows, (long long)D, scale,
-                         (int)accumulate, dtable);
+    const dim3 grid((unsigned)V, V * blocks <= 8192 ? (unsigned)blocks : 1), block(64 * waves);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, block, 0, st, dout, index, (int)rows, (long long)D, scale, (int)accumulate, dtable);
+    };
+    if (waves == 4)
+      vec ? launch(embedding_direct_kernel<4, 4>) : launch(embedding_direct_kernel<1, 4>);
     else
-      hipLaunchKernelGGL(embedding_direct_kernel<1>, grid, dim3(TPB), 0, st, dout, index, (int)rows, (long long)D, scale,
-                         (int)accumulate, dtable);
+      vec ? launch(embedding_direct_kernel<4, 16>) : launch(embedding_direct_kernel<1, 16>);
     return vitk::check_launch("vitk_embedding_bwd");
   }
   const Plan p = make_plan(rows, V, D);
