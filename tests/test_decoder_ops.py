@@ -196,7 +196,7 @@ def test_cross_attention_every_block_size(K, dh):
 def test_cross_attention_every_block_size_with_many_heads(K, dh):
     """Blocks of 64 as four waves, which at least one workgroup a CU takes: alone, as 3 and 5 blocks, over keys of
     every kind of count."""
-    for Nq, Nk in ((40, 33), (60, 130), (131, 50), (190, 200), (120, 64), (259, 20), (20, 150)):
+    for Nq, Nk in ((40, 33), (60, 130), (131, 50), (190, 200), (120, 64), (259, 20), (20, 150), (140, 300)):
         g = rng(1000 * Nq + Nk)
         B, Hkv = 40, 8  # 320 workgroups
         q, k, v, dout = (randn(g, B, n, Hkv, dh) for n in (Nq, Nk, Nk, Nq))

@@ -352,9 +352,9 @@ struct Stage {
 // many such workgroups as CUs; otherwise eight, so that two share a group's other side (64 columns, forward, eight
 // waves -> four: 64 x 64, 2048 heads: 40 -> 33 us; 50 x 900, 24 heads: 18 -> 23).  More than 64 rows are cut into
 // blocks of 64 where the last block of 128 were half empty and that is a sixth of the rows or more (147 x 197, 320
-// heads: forward 42 -> 33, row gradient 19 less), up to `half` on the other side, and up to `any` on the other
-// side always (row gradient of 512 x 128, 192 heads: 5 less; 512 x 197: 2 more; key gradients of 16 rows x 1000, 128
-// heads of 96: 7 less).
+// heads: forward 42 -> 33, row gradient 19 less; 300 x 500 x 96, 96 heads: 72 -> 48 and 50 less; 150 x 1000 x 128:
+// 91 -> 102), up to `half` on the other side, and up to `any` on the other side always (row gradient of 512 x 128,
+// 192 heads: 5 less; 512 x 197: 2 more; key gradients of 16 rows x 1000, 128 heads of 96: 7 less).
 struct Block {
   int groups, waves;
 };

@@ -511,7 +511,7 @@ FwdPlan plan_fwd(Params *p) {
   } else {
     // A workgroup of 64 rows with one buffer is worth its empty waves even for 9 to 32 rows: more of them are on a
     // CU (16 x 1000, 320 heads of 64: 49 -> 38 us, of 128: 220 -> 133; of 32 no difference).
-    f.block = plan_block(p->rows, p->Nk, heads, true, 256, 0);
+    f.block = plan_block(p->rows, p->Nk, heads, true, p->dh <= 96 ? 1024 : 512, 0);
     const long long cus = vitk::cu_count();
     if (p->rows <= 32 && p->dh > 32 && 4 * heads >= cus && heads * stages >= cus) f.block = {4, 4};
     const int groups = f.block.groups;

@@ -449,7 +449,7 @@ struct Side {
 };
 Side plan_side(long long own, long long other, long long heads, int dh, bool keys, double part_us) {
   Side s;
-  s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 256, keys ? 64 : 128);
+  s.block = plan_block(own, other, heads, dh <= 96, keys ? 0 : 1024, keys ? 64 : 128);
   // Up to 32 keys, or rows of wide heads: eight waves, half of which only load (668 x 14 x 128, 24 key heads: 109 -> 88 us,
   // 98 x 24 x 80, 128: 49 -> 41; rows: 10 x 814 x 128, 42 heads: 94 -> 74; of 80 columns no difference).
   if (own <= 32 && (keys || dh > 96)) s.block = {4, 8};
