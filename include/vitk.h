@@ -450,8 +450,9 @@ int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float 
  *   y = x / (|x|_F + eps);  `steps` times: g = y y^T, y = a y + (b g + c g g) y;  out = y
  * (y^T y on the other side where rows > cols: the same polynomial of the singular values.)  The
  * Frobenius norm is summed in double precision; between products y and g are pairs of fp16 numbers, 32
- * bits within 2^-23 of the value, and a product is three matrix products of parts with fp32 sums: as
- * close to the exact result as the same steps in fp32.  A zero matrix gives zeros (NaN with eps = 0).
+ * bits within 2^-23 of the value (y below 2^-25 within 2^-48, g below 2^-23 within 2^-46), and a product is
+ * three matrix products of parts with fp32 sums: each row of the shorter side is as close to the exact result as
+ * the same steps in fp32, with a few 2^-23 of its own size a step.  A zero matrix gives zeros (NaN with eps = 0).
  * out may be x, with one layout for both; no other overlap.
  * 0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1] within [-4, 4], with
  * |b t^2 + c t^4| below 31 (checked from the largest values of each step), which every useful triple does.

@@ -653,6 +653,55 @@ def test_newton_schulz_scales(K):
         assert err <= ns_tolerance(h, want, 5, COEF, 1e-38) + floor, (i, err)
 
 
+def graded(kind, level, batch, r, c, seed):
+    """Matrices whose entries span many magnitudes: half of the rows `level` of the others, or one entry of 1 over a
+    floor of `level`."""
+    x = randn(rng(seed), batch, r, c)
+    if kind == "cold rows":
+        x[:, r // 2:] *= level
+    else:
+        x *= level
+        x[:, r // 3, c // 4] = 1.0
+    return x
+
+
+def graded_tolerance(x, want, steps, rowwise):
+    """Bound of each row's (column's) norm.  An operand is within 2 u of its value and the dropped product of two lo
+    parts within 4 u, so a product is off by 8 u of its terms; a step rounds y (2 u), forms and rounds y y^T (8 + 2 u) and
+    the polynomial (8 + 2 u), and multiplies (8 u): 30 u of a row, in five steps 150 u, passed on with a factor of at most
+    4 relative to the row, which grows as its error does: 600 u.  The sums are those of the same steps in fp32, of
+    which four times the error is taken.  Below 2^-25 a pair of y is within 2^-48: sqrt(n) of those a row, times 3.4445 a
+    step and 1.41 for all of them."""
+    axis = 1 if rowwise else 0
+    plain = newton_schulz(x, steps, COEF, 1e-30, np.float32)
+    norm = lambda z: np.linalg.norm(z, axis=axis)  # noqa: E731
+    return 4 * norm(plain - want) + 600 * U * norm(want) + 1.41 * 3.4445 ** steps * np.sqrt(x.shape[axis]) * 2.0 ** -48
+
+
+@gpu
+@pytest.mark.parametrize("kind, level", [("cold rows", 1e-3), ("cold rows", 1e-6), ("cold rows", 1e-7), ("spike", 1e-6),
+                                         ("spike", 1e-8)])
+@pytest.mark.parametrize("cus, batch, r, c", [(0, 2, 70, 90), (0, 1, 128, 96), (0, 1, 200, 300), (0, 1, 513, 514),
+                                              (10, 1, 200, 300), (4, 1, 200, 300), (4, 1, 300, 200)],
+                         ids=["one", "one_tall", "small", "lower", "64", "128", "128_tall"])
+def test_newton_schulz_keeps_small_entries(K, kind, level, cus, batch, r, c):
+    """Each row is as close as its own size allows, however large the others are.  (cus: tiles of 64 and 128 at these
+    sizes, as a device with so few CUs would take them.)"""
+    K.planning_cu_count(cus)
+    try:
+        x = graded(kind, level, batch, r, c, 350)
+        out = torch.empty_like(x)
+        K.newton_schulz(K.newton_schulz_args(x, out, steps=5, coefficients=COEF, eps=1e-30))
+        for b in range(batch):
+            h = x[b].cpu().numpy()
+            want = newton_schulz(h, 5, COEF, 1e-30, np.float64)
+            err = np.linalg.norm(out[b].double().cpu().numpy() - want, axis=1)
+            over = err / graded_tolerance(h, want, 5, True)
+            assert (over <= 1).all(), (b, int(over.argmax()), over.max(), (err / np.linalg.norm(want, axis=1)).max())
+    finally:
+        K.planning_cu_count(0)
+
+
 @gpu
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("shape", [(96, 288, 3), (288, 96, 2), (10, 192, 1)])

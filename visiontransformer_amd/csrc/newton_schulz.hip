@@ -4,16 +4,21 @@
 // The matrices are held with their shorter side (r) as rows (a taller matrix is transposed on the way in and
 // out: the polynomial acts on singular values only), padded with zeros to whole tiles.
 // Products run on v_mfma_f32_32x32x16_f16 with every fp32 operand x split in two fp16 parts,
-//   2^S x = hi + lo,  hi = fp16(2^S x), lo = fp16(2^S x - hi),
-// and x y = hi hi' + hi lo' + lo hi' with fp32 sums, on matrix cores that do fp16 at 16 times the rate of
-// fp32.  hi is off by at most half a step of 11 bits and lo, which has a sign, by half a step of 11
+//   2^S x = hi + 2^-11 lo,  hi = fp16(2^S x), lo = fp16(2^11 (2^S x - hi)),
+// and x y = hi hi' + 2^-11 (hi lo' + lo hi') with fp32 sums of both, on matrix cores that do fp16 at 16 times
+// the rate of fp32.  hi is off by at most half a step of 11 bits and lo, which has a sign, by half a step of 11
 // more: a pair is within 2^-23 of x, one bit short of fp32, in the same 32 bits; the dropped lo lo' is
-// below 2^-22.  The steps are normalised, so the range is known and the scales are constants: |y| <= 4
-// with S = 12 (a head room of 4), |y y^T| <= 16 and |b g + c g g| < 31 with S = 10 (head rooms 4 and 2).
-// Against 64 bits the result is as close as the same steps in fp32 throughout (the error is that of the
-// long sums, not of the operands).  Sums are fp32, the norm is fp64; the pairs are also where y and g
-// are kept between products: what the products move is what bounds them, and an fp32 copy beside the
-// pairs would double it.
+// below 2^-22.  lo is as large as hi, so it keeps its bits as far down as hi does: that holds for |2^S x| >= 2^-13,
+// and below that a pair is within 2^-36 of 2^S x.  (With lo unscaled its bits were lost below |2^S x| = 2^-2: rows
+// 1e-7 of the others were off by 1e-2, now by 5e-6.  The second sum takes registers: 3 % of the time of the
+// 128-wide tiles and 2 to 4 % of the small forms.)
+// The steps are normalised, so the range is known and the scales are constants: |y| <= 4
+// with S = 12 (a head room of 4), |y y^T| <= 16 and |b g + c g g| < 31 with S = 10 (head rooms 4 and 2): y is within
+// 2^-23 of its value from 2^-25 on, and within 2^-48 below; g from 2^-23 on, and within 2^-46.
+// Against 64 bits the result is as close as the same steps in fp32 where sums are long (the error is theirs,
+// not that of the operands), and off by a few 2^-23 a step where one entry makes up a matrix.  Sums are fp32, the
+// norm is fp64; the pairs are also where y and g are kept between products: what the products move is what bounds
+// them, and an fp32 copy beside the pairs would double it.
 //
 // A split matrix ("planes") lies in memory as [row][column / 32][part][32]: the two parts of 32 columns are
 // one 128-byte line, 8 units of 16 bytes.
@@ -42,6 +47,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int PARTS = 64;                  // partial sums of a norm
 constexpr float kY = 4096.f, kG = 1024.f;  // 2^S of the planes of y and of g, b g + c g g
+constexpr float kLo = 2048.f;              // 2^11: lo parts are held times this
 constexpr int ONE = 128;                   // largest side of the one-launch form
 
 struct NsParams {
@@ -65,15 +71,15 @@ struct NsParams {
 // ------------------------------------------------------------------------------------- the planes
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ void split4(f32x4 v, float scale, f16x4 &hi, f16x4 &lo) {  // two elements an instruction
+__device__ __forceinline__ void split4(f32x4 v, float scale, f16x4 &hi, f16x4 &lo) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const f32x2 x = {v[2 * h] * scale, v[2 * h + 1] * scale};
     const f16x2 a = __builtin_convertvector(x, f16x2);
-    const f32x2 r = {x[0] - (float)a[0], x[1] - (float)a[1]};
-    const f16x2 b = __builtin_convertvector(r, f16x2);
     hi[2 * h] = a[0], hi[2 * h + 1] = a[1];
-    lo[2 * h] = b[0], lo[2 * h + 1] = b[1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)  // (one mixed-precision instruction: what is left is exact in fp32)
+      lo[2 * h + e] = (_Float16)fmaf((float)a[e], -kLo, v[2 * h + e] * (scale * kLo));
   }
 }
 // fp16 offset of the hi part of element (row, col) of a matrix of `cols` columns; the lo part lies 32 behind
@@ -96,16 +102,24 @@ __device__ __forceinline__ f16x4 read_transposed(const _Float16 *at) {
 __device__ __forceinline__ f16x8 join(f16x4 a, f16x4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ __forceinline__ f32x16 product3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
-}
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll
   for (int i = 0; i < 16; ++i) z[i] = 0.f;
   return z;
+}
+// The sums of hi hi' and of hi lo' + lo hi', which are kLo times as large.
+struct Sum {
+  f32x16 hh = zero16(), cross = zero16();
+  __device__ __forceinline__ float operator[](int e) const { return hh[e] + cross[e] * (1.f / kLo); }
+};
+__device__ __forceinline__ void product(f16x8 a, f16x8 b, f32x16 &acc) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void product3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, Sum &acc) {
+  product(ah, bl, acc.cross);
+  product(ah, bh, acc.hh);
+  product(al, bh, acc.cross);
 }
 
 // ----------------------------------------------------------------------------- norm and first y
@@ -298,7 +312,7 @@ __device__ __forceinline__ f32x4 finish(const NsParams &p, int flip, long long k
   f32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float x = (float)add.hi[e] + (float)add.lo[e];
+    const float x = (float)add.hi[e] + (float)add.lo[e] * (1.f / kLo);
     if constexpr (MODE == GRAM)
       v[e] = acc[e] * (1.f / (kY * kY));
     else if constexpr (MODE == POLY)
@@ -348,12 +362,12 @@ __device__ __forceinline__ f16x8 load_unit(const _Float16 *base, int voff, int s
 // 2000 to 3000 cycles away.
 // The workgroups of an XCD (every eighth) take neighbouring tiles, so that they share operands in its L2.
 template <int MODE, int T, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const NsParams p, int flip, int total) {
+__global__ __launch_bounds__(64 * NW, 4) void ns_tile_kernel(const NsParams p, int flip, int total) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
   constexpr int NX = T / 64, NY = 2 * T / NW / 32;  // 32-wide blocks of a wave in each direction
   constexpr int UNITS = T * 8;                      // 16-byte units of an operand's slab
   constexpr int THREADS = 64 * NW, LOADS = UNITS / THREADS;
-  constexpr int DIST = T == 128 ? 2 : 4;
+  constexpr int DIST = 2;
   constexpr int SP = T + 4;  // pitch of the sums in the epilogue
   constexpr int LDS_BYTES = T * SP * 4 > 4 * UNITS * 16 ? T * SP * 4 : 4 * UNITS * 16;
   __shared__ __attribute__((aligned(16))) char lds_bytes[LDS_BYTES];
@@ -385,11 +399,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const
   const int qd = TR ? qrow * (T / 4) + (qunit ^ tr_swizzle(qrow)) : pd;
   const long long qslab = TR ? 32ll * 2 * cols : 64;
 
-  f32x16 acc[NX][NY];
-#pragma unroll
-  for (int x = 0; x < NX; ++x)
-#pragma unroll
-    for (int y = 0; y < NY; ++y) acc[x][y] = zero16();
+  Sum acc[NX][NY];
   f16x8 pr[DIST][LOADS], qr[DIST][LOADS];
   const int slabs = depth / 32;
   auto fetch = [&](int s, f16x8 (&x)[LOADS], f16x8 (&y)[LOADS]) {
@@ -416,32 +426,44 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void ns_tile_kernel(const
   // branch: where loads may or may not have been issued the compiler waits for all of them.
   auto multiply = [&](int s, int h) {
     const f16x8 *lp = lds[s & 1][0], *lq = lds[s & 1][1];
-    f16x8 a[NX][2], b[NY][2];  // [block][part] of P (columns of the result tile's MFMA form) and Q
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
+    // blocks of P (columns of the result tile's MFMA form) and of Q
+    auto read_p = [&](int part, f16x8 (&to)[NX]) {
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
         const int row = wi + 32 * x + c;
-        a[x][part] = lp[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
+        to[x] = lp[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
       }
+    };
+    auto read_q = [&](int part, f16x8 (&to)[NY]) {
 #pragma unroll
       for (int y = 0; y < NY; ++y) {
         if constexpr (TR) {
           const int sub = (lane >> 4) & 1, k0 = 16 * h + 8 * g + ((lane & 15) >> 2);
           const int unit = ((wj >> 5) + y) * 8 + 4 * part + 2 * sub + ((lane & 3) >> 1);
           const _Float16 *base = reinterpret_cast<const _Float16 *>(lq) + 4 * (lane & 1);
-          b[y][part] = join(read_transposed(base + (k0 * (T / 4) + (unit ^ tr_swizzle(k0))) * 8),
-                            read_transposed(base + ((k0 + 4) * (T / 4) + (unit ^ tr_swizzle(k0 + 4))) * 8));
+          to[y] = join(read_transposed(base + (k0 * (T / 4) + (unit ^ tr_swizzle(k0))) * 8),
+                       read_transposed(base + ((k0 + 4) * (T / 4) + (unit ^ tr_swizzle(k0 + 4))) * 8));
         } else {
           const int row = wj + 32 * y + c;
-          b[y][part] = lq[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
+          to[y] = lq[row * 8 + ((4 * part + 2 * h + g) ^ row_swizzle(row))];
         }
       }
-    }
+    };
+    // the sums of all blocks in turn, operands in the order of their use: registers are short
+    f16x8 ph[NX], pl[NX], qh[NY], ql[NY];
+    read_p(0, ph), read_q(0, qh), read_q(1, ql), read_p(1, pl);
 #pragma unroll
     for (int x = 0; x < NX; ++x)
 #pragma unroll
-      for (int y = 0; y < NY; ++y) acc[x][y] = product3(b[y][0], b[y][1], a[x][0], a[x][1], acc[x][y]);
+      for (int y = 0; y < NY; ++y) product(qh[y], ph[x], acc[x][y].hh);
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int y = 0; y < NY; ++y) product(ql[y], ph[x], acc[x][y].cross);
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int y = 0; y < NY; ++y) product(qh[y], pl[x], acc[x][y].cross);
   };
   auto step = [&](int s, f16x8 (&x)[LOADS], f16x8 (&y)[LOADS]) {
     multiply(s, 0);
@@ -538,7 +560,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
   const int i = threadIdx.x >> 3, j = (threadIdx.x & 7) * 4;  // this thread's elements of the result
   Parts add = {};
   if (threadIdx.x < 256) add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
-  f32x16 acc = zero16();
+  Sum acc;
   [[maybe_unused]] _Float16 *qt = reinterpret_cast<_Float16 *>(lds[wave]);
   for (int s = s0; s < s1; s += U) {
     f16x8 a[U][2], b[U][2];
@@ -578,7 +600,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc = product3(b[u][0], b[u][1], a[u][0], a[u][1], acc);
+    for (int u = 0; u < U; ++u) product3(b[u][0], b[u][1], a[u][0], a[u][1], acc);
   }
   float *own = reinterpret_cast<float *>(lds[wave]);
 #pragma unroll
@@ -638,7 +660,7 @@ __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int
   const int i = lane >> 2, j = (lane & 3) * 4;  // the first wave's elements of the result
   Parts add = {};
   if (wave == 0) add = addend<MODE>(p, flip, k, i0 + i, j0 + j);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f}, cross = acc;
   for (int s = s0; s < s1; s += U) {
     f16x8 a[U][2], b[U][2];
 #pragma unroll
@@ -653,11 +675,13 @@ __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s + u >= s1) a[u][0] = a[u][1] = f16x8{};  // (a step that was loaded twice adds nothing)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][0], a[u][1], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][1], a[u][0], acc, 0, 0, 0);
+      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][0], a[u][1], cross, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][0], a[u][0], acc, 0, 0, 0);
+      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u][1], a[u][0], cross, 0, 0, 0);
     }
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] += cross[e] * (1.f / kLo);
   *reinterpret_cast<f32x4 *>(lds[wave] + c * PITCH + 4 * g) = acc;
   __syncthreads();
   if (wave > 0) return;
@@ -699,7 +723,7 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
   // this wave's block of y and of g
   const int yi = wave / tn, yj = wave % tn, gi = wave / tr, gj = wave % tr;
   const bool y_mine = yi < tr, g_mine = gi < tr;
-  float y[16];
+  float y[16];  // behind the norm: times kY
   double s = 0.0;
   // Element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4.  Every load is issued, its place
 // clamped: a branch around each would wait for one after the other (96 x 96 without a step: 11 us instead of 6).
@@ -752,7 +776,7 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
   const float norm = (float)sqrt(s) + p.eps;
 #pragma unroll
   for (int e = 0; e < 16; ++e)
-    if (row < p.r && col + 8 * (e / 4) + e % 4 < p.n) y[e] /= norm;
+    if (row < p.r && col + 8 * (e / 4) + e % 4 < p.n) y[e] = y[e] / norm * kY;
   // block (bi, bj) of a matrix with `blocks` column blocks, from the registers' layout
   auto store = [&](f16x8 *m, int pitch, int bi, int bj, const float (&x)[16], float scale) {
     const int row = 32 * bi + c;
@@ -766,92 +790,83 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
     }
   };
   struct Operand {
-    f16x8 x[2][2];  // [16 k][part]
+    f16x8 part[2];  // of 16 k
   };
-  // row 32 block + c, columns of column block cb
-  auto rows = [&](const f16x8 *m, int pitch, int block, int cb) {
-    Operand o;
-    const f16x8 *at = m + (32 * block + c) * pitch + 8 * cb + g;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int part = 0; part < 2; ++part) o.x[h][part] = at[4 * part + 2 * h];
-    return o;
+  // row 32 block + c, columns 16 t .. + 15
+  auto rows = [&](const f16x8 *m, int pitch, int block, int t) {
+    const f16x8 *at = m + (32 * block + c) * pitch + 8 * (t >> 1) + 2 * (t & 1) + g;
+    return Operand{{at[0], at[4]}};
   };
-  // columns 32 cb + c of y, rows of row block rb
-  auto columns = [&](int rb, int cb) {
+  // column 32 cb + c of y, rows 16 t .. + 15
+  auto columns = [&](int t, int cb) {
     Operand o;
-    const _Float16 *at = reinterpret_cast<const _Float16 *>(yl + (32 * rb + 8 * g + ((lane & 15) >> 2)) * yp + 8 * cb) +
+    const _Float16 *at = reinterpret_cast<const _Float16 *>(yl + (16 * t + 8 * g + ((lane & 15) >> 2)) * yp + 8 * cb) +
                          16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int part = 0; part < 2; ++part)
-        o.x[h][part] = join(read_transposed(at + 16 * h * yp * 8 + 32 * part),
-                            read_transposed(at + (16 * h + 4) * yp * 8 + 32 * part));
+    for (int part = 0; part < 2; ++part)
+      o.part[part] = join(read_transposed(at + 32 * part), read_transposed(at + 4 * yp * 8 + 32 * part));
     return o;
   };
-  auto multiply = [&](const Operand &a, const Operand &b, f32x16 acc) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) acc = product3(a.x[h][0], a.x[h][1], b.x[h][0], b.x[h][1], acc);
+  // sum over `blocks` times 32 k; the next operands are on their way behind each product.  (The first product is
+  // written out: it takes constants where the others take the registers of the sums.)
+  auto contract = [&](int blocks, auto left, auto right) {
+    Sum acc;
+    auto multiply = [&](const Operand &a, const Operand &b) { product3(a.part[0], a.part[1], b.part[0], b.part[1], acc); };
+    Operand a0 = left(0), b0 = right(0), a1 = left(1), b1 = right(1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(a0, b0);
+#pragma unroll 1
+    for (int t = 2; t < 2 * blocks; t += 2) {
+      a0 = left(t), b0 = right(t);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a1, b1);
+      a1 = left(t + 1), b1 = right(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a0, b0);
+    }
+    multiply(a1, b1);
     return acc;
   };
-  // sum over k of row blocks bi and bj of one matrix; the next operands are on their way behind each product
+  // of row blocks bi and bj of one matrix
   auto symmetric = [&](const f16x8 *m, int pitch, int blocks, int bi, int bj) {
-    f32x16 acc = zero16();
-    Operand a = rows(m, pitch, bj, 0), b = rows(m, pitch, bi, 0);
-#pragma unroll 1
-    for (int cb = 1; cb < blocks; ++cb) {
-      const Operand na = rows(m, pitch, bj, cb), nb = rows(m, pitch, bi, cb);
-      acc = multiply(a, b, acc);
-      a = na, b = nb;
-    }
-    return multiply(a, b, acc);
+    return contract(blocks, [&](int t) { return rows(m, pitch, bj, t); }, [&](int t) { return rows(m, pitch, bi, t); });
   };
-  if (p.steps > 0) {
-      if (y_mine) store(yl, yp, yi, yj, y, kY);
-  }
+  if (p.steps > 0 && y_mine) store(yl, yp, yi, yj, y, 1.f);
   __syncthreads();
 #pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
     // (the compiler would compute every address of the body before the loop and run out of registers)
     asm volatile("" : "+v"(lane), "+v"(c), "+v"(g));
-    float v[16];
+    float v[16];  // g times kY^2
     if (g_mine) {  // g = y y^T
-      const f32x16 acc = symmetric(yl, yp, tn, gi, gj);
+      const Sum acc = symmetric(yl, yp, tn, gi, gj);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[e] * (1.f / (kY * kY));
-      store(gl, gp, gi, gj, v, kG);
+      for (int e = 0; e < 16; ++e) v[e] = acc[e];
+      store(gl, gp, gi, gj, v, kG / (kY * kY));
     }
     __syncthreads();
     if (g_mine) {  // b g + c g g
-      const f32x16 acc = symmetric(gl, gp, tr, gi, gj);
+      const Sum acc = symmetric(gl, gp, tr, gi, gj);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = p.b * v[e] + p.c * (acc[e] * (1.f / (kG * kG)));
+      for (int e = 0; e < 16; ++e) v[e] = p.b * (1.f / (kY * kY)) * v[e] + p.c * (1.f / (kG * kG)) * acc[e];
     }
     __syncthreads();
     if (g_mine) store(gl, gp, gi, gj, v, kG);
     __syncthreads();
     if (y_mine) {  // y = a y + that y
-      f32x16 acc = zero16();
-      Operand x = columns(0, yj), w = rows(gl, gp, yi, 0);
-#pragma unroll 1
-      for (int rb = 1; rb < tr; ++rb) {
-        const Operand nx = columns(rb, yj), nw = rows(gl, gp, yi, rb);
-        acc = multiply(x, w, acc);
-        x = nx, w = nw;
-      }
-      acc = multiply(x, w, acc);
+      const Sum acc = contract(tr, [&](int t) { return columns(t, yj); }, [&](int t) { return rows(gl, gp, yi, t); });
 #pragma unroll
-      for (int e = 0; e < 16; ++e) y[e] = p.a * y[e] + acc[e] * (1.f / (kG * kY));
+      for (int e = 0; e < 16; ++e) y[e] = p.a * y[e] + acc[e] * (1.f / kG);
     }
     if (step + 1 < p.steps) {
       __syncthreads();
-      if (y_mine) store(yl, yp, yi, yj, y, kY);
+      if (y_mine) store(yl, yp, yi, yj, y, 1.f);
       __syncthreads();
     }
   }
   if (row >= p.r) return;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e] *= 1.f / kY;
   const long long si = p.tall ? 1 : p.ld_out, sj = p.tall ? p.ld_out : 1, line = k * p.stride_out + row * si;
   if (p.vec && !p.tall && p.cols % 4 == 0) {
     f32x4 old[4];
