@@ -916,6 +916,31 @@ def test_newton_schulz_takes_every_triple_that_stays_and_no_other():
     assert seen == {True, False}
 
 
+def taken(a, b, c, steps):
+    """Are these coefficients accepted?  (The call is refused either way, for its workspace.)"""
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    args = _nargs(vitk, vitk.NewtonSchulzArgs, a=a, b=b, c=c, steps=steps, workspace=0)
+    assert d.vitk_newton_schulz_f32(C.byref(args), None) != 0
+    message = d.vitk_last_error().decode()
+    assert "bounded" in message or "workspace" in message
+    return "bounded" not in message
+
+
+@pytest.mark.parametrize("c", [0.0] + [sign * 10.0 ** e for e in (-30, -20, -16, -15, -13, -12, -9, -6) for sign in (1, -1)])
+@pytest.mark.parametrize("a, b", [(15.0, -14.0), (8.0, -7.5), (-15.0, 14.0), (2.0, -1.0), (1.5, -0.5), (-1.5, 0.5), (0.5, 0.25)])
+def test_newton_schulz_coefficients_next_to_a_cubic(a, b, c):
+    """A fifth-order term that is too small to matter changes nothing: the extremum is that of a t + b t^3."""
+    t, stays = np.linspace(0.0, 1.0, 20001), True
+    for _ in range(5):
+        poly = b * t ** 2 + c * t ** 4
+        t = a * t + poly * t
+        stays = stays and bool((np.abs(poly) < 31.0).all() and (np.abs(t) <= 4.0).all())
+        if not stays:
+            break
+    assert taken(a, b, c, 5) == stays
+
+
 # ---------------------------------------------------------------------------- the run together
 @gpu
 def test_all_of_them_captured_in_one_graph(K):

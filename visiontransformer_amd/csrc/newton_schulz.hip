@@ -944,9 +944,11 @@ bool bounded(double a, double b, double c, int steps) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
   double top = 1.0;
   for (int s = 0; s < steps; ++s) {
+    // the roots of a + 3 b q + 5 c q^2 without a difference of neighbours (c may be tiny, or 0: then one of them is
+    // an infinity, whose place the end takes, or no number)
     const double end = top * top, root = std::sqrt(std::max(9.0 * b * b - 20.0 * a * c, 0.0));
-    const double at[] = {end, c != 0.0 ? -b / (2.0 * c) : end, c != 0.0 ? (-3.0 * b + root) / (10.0 * c) : -a / (3.0 * b),
-                         c != 0.0 ? (-3.0 * b - root) / (10.0 * c) : end};
+    const double t = -0.5 * (3.0 * b + std::copysign(root, b));
+    const double at[] = {end, -b / (2.0 * c), t / (5.0 * c), a / t};
     double next = 0.0;
     for (const double x : at) {
       if (!(x >= 0.0)) continue;
