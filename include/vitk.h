@@ -455,7 +455,8 @@ int vitk_adam_l2(float *p, const float *g, float *m, float *v, int64_t n, float 
  * the same steps in fp32, with a few 2^-23 of its own size a step.  A zero matrix gives zeros (NaN with eps = 0).
  * out may be x, with one layout for both; no other overlap.
  * 0 <= steps <= 32.  The iteration t -> a t + b t^3 + c t^5 has to keep [0, 1] within [-4, 4], with
- * |b t^2 + c t^4| below 31 (checked from the largest values of each step), which every useful triple does.
+ * |b t^2 + c t^4| below 31 (checked from the largest values of each step, each taken 2^-14 larger for the
+ * rounding), which every useful triple does.
  * vitk_muon_f32 (p, g, m share ld and stride, as arenas of one layout do):
  *   m = momentum*m + grad_scale*g;  u = nesterov ? grad_scale*g + momentum*m : m
  *   p = p * (1 - lr*weight_decay) - lr*update_scale * NS(u)

@@ -941,6 +941,32 @@ def test_newton_schulz_coefficients_next_to_a_cubic(a, b, c):
     assert taken(a, b, c, 5) == stays
 
 
+KEEPING = [COEF, (15 / 8, -10 / 8, 3 / 8), (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (3.0, -3.0, 1.0)]
+
+
+@pytest.mark.parametrize("a, b, c", [(5.0, -20.0, 16.0), (3.0, -4.0, 0.0), (3.0, -2.0, 0.0), (-5.0, 20.0, -16.0)])
+def test_newton_schulz_refuses_coefficients_that_rounding_carries_out_of_range(a, b, c):
+    """Exactly, each of these keeps [0, 1] (or what it makes of it) for ever; beside the end it grows by 9 to 25 a step."""
+    assert taken(a, b, c, 1)
+    assert not taken(a, b, c, 12)
+
+
+@pytest.mark.parametrize("coef", KEEPING)
+def test_newton_schulz_takes_convergent_coefficients_for_every_number_of_steps(coef):
+    assert all(taken(*coef, steps) for steps in range(33))
+
+
+@gpu
+@pytest.mark.parametrize("coef", KEEPING)
+@pytest.mark.parametrize("shape", [(96, 120), (150, 200)])
+def test_newton_schulz_of_one_direction_stays_in_range(K, shape, coef):
+    """The one singular value starts at 1 but for its rounding; in each of 32 steps it stays below 4."""
+    x = randn(rng(360), shape[0], 1) * randn(rng(361), 1, shape[1])
+    out = torch.empty_like(x)
+    K.newton_schulz(K.newton_schulz_args(x, out, steps=32, coefficients=coef, eps=0.0))
+    assert torch.isfinite(out).all() and torch.linalg.norm(out.double().cpu()) <= 4.0 * min(shape) ** 0.5
+
+
 # ---------------------------------------------------------------------------- the run together
 @gpu
 def test_all_of_them_captured_in_one_graph(K):

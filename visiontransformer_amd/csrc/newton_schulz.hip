@@ -939,10 +939,14 @@ bool size_ok(int64_t rows, int64_t cols, int64_t batch) {
 }
 
 // Does the iteration t -> a t + b t^3 + c t^5 stay where the fixed scales hold?  From |t| <= top, the largest values
-// of the odd polynomial, and of b q + c q^2 with q = t^2, are at the ends or where their derivatives vanish.
+// of the odd polynomial, and of b q + c q^2 with q = t^2, are at the ends or where their derivatives vanish.  Rounding
+// may carry a value over an end, and a polynomial that is steep there carries it on and out of the range within
+// a few steps (5 t - 20 t^3 + 16 t^5 multiplies what is above 1 by 25), so each step starts from 2^-14 more: sums of
+// 16384 terms are not off by as much.
+constexpr double SLACK = 1.0 + 1.0 / 16384;
 bool bounded(double a, double b, double c, int steps) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-  double top = 1.0;
+  double top = SLACK;
   for (int s = 0; s < steps; ++s) {
     // the roots of a + 3 b q + 5 c q^2 without a difference of neighbours (c may be tiny, or 0: then one of them is
     // an infinity, whose place the end takes, or no number)
@@ -957,7 +961,7 @@ bool bounded(double a, double b, double c, int steps) {
       next = std::max(next, std::fabs(std::sqrt(q) * (a + poly)));
     }
     if (!(next <= 4.0)) return false;
-    top = next;
+    top = next * SLACK;
   }
   return true;
 }
