@@ -424,11 +424,7 @@ int sdpa_bwd16_launch(const float *q, const float *k, const float *v, long long 
                       float *dq, float *dk, float *dv, long long ldg, hipStream_t st) {
   const size_t lds = F_TOTAL * sizeof(float);
   static std::atomic<unsigned long long> configured{0};  // raise the dynamic LDS limit once per device
-  if (vitk::first_use_on_device(&configured)) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_bwd16_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    VITK_REQUIRE(e == hipSuccess, "vitk_sdpa_bwd: cannot reserve %zu bytes of LDS: %s", lds, hipGetErrorString(e));
-  }
+  if (vitk::reserve_lds("vitk_sdpa_bwd", reinterpret_cast<const void *>(&sdpa_bwd16_kernel), lds, &configured)) return 1;
   Bwd16Params p;
   p.q = q; p.k = k; p.v = v; p.ld = (int)ld; p.o = o; p.dout = dout; p.ldo = (int)ldo; p.stats = stats;
   p.dq = dq; p.dk = dk; p.dv = dv; p.ldg = (int)ldg;

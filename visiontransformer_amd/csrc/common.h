@@ -43,8 +43,9 @@ int sdpa_bwd16_launch(const float *q, const float *k, const float *v, long long 
 // Compute units of the current device (hipDeviceProp_t::multiProcessorCount), cached per device;
 // 256 if the query fails.
 int cu_count();
-// first call with this flag word on the current device?
-bool first_use_on_device(std::atomic<unsigned long long> *done);
+// Raises a kernel's dynamic LDS limit on the current device; `done` keeps a bit per device on which that has been done.
+// Returns 0 or records the error.
+int reserve_lds(const char *who, const void *kernel, size_t bytes, std::atomic<unsigned long long> *done);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

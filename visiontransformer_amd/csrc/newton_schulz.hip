@@ -1010,12 +1010,8 @@ int run(const char *who, NsParams *p, float *workspace, size_t bytes, hipStream_
   if (form == FORM_ONE) {
     const int tr = (p->r + 31) / 32, tn = (p->n + 31) / 32;
     const size_t lds = (size_t)tr * 32 * (one_pitch(tn) + one_pitch(tr)) * 16;
-    if (vitk::first_use_on_device(&g_one_lds)) {
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(ns_one_kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               2 * ONE * one_pitch(ONE / 32) * 16);
-      VITK_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
-    }
+    if (vitk::reserve_lds(who, reinterpret_cast<const void *>(ns_one_kernel), 2 * ONE * one_pitch(ONE / 32) * 16, &g_one_lds))
+      return 1;
     hipLaunchKernelGGL(ns_one_kernel, dim3(p->batch), dim3(64 * ONE_WAVES), lds, st, *p);
     return vitk::check_launch(who);
   }

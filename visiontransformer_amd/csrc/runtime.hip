@@ -38,13 +38,17 @@ int cu_count() {
   return cached[dev];
 }
 
-// True the first time it is called with `done` on the current device (one bit per device), so that
-// per-function attributes are set on every device a process uses, not just the first.
-bool first_use_on_device(std::atomic<unsigned long long> *done) {
+// Once per device a process uses, not just the first.  The bit is set when the attribute is: a second thread that
+// comes before that sets it as well (the same value), and one that failed is tried again by the next call.
+int reserve_lds(const char *who, const void *kernel, size_t bytes, std::atomic<unsigned long long> *done) {
   int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return true;  // unknown device: set again (idempotent)
-  const unsigned long long bit = 1ull << dev;
-  return (done->fetch_or(bit) & bit) == 0;
+  const bool known = hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64;
+  const unsigned long long bit = known ? 1ull << dev : 0;
+  if (done->load(std::memory_order_acquire) & bit) return 0;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  VITK_REQUIRE(e == hipSuccess, "%s: cannot reserve %zu bytes of LDS: %s", who, bytes, hipGetErrorString(e));
+  done->fetch_or(bit, std::memory_order_release);
+  return 0;
 }
 
 }  // namespace vitk
