@@ -873,6 +873,41 @@ def test_bindings_refuse_wrong_tensors():
         vitk.muon_args(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), lr=0.1)
 
 
+def test_a_workspace_with_gaps_or_repeated_elements_is_refused():
+    from visiontransformer_amd import vitk
+
+    class OnTheDevice:  # a tensor's strides where there is no device
+        is_cuda = True
+
+        def __init__(self, t):
+            self.is_contiguous, self.numel, self.element_size, self.data_ptr = t.is_contiguous, t.numel, t.element_size, t.data_ptr
+
+    whole = torch.empty(64)
+    assert vitk._room(OnTheDevice(whole)) == (whole.data_ptr(), 256)
+    for t in (whole[:1].expand(1 << 20), whole[::2], whole.view(8, 8).t()):
+        with pytest.raises(vitk.VitkError, match="contiguous"):
+            vitk._room(OnTheDevice(t))
+    with pytest.raises(vitk.VitkError, match="CUDA"):
+        vitk._room(whole)
+
+
+@gpu
+def test_the_bindings_refuse_a_repeated_workspace(K):
+    g = rng(6)
+    one = torch.zeros(1, device="cuda").expand(1 << 24)
+    q, k = randn(g, 1, 1, 1, 64), randn(g, 1, 20000, 1, 64)
+    with pytest.raises(K.VitkError, match="contiguous"):
+        K.cross_sdpa_args(q, k, k, torch.empty_like(q), workspace=one)
+    w = randn(g, 200, 200)
+    with pytest.raises(K.VitkError, match="contiguous"):
+        K.newton_schulz_args(w, torch.empty_like(w), workspace=one)
+    with pytest.raises(K.VitkError, match="contiguous"):
+        K.muon_args(w, randn(g, 200, 200), randn(g, 200, 200), lr=0.1, workspace=one)
+    index = torch.zeros(20000, dtype=torch.int32, device="cuda")
+    with pytest.raises(K.VitkError, match="contiguous"):
+        K.embedding_bwd(randn(g, 20000, 4), index, torch.empty(3000, 4, device="cuda"), workspace=one)
+
+
 @gpu
 def test_the_bindings_refuse_another_device(K):
     g = rng(5)

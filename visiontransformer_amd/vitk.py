@@ -294,6 +294,12 @@ def _f32(name, t, shape=None):
     _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {shape}")
 
 
+def _room(workspace):
+    """Address and bytes of a workspace; a tensor with gaps or repeated elements (`expand`) has another extent."""
+    _need(workspace.is_cuda and workspace.is_contiguous(), "workspace: a contiguous CUDA tensor is needed")
+    return ptr(workspace), workspace.numel() * workspace.element_size()
+
+
 def _head_rows(name, t, shape):
     """Pitch of a [B, N, heads, dh] tensor whose rows (b, n) lie one after the other, heads packed."""
     _f32(name, t, shape)
@@ -344,7 +350,7 @@ def cross_sdpa_args(q, k, v, out, *, key_len=None, scale=None, stats=None, dout=
         import torch
         workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=q.device)
     if workspace is not None:
-        a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
+        a.workspace, a.workspace_bytes = _room(workspace)
     a.keep = (q, k, v, out, key_len, stats, dout, dq, dk, dv, workspace)
     a.device = _one_device(*a.keep)
     return a
@@ -385,9 +391,9 @@ def embedding_bwd(dout, index, dtable, *, scale=1.0, accumulate=False, workspace
         need = dll().vitk_embedding_bwd_workspace_bytes(rows, V, D)
         _need(need == 0 or st is None, "embedding_bwd: another stream than the current one needs a workspace of its own")
         workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=dout.device)
+    room = _room(workspace)
     current = stream(_one_device(dout, index, dtable, workspace))
-    check(dll().vitk_embedding_bwd(ptr(dout), ptr(index), rows, V, D, scale, int(bool(accumulate)), ptr(dtable),
-                                   ptr(workspace), workspace.numel() * workspace.element_size(),
+    check(dll().vitk_embedding_bwd(ptr(dout), ptr(index), rows, V, D, scale, int(bool(accumulate)), ptr(dtable), *room,
                                    current if st is None else st))
     return workspace
 
@@ -438,7 +444,7 @@ def _with_workspace(a, need, workspace, like, keep):
         import torch
         workspace = torch.empty((need + 3) // 4, dtype=torch.float32, device=like.device)
     if workspace is not None:
-        a.workspace, a.workspace_bytes = ptr(workspace), workspace.numel() * workspace.element_size()
+        a.workspace, a.workspace_bytes = _room(workspace)
     a.keep = keep + (workspace,)
     a.device = _one_device(*a.keep)
     return a
