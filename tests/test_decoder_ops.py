@@ -506,6 +506,18 @@ def test_embedding_unaligned_and_empty(K):
 
 
 @gpu
+def test_embedding_lookup_of_more_rows_than_one_launch_takes(K):
+    rows, V = 2 ** 29 + 5, 1000  # eight rows to a workgroup of 64 threads: 2^32 threads and a few
+    table = randn(rng(203), V, 1)
+    index = torch.arange(rows, dtype=torch.int32, device="cuda").remainder_(V)
+    out = torch.full((rows, 1), 7.0, device="cuda")
+    K.embedding_fwd(table, index, out, scale=0.5)
+    whole = rows // V * V
+    assert (out[:whole].view(-1, V) == 0.5 * table[:, 0]).all()
+    assert torch.equal(out[whole:, 0], 0.5 * table[:rows - whole, 0])
+
+
+@gpu
 def test_embedding_gradient_captured_and_replayed(K):
     g = rng(202)
     V, D, rows = 3000, 96, 6000
@@ -774,6 +786,39 @@ def test_cross_attention_refuses(change, message):
     for fn in (d.vitk_cross_sdpa_fwd, d.vitk_cross_sdpa_bwd):
         assert fn(C.byref(_xargs(vitk, **change)), None) != 0
         assert message in d.vitk_last_error().decode()
+
+
+@pytest.mark.parametrize("change, forward, backward", [
+    (dict(B=2 ** 21, H=8, Hkv=8, Nq=1, Nk=5), True, True),  # 2^24 workgroups of four waves
+    (dict(B=2 ** 20, H=15, Hkv=15, Nq=1, Nk=5), False, False),
+    (dict(B=2 ** 20, H=8, Hkv=8, Nq=40, Nk=70), False, True),  # 2^23 of eight waves
+    (dict(B=2 ** 21, H=8, Hkv=8, Nq=40, Nk=70), True, True),
+    (dict(B=1, H=1, Hkv=1, Nq=2 ** 30, Nk=5), True, False)])  # 2^24 blocks of 64 rows
+def test_cross_attention_refuses_more_threads_than_a_launch_has(change, forward, backward):
+    """Before anything is launched (what is not refused fails here only for want of a device)."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    a = _xargs(vitk, dh=1, workspace_bytes=1 << 62, **{"ld_" + n: 16 for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")},
+               **change)
+    for fn, refused in ((d.vitk_cross_sdpa_fwd, forward), (d.vitk_cross_sdpa_bwd, backward)):
+        assert fn(C.byref(a), None) != 0
+        assert ("too many rows" in d.vitk_last_error().decode()) == refused, d.vitk_last_error()
+
+
+@pytest.mark.parametrize("batch, cols, refused", [(2 ** 22, 16, True), (2 ** 22 - 1, 16, False), (2 ** 18, 130, True),
+                                                  (2 ** 18 - 1, 130, False)])
+def test_newton_schulz_refuses_more_threads_than_a_launch_has(batch, cols, refused):
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    change = dict(batch=batch, rows=16, cols=cols, steps=1, workspace_bytes=1 << 62)
+    for fn, a in ((d.vitk_newton_schulz_f32, _nargs(vitk, vitk.NewtonSchulzArgs, **change)),
+                  (d.vitk_muon_f32, _nargs(vitk, vitk.MuonArgs, **change))):
+        assert fn(C.byref(a), None) != 0
+        assert ("too many matrices" in d.vitk_last_error().decode()) == refused, d.vitk_last_error()
 
 
 @pytest.mark.parametrize("change, message", [

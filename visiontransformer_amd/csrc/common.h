@@ -52,6 +52,9 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 constexpr int kWave = 64;
 constexpr int kMaxGridBlocks = 2048;  // 256 CUs x 8 resident blocks; larger problems grid-stride
 
+// A launch has fewer than 2^32 threads in a dimension.
+inline bool fits_one_launch(long long blocks, int threads) { return blocks < (1ll << 32) / threads; }
+
 inline int grid_for(int64_t work_items, int per_block) {
   int64_t b = (work_items + per_block - 1) / per_block;
   if (b < 1) b = 1;

@@ -596,7 +596,12 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
   VITK_REQUIRE(need == 0 || vitk::aligned16(a->workspace), "vitk_cross_sdpa_fwd: workspace is not 16-byte aligned");
   p.part = a->workspace;
   const long long wgs = (long long)p.B * p.Hkv * p.blocks * p.splits;
-  VITK_REQUIRE(wgs < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
+  const long long rows = (long long)p.B * p.H * p.Nq;  // of the join
+  const int lp = p.splits > JOIN_FEW ? 64 : p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32;
+  const long long blocks = (rows * lp + 255) / 256;
+  VITK_REQUIRE(vitk::fits_one_launch(wgs, 64 * plan.block.waves) &&
+                   (p.splits == 1 || (p.splits > 64 ? vitk::fits_one_launch(rows, 64 * JOIN_WAVES) : vitk::fits_one_launch(blocks, 256))),
+               "vitk_cross_sdpa_fwd: too many rows for one launch");
   hipStream_t st = vitk::as_stream(stream);
   const unsigned grid = (unsigned)wgs;
   if (plan.block.groups == 0) {
@@ -616,11 +621,8 @@ extern "C" int vitk_cross_sdpa_fwd(const vitk_cross_sdpa_args *a, vitk_stream_t 
     launch_fwd<128>(p, plan.block, grid, st);
   }
   if (p.splits > 1) {
-    const int lp = p.splits > JOIN_FEW ? 64 : p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32;
-    const long long blocks = ((long long)p.B * p.H * p.Nq * lp + 255) / 256;
-    VITK_REQUIRE(blocks < (1ll << 31), "vitk_cross_sdpa_fwd: too many rows for one launch");
     if (p.splits > 64)
-      hipLaunchKernelGGL(cross_join_many_kernel<JOIN_WAVES>, dim3((unsigned)(p.B * p.H * p.Nq)), dim3(64 * JOIN_WAVES), 0, st, p);
+      hipLaunchKernelGGL(cross_join_many_kernel<JOIN_WAVES>, dim3((unsigned)rows), dim3(64 * JOIN_WAVES), 0, st, p);
     else if (lp == 64)
       hipLaunchKernelGGL(cross_join_many_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     else if (lp == 8)

@@ -533,7 +533,9 @@ template <int DH>
 int launch(Params p, const Plan &n, hipStream_t st) {
   const long long heads = (long long)p.B * p.Hkv;
   const long long qw = heads * n.rows.blocks * n.rows.splits, kw = heads * n.keys.blocks * n.keys.splits;
-  VITK_REQUIRE(qw < (1ll << 31) && kw < (1ll << 31), "vitk_cross_sdpa_bwd: too many rows for one launch");
+  VITK_REQUIRE((n.few_keys || vitk::fits_one_launch(qw, DH > 96 ? 512 : 64 * n.rows.block.waves)) &&
+                   vitk::fits_one_launch(kw, n.few_keys ? 256 : 64 * n.keys.block.waves),
+               "vitk_cross_sdpa_bwd: too many rows for one launch");
   if (p.Nq > 0 && !n.few_keys) {
     p.blocks = n.rows.blocks, p.splits = n.rows.splits, p.chunk = n.rows.chunk;
     launch_dq<DH>(p, n.rows.block, (unsigned)qw, st);

@@ -1009,6 +1009,7 @@ int run(const char *who, NsParams *p, float *workspace, size_t bytes, hipStream_
   const dim3 block(256);
   if (form == FORM_ONE) {
     const int tr = (p->r + 31) / 32, tn = (p->n + 31) / 32;
+    VITK_REQUIRE(vitk::fits_one_launch(p->batch, 64 * ONE_WAVES), "%s: too many matrices for one launch", who);
     const size_t lds = (size_t)tr * 32 * (one_pitch(tn) + one_pitch(tr)) * 16;
     if (vitk::reserve_lds(who, reinterpret_cast<const void *>(ns_one_kernel), 2 * ONE * one_pitch(ONE / 32) * 16, &g_one_lds))
       return 1;
@@ -1020,7 +1021,7 @@ int run(const char *who, NsParams *p, float *workspace, size_t bytes, hipStream_
   VITK_REQUIRE(vitk::aligned16(workspace), "%s: workspace is not 16-byte aligned", who);
   plan(p, workspace, &form);
   const long long yb = (long long)p->batch * (p->rp / 64) * (p->np / 64);
-  VITK_REQUIRE(4 * yb < (1ll << 31) - 8 && p->batch * (long long)PARTS < (1ll << 31),
+  VITK_REQUIRE(vitk::fits_one_launch(yb + 8, 256) && vitk::fits_one_launch(p->batch * (long long)PARTS, 256),
                "%s: too many matrices for one launch", who);
   hipLaunchKernelGGL(ns_norm_kernel, dim3(p->batch * PARTS), block, 0, st, *p);
   hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)yb), block, 0, st, *p, p->steps == 0 ? 1 : 0);

@@ -513,15 +513,15 @@ extern "C" int vitk_embedding_fwd(const float *table, int64_t V, const int32_t *
   hipStream_t st = vitk::as_stream(stream);
   const long long threads = vec ? D / 4 : D, groups = (rows + ROWS - 1) / ROWS;
   const unsigned tpb = threads_for(threads);
-  VITK_REQUIRE(groups < (1ll << 31) && D <= kMaxWidth, "vitk_embedding_fwd: %lld rows of %lld in one launch",
-               (long long)rows, (long long)D);
-  const dim3 grid((unsigned)groups, (unsigned)((threads + tpb - 1) / tpb));
-  if (vec)
-    hipLaunchKernelGGL(embedding_fwd_kernel<4>, grid, dim3(tpb), 0, st, table, (long long)V, index, (long long)rows,
-                       (long long)D, scale, out);
-  else
-    hipLaunchKernelGGL(embedding_fwd_kernel<1>, grid, dim3(tpb), 0, st, table, (long long)V, index, (long long)rows,
-                       (long long)D, scale, out);
+  VITK_REQUIRE(rows <= INT64_MAX - ROWS && D <= kMaxWidth, "vitk_embedding_fwd: %lld rows of %lld", (long long)rows,
+               (long long)D);
+  auto kernel = vec ? embedding_fwd_kernel<4> : embedding_fwd_kernel<1>;
+  const long long most = (1ll << 32) / tpb - 1;  // groups of one launch, which has fewer than 2^32 threads in a dimension
+  for (long long g0 = 0; g0 < groups; g0 += most) {
+    const dim3 grid((unsigned)std::min(most, groups - g0), (unsigned)((threads + tpb - 1) / tpb));
+    hipLaunchKernelGGL(kernel, grid, dim3(tpb), 0, st, table, (long long)V, index + g0 * ROWS, (long long)rows - g0 * ROWS,
+                       (long long)D, scale, out + g0 * ROWS * D);
+  }
   return vitk::check_launch("vitk_embedding_fwd");
 }
 
@@ -563,6 +563,8 @@ extern "C" int vitk_embedding_bwd(const float *dout, const int32_t *index, int64
                "vitk_embedding_bwd: workspace of %zu bytes needed, %zu given", (size_t)p.total * 4,
                workspace ? workspace_bytes : 0);
   VITK_REQUIRE(vitk::aligned16(workspace), "vitk_embedding_bwd: workspace is not 16-byte aligned");
+  VITK_REQUIRE(vitk::fits_one_launch(p.chunks[0], (int)threads_for(vec ? D / 4 : D)),
+               "vitk_embedding_bwd: %lld tokens of %lld in one launch", (long long)rows, (long long)D);
   int32_t *iw = reinterpret_cast<int32_t *>(workspace);
   Sort s = {};
   s.n = (int)rows, s.V = (int)V, s.chunk = p.chunk, s.blocks = p.blocks, s.hist = iw + p.hist;
