@@ -486,6 +486,34 @@ def test_embedding_lookup_and_gradient(K, name):
 
 
 @gpu
+@pytest.mark.parametrize("V, D, rows, kind", [
+    (2 ** 24 + 3, 1, 700001, "uniform"),     # four digits, every sort block with its largest share of tokens
+    (2 ** 24 + 3, 1, 9000, "outside"),
+    (100, 2, 1200007, "rank"),               # three levels of sums, runs over many chunks of each
+    (3, 4, 2300000, "same"),
+    (70000, 3, 1100000, "padded"),
+    (255, 1, 1048577, "uniform"),            # one digit, and the padding's key behind it
+    (256, 1, 1048576, "padded"),
+])
+def test_embedding_gradient_of_many_tokens(K, V, D, rows, kind):
+    g = rng(204)
+    index, dout = tokens(kind, V, rows, 7), randn(g, rows, D)
+    there = (index >= 0) & (index < V)
+    dout[~there] = float("nan")
+    dt = torch.full((V, D), float("nan"), device="cuda")
+    K.embedding_bwd(dout, index, dt, scale=0.5)
+    there, safe = there.cpu(), torch.where(there, index, 0).long().cpu()
+    clean = torch.where(there[:, None], dout.cpu(), 0.0).double()
+    want = torch.zeros(V, D, dtype=torch.float64).index_add_(0, safe, clean) * 0.5
+    mag = torch.zeros(V, D, dtype=torch.float64).index_add_(0, safe, clean.abs()) * 0.5
+    count = torch.zeros(V, dtype=torch.float64).index_add_(0, safe, there.double())
+    within(dt, want, (LAM * count.sqrt()[:, None] + 2) * U * mag, "dtable")
+    again = torch.full((V, D), float("nan"), device="cuda")
+    K.embedding_bwd(dout, index, again, scale=0.5)
+    assert torch.equal(dt, again)
+
+
+@gpu
 def test_embedding_unaligned_and_empty(K):
     g = rng(201)
     V, D, rows = 50, 64, 200
@@ -739,6 +767,77 @@ def test_muon_steps(K, nesterov, shape):
             e = ns_tolerance(u[i].astype(np.float32), o, 5, COEF, 1e-7) + 12 * U * 485
             err = np.linalg.norm(p[i].double().cpu().numpy() - p64[i])
             assert err <= (step + 1) * (lr * us * e + 4 * U * np.linalg.norm(p64[i])), (step, i, err)
+
+
+MUON = {
+    # CUs to plan for, batch, rows, cols, floats between rows, between matrices, in front
+    "one": (0, 3, 33, 128, 0, 0, 0),
+    "one_tall": (0, 2, 128, 97, 0, 0, 0),
+    "one_odd": (0, 2, 70, 90, 0, 0, 0),
+    "one_padded": (0, 2, 64, 96, 4, 8, 4),
+    "one_padded_odd": (0, 2, 96, 64, 3, 5, 1),
+    "one_row": (0, 2, 1, 100, 0, 0, 1),
+    "small": (0, 2, 150, 200, 0, 0, 0),
+    "small_padded": (0, 2, 150, 200, 4, 4, 0),
+    "small_unaligned": (0, 1, 200, 131, 0, 0, 1),
+    "small_tall_padded_odd": (0, 2, 300, 130, 1, 2, 3),
+    "64": (10, 1, 200, 300, 0, 0, 0),
+    "64_tall": (10, 1, 300, 200, 0, 0, 0),
+    "64_padded": (20, 2, 190, 300, 4, 12, 4),
+    "64_tall_odd": (20, 2, 301, 190, 2, 1, 1),
+    "128": (4, 1, 200, 300, 0, 0, 0),
+    "128_tall": (4, 1, 300, 200, 0, 0, 0),
+    "128_padded": (8, 2, 200, 300, 4, 0, 0),
+    "128_odd": (8, 2, 129, 259, 0, 0, 1),
+    "128_tall_odd": (8, 2, 259, 130, 3, 7, 2),
+}
+
+
+@gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("name", list(MUON))
+def test_muon_in_every_form_and_layout(K, name, nesterov):
+    """p and m of three steps, and nothing else of their buffers: what lies between rows and matrices stays as it was."""
+    cus, batch, r, c, pad, gap, front = MUON[name]
+    ld, g = c + pad, rng(370 + list(MUON).index(name))
+    stride = r * ld + gap
+    size = front + batch * stride
+
+    def matrices(flat):
+        return flat.as_strided((batch, r, c), (stride, ld, 1), front)
+
+    buffers = [randn(g, size) * s for s in (0.02, 1e-2, 3e-3)]
+    p, grad, m = (matrices(b) for b in buffers)
+    p64, m64 = p.double().cpu().numpy(), m.double().cpu().numpy()
+    lr, mu, wd, us, gs = 0.02, 0.9, 0.2, 1.5, 0.25
+    outside = torch.ones(size, dtype=torch.bool, device="cuda")
+    matrices(outside)[:] = False
+    kept = [b[outside].clone() for b in buffers]
+    K.planning_cu_count(cus)
+    try:
+        args = K.muon_args(p, grad, m, lr=lr, momentum=mu, weight_decay=wd, update_scale=us, grad_scale=gs, nesterov=nesterov)
+        for step in range(3):
+            grad.copy_(randn(g, batch, r, c) * 1e-2)
+            before = grad.clone()
+            K.muon(args)
+            assert torch.equal(grad, before)
+            gd = grad.double().cpu().numpy() * gs
+            m64 = mu * m64 + gd
+            # three roundings of at most u of each term, a step
+            tol_m = (step + 1) * 4 * U * (np.abs(m64) + np.abs(gd) + 1e-2)
+            assert (np.abs(m.double().cpu().numpy() - m64) <= tol_m).all(), step
+            u = gd + mu * m64 if nesterov else m64
+            for i in range(batch):
+                o = newton_schulz(u[i].astype(np.float32), 5, COEF, 1e-7, np.float64)
+                p64[i] = p64[i] * (1 - lr * wd) - lr * us * o
+                # the direction: bound of the products plus what 12 u in u becomes (a factor of at most 3.4445^5)
+                e = ns_tolerance(u[i].astype(np.float32), o, 5, COEF, 1e-7) + 12 * U * 485
+                err = np.linalg.norm(p[i].double().cpu().numpy() - p64[i])
+                assert err <= (step + 1) * (lr * us * e + 4 * U * np.linalg.norm(p64[i])), (step, i, err)
+    finally:
+        K.planning_cu_count(0)
+    for b, k in zip(buffers, kept):
+        assert torch.equal(b[outside], k)
 
 
 @gpu
