@@ -308,9 +308,11 @@ int vitk_sdpa_row_bwd(const float *q, int64_t ld_q, const float *k, const float 
  * stats (optional in the forward, required by the backward; [B*H][Nq][2]): {row maximum of the
  * scaled scores times log2(e), row sum of exp(score - maximum)}.
  * Any Nq, Nk >= 0, 1 <= dh <= 128, any alignment.  Products are formed to fp32 accuracy from three
- * bf16 parts of each operand: finite numbers below 3.38e38 (an infinity among them gives NaN), and
- * scores that are finite in fp32;
- * numbers below 2^-100 keep fewer than 24 bits.  Outputs must not overlap inputs or each other.  The sum over
+ * bf16 parts of each operand: finite numbers below 3.38e38, and scores that are finite in fp32;
+ * numbers below 2^-100 keep fewer than 24 bits.  What is formed from an infinity or NaN is not defined beyond this:
+ * a NaN gives NaN; an infinity gives NaN, or what fp32 arithmetic makes of it (few rows, whose products
+ * are plain fp32: an infinite value in v an infinity, a score of -inf a weight of 0); results that are not formed
+ * from it keep their bits.  Outputs must not overlap inputs or each other.  The sum over
  * a row's keys may be split over workgroups, a rule on the sizes; every result has a fixed order of sums.
  * workspace: vitk_cross_sdpa_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments (0 =
  * none needed); one call at a time may use it (two captured graphs replayed at once need two). */

@@ -325,6 +325,52 @@ def test_cross_attention_extreme_scores(K, amplitude):
 
 
 @gpu
+@pytest.mark.parametrize("Nq, Nk, dh", [(1, 197, 64), (2, 40, 128), (40, 197, 64), (150, 500, 96), (70, 50, 32)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_cross_attention_keeps_what_is_not_finite_to_its_own(K, Nq, Nk, dh, value):
+    """An infinity or NaN reaches the results that are formed from it and no others: those keep their bits."""
+    g, B, H, Hkv = rng(380), 2, 4, 2
+    q, k, v, dout = randn(g, B, Nq, H, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nk, Hkv, dh), randn(g, B, Nq, H, dh)
+    inputs = dict(q=q, k=k, v=v, dout=dout)
+    names = ("out", "dq", "dk", "dv")
+
+    def run():
+        o, dq, dk, dv = (torch.full_like(t, 7.0) for t in (q, q, k, v))
+        args = K.cross_sdpa_args(q, k, v, o, stats=torch.empty(B * H, Nq, 2, device="cuda"), dout=dout, dq=dq, dk=dk, dv=dv)
+        K.cross_sdpa_fwd(args)
+        K.cross_sdpa_bwd(args)
+        return dict(zip(names, (o, dq, dk, dv)))
+
+    clean = run()
+    row, key, col = Nq - 1, Nk // 2, dh // 2
+    all_ = slice(None)
+    # the element of each input, and what is formed from it: (batch, token, heads, column) of each result
+    head = dict(q=(1, row, 3, col), dout=(1, row, 3, col), k=(1, key, 1, col), v=(1, key, 1, col))
+    reach = {
+        "q": dict(out=(1, row, 3), dq=(1, row, 3), dk=(1, all_, 1), dv=(1, all_, 1)),
+        "dout": dict(dq=(1, row, 3), dk=(1, all_, 1), dv=(1, all_, 1)),
+        "k": dict(out=(1, all_, slice(2, 4)), dq=(1, all_, slice(2, 4)), dk=(1, all_, 1), dv=(1, all_, 1)),
+        "v": dict(out=(1, all_, slice(2, 4), col), dq=(1, all_, slice(2, 4)), dk=(1, all_, 1)),
+    }
+    for name, x in inputs.items():
+        old = x[head[name]].clone()
+        x[head[name]] = value
+        got = run()
+        x[head[name]] = old
+        for n in names:
+            same = torch.ones_like(got[n], dtype=torch.bool)
+            if n in reach[name]:
+                same[reach[name][n]] = False
+            assert torch.equal(got[n][same], clean[n][same]), (name, n)
+        if value != value:  # NaN stays NaN
+            assert name not in ("q", "k") or torch.isnan(got["out"][1, row, 3]).all(), name
+            assert name not in ("k", "v") or torch.isnan(got["out"][1, :, 2:4, col]).all(), name
+            assert torch.isnan(got["dq"][1, row, 3]).all(), name
+        if name == "v" and abs(value) == float("inf"):  # every probability is above 0 here
+            assert not torch.isfinite(got["out"][1, :, 2:4, col]).any()
+
+
+@gpu
 def test_cross_attention_gradients_against_differences(K):
     """Central differences of sum(out * dout) in float64 of the definition, at single entries."""
     g = rng(8)
