@@ -370,6 +370,59 @@ def test_cross_attention_keeps_what_is_not_finite_to_its_own(K, Nq, Nk, dh, valu
             assert not torch.isfinite(got["out"][1, :, 2:4, col]).any()
 
 
+def check_attention(K, q, k, v, lens, scale, dout, like=torch.empty_like):
+    """Forward, statistics and gradients of one call against attention64."""
+    B, Nq, H, dh = q.shape
+    out, dq, dk, dv = (like(t).fill_(7.0) for t in (q, q, k, v))
+    stats = torch.empty(B * H, Nq, 2, device="cuda")
+    klen = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    args = K.cross_sdpa_args(q, k, v, out, key_len=klen, scale=scale, stats=stats, dout=dout, dq=dq, dk=dk, dv=dv)
+    K.cross_sdpa_fwd(args)
+    K.cross_sdpa_bwd(args)
+    want, tol, _ = attention64(q, k, v, lens, scale, dout)
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        within(got, want[name], tol[name] + 1e-30, name)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, -2.0])
+@pytest.mark.parametrize("Nq, Nk, dh", [(1, 197, 64), (37, 40, 64), (40, 150, 96), (5, 2100, 32)])
+def test_cross_attention_scales_of_any_sign(K, scale, Nq, Nk, dh):
+    g = rng(390)
+    q, dout = randn(g, 2, Nq, 4, dh), randn(g, 2, Nq, 4, dh)
+    k, v = randn(g, 2, Nk, 2, dh) * 0.5, randn(g, 2, Nk, 2, dh)
+    check_attention(K, q, k, v, [Nk, Nk // 2], scale, dout)
+
+
+@gpu
+@pytest.mark.parametrize("Nq, Nk", [(1, 90), (20, 90), (20, 40), (130, 70)])
+def test_cross_attention_ragged_batches_of_more_than_a_wave(K, Nq, Nk):
+    g, B = rng(391), 70
+    lens = [(17 * b) % (Nk + 1) for b in range(B)]
+    q, dout, k, v = randn(g, B, Nq, 2, 16), randn(g, B, Nq, 2, 16), randn(g, B, Nk, 1, 16), randn(g, B, Nk, 1, 16)
+    check_attention(K, q, k, v, lens, 0.25, dout)
+
+
+@gpu
+@pytest.mark.parametrize("Nq, Nk, dh", [(1, 1100, 64), (1100, 70, 32), (33, 1100, 64), (1100, 9, 64)])
+def test_cross_attention_offsets_past_32_bits(K, Nq, Nk, dh):
+    """Rows 2^21 floats apart: the last ones lie more than 2^31 elements behind the first."""
+    g, H, ld = rng(392), 2, 2 ** 21
+    need = max(Nq, Nk) * ld
+    assert need > 2 ** 31
+    room = torch.empty(need, device="cuda")
+    place = [0]
+
+    def far(t):  # rows of all tensors lie side by side
+        B, N, heads, d = t.shape
+        r = room.as_strided((B, N, heads, d), (N * ld, ld, d, 1), place[0])
+        place[0] += heads * d
+        return r.copy_(t)
+
+    q, dout, k, v = (far(randn(g, 1, n, H, dh)) for n in (Nq, Nq, Nk, Nk))
+    check_attention(K, q, k, v, None, 0.2, dout, like=lambda t: far(torch.zeros(t.shape, device="cuda")))
+
+
 @gpu
 def test_cross_attention_gradients_against_differences(K):
     """Central differences of sum(out * dout) in float64 of the definition, at single entries."""
@@ -557,6 +610,30 @@ def test_embedding_gradient_of_many_tokens(K, V, D, rows, kind):
     again = torch.full((V, D), float("nan"), device="cuda")
     K.embedding_bwd(dout, index, again, scale=0.5)
     assert torch.equal(dt, again)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [300, 5000, 20000])
+def test_embedding_offsets_past_32_bits(K, rows):
+    V, D = 2 ** 21 + 11, 1025
+    index = torch.randint(V - 900, V, (rows,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    index[::5] = torch.arange(len(index[::5]), dtype=torch.int32)
+    table, index = torch.empty(V, D, device="cuda"), index.cuda()
+    used = index.long().unique()
+    table[used] = randn(rng(205), len(used), D)
+    out = torch.empty(rows, D, device="cuda")
+    K.embedding_fwd(table, index, out, scale=2.0)
+    assert torch.equal(out, table[index.long()] * 2.0)
+    dout = randn(rng(206), rows, D)
+    K.embedding_bwd(dout, index, table, scale=0.5)  # into the same room
+    want = torch.zeros(len(used), D, dtype=torch.float64, device="cuda")
+    at = torch.searchsorted(used, index.long())
+    want.index_add_(0, at, dout.double())
+    mag = torch.zeros_like(want).index_add_(0, at, dout.double().abs())
+    count = torch.bincount(at, minlength=len(used)).double()
+    within(table[used], 0.5 * want, 0.5 * (LAM * count.sqrt()[:, None] + 2) * U * mag, "dtable")
+    table[used] = 0
+    assert not table.view(-1)[: 2 ** 31].any() and not table.view(-1)[2 ** 31:].any()
 
 
 @gpu
@@ -884,6 +961,26 @@ def test_muon_in_every_form_and_layout(K, name, nesterov):
         K.planning_cu_count(0)
     for b, k in zip(buffers, kept):
         assert torch.equal(b[outside], k)
+
+
+@gpu
+@pytest.mark.parametrize("r, c", [(60, 100), (140, 100), (300, 500)])
+def test_muon_offsets_past_32_bits(K, r, c):
+    """Rows and matrices far apart: the second matrix starts more than 2^31 elements behind the first."""
+    ld, stride, g = 2 ** 20, 2 ** 31 + 64, rng(395)
+    room = torch.empty(stride + r * ld, device="cuda")
+    p, grad, m = (room.as_strided((2, r, c), (stride, ld, 1), i * 1024).copy_(randn(g, 2, r, c) * x)
+                  for i, x in enumerate((0.02, 1e-2, 3e-3)))
+    near = [t.contiguous() for t in (p, grad, m)]
+    for t in ((p, grad, m), near):
+        K.muon(K.muon_args(*t, lr=0.1, weight_decay=0.1))
+    assert torch.equal(m, near[2])
+    # a row pitch may choose other loads, not other sums
+    assert (p - near[0]).abs().max() <= 4 * U
+    out = torch.empty_like(near[1])
+    K.newton_schulz(K.newton_schulz_args(near[1], out))
+    K.newton_schulz(K.newton_schulz_args(grad, p))
+    assert torch.equal(p, out)
 
 
 @gpu
