@@ -468,8 +468,8 @@ __global__ __launch_bounds__(64 * NW, 4) void ns_tile_kernel(const NsParams p, i
   auto step = [&](int s, f16x8 (&x)[LOADS], f16x8 (&y)[LOADS]) {
     multiply(s, 0);
     put((s + 1) & 1, x, y);
-    multiply(s, 1);
     fetch(s + 1 + DIST, x, y);
+    multiply(s, 1);
     __syncthreads();
   };
   int s0 = 0;
