@@ -1167,7 +1167,7 @@ def test_a_workspace_with_gaps_or_repeated_elements_is_refused():
         is_cuda = True
 
         def __init__(self, t):
-            self.is_contiguous, self.numel, self.element_size, self.data_ptr = t.is_contiguous, t.numel, t.element_size, t.data_ptr
+            self.is_contiguous, self.nbytes, self.data_ptr = t.is_contiguous, t.nbytes, t.data_ptr
 
     whole = torch.empty(64)
     assert vitk._room(OnTheDevice(whole)) == (whole.data_ptr(), 256)

@@ -296,8 +296,9 @@ def _f32(name, t, shape=None):
 
 def _room(workspace):
     """Address and bytes of a workspace; a tensor with gaps or repeated elements (`expand`) has another extent."""
-    _need(workspace.is_cuda and workspace.is_contiguous(), "workspace: a contiguous CUDA tensor is needed")
-    return ptr(workspace), workspace.numel() * workspace.element_size()
+    if not (workspace.is_cuda and workspace.is_contiguous()):
+        raise VitkError("workspace: a contiguous CUDA tensor is needed")
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def _head_rows(name, t, shape):
