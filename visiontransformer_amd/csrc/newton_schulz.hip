@@ -29,8 +29,8 @@
 //     workgroup, operands straight from memory (every load of a wave in flight: a few round trips);
 //   otherwise: 64 x 64 or 128 x 128 tiles staged through LDS.
 // y y^T and g g are symmetric: only tiles on and below the diagonal are computed, and mirrored.
-// Twelve 768 x 2304 (272 GFLOP): 1050 us, matrix cores: y y^T 66 us, the polynomial 29, the step of y 118, which is 860,
-// 650 and 830 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 26 us, 1000 x 257:
+// Twelve 768 x 2304 (272 GFLOP): 1075 - 1110 us, matrix cores: y y^T 60 us, the polynomial 27, the step of y 113, which is
+// 950, 710 and 870 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 27 us, 1000 x 257:
 // 96 us, the latency of 15 dependent products.
 #include "common.h"
 
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(64 * NW, 4) void ns_tile_kernel(const NsParams p, i
 }
 
 // 32 x 32 tiles, the contraction dealt to NW waves, operands straight from memory: the step of y of 257 x 1000 takes
-// 7.7 us (288 workgroups), mostly round trips to memory.
+// 7.5 us (288 workgroups), mostly round trips to memory.
 template <int MODE, int NW>
 __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int flip, int ti) {
   constexpr bool LOWER = MODE <= POLY, TR = MODE >= APPLY;
@@ -639,7 +639,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const NsParams p, int
 
 // The symmetric products where 32 x 32 tiles leave half of the CUs without work: 16 x 16 tiles, half as much for each to read.
 // The contraction is dealt to the waves, 32 k a step, a line of planes for 16 rows; the first wave adds the sums.
-// 257 x 1000: y y^T 6.7 us, the polynomial 4.4 (32 x 32 tiles: 10.8 and 6.2).
+// 257 x 1000: y y^T 6.6 us, the polynomial 4.7 (32 x 32 tiles: 10.8 and 6.2).
 template <int MODE, int NW>
 __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int flip, int ti) {
   static_assert(MODE <= POLY, "the symmetric products");
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(64 * NW) void ns_lower_kernel(const NsParams p, int
 // Both sides <= 128: everything in one launch.  Sixteen waves, one 32 x 32 block of g and of y each; the planes of
 // y and of g, then b g + c g g, are in LDS (70 KiB each), what a wave adds to its products in registers.  All
 // blocks of g are computed: writing a block's mirror image, two bytes at a time, takes longer than its product.
-// 96 x 96, five steps: 26 us, 1.3 a product: operands from LDS 0.7, matrix cores 0.7, one after the other.
+// 96 x 96, five steps: 27 us, 1.4 a product: operands from LDS 0.7, matrix cores 0.7, one after the other.
 // A row of planes takes 3 mod 16 units of 16 bytes, so that 16 rows of one unit, and mostly four rows of four
 // neighbouring ones, are on different banks.
 constexpr int ONE_WAVES = 16;
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(64 * ONE_WAVES) void ns_one_kernel(const NsParams p
   float y[16];  // behind the norm: times kY
   double s = 0.0;
   // Element e of the lane: row 32 yi + c, column 32 yj + 4 g + 8 (e / 4) + e % 4.  Every load is issued, its place
-// clamped: a branch around each would wait for one after the other (96 x 96 without a step: 11 us instead of 6).
+  // clamped: a branch around each would wait for one after the other (96 x 96 without a step: 11 us instead of 6).
   const int row = 32 * yi + c, col = 32 * yj + 4 * g;
   const bool quads = p.flat && !p.tall && p.cols % 4 == 0;
   {
