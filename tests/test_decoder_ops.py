@@ -1030,6 +1030,14 @@ def test_cross_attention_refuses(change, message):
         assert message in d.vitk_last_error().decode()
 
 
+@pytest.mark.parametrize("change", [dict(Nq=2 ** 30, H=8), dict(Nq=2 ** 31 - 1, H=2), dict(Nk=2 ** 31 - 1)])
+def test_cross_attention_needs_no_workspace_for_what_it_refuses(change):
+    from visiontransformer_amd import vitk
+    d = vitk.dll()
+    a = _xargs(vitk, **change)
+    assert d.vitk_cross_sdpa_fwd_workspace_bytes(C.byref(a)) == 0 and d.vitk_cross_sdpa_bwd_workspace_bytes(C.byref(a)) == 0
+
+
 @pytest.mark.parametrize("change, forward, backward", [
     (dict(B=2 ** 21, H=8, Hkv=8, Nq=1, Nk=5), True, True),  # 2^24 workgroups of four waves
     (dict(B=2 ** 20, H=15, Hkv=15, Nq=1, Nk=5), False, False),

@@ -382,6 +382,11 @@ inline int plan_splits(long long wgs, long long places, long long stages, double
   return best;
 }
 
+// Query rows of a key head and keys that the kernels' row numbers (and what they add to them) hold.
+inline bool few_enough_rows(const vitk_cross_sdpa_args *a) {
+  return (long long)(a->H / a->Hkv) * a->Nq < 2147482624 && a->Nk < 2147482624;
+}
+
 // Argument checks both directions share; fills everything but the launch plan.
 int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Params *p);
 

@@ -27,8 +27,7 @@ int check_args(const char *who, const vitk_cross_sdpa_args *a, bool backward, Pa
   VITK_REQUIRE(std::isfinite(a->scale), "%s: scale is not a finite number", who);
   const long long wq = (long long)a->H * a->dh, wk = (long long)a->Hkv * a->dh;
   const bool any_q = a->B > 0 && a->Nq > 0, any_k = a->B > 0 && a->Nk > 0;
-  VITK_REQUIRE((long long)(a->H / a->Hkv) * a->Nq < 2147482624 && a->Nk < 2147482624,
-               "%s: too many rows", who);
+  VITK_REQUIRE(few_enough_rows(a), "%s: too many rows", who);
   if (any_q) {
     VITK_REQUIRE(a->q && a->out, "%s: null pointer", who);
     VITK_REQUIRE(a->ld_q >= wq && a->ld_out >= wq, "%s: row pitch below H*dh", who);
@@ -577,7 +576,8 @@ size_t fwd_bytes(const Params &p) {
 }  // namespace
 
 extern "C" size_t vitk_cross_sdpa_fwd_workspace_bytes(const vitk_cross_sdpa_args *a) {
-  if (!a || a->B <= 0 || a->Nq <= 0 || a->Nk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->dh < 1) return 0;
+  if (!a || a->B <= 0 || a->Nq <= 0 || a->Nk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->dh < 1 || !few_enough_rows(a))
+    return 0;
   Params p = {};
   p.B = a->B, p.H = a->H, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Nq = a->Nq, p.Nk = a->Nk, p.dh = a->dh;
   p.rows = p.G * p.Nq;

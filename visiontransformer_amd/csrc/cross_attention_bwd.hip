@@ -556,7 +556,9 @@ int launch(Params p, const Plan &n, hipStream_t st) {
 }  // namespace
 
 extern "C" size_t vitk_cross_sdpa_bwd_workspace_bytes(const vitk_cross_sdpa_args *a) {
-  if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->Nq < 0 || a->Nk < 0 || a->dh < 1) return 0;
+  if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->Nq < 0 || a->Nk < 0 || a->dh < 1 ||
+      !few_enough_rows(a))
+    return 0;
   Params p = {};
   p.B = a->B, p.H = a->H, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Nq = a->Nq, p.Nk = a->Nk, p.dh = a->dh;
   p.rows = p.G * p.Nq;
