@@ -29,7 +29,7 @@
 //     workgroup, operands straight from memory (every load of a wave in flight: a few round trips);
 //   otherwise: 64 x 64 or 128 x 128 tiles staged through LDS.
 // y y^T and g g are symmetric: only tiles on and below the diagonal are computed, and mirrored.
-// Twelve 768 x 2304 (272 GFLOP): 1075 - 1110 us, matrix cores: y y^T 60 us, the polynomial 27, the step of y 113, which is
+// Twelve 768 x 2304 (272 GFLOP): 1075 - 1150 us, matrix cores: y y^T 60 us, the polynomial 27, the step of y 113, which is
 // 950, 710 and 870 TFLOP/s of fp16 products; norm and first y 50 us each, 5 TB/s.  One 96 x 96: 27 us, 1000 x 257:
 // 96 us, the latency of 15 dependent products.
 #include "common.h"
